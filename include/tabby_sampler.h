@@ -41,7 +41,7 @@ typedef enum {
   TABBY_ECAPACITY = 5  /* request exceeds what the handle was created for */
 } tabby_status;
 
-typedef enum { TABBY_F32 = 0, TABBY_F16 = 1 } tabby_dtype;
+typedef enum { TABBY_F32 = 0, TABBY_F16 = 1, TABBY_BF16 = 2 } tabby_dtype;
 
 /* Per-row sampling parameters: SamplingParams (sampler.ts:83-98) plus the uniform that
  * SeededRandom.next() (sampler.ts:112-118) would return for this row. All f64, as JS
@@ -199,6 +199,109 @@ TABBY_API int tabby_sampler_sample_lmhead_q4_device(tabby_sampler *sampler, cons
                                                     int32_t block_size,
                                                     const tabby_row_params *params_dev,
                                                     tabby_row_result *results_dev, void *stream);
+/*
+ * Microscaled 4-bit floating point (MXFP4) beside the int4 weights of the reference's
+ * encodeQuantMatmul (src/engine/forward.ts:732-770): values of 4 bits (e2m1: 0, 1/2, 1, 3/2,
+ * 2, 3, 4, 6 and a sign) in blocks of 32 along a row, each block with a power of two as a
+ * biased 8-bit exponent. A matrix [rows, cols] is held as two device arrays in this
+ * library's panel layout; this call gives their sizes (both multiples of 256).
+ */
+TABBY_API int tabby_mx4_bytes(int32_t rows, int32_t cols, int64_t *code_bytes, int64_t *scale_bytes);
+/*
+ * x_dev [rows, cols] of `dtype` (TABBY_F32, TABBY_F16 or TABBY_BF16; rows row_stride elements
+ * apart) to MXFP4, as a loader would convert weights for encodeQuantMatmul
+ * (src/engine/forward.ts:732-770). A block's power is floor(log2(max |x|)) - 2, held to
+ * [-127, 127]; a value is divided by it, rounded to the nearest of the sixteen codes (ties to
+ * the even one) and held to 6. A block that holds a NaN or an infinity is NaN as a whole.
+ * codes_dev is 16-byte aligned, scales_dev 4-byte. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_mx4_quantize_device(const void *x_dev, int32_t dtype, int32_t rows, int32_t cols,
+                                        int64_t row_stride, void *codes_dev, void *scales_dev, void *stream);
+/*
+ * The way back: out_dev [rows, cols] of `dtype` receives the values that the codes stand for,
+ * as encodeQuantMatmul's shader expands its codes (src/engine/forward.ts:732-770): exact in
+ * f32 and bf16 (above their range: infinity), rounded to nearest even in f16. Asynchronous on
+ * `stream`.
+ */
+TABBY_API int tabby_mx4_dequantize_device(const void *codes_dev, const void *scales_dev, int32_t rows,
+                                          int32_t cols, void *out_dev, int32_t dtype, int64_t row_stride,
+                                          void *stream);
+/*
+ * A checkpoint's MXFP4 weights, repacked once as the int4 ones are for encodeQuantMatmul
+ * (src/engine/forward.ts:732-770). Input: row_codes_dev [rows][ceil(cols / 32)][16], two codes
+ * to a byte with the lower column in the low half, and row_scales_dev
+ * [rows][ceil(cols / 32)], the biased exponents (255: a block of NaN). Codes past the last
+ * column are taken as 0. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_mx4_pack_device(const void *row_codes_dev, const void *row_scales_dev, int32_t rows,
+                                    int32_t cols, void *codes_dev, void *scales_dev, void *stream);
+/*
+ * The product that stands in encodeQuantMatmul's place (src/engine/forward.ts:732-770) where
+ * both sides are MXFP4: out_dev [rows, n] of `out_dtype` (rows out_stride elements apart) =
+ * x [rows, k] times the transpose of w [n, k], plus bias_dev [n] (f32, may be NULL). Products
+ * are exact, their sums f32, rounded once to out_dtype. Asynchronous on `stream`; no scratch.
+ */
+TABBY_API int tabby_mx4_matmul_device(const void *x_codes_dev, const void *x_scales_dev, int32_t rows,
+                                      const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,
+                                      int32_t n, int32_t k, void *out_dev, int32_t out_dtype,
+                                      int64_t out_stride, void *stream);
+/*
+ * The same from activations as the lm_head finds them (src/engine/forward.ts:408-428): x_dev
+ * [rows, k] of `x_dtype`, rows x_stride elements apart, is quantised to MXFP4 in the call. The
+ * caller's workspace_dev (16-byte aligned) holds at least code_bytes + scale_bytes of
+ * [rows, k]; calls that may overlap need a workspace each. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64_t x_stride, int32_t rows,
+                                      const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,
+                                      int32_t n, int32_t k, void *out_dev, int32_t out_dtype,
+                                      int64_t out_stride, void *workspace_dev, int64_t workspace_bytes,
+                                      void *stream);
+/*
+ * Bytes of the workspace of the beam selection declared next, which stands where a search has
+ * more than sampleFromTopK's one continuation (src/engine/sampler.ts:147-212).
+ */
+TABBY_API int tabby_beam_workspace(int32_t groups, int32_t beams, int32_t vocab, int32_t count, int64_t *bytes);
+/*
+ * Beam search's selection, in the place of encodeSampling and sampleFromTopK
+ * (src/engine/forward.ts:522-601, src/engine/sampler.ts:147-212). Row g * beams + b of
+ * logits_dev [groups * beams, vocab] (`dtype` TABBY_F32, TABBY_F16 or TABBY_BF16, rows
+ * row_stride elements apart) holds the logits of beam b of group g, whose score so far is
+ * scores_dev [groups, beams] (f32). A continuation by token t scores
+ *   scores[g, b] + (x_t - log sum over the row's allowed entries of exp(x)),
+ * in 64 bits. allowed_dev (may be NULL: everything) has ceil(vocab / 32) words to a row, entry t
+ * at bit t % 32 of word t / 32; what is not allowed is never looked at, NaN included.
+ * done_dev [groups, beams] (may be NULL): a beam with a nonzero entry has ended, and its one
+ * continuation is pad_id at its own score; its logits are not read. A beam whose score is
+ * -inf has no continuations, nor has an entry of -inf or a row in which nothing is allowed.
+ * The `count` (1..128) best of each group's beams (1..64), equal scores in the order of (beam,
+ * token), go to tokens_dev, parents_dev (the beam within its group) and out_scores_dev, each
+ * [groups, count]; where there are fewer the rest is -1, -1 and -inf. status_dev [groups] (may
+ * be NULL) receives TABBY_OK, TABBY_EEMPTY (no continuation at all) or TABBY_EDOMAIN (an
+ * allowed entry of a row that is read is NaN or +inf, or a score is NaN or +inf; the group's
+ * outputs are as if it had none). workspace_dev: 16-byte aligned, of the size given above;
+ * calls that may overlap need one each. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_beam_select_device(const void *logits_dev, int32_t dtype, int64_t row_stride, int32_t groups,
+                                       int32_t beams, int32_t vocab, const float *scores_dev,
+                                       const uint32_t *allowed_dev, const int32_t *done_dev, int32_t pad_id,
+                                       int32_t count, int32_t *tokens_dev, int32_t *parents_dev,
+                                       float *out_scores_dev, int32_t *status_dev, void *workspace_dev,
+                                       int64_t workspace_bytes, void *stream);
+/*
+ * The cached states (the reference's KV cache, src/engine/kvcache.ts:14-104, or anything else
+ * kept by row) follow the beams that survived a selection. src_dev and dst_dev are host arrays
+ * of `states` device addresses, all of one shape: groups * beams rows, row_stride bytes apart,
+ * each of `segments` segments, segment_stride bytes apart, of `capacity` positions of unit_bytes
+ * each. In every segment the first lengths_dev[g] positions (NULL: all; held to
+ * [0, capacity]) of row (g, b) of dst become those of row (g, parents_dev[g, b]) of src; the rest
+ * of dst stays. parents_dev [groups, beams]; a row whose parent is not within [0, beams) stays
+ * as it is. Every state's dst is its src (in place, any parents), or none is, and then they do
+ * not overlap. beams 1..64. Asynchronous on `stream`; no scratch.
+ */
+TABBY_API int tabby_beam_reorder_device(const void *const *src_dev, void *const *dst_dev, int32_t states,
+                                        int32_t groups, int32_t beams, int32_t segments, int64_t capacity,
+                                        int64_t unit_bytes, int64_t row_stride, int64_t segment_stride,
+                                        const int32_t *parents_dev, const int32_t *lengths_dev, void *stream);
 /* Message of the calling thread's last failure ("" if none). */
 TABBY_API const char *tabby_last_error(void);
 

@@ -37,6 +37,13 @@ int handle_view(const tabby_sampler *h, HandleView *out);
 // hidden); TABBY_EINVAL with a message otherwise.
 int check_q4_shape(int32_t vocab, int32_t hidden, int32_t block);
 
+// MXFP4 matrices: the sizes a matrix may have, the pointers of one, and the conversion itself
+// (arguments checked by the caller).
+int check_mx4_shape(int32_t rows, int32_t cols);
+int check_mx4_operand(const void *codes, const void *scales);
+int mx4_quantize(const void *x, int32_t dtype, int32_t rows, int32_t cols, int64_t stride, uint8_t *codes,
+                 uint8_t *scales, hipStream_t s);
+
 }  // namespace tabby
 
 #define TABBY_HIP_CHECK(expr)                                            \

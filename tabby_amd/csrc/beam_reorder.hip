@@ -1,0 +1,159 @@
+// Beam search's states follow the beams that survived: row (g, b) of every state becomes what row
+// (g, parent[g, b]) was, in the first len_g positions of each of its segments, for many states in one
+// launch, in place or into a second set of buffers.
+//
+// One lane owns one column -- kWidth consecutive bytes at one place of the group's rows -- and holds it for
+// all of the group's beams: it loads the columns of the parents, then stores them. So a lane never
+// reads what another writes and the move may run in place, whatever the parents; and a parent with
+// several children is fetched from memory once, its further reads close behind in the cache. Bound by
+// HBM: every surviving row read once, every moved row written once.
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <string>
+
+#include "abi_internal.h"
+#include "loads.h"
+
+namespace tabby {
+namespace {
+
+constexpr int kReorderBlock = 256;
+constexpr int kReorderBeams = 64;
+constexpr int kStatesPerLaunch = 64;  // their addresses travel as arguments
+
+struct ReorderArgs {
+  const char *src[kStatesPerLaunch];
+  char *dst[kStatesPerLaunch];
+  int beams, segments;
+  int64_t capacity;  // positions of a segment
+  int64_t unit;      // bytes of a position
+  int64_t row_stride, segment_stride;
+  const int32_t *parents, *lengths;
+  int64_t chunks;  // workgroups to a segment
+};
+
+template <int BYTES>
+struct ColumnOf;
+template <>
+struct ColumnOf<16> { using T = u32x4; };
+template <>
+struct ColumnOf<8> { using T = uint2; };
+template <>
+struct ColumnOf<4> { using T = uint32_t; };
+template <>
+struct ColumnOf<2> { using T = uint16_t; };
+template <>
+struct ColumnOf<1> { using T = uint8_t; };
+
+// NB: beams held at once. Grid: ((group * segments + segment) * chunks + chunk, state).
+template <int BYTES, int NB, bool IN_PLACE>
+__global__ __launch_bounds__(kReorderBlock) void beam_reorder_kernel(ReorderArgs a) {
+  using T = typename ColumnOf<BYTES>::T;
+  const uint32_t line = blockIdx.x / (uint32_t)a.chunks, chunk = blockIdx.x - line * (uint32_t)a.chunks;
+  const int g = (int)(line / (uint32_t)a.segments), seg = (int)(line - (uint32_t)g * a.segments);
+  int64_t length = a.capacity;
+  if (a.lengths) length = min(length, (int64_t)max(a.lengths[g], 0));
+  const int64_t at = ((int64_t)chunk * kReorderBlock + threadIdx.x) * BYTES;
+  if (at >= length * a.unit) return;
+  const int64_t first = (int64_t)g * a.beams * a.row_stride + seg * a.segment_stride + at;
+  const char *src = a.src[blockIdx.y] + first;
+  char *dst = a.dst[blockIdx.y] + first;
+  const int32_t *parents = a.parents + (int64_t)g * a.beams;
+  T v[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    if (b >= a.beams) break;
+    const uint32_t p = (uint32_t)parents[b];
+    if (p < (uint32_t)a.beams && !(IN_PLACE && p == (uint32_t)b)) v[b] = *reinterpret_cast<const T *>(src + p * a.row_stride);
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    if (b >= a.beams) break;
+    const uint32_t p = (uint32_t)parents[b];
+    if (p < (uint32_t)a.beams && !(IN_PLACE && p == (uint32_t)b)) *reinterpret_cast<T *>(dst + b * a.row_stride) = v[b];
+  }
+}
+
+template <int BYTES, int NB>
+int launch_width(const ReorderArgs &a, dim3 grid, bool in_place, hipStream_t s) {
+  if (in_place) hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, true>), grid, dim3(kReorderBlock), 0, s, a);
+  else hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, false>), grid, dim3(kReorderBlock), 0, s, a);
+  TABBY_HIP_CHECK(hipGetLastError());
+  return TABBY_OK;
+}
+
+template <int BYTES>
+int launch_reorder(ReorderArgs &a, int groups, int states, bool in_place, hipStream_t s) {
+  a.chunks = (a.capacity * a.unit + (int64_t)kReorderBlock * BYTES - 1) / ((int64_t)kReorderBlock * BYTES);
+  const int64_t rows = (int64_t)groups * a.segments;
+  if (a.chunks > INT32_MAX / rows) return record_failure(TABBY_EINVAL, "the states are too large for one launch");
+  const dim3 grid((unsigned)(a.chunks * rows), (unsigned)states);
+  if (a.beams <= 4) return launch_width<BYTES, 4>(a, grid, in_place, s);
+  if (a.beams <= 8) return launch_width<BYTES, 8>(a, grid, in_place, s);
+  if (a.beams <= 16) return launch_width<BYTES, 16>(a, grid, in_place, s);
+  return launch_width<BYTES, 64>(a, grid, in_place, s);
+}
+
+}  // namespace
+}  // namespace tabby
+
+using namespace tabby;
+
+extern "C" int tabby_beam_reorder_device(const void *const *src_dev, void *const *dst_dev, int32_t states,
+                                         int32_t groups, int32_t beams, int32_t segments, int64_t capacity,
+                                         int64_t unit_bytes, int64_t row_stride, int64_t segment_stride,
+                                         const int32_t *parents_dev, const int32_t *lengths_dev, void *stream) {
+  if (!src_dev || !dst_dev || !parents_dev) return record_failure(TABBY_EINVAL, "null pointer");
+  if (states < 1 || groups < 1 || segments < 1 || capacity < 1 || unit_bytes < 1)
+    return record_failure(TABBY_EINVAL, "states, groups, segments, capacity and unit_bytes must be >= 1");
+  if (beams < 1 || beams > kReorderBeams)
+    return record_failure(TABBY_EINVAL, "beams must be between 1 and " + std::to_string(kReorderBeams) + ", got " + std::to_string(beams));
+  if (capacity > INT64_MAX / unit_bytes) return record_failure(TABBY_EINVAL, "a segment must fit 63 bits");
+  const int64_t segment = capacity * unit_bytes;
+  if (segments > 1 && segment_stride < segment)
+    return record_failure(TABBY_EINVAL, "segment_stride must be at least capacity x unit_bytes");
+  if ((int64_t)groups * segments > INT32_MAX) return record_failure(TABBY_EINVAL, "groups x segments must fit 32 bits");
+  const int64_t rows = (int64_t)groups * beams;
+  const int64_t last = (segments - 1) * segment_stride;  // where a row's last segment starts
+  if (rows > 1 && row_stride < last + segment) return record_failure(TABBY_EINVAL, "rows must not overlap: row_stride is too small");
+  const int64_t span = (rows - 1) * row_stride + last + segment;
+  // The widest column that every address is a multiple of.
+  uint64_t bits = (uint64_t)unit_bytes | (rows > 1 ? (uint64_t)row_stride : 0) | (segments > 1 ? (uint64_t)segment_stride : 0);
+  const bool in_place = src_dev[0] == dst_dev[0];
+  for (int i = 0; i < states; ++i) {
+    const char *from = (const char *)src_dev[i], *to = (const char *)dst_dev[i];
+    if (!from || !to) return record_failure(TABBY_EINVAL, "null pointer");
+    if ((from == to) != in_place) return record_failure(TABBY_EINVAL, "either every state or none is moved in place");
+    if (from != to && from < to + span && to < from + span)
+      return record_failure(TABBY_EINVAL, "a state's source and destination must be the same or not overlap");
+    bits |= (uint64_t)(uintptr_t)from | (uint64_t)(uintptr_t)to;
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  for (int i0 = 0; i0 < states; i0 += kStatesPerLaunch) {
+    const int n = std::min(kStatesPerLaunch, states - i0);
+    ReorderArgs a{};
+    for (int i = 0; i < n; ++i) {
+      a.src[i] = (const char *)src_dev[i0 + i];
+      a.dst[i] = (char *)dst_dev[i0 + i];
+    }
+    a.beams = beams;
+    a.segments = segments;
+    a.capacity = capacity;
+    a.unit = unit_bytes;
+    a.row_stride = row_stride;
+    a.segment_stride = segment_stride;
+    a.parents = parents_dev;
+    a.lengths = lengths_dev;
+    int rc;
+    if (bits % 16 == 0) rc = launch_reorder<16>(a, groups, n, in_place, s);
+    else if (bits % 8 == 0) rc = launch_reorder<8>(a, groups, n, in_place, s);
+    else if (bits % 4 == 0) rc = launch_reorder<4>(a, groups, n, in_place, s);
+    else if (bits % 2 == 0) rc = launch_reorder<2>(a, groups, n, in_place, s);
+    else rc = launch_reorder<1>(a, groups, n, in_place, s);
+    if (rc) return rc;
+  }
+  return TABBY_OK;
+}

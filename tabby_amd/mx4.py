@@ -1,0 +1,212 @@
+"""Microscaled 4-bit floating point (MXFP4) on the GPU: conversion, the way back, and the
+product of two such matrices, over the C ABI's ``tabby_mx4_*`` entries.
+
+It stands beside ``sampler.LmHeadQ4`` (the reference's int4 lm_head, src/engine/forward.ts:
+408-428, 732-770) for checkpoints whose weights are MXFP4: values of 4 bits (e2m1) in blocks
+of 32 along a row, each block with a power of two of its own. ``LmHeadMx4.logits`` quantises the
+hidden states as well, so that the product runs on the matrix cores' scaled 4-bit instructions.
+
+Every call is asynchronous on the given stream (default: torch's current one) and checks its
+arguments before any GPU work.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Optional
+
+from .sampler import TABBY_BF16, TABBY_F16, TABBY_F32, _check, load_library
+
+BLOCK = 32  # values to a scale
+
+
+def dtype_code(dtype) -> int:
+    import torch
+    codes = {torch.float32: TABBY_F32, torch.float16: TABBY_F16, torch.bfloat16: TABBY_BF16}
+    if dtype not in codes:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {dtype}")
+    return codes[dtype]
+
+
+def rows_of(x, what: str):
+    """A CUDA tensor as rows: 1-D becomes one row; a row's elements must be adjacent."""
+    if not x.is_cuda:
+        raise ValueError(f"{what} must be a device (cuda) tensor")
+    if x.dim() not in (1, 2):
+        raise ValueError(f"{what} must have one or two dimensions, got {x.dim()}")
+    x = x if x.dim() == 2 else x.unsqueeze(0)
+    if x.shape[0] < 1 or x.shape[1] < 1:
+        raise ValueError(f"{what} must not be empty, got {tuple(x.shape)}")
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"{what} must hold its rows' elements adjacent and its rows apart")
+    return x
+
+
+def on_device(device, *tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors lie on {device} and on {t.device}")
+
+
+@contextlib.contextmanager
+def _guard(device, stream):
+    import torch
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def call_on(device, stream):
+    """(context, stream handle) of a call on ``device``: the device is made current where it is
+    not, and what the call allocates belongs to its stream."""
+    import torch
+    if stream is None:
+        if device.index == torch.cuda.current_device():
+            return contextlib.nullcontext(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        stream = torch.cuda.current_stream(device)
+    elif stream.device != device:
+        raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+    return _guard(device, stream), ctypes.c_void_p(stream.cuda_stream)
+
+
+def sizes(rows: int, cols: int):
+    """Bytes of a matrix's codes and scales."""
+    code, scale = ctypes.c_int64(), ctypes.c_int64()
+    _check(load_library().tabby_mx4_bytes(rows, cols, ctypes.byref(code), ctypes.byref(scale)))
+    return code.value, scale.value
+
+
+class Mx4Matrix:
+    """A [rows, cols] matrix in MXFP4 on the device, in the library's panel layout. Its buffers may
+    be written again with ``quantize(x, out=matrix)``."""
+
+    def __init__(self, rows: int, cols: int, device="cuda"):
+        import torch
+        code, scale = sizes(rows, cols)
+        self.rows, self.cols = int(rows), int(cols)
+        self.codes = torch.empty(code, dtype=torch.uint8, device=device)
+        self.scales = torch.empty(scale, dtype=torch.uint8, device=device)
+
+    @classmethod
+    def quantize(cls, x, out: Optional["Mx4Matrix"] = None, stream=None) -> "Mx4Matrix":
+        """``x`` ([rows, cols] or [cols], float32, float16 or bfloat16) rounded to MXFP4: a block's
+        power of two is floor(log2(max |x|)) - 2, values go to the nearest code (ties to even, at
+        most 6); a block with a NaN or an infinity becomes NaN."""
+        x = rows_of(x, "x")
+        code = dtype_code(x.dtype)
+        rows, cols = int(x.shape[0]), int(x.shape[1])
+        ctx, handle = call_on(x.device, stream)
+        with ctx:
+            m = cls(rows, cols, x.device) if out is None else out
+            if (m.rows, m.cols) != (rows, cols):
+                raise ValueError(f"out is {m.rows} x {m.cols}, x is {rows} x {cols}")
+            on_device(x.device, m.codes)
+            _check(load_library().tabby_mx4_quantize_device(
+                x.data_ptr(), code, rows, cols, x.stride(0), m.codes.data_ptr(), m.scales.data_ptr(), handle))
+        return m
+
+    @classmethod
+    def from_rowmajor(cls, codes, scales, cols: int, stream=None) -> "Mx4Matrix":
+        """A checkpoint's layout, repacked once: ``codes`` uint8 [rows, ceil(cols / 32) * 16], two to a
+        byte with the lower column in the low half, ``scales`` uint8 [rows, ceil(cols / 32)], the
+        biased exponents."""
+        import torch
+        blocks = -(-int(cols) // BLOCK)
+        if not codes.is_cuda or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError("codes and scales must be uint8 device (cuda) tensors")
+        if codes.dim() != 2 or codes.shape[0] < 1 or cols < 1 or codes.shape[1] != blocks * BLOCK // 2:
+            raise ValueError(f"codes must have shape (rows, {blocks * BLOCK // 2}), got {tuple(codes.shape)}")
+        if tuple(scales.shape) != (codes.shape[0], blocks):
+            raise ValueError(f"scales must have shape ({codes.shape[0]}, {blocks}), got {tuple(scales.shape)}")
+        if not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("codes and scales must be contiguous")
+        on_device(codes.device, scales)
+        ctx, handle = call_on(codes.device, stream)
+        with ctx:
+            m = cls(int(codes.shape[0]), int(cols), codes.device)
+            _check(load_library().tabby_mx4_pack_device(
+                codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, m.codes.data_ptr(), m.scales.data_ptr(), handle))
+        return m
+
+    def dequantize(self, dtype=None, out=None, stream=None):
+        """The values that the codes stand for, [rows, cols]: exact in float32 (the default) and
+        bfloat16, rounded once in float16."""
+        import torch
+        if out is None:
+            code = dtype_code(dtype or torch.float32)
+        else:
+            if dtype is not None and out.dtype != dtype:
+                raise ValueError(f"out is {out.dtype}, asked for {dtype}")
+            code = dtype_code(out.dtype)
+            out = rows_of(out, "out")
+            if tuple(out.shape) != (self.rows, self.cols):
+                raise ValueError(f"out must have shape ({self.rows}, {self.cols}), got {tuple(out.shape)}")
+            on_device(self.codes.device, out)
+        ctx, handle = call_on(self.codes.device, stream)
+        with ctx:
+            if out is None:
+                out = torch.empty((self.rows, self.cols), dtype=dtype or torch.float32, device=self.codes.device)
+            _check(load_library().tabby_mx4_dequantize_device(
+                self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.cols, out.data_ptr(), code,
+                out.stride(0), handle))
+        return out
+
+
+def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
+    """x W^T (+ bias), [rows, w.rows] of ``dtype`` (float32 by default): ``x`` is an ``Mx4Matrix``
+    or a float tensor ([rows, k] or [k]), which is quantised in the call. Products of codes are
+    exact, their sums float32, rounded once to ``dtype``."""
+    import torch
+    device = w.codes.device
+    quantized = isinstance(x, Mx4Matrix)
+    if not quantized:
+        x = rows_of(x, "x")
+        x_code = dtype_code(x.dtype)
+        on_device(device, x)
+    else:
+        on_device(device, x.codes)
+    rows, k = (x.rows, x.cols) if quantized else (int(x.shape[0]), int(x.shape[1]))
+    if k != w.cols:
+        raise ValueError(f"x has {k} columns, the weights {w.cols}")
+    if bias is not None:
+        on_device(device, bias)
+        if bias.dtype != torch.float32 or not bias.is_contiguous() or tuple(bias.shape) != (w.rows,):
+            raise ValueError(f"bias must be a contiguous float32 tensor of {w.rows} entries")
+    if out is None:
+        dtype = dtype or torch.float32
+        code = dtype_code(dtype)
+    else:
+        if dtype is not None and out.dtype != dtype:
+            raise ValueError(f"out is {out.dtype}, asked for {dtype}")
+        code = dtype_code(out.dtype)
+        out = rows_of(out, "out")
+        if tuple(out.shape) != (rows, w.rows):
+            raise ValueError(f"out must have shape ({rows}, {w.rows}), got {tuple(out.shape)}")
+        on_device(device, out)
+    lib = load_library()
+    bias_ptr = bias.data_ptr() if bias is not None else None
+    ctx, handle = call_on(device, stream)
+    with ctx:
+        if out is None:
+            out = torch.empty((rows, w.rows), dtype=dtype, device=device)
+        if quantized:
+            _check(lib.tabby_mx4_matmul_device(
+                x.codes.data_ptr(), x.scales.data_ptr(), rows, w.codes.data_ptr(), w.scales.data_ptr(), bias_ptr,
+                w.rows, k, out.data_ptr(), code, out.stride(0), handle))
+        else:
+            space = torch.empty(sum(sizes(rows, k)), dtype=torch.uint8, device=device)
+            _check(lib.tabby_mx4_linear_device(
+                x.data_ptr(), x_code, x.stride(0), rows, w.codes.data_ptr(), w.scales.data_ptr(), bias_ptr,
+                w.rows, k, out.data_ptr(), code, out.stride(0), space.data_ptr(), space.numel(), handle))
+    return out
+
+
+class LmHeadMx4:
+    """An lm_head with MXFP4 weights [vocab, hidden] and an optional float32 bias [vocab]."""
+
+    def __init__(self, weight: Mx4Matrix, bias=None):
+        self.weight, self.bias = weight, bias
+        self.vocab, self.hidden = weight.rows, weight.cols
+
+    def logits(self, hidden_states, dtype=None, out=None, stream=None):
+        """Logits [rows, vocab] (float32 by default) of hidden states [rows, hidden] or [hidden]."""
+        return matmul(hidden_states, self.weight, self.bias, dtype=dtype, out=out, stream=stream)

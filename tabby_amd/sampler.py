@@ -29,7 +29,7 @@ import numpy as np
 from .build import LIB_PATH
 
 TABBY_OK, TABBY_EINVAL, TABBY_EHIP, TABBY_EEMPTY, TABBY_EDOMAIN, TABBY_ECAPACITY = range(6)
-TABBY_F32, TABBY_F16 = 0, 1
+TABBY_F32, TABBY_F16, TABBY_BF16 = 0, 1, 2  # bf16: the MXFP4 and beam operators only
 TABBY_FLAG_FULL_VOCAB = 1
 
 PARAMS_DTYPE = np.dtype([
@@ -50,6 +50,9 @@ EXPORTED_SYMBOLS = (
     "tabby_argmax_device", "tabby_softmax_rows_device", "tabby_debug_stream_read",
     "tabby_debug_exp_f32", "tabby_lmhead_q4_pack_device", "tabby_lmhead_q4_device",
     "tabby_sampler_sample_lmhead_q4_device",
+    "tabby_mx4_bytes", "tabby_mx4_quantize_device", "tabby_mx4_dequantize_device", "tabby_mx4_pack_device",
+    "tabby_mx4_matmul_device", "tabby_mx4_linear_device", "tabby_beam_workspace", "tabby_beam_select_device",
+    "tabby_beam_reorder_device",
 )
 
 
@@ -90,6 +93,18 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     L.tabby_lmhead_q4_pack_device.argtypes = [vp, vp, i32, i32, i32, vp, vp, vp]
     L.tabby_lmhead_q4_device.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]
     L.tabby_sampler_sample_lmhead_q4_device.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp]
+    pi64 = ctypes.POINTER(i64)
+    L.tabby_mx4_bytes.argtypes = [i32, i32, pi64, pi64]
+    L.tabby_mx4_quantize_device.argtypes = [vp, i32, i32, i32, i64, vp, vp, vp]
+    L.tabby_mx4_dequantize_device.argtypes = [vp, vp, i32, i32, vp, i32, i64, vp]
+    L.tabby_mx4_pack_device.argtypes = [vp, vp, i32, i32, vp, vp, vp]
+    L.tabby_mx4_matmul_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp]
+    L.tabby_mx4_linear_device.argtypes = [vp, i32, i64, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp, i64, vp]
+    L.tabby_beam_workspace.argtypes = [i32, i32, i32, i32, pi64]
+    L.tabby_beam_select_device.argtypes = [vp, i32, i64, i32, i32, i32, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, i64, vp]
+    L.tabby_beam_reorder_device.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, i64, i64, vp, vp, vp]
+    for name in EXPORTED_SYMBOLS[-9:]:
+        getattr(L, name).restype = ctypes.c_int
     for name in ("tabby_sampler_create", "tabby_sampler_destroy", "tabby_sampler_sample_device",
                  "tabby_sampler_sample", "tabby_debug_exp", "tabby_debug_seq_sum",
                  "tabby_debug_first_above", "tabby_sampler_sample_device_noalloc",

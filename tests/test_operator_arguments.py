@@ -1,0 +1,109 @@
+"""The C entries of the MXFP4 and beam operators refuse bad arguments before any GPU work: no
+GPU is needed to be refused. The addresses are never read."""
+import ctypes
+
+import pytest
+
+from tabby_amd import sampler as S
+
+A = 1 << 20  # an aligned address that nothing reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return S.load_library()
+
+
+def _refused(lib, rc, text, status=S.TABBY_EINVAL):
+    assert rc == status
+    assert text in lib.tabby_last_error().decode()
+
+
+def test_mx4_sizes(lib):
+    code, scale = ctypes.c_int64(), ctypes.c_int64()
+    for rows, cols, panels in ((1, 1, 1), (64, 128, 1), (65, 128, 2), (64, 129, 2), (151936, 896, 2374 * 7)):
+        assert lib.tabby_mx4_bytes(rows, cols, ctypes.byref(code), ctypes.byref(scale)) == 0
+        assert (code.value, scale.value) == (panels * 4096, panels * 256)
+    big = 2 ** 31 - 129
+    assert lib.tabby_mx4_bytes(big, big, ctypes.byref(code), ctypes.byref(scale)) == 0
+    assert code.value == -(-big // 64) * -(-big // 128) * 4096
+    _refused(lib, lib.tabby_mx4_bytes(0, 5, ctypes.byref(code), ctypes.byref(scale)), ">= 1")
+    _refused(lib, lib.tabby_mx4_bytes(5, 2 ** 31 - 1, ctypes.byref(code), ctypes.byref(scale)), "padding")
+    _refused(lib, lib.tabby_mx4_bytes(5, 5, None, ctypes.byref(scale)), "null")
+
+
+def test_mx4_conversion_arguments(lib):
+    q, d, p = lib.tabby_mx4_quantize_device, lib.tabby_mx4_dequantize_device, lib.tabby_mx4_pack_device
+    _refused(lib, q(None, 0, 1, 32, 32, A, A, None), "null")
+    _refused(lib, q(A, 0, 1, 32, 32, A + 8, A, None), "aligned")
+    _refused(lib, q(A, 0, 1, 32, 32, A, A + 2, None), "aligned")
+    _refused(lib, q(A, 3, 1, 32, 32, A, A, None), "dtype")
+    _refused(lib, q(A, 0, 2, 32, 31, A, A, None), "row_stride")
+    _refused(lib, q(A + 2, 0, 1, 32, 32, A, A, None), "elements")
+    _refused(lib, q(A, 0, 0, 32, 32, A, A, None), ">= 1")
+    _refused(lib, d(A, A, 1, 32, None, 0, 32, None), "null")
+    _refused(lib, d(A, A, 1, 32, A, -1, 32, None), "dtype")
+    _refused(lib, d(A, A, 2, 32, A, 0, 5, None), "row_stride")
+    _refused(lib, d(A, None, 1, 32, A, 0, 32, None), "null")
+    _refused(lib, p(None, A, 1, 32, A, A, None), "null")
+    _refused(lib, p(A, A, 1, 0, A, A, None), ">= 1")
+
+
+def test_mx4_product_arguments(lib):
+    m, f = lib.tabby_mx4_matmul_device, lib.tabby_mx4_linear_device
+    _refused(lib, m(A, A, 1, None, A, None, 64, 128, A, 0, 64, None), "null")
+    _refused(lib, m(A, A, 1, A, A, None, 64, 0, A, 0, 64, None), ">= 1")
+    _refused(lib, m(A, A, 2, A, A, None, 64, 128, A, 0, 63, None), "out_stride")
+    _refused(lib, m(A, A, 1, A, A, None, 64, 128, A, 5, 64, None), "dtype")
+    _refused(lib, m(A, A, 1, A, A, None, 64, 128, A + 1, 1, 64, None), "elements")
+    _refused(lib, f(A, 0, 128, 1, A, A, None, 64, 128, A, 0, 64, None, 1 << 20, None), "null")
+    _refused(lib, f(A, 9, 128, 1, A, A, None, 64, 128, A, 0, 64, A, 1 << 20, None), "dtype")
+    _refused(lib, f(A, 0, 100, 2, A, A, None, 64, 128, A, 0, 64, A, 1 << 20, None), "x_stride")
+    _refused(lib, f(A, 0, 128, 1, A, A, None, 64, 128, A, 0, 64, A, 4351, None), "workspace")
+    _refused(lib, f(A, 0, 128, 1, A, A, None, 64, 128, A, 0, 64, A + 8, 1 << 20, None), "workspace")
+
+
+def test_beam_selection_arguments(lib):
+    size = ctypes.c_int64()
+    _refused(lib, lib.tabby_beam_workspace(1, 65, 10, 4, ctypes.byref(size)), "beams must be between 1 and 64, got 65")
+    _refused(lib, lib.tabby_beam_workspace(1, 4, 10, 129, ctypes.byref(size)), "count must be between 1 and 128, got 129")
+    _refused(lib, lib.tabby_beam_workspace(0, 4, 10, 4, ctypes.byref(size)), ">= 1")
+    assert lib.tabby_beam_workspace(3, 4, 1000, 8, ctypes.byref(size)) == 0
+    need = size.value
+
+    def call(logits=A, dtype=0, stride=1000, groups=3, beams=4, vocab=1000, scores=A, pad=0, count=8, tokens=A, space=A,
+             bytes_=need):
+        return lib.tabby_beam_select_device(logits, dtype, stride, groups, beams, vocab, scores, None, None, pad, count,
+                                            tokens, A, A, None, space, bytes_, None)
+    _refused(lib, call(logits=None), "null")
+    _refused(lib, call(scores=None), "null")
+    _refused(lib, call(space=None), "null")
+    _refused(lib, call(dtype=7), "dtype")
+    _refused(lib, call(stride=999), "row_stride")
+    _refused(lib, call(logits=A + 2), "elements")
+    _refused(lib, call(pad=-1), "pad_id")
+    _refused(lib, call(count=0), "count")
+    _refused(lib, call(vocab=0), ">= 1")
+    _refused(lib, call(groups=2 ** 26, beams=64), "32 bits")
+    _refused(lib, call(bytes_=need - 1), "workspace")
+    _refused(lib, call(space=A + 8), "workspace")
+
+
+def test_beam_reorder_arguments(lib):
+    def call(src=(A, 2 * A), dst=(3 * A, 4 * A), groups=2, beams=4, segments=2, capacity=16, unit=128, row=4096, segment=2048,
+             parents=A):
+        n = len(src)
+        arr = ctypes.c_void_p * n
+        return lib.tabby_beam_reorder_device(arr(*src), arr(*dst), n, groups, beams, segments, capacity, unit, row, segment,
+                                             parents, None, None)
+    _refused(lib, call(parents=None), "null")
+    _refused(lib, call(src=(A, None)), "null")
+    _refused(lib, call(beams=65), "beams must be between 1 and 64, got 65")
+    _refused(lib, call(capacity=0), ">= 1")
+    _refused(lib, call(unit=0), ">= 1")
+    _refused(lib, call(segment=2047), "segment_stride")
+    _refused(lib, call(row=4095), "row_stride")
+    _refused(lib, call(capacity=2 ** 62, unit=8), "63 bits")
+    _refused(lib, call(dst=(A, 4 * A)), "in place")
+    _refused(lib, call(dst=(A + 4096, 4 * A)), "overlap")
+    _refused(lib, call(groups=2 ** 20, segments=2 ** 20), "32 bits")
