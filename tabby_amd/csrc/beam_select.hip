@@ -490,7 +490,7 @@ int check_beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count
   if (count < 1 || count > kCountMax)
     return record_failure(TABBY_EINVAL, "count must be between 1 and " + std::to_string(kCountMax) + ", got " + std::to_string(count));
   if (vocab > kVocabMax) return record_failure(TABBY_EINVAL, "vocab must be at most " + std::to_string(kVocabMax));
-  if ((int64_t)groups * beams > INT32_MAX / kPartsMax) return record_failure(TABBY_EINVAL, "groups x beams must fit 27 bits");
+  if ((int64_t)groups * beams > INT32_MAX / kPartsMax) return record_failure(TABBY_EINVAL, "groups x beams x " + std::to_string(kPartsMax) + " must fit 32 bits");
   return TABBY_OK;
 }
 
