@@ -30,7 +30,7 @@ constexpr int kMxPanelScales = 256;    // scales of a panel
 constexpr uint32_t kMxScaleOne = 127;  // 2^0
 constexpr uint32_t kMxScaleNan = 255;
 
-__host__ __device__ __forceinline__ int64_t mx_panels(int64_t size, int to) { return (size + to - 1) / to; }
+__host__ __device__ __forceinline__ int64_t mx_panels(int64_t size, int64_t to) { return (size + to - 1) / to; }
 
 struct Mx4Matrix {
   const uint8_t *codes;
