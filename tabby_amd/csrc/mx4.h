@@ -18,6 +18,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "elem.h"
+
 namespace tabby {
 
 constexpr int kMxBlock = 32;           // values to a scale
@@ -38,5 +40,54 @@ struct Mx4Matrix {
   int rows, cols;
   __host__ __device__ int col_panels() const { return (cols + kMxPanelCols - 1) / kMxPanelCols; }
 };
+
+// The block's biased exponent from the largest magnitude's bits (f32).
+__device__ __forceinline__ uint32_t block_scale(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return kMxScaleNan;
+  const int e = (int)(amax_bits >> 23) - 2;  // a subnormal's field is 0: below the range all the same
+  return (uint32_t)max(e, 0);
+}
+
+// The values of one row from column `col` on, widened; zero past the last column.
+template <int DT, bool VEC>
+__device__ __forceinline__ void load_block(const typename Elem<DT>::Bits *src, int col, int cols, float (&v)[kMxBlock]) {
+  using E = Elem<DT>;
+  if (VEC && col + kMxBlock <= cols) {
+#pragma unroll
+    for (int i = 0; i < kMxBlock; i += E::kVec) {
+      float w[E::kVec];
+      E::widen16(*reinterpret_cast<const u32x4 *>(src + col + i), w);
+#pragma unroll
+      for (int j = 0; j < E::kVec; ++j) v[i + j] = w[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kMxBlock; ++i) v[i] = col + i < cols ? E::widen(src[col + i]) : 0.0f;
+  }
+}
+
+// A block's codes and biased exponent E + 127 from its values. E = floor(log2(max|x|)) - 2, the power of two
+// that puts the largest value into [4, 8), held to [-127, 127] (a block of zeros: -127). A value's code
+// is x / 2^E rounded to the nearest of the eight magnitudes, ties to the even code, and what lies above
+// 6 becomes 6. A block with a NaN or an infinity is NaN as a whole, its codes 0. The rounding is the
+// hardware's scaled conversion; the division by a power of two is exact, so there is one rounding to a
+// value.
+__device__ __forceinline__ uint32_t encode_block(const float (&v)[kMxBlock], u32x4 &codes) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kMxBlock; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  const uint32_t s = block_scale(top);
+  const float scale = __uint_as_float(s << 23);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t word = 0;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i], v[8 * i + 1], scale, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 2], v[8 * i + 3], scale, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 4], v[8 * i + 5], scale, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 6], v[8 * i + 7], scale, 3);
+    codes[i] = s != kMxScaleNan ? word : 0u;
+  }
+  return s;
+}
 
 }  // namespace tabby

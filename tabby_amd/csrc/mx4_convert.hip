@@ -1,11 +1,5 @@
 // MXFP4 conversions: a matrix to codes and scales (mx4.h has the layout), the way back, and the
 // repacking of a checkpoint's row-major codes.
-//
-// A block's exponent is E = floor(log2(max|x|)) - 2, the power of two that puts its largest value
-// into [4, 8), held to [-127, 127] (a block of zeros: -127). A value's code is x / 2^E rounded to the
-// nearest of the eight magnitudes, ties to the even code, and what lies above 6 becomes 6. A block
-// with a NaN or an infinity is NaN as a whole. The rounding is the hardware's scaled conversion; the
-// division by a power of two is exact, so there is one rounding to a value.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,31 +16,6 @@ namespace {
 
 constexpr int kConvertBlock = 256;  // 16 rows x 16 blocks: one tile to a wave
 
-// The block's biased exponent from the largest magnitude's bits (f32).
-__device__ __forceinline__ uint32_t block_scale(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return kMxScaleNan;
-  const int e = (int)(amax_bits >> 23) - 2;  // a subnormal's field is 0: below the range all the same
-  return (uint32_t)max(e, 0);
-}
-
-// Row `row`'s values of block `block`, widened; zero past the last column.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_block(const typename Elem<DT>::Bits *src, int col, int cols, float (&v)[kMxBlock]) {
-  using E = Elem<DT>;
-  if (VEC && col + kMxBlock <= cols) {
-#pragma unroll
-    for (int i = 0; i < kMxBlock; i += E::kVec) {
-      float w[E::kVec];
-      E::widen16(*reinterpret_cast<const u32x4 *>(src + col + i), w);
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) v[i + j] = w[j];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kMxBlock; ++i) v[i] = col + i < cols ? E::widen(src[col + i]) : 0.0f;
-  }
-}
-
 template <int DT, bool VEC>
 __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typename Elem<DT>::Bits *x, int rows, int cols,
                                                                      int64_t stride, uint8_t *codes, uint8_t *scales) {
@@ -60,24 +29,10 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
     if (row >= rows) continue;
     float v[kMxBlock];
     load_block<DT, VEC>(x + (int64_t)row * stride, col, cols, v);
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < kMxBlock; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    const uint32_t s = block_scale(top);
-    const float scale = __uint_as_float(s << 23);
-    uint32_t word[4] = {0, 0, 0, 0};
-    if (s != kMxScaleNan) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        word[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word[i], v[8 * i], v[8 * i + 1], scale, 0);
-        word[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word[i], v[8 * i + 2], v[8 * i + 3], scale, 1);
-        word[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word[i], v[8 * i + 4], v[8 * i + 5], scale, 2);
-        word[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word[i], v[8 * i + 6], v[8 * i + 7], scale, 3);
-      }
-    }
+    u32x4 word;
+    const uint32_t s = encode_block(v, word);
     const int64_t panel = (int64_t)(tile >> 2) * col_panels + panel_col;
-    *reinterpret_cast<u32x4 *>(codes + panel * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16) =
-        u32x4{word[0], word[1], word[2], word[3]};
+    *reinterpret_cast<u32x4 *>(codes + panel * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16) = word;
     scales[panel * kMxPanelScales + lane * 4 + (tile & 3)] = (uint8_t)(col < cols ? s : kMxScaleOne);
   }
 }

@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "abi_internal.h"
 #include "elem.h"
@@ -298,36 +299,173 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mx4_tile_kernel(Mx4Product p, 
   }
 }
 
-// One wave to 64 columns and 16 rows of Y.
-template <int DT>
-__global__ __launch_bounds__(64) void mx4_panel_kernel(Mx4Product p) {
-  const int lane = (int)threadIdx.x;
-  const int kp = p.w.col_panels();
-  const int64_t wp = (int64_t)blockIdx.x * kp;
-  for (int tile = (int)blockIdx.y; tile * kMxTileRows < p.x.rows; tile += (int)gridDim.y) {
-    const int64_t xp = (int64_t)(tile >> 2) * kp;
-    f32x4 acc[4] = {};
-    for (int k = 0; k < kp; ++k) {
-      const uint8_t *wc = p.w.codes + (wp + k) * kMxPanelBytes + lane * 16;
-      const uint8_t *xc = p.x.codes + (xp + k) * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16;
-      const uint32_t sw = *reinterpret_cast<const uint32_t *>(p.w.scales + (wp + k) * kMxPanelScales + lane * 4);
-      const uint32_t sx = *reinterpret_cast<const uint32_t *>(p.x.scales + (xp + k) * kMxPanelScales + lane * 4) >> (8 * (tile & 3));
-      const u32x4 b = *reinterpret_cast<const u32x4 *>(xc);
-      u32x4 a[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) a[t] = *reinterpret_cast<const u32x4 *>(wc + t * kMxTileBytes);
-      acc[0] = mx4_mfma<0, 0>(a[0], b, acc[0], sw, sx);
-      acc[1] = mx4_mfma<1, 0>(a[1], b, acc[1], sw, sx);
-      acc[2] = mx4_mfma<2, 0>(a[2], b, acc[2], sw, sx);
-      acc[3] = mx4_mfma<3, 0>(a[3], b, acc[3], sw, sx);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      store4<DT>(p, tile * kMxTileRows + (lane & 15), (int)blockIdx.x * kMxPanelRows + t * kMxTileRows + (lane >> 4) * 4, acc[t]);
+// Few rows: W is streamed from memory straight into registers, a wave to a panel of 64 columns of Y and
+// NT tiles of 16 rows. Bound by HBM where W is large (1 x 151936, k = 896: 12 us, 5.9 TB/s); where it is
+// small, by how long a wave takes for its share of k, so `slices` waves of the workgroup take a part of
+// k each and add up through LDS.
+struct FewShape {
+  int waves, slices;  // of a workgroup; powers of two
+};
+constexpr int kSlicesMax = 8;
+constexpr int kSumsMax = 16;        // slices * NT: the upper half of the slices' sums lie in LDS, 4 KB to a tile of rows
+constexpr int kFewLds = kSumsMax / 2 * 4096;
+constexpr int kStepBytes = kMxTileBytes + 64;      // codes and scales of 16 rows, 128 columns
+constexpr int kFloatPanels = kFewLds / kStepBytes;  // of k, of X quantised in the workgroup
+
+// The tiles of X as they are held.
+template <int NT>
+struct HeldTiles {
+  using Args = Mx4Matrix;
+  static constexpr int kTiles = NT;
+  struct Raw { u32x4 codes[NT]; uint32_t scales; };
+  const uint8_t *codes, *scales;
+  uint32_t shift;
+  __device__ __forceinline__ HeldTiles(const Mx4Matrix &m, const uint8_t *, int tile, int lane) {
+    // NT tiles from `tile` on lie in one panel.
+    const int64_t panel = (int64_t)(tile >> 2) * m.col_panels();
+    codes = m.codes + panel * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16;
+    scales = m.scales + panel * kMxPanelScales + lane * 4;
+    shift = 8 * (tile & 3);
   }
+  static __device__ __forceinline__ void fill(const Mx4Matrix &, uint8_t *, int) {}
+  __device__ __forceinline__ void load(int k, Raw &r) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) r.codes[t] = *reinterpret_cast<const u32x4 *>(codes + (int64_t)k * kMxPanelBytes + t * kMxTileBytes);
+    r.scales = *reinterpret_cast<const uint32_t *>(scales + (int64_t)k * kMxPanelScales);
+  }
+  __device__ __forceinline__ uint32_t tiles(const Raw &r, int, u32x4 (&c)[NT]) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) c[t] = r.codes[t];
+    return r.scales >> shift;
+  }
+};
+
+// Up to 16 rows of x's own values: every workgroup quantises all of them into LDS, a block of one row to a
+// thread, which costs it less than a launch before this one does. Rows past the last hold anything.
+struct FloatRows {
+  const void *x;
+  int64_t stride;
+  int rows, cols;
+  int wide;  // 16-byte loads
+};
+
+template <int XDT>
+struct FloatTiles {
+  using Args = FloatRows;
+  static constexpr int kTiles = 1;
+  struct Raw {};
+  const uint8_t *codes;
+  __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int lane) : codes(lds) { (void)lane; }
+  static __device__ __forceinline__ void fill(const FloatRows &a, uint8_t *lds, int kp) {
+    using E = Elem<XDT>;
+    for (int i = (int)threadIdx.x; i < a.rows * kp * 4; i += (int)blockDim.x) {
+      const int r = i / (kp * 4), b = i - r * (kp * 4), col = b * kMxBlock;
+      const auto *row = (const typename E::Bits *)a.x + (int64_t)r * a.stride;
+      float v[kMxBlock];
+      u32x4 word;
+      if (a.wide) load_block<XDT, true>(row, col, a.cols, v);
+      else load_block<XDT, false>(row, col, a.cols, v);
+      const uint32_t s = encode_block(v, word);
+      uint8_t *to = lds + (b >> 2) * kStepBytes;
+      const int lane = r + 16 * (b & 3);
+      *reinterpret_cast<u32x4 *>(to + lane * 16) = word;
+      to[kMxTileBytes + lane] = (uint8_t)(col < a.cols ? s : kMxScaleOne);
+    }
+  }
+  __device__ __forceinline__ void load(int, Raw &) const {}
+  __device__ __forceinline__ uint32_t tiles(const Raw &, int k, u32x4 (&c)[1]) const {
+    const uint8_t *at = codes + k * kStepBytes;
+    c[0] = *reinterpret_cast<const u32x4 *>(at + (threadIdx.x & 63) * 16);
+    return at[kMxTileBytes + (threadIdx.x & 63)];
+  }
+};
+
+template <int DT, typename Rows>
+__global__ __launch_bounds__(kSlicesMax * 64) void mx4_few_kernel(Mx4Product p, typename Rows::Args xs, FewShape shape) {
+  constexpr int NT = Rows::kTiles;
+  __shared__ __align__(16) uint8_t lds[kFewLds];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int slice = wave & (shape.slices - 1);
+  const int panel = (int)blockIdx.x * (shape.waves / shape.slices) + wave / shape.slices;
+  const int kp = p.w.col_panels();
+  const int tile = (int)blockIdx.y * NT;
+  f32x4 acc[4][NT] = {};
+  struct Step {
+    u32x4 w[4];
+    uint32_t sw;
+    typename Rows::Raw x;
+  };
+  // A wave past the last panel has nothing to do but to meet the others.
+  const bool works = panel * kMxPanelRows < p.w.rows;
+  const Rows rows(xs, lds, tile, lane);
+  const uint8_t *wc = p.w.codes + (int64_t)panel * kp * kMxPanelBytes + lane * 16;
+  const uint8_t *ws = p.w.scales + (int64_t)panel * kp * kMxPanelScales + lane * 4;
+  int k = (int)((int64_t)kp * slice / shape.slices);
+  const int end = works ? (int)((int64_t)kp * (slice + 1) / shape.slices) : k;
+  auto load = [&](int at, Step &s) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s.w[t] = *reinterpret_cast<const u32x4 *>(wc + (int64_t)at * kMxPanelBytes + t * kMxTileBytes);
+    s.sw = *reinterpret_cast<const uint32_t *>(ws + (int64_t)at * kMxPanelScales);
+    rows.load(at, s.x);
+  };
+  auto multiply = [&](int at, const Step &s) {
+    u32x4 x[NT];
+    const uint32_t sx = rows.tiles(s.x, at, x);
+    unrolled<4>([&](auto t) {
+      unrolled<NT>([&](auto u) {
+        constexpr int T = decltype(t)::value, U = decltype(u)::value;
+        acc[T][U] = mx4_mfma<T, U>(s.w[T], x[U], acc[T][U], s.sw, sx);
+      });
+    });
+  };
+  Step now, next;
+  if (k < end) load(k, now);
+  if constexpr (!std::is_same<typename Rows::Args, Mx4Matrix>::value) {
+    Rows::fill(xs, lds, kp);
+    __syncthreads();
+  }
+  if (k < end) {
+    for (; k + 1 < end; ++k) {
+      load(k + 1, next);
+      multiply(k, now);
+      now = next;
+    }
+    multiply(k, now);
+  }
+  // The slices in halves: the upper half's sums go through LDS to the lower half's waves.
+  if constexpr (!std::is_same<typename Rows::Args, Mx4Matrix>::value) {
+    if (shape.slices > 1) __syncthreads();
+  }
+  f32x4 *const sums = reinterpret_cast<f32x4 *>(lds) + lane;
+  for (int half = shape.slices / 2; half > 0; half /= 2) {
+    const int at = (wave / shape.slices * half + (slice & (half - 1))) * NT * 4;
+    if (slice >= half && slice < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) sums[(at + i) * 64] = acc[i / NT][i % NT];
+    }
+    __syncthreads();
+    if (slice < half) {
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) acc[i / NT][i % NT] += sums[(at + i) * 64];
+    }
+    __syncthreads();
+  }
+  if (!works || slice != 0) return;
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+    store_panel<DT>(p, (tile + u) * kMxTileRows + (lane & 15), panel * kMxPanelRows, acc[0][u], acc[1][u], acc[2][u], acc[3][u]);
 }
 
+constexpr int kCus = 256;             // an MI355X's compute units
 constexpr int64_t kTilesMax = 1 << 22;  // of a launch: 2^32 threads are too many
+
+// Whether W is streamed into registers: up to 64 rows, which one wave takes, and where tiles of 128 x 128
+// would leave half the units idle (128 x 4864, k = 4096: 10.9 us in tiles, 8.6 so; 100 x 50257, k = 800, with
+// 393 tiles: 14.4 and 18.4).
+bool few_rows(int n, int rows) {
+  return rows <= kMxPanelRows || mx_panels(n, 128) * mx_panels(rows, 128) <= kCus / 2;
+}
 
 template <int DT, int PM, int PN, int WM, int WN>
 int launch_tiles(const Mx4Product &p, hipStream_t s) {
@@ -339,9 +477,6 @@ int launch_tiles(const Mx4Product &p, hipStream_t s) {
   return TABBY_OK;
 }
 
-constexpr int kTileRowsMin = 64;  // rows of X from which a tile pays
-constexpr int kCus = 256;         // an MI355X's compute units
-
 // Whether tiles of 256 x 256 are the better choice, else 128 x 128. A unit holds one of the large tiles,
 // and they do the same work in 3.5/4 of the time (4096 x 16384, k = 8192: 243 us and 270), but a last
 // round of them that few units take part in costs as much as a full one: 318 x 44368, k = 6704: 86 us
@@ -351,14 +486,35 @@ bool large_tiles(int n, int rows) {
   return 7 * mx_panels(large, kCus) <= 2 * mx_panels(small, kCus);
 }
 
-template <int DT>
-int launch_product(const Mx4Product &p, hipStream_t s) {
-  if (p.x.rows >= kTileRowsMin) return large_tiles(p.w.rows, p.x.rows) ? launch_tiles<DT, 2, 1, 2, 4>(p, s) : launch_tiles<DT, 1, 1, 2, 2>(p, s);
-  const int64_t tiles = mx_panels(p.x.rows, kMxTileRows);
-  hipLaunchKernelGGL(mx4_panel_kernel<DT>, dim3((unsigned)mx_panels(p.w.rows, kMxPanelRows), (unsigned)std::min<int64_t>(tiles, 65535)),
-                     dim3(64), 0, s, p);
+// The slices of k: enough waves to fill the chip, eight to a unit, while every one has a panel of k.
+FewShape few_shape(int64_t panels, int kp, int tiles, bool fills) {
+  int slices = 1;
+  while (slices < kSlicesMax && slices * 2 <= kp && slices * 2 * tiles <= kSumsMax && panels * slices < 8 * kCus) slices *= 2;
+  return {fills ? kSlicesMax : std::max(slices, 4), slices};
+}
+
+template <int DT, typename Rows>
+int launch_few(const Mx4Product &p, const typename Rows::Args &xs, hipStream_t s) {
+  constexpr int NT = Rows::kTiles;
+  const int64_t panels = mx_panels(p.w.rows, kMxPanelRows), groups = mx_panels(p.x.rows, kMxTileRows * NT);
+  const FewShape shape = few_shape(panels * groups, p.w.col_panels(), NT, !std::is_same<typename Rows::Args, Mx4Matrix>::value);
+  const int64_t blocks = mx_panels(panels, shape.waves / shape.slices);
+  hipLaunchKernelGGL((mx4_few_kernel<DT, Rows>), dim3((unsigned)blocks, (unsigned)groups), dim3(64 * shape.waves), 0, s, p, xs, shape);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
+}
+
+// X as it is held.
+template <int DT>
+int launch_product(const Mx4Product &p, hipStream_t s) {
+  if (!few_rows(p.w.rows, p.x.rows)) return large_tiles(p.w.rows, p.x.rows) ? launch_tiles<DT, 2, 1, 2, 4>(p, s) : launch_tiles<DT, 1, 1, 2, 2>(p, s);
+  const Mx4Matrix &xs = p.x;
+  switch (mx_panels(p.x.rows, kMxTileRows)) {
+    case 1: return launch_few<DT, HeldTiles<1>>(p, xs, s);
+    case 2: return launch_few<DT, HeldTiles<2>>(p, xs, s);
+    case 3: return launch_few<DT, HeldTiles<3>>(p, xs, s);
+    default: return launch_few<DT, HeldTiles<4>>(p, xs, s);
+  }
 }
 
 int product(const Mx4Product &p, int32_t out_dtype, hipStream_t s) {
@@ -366,6 +522,24 @@ int product(const Mx4Product &p, int32_t out_dtype, hipStream_t s) {
     case TABBY_F32: return launch_product<TABBY_F32>(p, s);
     case TABBY_F16: return launch_product<TABBY_F16>(p, s);
     default: return launch_product<TABBY_BF16>(p, s);
+  }
+}
+
+// X quantised in the product's own launch.
+template <int DT>
+int launch_linear(const Mx4Product &p, const FloatRows &x, int x_dtype, hipStream_t s) {
+  switch (x_dtype) {
+    case TABBY_F32: return launch_few<DT, FloatTiles<TABBY_F32>>(p, x, s);
+    case TABBY_F16: return launch_few<DT, FloatTiles<TABBY_F16>>(p, x, s);
+    default: return launch_few<DT, FloatTiles<TABBY_BF16>>(p, x, s);
+  }
+}
+
+int linear(const Mx4Product &p, const FloatRows &x, int x_dtype, int32_t out_dtype, hipStream_t s) {
+  switch (out_dtype) {
+    case TABBY_F32: return launch_linear<TABBY_F32>(p, x, x_dtype, s);
+    case TABBY_F16: return launch_linear<TABBY_F16>(p, x, x_dtype, s);
+    default: return launch_linear<TABBY_BF16>(p, x, x_dtype, s);
   }
 }
 
@@ -417,9 +591,13 @@ extern "C" int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64
   if ((uintptr_t)workspace_dev % 16 != 0 || workspace_bytes < code_bytes + scale_bytes)
     return record_failure(TABBY_EINVAL, "workspace must be 16-byte aligned and hold the quantised x (tabby_mx4_bytes)");
   uint8_t *codes = (uint8_t *)workspace_dev, *scales = codes + code_bytes;
-  rc = mx4_quantize(x_dev, x_dtype, rows, k, x_stride, codes, scales, (hipStream_t)stream);
-  if (rc) return rc;
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
                      {codes, scales, rows, k}, bias_dev, out_dev, out_stride};
+  if (rows <= kMxTileRows && p.w.col_panels() <= kFloatPanels) {
+    const bool wide = (uintptr_t)x_dev % 16 == 0 && (rows == 1 || x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0);
+    return linear(p, FloatRows{x_dev, x_stride, rows, k, wide}, x_dtype, out_dtype, (hipStream_t)stream);
+  }
+  rc = mx4_quantize(x_dev, x_dtype, rows, k, x_stride, codes, scales, (hipStream_t)stream);
+  if (rc) return rc;
   return product(p, out_dtype, (hipStream_t)stream);
 }

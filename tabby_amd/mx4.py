@@ -15,61 +15,80 @@ import contextlib
 import ctypes
 from typing import Optional
 
+import torch
+
 from .sampler import TABBY_BF16, TABBY_F16, TABBY_F32, _check, load_library
 
 BLOCK = 32  # values to a scale
+PANEL_ROWS, PANEL_COLS = 64, 128  # a panel's codes take 4,096 bytes, its scales 256
+
+_CODES = {torch.float32: TABBY_F32, torch.float16: TABBY_F16, torch.bfloat16: TABBY_BF16}
 
 
 def dtype_code(dtype) -> int:
-    import torch
-    codes = {torch.float32: TABBY_F32, torch.float16: TABBY_F16, torch.bfloat16: TABBY_BF16}
-    if dtype not in codes:
+    code = _CODES.get(dtype)
+    if code is None:
         raise TypeError(f"expected float32, float16 or bfloat16, got {dtype}")
-    return codes[dtype]
+    return code
 
 
 def rows_of(x, what: str):
     """A CUDA tensor as rows: 1-D becomes one row; a row's elements must be adjacent."""
     if not x.is_cuda:
         raise ValueError(f"{what} must be a device (cuda) tensor")
-    if x.dim() not in (1, 2):
-        raise ValueError(f"{what} must have one or two dimensions, got {x.dim()}")
-    x = x if x.dim() == 2 else x.unsqueeze(0)
-    if x.shape[0] < 1 or x.shape[1] < 1:
+    if x.dim() != 2:
+        if x.dim() != 1:
+            raise ValueError(f"{what} must have one or two dimensions, got {x.dim()}")
+        x = x.unsqueeze(0)
+    rows, cols = x.shape
+    if rows < 1 or cols < 1:
         raise ValueError(f"{what} must not be empty, got {tuple(x.shape)}")
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+    row_stride, stride = x.stride()
+    if (cols > 1 and stride != 1) or (rows > 1 and row_stride < cols):
         raise ValueError(f"{what} must hold its rows' elements adjacent and its rows apart")
     return x
 
 
 def on_device(device, *tensors):
     for t in tensors:
-        if t is not None and t.device != device:
+        if t.device != device:
             raise ValueError(f"tensors lie on {device} and on {t.device}")
+
+
+_HERE = contextlib.nullcontext()
 
 
 @contextlib.contextmanager
 def _guard(device, stream):
-    import torch
     with torch.cuda.device(device), torch.cuda.stream(stream):
         yield
+
+
+def _current_handle(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The current stream's handle without the object around it, which takes longer to make than a launch.
+_current_handle = getattr(torch._C, "_cuda_getCurrentRawStream", _current_handle)
 
 
 def call_on(device, stream):
     """(context, stream handle) of a call on ``device``: the device is made current where it is
     not, and what the call allocates belongs to its stream."""
-    import torch
     if stream is None:
         if device.index == torch.cuda.current_device():
-            return contextlib.nullcontext(), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+            return _HERE, _current_handle(device.index)
         stream = torch.cuda.current_stream(device)
     elif stream.device != device:
         raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
-    return _guard(device, stream), ctypes.c_void_p(stream.cuda_stream)
+    return _guard(device, stream), stream.cuda_stream
 
 
 def sizes(rows: int, cols: int):
     """Bytes of a matrix's codes and scales."""
+    if rows < 2 ** 20 and cols < 2 ** 20 and rows > 0 and cols > 0:
+        panels = -(-rows // PANEL_ROWS) * -(-cols // PANEL_COLS)
+        return panels * 4096, panels * 256
     code, scale = ctypes.c_int64(), ctypes.c_int64()
     _check(load_library().tabby_mx4_bytes(rows, cols, ctypes.byref(code), ctypes.byref(scale)))
     return code.value, scale.value
@@ -80,11 +99,21 @@ class Mx4Matrix:
     be written again with ``quantize(x, out=matrix)``."""
 
     def __init__(self, rows: int, cols: int, device="cuda"):
-        import torch
-        code, scale = sizes(rows, cols)
         self.rows, self.cols = int(rows), int(cols)
-        self.codes = torch.empty(code, dtype=torch.uint8, device=device)
-        self.scales = torch.empty(scale, dtype=torch.uint8, device=device)
+        self._code_bytes, scale = sizes(self.rows, self.cols)
+        self.data = torch.empty(self._code_bytes + scale, dtype=torch.uint8, device=device)  # codes, then scales
+
+    @property
+    def codes(self):
+        return self.data[:self._code_bytes]
+
+    @property
+    def scales(self):
+        return self.data[self._code_bytes:]
+
+    def _addresses(self):
+        at = self.data.data_ptr()
+        return at, at + self._code_bytes
 
     @classmethod
     def quantize(cls, x, out: Optional["Mx4Matrix"] = None, stream=None) -> "Mx4Matrix":
@@ -93,15 +122,15 @@ class Mx4Matrix:
         most 6); a block with a NaN or an infinity becomes NaN."""
         x = rows_of(x, "x")
         code = dtype_code(x.dtype)
-        rows, cols = int(x.shape[0]), int(x.shape[1])
+        rows, cols = x.shape
         ctx, handle = call_on(x.device, stream)
         with ctx:
             m = cls(rows, cols, x.device) if out is None else out
             if (m.rows, m.cols) != (rows, cols):
                 raise ValueError(f"out is {m.rows} x {m.cols}, x is {rows} x {cols}")
-            on_device(x.device, m.codes)
+            on_device(x.device, m.data)
             _check(load_library().tabby_mx4_quantize_device(
-                x.data_ptr(), code, rows, cols, x.stride(0), m.codes.data_ptr(), m.scales.data_ptr(), handle))
+                x.data_ptr(), code, rows, cols, x.stride(0), *m._addresses(), handle))
         return m
 
     @classmethod
@@ -109,7 +138,6 @@ class Mx4Matrix:
         """A checkpoint's layout, repacked once: ``codes`` uint8 [rows, ceil(cols / 32) * 16], two to a
         byte with the lower column in the low half, ``scales`` uint8 [rows, ceil(cols / 32)], the
         biased exponents."""
-        import torch
         blocks = -(-int(cols) // BLOCK)
         if not codes.is_cuda or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise ValueError("codes and scales must be uint8 device (cuda) tensors")
@@ -124,13 +152,12 @@ class Mx4Matrix:
         with ctx:
             m = cls(int(codes.shape[0]), int(cols), codes.device)
             _check(load_library().tabby_mx4_pack_device(
-                codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, m.codes.data_ptr(), m.scales.data_ptr(), handle))
+                codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, *m._addresses(), handle))
         return m
 
     def dequantize(self, dtype=None, out=None, stream=None):
         """The values that the codes stand for, [rows, cols]: exact in float32 (the default) and
         bfloat16, rounded once in float16."""
-        import torch
         if out is None:
             code = dtype_code(dtype or torch.float32)
         else:
@@ -140,13 +167,13 @@ class Mx4Matrix:
             out = rows_of(out, "out")
             if tuple(out.shape) != (self.rows, self.cols):
                 raise ValueError(f"out must have shape ({self.rows}, {self.cols}), got {tuple(out.shape)}")
-            on_device(self.codes.device, out)
-        ctx, handle = call_on(self.codes.device, stream)
+            on_device(self.data.device, out)
+        ctx, handle = call_on(self.data.device, stream)
         with ctx:
             if out is None:
-                out = torch.empty((self.rows, self.cols), dtype=dtype or torch.float32, device=self.codes.device)
+                out = torch.empty((self.rows, self.cols), dtype=dtype or torch.float32, device=self.data.device)
             _check(load_library().tabby_mx4_dequantize_device(
-                self.codes.data_ptr(), self.scales.data_ptr(), self.rows, self.cols, out.data_ptr(), code,
+                *self._addresses(), self.rows, self.cols, out.data_ptr(), code,
                 out.stride(0), handle))
         return out
 
@@ -155,16 +182,15 @@ def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
     """x W^T (+ bias), [rows, w.rows] of ``dtype`` (float32 by default): ``x`` is an ``Mx4Matrix``
     or a float tensor ([rows, k] or [k]), which is quantised in the call. Products of codes are
     exact, their sums float32, rounded once to ``dtype``."""
-    import torch
-    device = w.codes.device
+    device = w.data.device
     quantized = isinstance(x, Mx4Matrix)
     if not quantized:
         x = rows_of(x, "x")
         x_code = dtype_code(x.dtype)
         on_device(device, x)
     else:
-        on_device(device, x.codes)
-    rows, k = (x.rows, x.cols) if quantized else (int(x.shape[0]), int(x.shape[1]))
+        on_device(device, x.data)
+    rows, k = (x.rows, x.cols) if quantized else x.shape
     if k != w.cols:
         raise ValueError(f"x has {k} columns, the weights {w.cols}")
     if bias is not None:
@@ -190,12 +216,12 @@ def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
             out = torch.empty((rows, w.rows), dtype=dtype, device=device)
         if quantized:
             _check(lib.tabby_mx4_matmul_device(
-                x.codes.data_ptr(), x.scales.data_ptr(), rows, w.codes.data_ptr(), w.scales.data_ptr(), bias_ptr,
+                *x._addresses(), rows, *w._addresses(), bias_ptr,
                 w.rows, k, out.data_ptr(), code, out.stride(0), handle))
         else:
             space = torch.empty(sum(sizes(rows, k)), dtype=torch.uint8, device=device)
             _check(lib.tabby_mx4_linear_device(
-                x.data_ptr(), x_code, x.stride(0), rows, w.codes.data_ptr(), w.scales.data_ptr(), bias_ptr,
+                x.data_ptr(), x_code, x.stride(0), rows, *w._addresses(), bias_ptr,
                 w.rows, k, out.data_ptr(), code, out.stride(0), space.data_ptr(), space.numel(), handle))
     return out
 
