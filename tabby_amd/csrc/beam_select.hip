@@ -33,10 +33,9 @@ constexpr int kVocabMax = 1 << 28;            // a part's bytes fit a buffer res
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
+constexpr int kKeyLow = 12;                   // a bound in the row need not be finer than 2^-11 of it
 constexpr int kListMax = 2048;                // entries above the bound that LDS holds
-constexpr int kMergeWaves = 16;
-constexpr int kMergeBlock = kMergeWaves * 64;
-static_assert(kBeamsMax * kCountMax <= kEntriesMax && kBeamsMax * kPartsMax <= kMergeBlock, "a group's entries and sums");
+static_assert(kBeamsMax * kCountMax <= kEntriesMax && kBeamsMax * kPartsMax <= 1024, "a group's entries and sums");
 
 // What the first kernel leaves of a row's part, beside its entries.
 struct RowSum {
@@ -68,14 +67,15 @@ __device__ __forceinline__ bool beam_reads(const BeamArgs &a, int row) {
   return a.scores[row] > -INFINITY && !(a.done && a.done[row]);
 }
 
-// 2^t in 64 bits for t in [-1000, 1000]: the nearest whole power by adding and taking away 1.5 * 2^52,
-// whose low word then holds it, and for the rest f in [-1/2, 1/2] the polynomial of degree 7 through
-// 2^f at the Chebyshev nodes, within 5e-11 of it. A sum of such terms decides the order of two
-// beams' continuations only where their scores are that close.
-__device__ __forceinline__ double exp2_64(double t) {
+// exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
+// and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]; for 2^f the
+// polynomial of degree 7 through it at the Chebyshev nodes, within 5e-11 of it. A sum of such terms
+// decides the order of two beams' continuations only where their scores are that close.
+__device__ __forceinline__ double exp_64(double d) {
+  constexpr double kLog2e = 1.4426950408889634;
   const double magic = 6755399441055744.0;
-  const double shifted = t + magic;
-  const double f = t - (shifted - magic);
+  const double shifted = __builtin_fma(d, kLog2e, magic);
+  const double f = __builtin_fma(d, kLog2e, -(shifted - magic));
   double p = 1.530370102315244e-05;
   p = __builtin_fma(p, f, 0.0001546972921563772);
   p = __builtin_fma(p, f, 0.0013333478472326247);
@@ -88,8 +88,8 @@ __device__ __forceinline__ double exp2_64(double t) {
   const uint64_t bits = (uint64_t)__double_as_longlong(p);
   return __longlong_as_double((long long)(((uint64_t)((uint32_t)(bits >> 32) + (n << 20)) << 32) | (uint32_t)bits));
 }
-
-constexpr double kLog2e = 1.4426950408889634;
+// The same for any d <= 690: below -690 nothing is left that a sum of at least 1 would hold.
+__device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, -690.0)); }
 
 // The larger of two, NaN if either is: a chunk's maximum shows that it holds a NaN.
 __device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -176,6 +176,65 @@ struct PartReader {
   }
 };
 
+// The k-th largest of the wave's 64 R values, its bits below LOW taken as zero: bit by bit from the top, the
+// largest value that k of them reach. 0 where there are fewer that are not.
+template <int LOW, int R>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[R], int k) {
+  uint32_t found = 0;
+#pragma unroll 4
+  for (int bit = 31; bit >= LOW; --bit) {
+    const uint32_t next = found | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) n += (int)__popcll(__ballot(v[r] >= next));
+    if (n >= k) found = next;
+  }
+  return found;
+}
+
+// The number of set lanes before this one.
+__device__ __forceinline__ uint32_t lanes_before(uint64_t who) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+}
+
+// A lower bound of the count-th largest of the keys that the workgroup's lanes hold, one each, from the
+// largest few of every wave. `offers` holds 256 words; the call meets the workgroup once.
+template <int LOW, int NW>
+__device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, uint32_t *offers) {
+  const int lane = wave_lane();
+  const int rows = count <= 16 ? 1 : count <= 64 ? 2 : 4;  // 64 offers each
+  const int each = 64 * rows / NW;
+  uint32_t *mine = offers + ((int)threadIdx.x >> 6) * each;
+  const bool in = key >= kth_largest<LOW>({key}, each);
+  const uint64_t who = __ballot(in);
+  const int at = (int)lanes_before(who);
+  if (in && at < each) mine[at] = key;
+  if (lane >= __popcll(who) && lane < each) mine[lane] = 0;
+  __syncthreads();
+  if (rows == 1) return kth_largest<LOW>({offers[lane]}, count);
+  if (rows == 2) return kth_largest<LOW>({offers[lane], offers[64 + lane]}, count);
+  return kth_largest<LOW>({offers[lane], offers[64 + lane], offers[128 + lane], offers[192 + lane]}, count);
+}
+
+// How many of the n things come before thing c, counted by `share` neighbouring lanes (a power of two up to
+// 64), every one of which returns it.
+template <class Before>
+__device__ __forceinline__ uint32_t rank_of(int share, uint32_t n, Before before) {
+  uint32_t rank = 0;
+#pragma unroll 4
+  for (uint32_t j = threadIdx.x & (share - 1); j < n; j += share) rank += before(j) ? 1u : 0u;
+#pragma unroll
+  for (int stride = 1; stride < 64; stride *= 2)
+    if (stride < share) rank += xor_lane_by(rank, stride);
+  return rank;
+}
+// The lanes to a thing where `lanes` of them rank n.
+__device__ __forceinline__ int share_of(int lanes, uint32_t n) {
+  int share = 1;
+  while (share < 64 && n * share * 2 <= (uint32_t)lanes) share *= 2;
+  return share;
+}
+
 // One workgroup of NW waves to a part of a row. HBM-bound: every element is read once.
 template <int DT, bool MASK, int NW>
 __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
@@ -183,30 +242,32 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   constexpr int kBlockN = NW * 64;
   __shared__ BlockScratchT<NW> scratch;
   __shared__ uint32_t hist[kBins];
-  __shared__ uint64_t list[kListMax];
-  __shared__ uint32_t first[NW * 64];  // the waves' largest lane maxima of their first chunks
+  __shared__ uint64_t list[kListMax];  // 0 where nothing is written yet
+  __shared__ uint32_t offers[256];
   __shared__ uint32_t listed, bad, bound;
   __shared__ double wave_sum_[NW];
   __shared__ float wave_ref[NW], wave_max_[NW];
   const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - row * a.parts;
   const int t = (int)threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int begin = part * a.part_len, len = min(a.part_len, a.vocab - begin);
+  const Reader reader(a, row, begin, len);
+  typename Reader::Raw raw, next;
+  float x[kLane];
+  int c = wave;
+  reader.load(c, raw);
+  reader.load(c + NW, next);
+  asm volatile("" ::: "memory");  // on their way before the row's state is asked for
   if (!beam_reads(a, row)) {
     if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, 0, 0};
     return;
   }
-  const int begin = part * a.part_len, len = min(a.part_len, a.vocab - begin);
-  const Reader reader(a, row, begin, len);
+  for (int i = t; i < kListMax; i += kBlockN) list[i] = 0;
   if (t == 0) {
     listed = 0;
     bad = 0;
     bound = kNegInfKey + 1;
   }
-
-  typename Reader::Raw raw;
-  float x[kLane];
-  int c = wave;
-  reader.load(c, raw);
   auto chunk_max = [&]() {
     float m = x[0];
 #pragma unroll
@@ -222,33 +283,8 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     for (int i = 0; i < kLane; ++i) x[i] = -INFINITY;
     top = -INFINITY;
   }
-  // The first bound: each wave offers the largest of its lanes' maxima, 64 R of them in all, and the
-  // count-th largest of those has `count` elements of the part at or above it.
-  const int wide = a.count > 64 ? 4 : 2;
-  const int offered = 64 * wide / NW;
-  {
-    uint32_t key[1] = {top == top ? key_of(top) : 0u};
-    wave_sort_desc<1>(key);
-    if (lane < offered) first[wave * offered + lane] = key[0];
-  }
-  __syncthreads();
-  uint32_t theta;
-  {
-    uint32_t k;
-    if (a.count > 64) {
-      uint32_t v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = first[r * 64 + lane];
-      wave_sort_desc<4>(v);
-      k = a.count > 64 ? v[1] : v[0];
-      k = (uint32_t)__builtin_amdgcn_readlane((int)k, (a.count - 1) & 63);
-    } else {
-      uint32_t v[2] = {first[lane], first[64 + lane]};
-      wave_sort_desc<2>(v);
-      k = (uint32_t)__builtin_amdgcn_readlane((int)v[0], a.count - 1);
-    }
-    theta = max(k, kNegInfKey + 1);
-  }
+  // The first bound, from the lanes' largest of the first chunks.
+  uint32_t theta = max(bound_of<kKeyLow, NW>(top == top ? key_of(top) : 0u, a.count, offers), kNegInfKey + 1);
 
   double sum = 0.0;
   float ref = 0.0f, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
@@ -256,34 +292,44 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     // Elements at or above the bound join the list; a NaN is neither.
     float least = value_of(theta);
     if (__ballot(!(top < least))) {
-      const uint32_t shared = *(volatile uint32_t *)&bound;
-      if (shared > theta) theta = shared;
+      theta = max(theta, *(volatile uint32_t *)&bound);
       if (__ballot(!(top < value_of(theta)))) {
         if (!(top < INFINITY)) bad = 1;
         if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count) {
           // Many lanes have one: the count-th largest of the lanes' maxima is a better bound.
-          uint32_t key[1] = {top == top ? key_of(top) : 0u};
-          wave_sort_desc<1>(key);
-          const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key[0], a.count - 1);
+          const uint32_t k = kth_largest<kKeyLow>({top == top ? key_of(top) : 0u}, a.count);
           if (k > theta) {
             theta = k;
             if (lane == 0) atomicMax(&bound, k);
           }
         }
         least = value_of(theta);
-        uint32_t mine = 0;
+        uint32_t found = 0;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) mine += x[i] >= least ? 1u : 0u;
-        const uint32_t upto = wave_inclusive_scan_u32(mine);
+        for (int i = 0; i < kLane; ++i) found += (uint32_t)__popcll(__ballot(x[i] >= least));
         uint32_t at = 0;
-        if (lane == 63) at = atomicAdd(&listed, upto);
-        at = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + upto - mine;
+        if (lane == 0) at = atomicAdd(&listed, found);
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+        const uint32_t from = at;
 #pragma unroll
         for (int i = 0; i < kLane; ++i) {
-          if (x[i] >= least) {
-            if (at < kListMax) list[at] = composite(key_of(x[i]), (uint32_t)reader.element(c, i));
-            ++at;
+          const uint64_t who = __ballot(x[i] >= least);
+          if (who) {
+            const uint32_t to = at + lanes_before(who);
+            if (x[i] >= least && to < kListMax) list[to] = composite(key_of(x[i]), (uint32_t)reader.element(c, i));
+            at += (uint32_t)__popcll(who);
           }
+        }
+        // Every 64 (or 256) entries the count-th largest of the last so many is a new bound.
+        const uint32_t span = a.count <= 32 ? 64 : 256;
+        if (from / span != at / span && at <= kListMax) {
+          wave_lds_sync();
+          const volatile uint32_t *high = reinterpret_cast<const volatile uint32_t *>(list + (at / span - 1) * span) + 1;
+          const uint32_t k = span == 64 ? kth_largest<kKeyLow>({high[lane * 2]}, a.count)
+                                        : kth_largest<kKeyLow>({high[lane * 2], high[128 + lane * 2], high[256 + lane * 2],
+                                                                high[384 + lane * 2]}, a.count);
+          theta = max(theta, k);
+          if (lane == 0) atomicMax(&bound, k);
         }
       }
     }
@@ -291,7 +337,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       // The first chunk with an element, or one far above: another reference.
       const float m = wave_max(top);
       if (m < INFINITY) {
-        sum *= exp2_64(fmax(((double)ref - (double)m) * kLog2e, -1000.0));
+        sum *= exp_or_none((double)ref - (double)m);
         ref = m;
         rise = m + 600.0f;
       }
@@ -301,13 +347,11 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       const double at = (double)ref;
       double part_sum[2] = {0.0, 0.0};
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) part_sum[i & 1] += exp2_64(fmax(((double)x[i] - at) * kLog2e, -1000.0));
+      for (int i = 0; i < kLane; ++i) part_sum[i & 1] += exp_or_none((double)x[i] - at);
       sum += part_sum[0] + part_sum[1];
     }
   };
-  typename Reader::Raw next;
   if (c < reader.chunks) {
-    reader.load(c + NW, next);
     take();
     for (c += NW; c < reader.chunks; c += NW) {
       raw = next;
@@ -332,25 +376,23 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   }
   const uint32_t need = min(n, (uint32_t)a.count);
   uint64_t *out = a.entries + (int64_t)blockIdx.x * a.count;
-  if (t == 0) {
-    float m = wave_max_[0];
-    for (int w = 1; w < NW; ++w) m = fmaxf(m, wave_max_[w]);
-    double s = 0.0;
-    for (int w = 0; w < NW; ++w)
-      if (wave_sum_[w] > 0.0) s += wave_sum_[w] * exp((double)wave_ref[w] - (double)m);
-    a.sums[blockIdx.x] = RowSum{s, m, (int)need, 0, 0};
+  if (wave == 0) {
+    const float m = wave_max(lane < NW ? wave_max_[lane] : -INFINITY);
+    double term = lane < NW ? wave_sum_[lane] : 0.0;
+    if (term > 0.0) term *= exp_or_none((double)wave_ref[lane] - (double)m);
+    term = wave_sum(term);
+    if (t == 0) a.sums[blockIdx.x] = RowSum{term, m, (int)need, 0, 0};
   }
   if (n <= (uint32_t)a.count) {
     for (uint32_t i = t; i < n; i += kBlockN) out[i] = list[i];
     return;
   }
   if (n <= (uint32_t)kBlockN) {
-    if (t < (int)n) {
-      const uint64_t v = list[t];
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; ++j) rank += list[j] > v ? 1u : 0u;
-      if (rank < need) out[rank] = v;
-    }
+    const int share = share_of(kBlockN, n);
+    const uint32_t i = (uint32_t)t / share;
+    const uint64_t v = i < n ? list[i] : 0;
+    const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return list[j] > v; });
+    if (i < n && rank < need) out[rank] = v;
     return;
   }
   auto pick = [&](auto for_each) {
@@ -388,93 +430,120 @@ __device__ __forceinline__ double score_of(uint64_t k) {
   return __longlong_as_double((long long)(k ^ (~(uint64_t)((int64_t)k >> 63) | 0x8000000000000000ull)));
 }
 
-// One workgroup to a group: its beams' entries become scores, and the best `count` are ranked by
-// counting, for each, those that come before it. Bound by the latency of its few steps.
-__global__ __launch_bounds__(kMergeBlock) void beam_merge_kernel(BeamArgs a) {
-  __shared__ BlockScratchT<kMergeWaves> scratch;
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint64_t keys[kEntriesMax];  // scores
-  __shared__ uint64_t tags[kEntriesMax];  // beam << 32 | token: the order of equal scores
-  __shared__ double space[kEntriesMax / 4];
-  double *const part_sum = space;  // the parts' sums, maxima and counts
-  float *const part_max = (float *)(space + kBeamsMax * kPartsMax);
-  int32_t *const part_count = (int32_t *)(part_max + kBeamsMax * kPartsMax);
-  uint16_t *const kept = (uint16_t *)space;  // once those are used up: the entries that are ranked
+// One workgroup of NW waves to a group of at most NW * 512 entries: its beams' entries become scores, those
+// that may be among the best `count` go to LDS, and there each is ranked by counting those that come
+// before it. Bound by the latency of its few steps.
+constexpr int kMergeEach = 8;  // entries to a lane
+
+template <int NW>
+__global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a) {
+  constexpr int kBlockN = NW * 64;
+  constexpr int kHeld = kBlockN * kMergeEach;
+  __shared__ uint64_t keys[kHeld];  // scores
+  __shared__ uint64_t tags[kHeld];  // beam << 32 | token: the order of equal scores
+  __shared__ double part_term[kBlockN];
+  __shared__ float part_max[kBlockN];
+  __shared__ int32_t part_count[kBlockN];
   __shared__ double base[kBeamsMax], norm[kBeamsMax];
-  __shared__ uint32_t total, left, bad;
-  const int g = (int)blockIdx.x, t = (int)threadIdx.x;
+  __shared__ uint32_t offers[256];
+  __shared__ uint32_t held, bad;
+  const int g = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
   const int row0 = g * a.beams;
-  const int lists = a.beams * a.parts;
-  if (t == 0) total = left = bad = 0;
-  __syncthreads();
+  const int lists = a.beams * a.parts;  // up to kBlockN
+  const int slots = lists * a.count;
+  uint64_t entry[kMergeEach];
+#pragma unroll
+  for (int j = 0; j < kMergeEach; ++j) {
+    const int i = j * kBlockN + t;
+    entry[j] = i < slots ? a.entries[(int64_t)row0 * a.parts * a.count + i] : 0;
+  }
+  RowSum rs{0.0, -INFINITY, 0, 0, 0};
+  if (t < lists) rs = a.sums[(int64_t)row0 * a.parts + t];
+  float score = 0.0f;
+  int ended = 0;
+  if (t < a.beams) {
+    score = a.scores[row0 + t];
+    ended = a.done ? a.done[row0 + t] : 0;
+  }
+  if (t == 0) held = bad = 0;
   if (t < lists) {
-    const RowSum rs = a.sums[(int64_t)row0 * a.parts + t];
-    part_sum[t] = rs.sum;
     part_max[t] = rs.max;
     part_count[t] = rs.count;
-    if (rs.bad) bad = 1;
   }
   __syncthreads();
-  if (t < a.beams) {
-    const int row = row0 + t;
-    const float s = a.scores[row];
-    if (!(s < INFINITY)) bad = 1;
+  if (rs.bad || !(score < INFINITY)) bad = 1;
+  if (t < lists) {
+    const int first = t / a.parts * a.parts;
     float m = -INFINITY;
-    for (int p = 0; p < a.parts; ++p) m = fmaxf(m, part_max[t * a.parts + p]);
+    for (int p = 0; p < a.parts; ++p) m = fmaxf(m, part_max[first + p]);
+    part_term[t] = rs.count > 0 ? rs.sum * exp_or_none((double)rs.max - (double)m) : 0.0;
+  }
+  __syncthreads();
+  const bool stays = t < a.beams && ended && score > -INFINITY;  // as it is: one continuation
+  if (t < a.beams) {
+    float m = -INFINITY;
     double sum = 0.0;
-    for (int p = 0; p < a.parts; ++p)
-      if (part_count[t * a.parts + p] > 0) sum += part_sum[t * a.parts + p] * exp((double)part_max[t * a.parts + p] - (double)m);
-    base[t] = (double)s;
+    for (int p = 0; p < a.parts; ++p) {
+      m = fmaxf(m, part_max[t * a.parts + p]);
+      sum += part_term[t * a.parts + p];
+    }
+    base[t] = (double)score;
     norm[t] = m > -INFINITY ? (double)m + log(sum) : 0.0;
-    if (a.done && a.done[row] && s > -INFINITY) {
-      const uint32_t at = atomicAdd(&total, 1u);
-      keys[at] = score_key((double)s);
-      tags[at] = ((uint64_t)t << 32) | (uint32_t)a.pad_id;
+  }
+  __syncthreads();
+  // Scores; 0 is below every one.
+  auto beam_of = [&](int i) { return i / a.count / a.parts; };
+  uint64_t key[kMergeEach];
+  uint64_t best = stays ? score_key((double)score) : 0;
+#pragma unroll
+  for (int j = 0; j < kMergeEach; ++j) {
+    const int i = j * kBlockN + t;
+    key[j] = 0;
+    if (i < slots) {
+      const int l = i / a.count, b = beam_of(i);
+      if (i - l * a.count < part_count[l]) {
+        key[j] = score_key(base[b] + ((double)value_of(composite_key(entry[j])) - norm[b]));
+        best = max(best, key[j]);
+      }
     }
   }
-  __syncthreads();
-  for (int i = t; i < lists * a.count; i += kMergeBlock) {
-    const int l = i / a.count, j = i - l * a.count;
-    if (j >= part_count[l]) continue;
-    const int b = l / a.parts;
-    const uint64_t c = a.entries[(int64_t)row0 * a.parts * a.count + i];
-    const uint32_t at = atomicAdd(&total, 1u);
-    keys[at] = score_key(base[b] + ((double)value_of(composite_key(c)) - norm[b]));
-    tags[at] = ((uint64_t)b << 32) | composite_index(c);
+  // A bound by the upper half of the keys, where it saves more than it takes.
+  uint32_t theta = 0;
+  if (slots > kBlockN / 4) theta = bound_of<0, NW>((uint32_t)(best >> 32), a.count, offers);
+  auto keep = [&](uint64_t k, auto tag) {
+    const bool in = k != 0 && (uint32_t)(k >> 32) >= theta;
+    const uint64_t who = __ballot(in);
+    if (!who) return;
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&held, (uint32_t)__popcll(who));
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+    if (in) {
+      at += lanes_before(who);
+      keys[at] = k;
+      tags[at] = tag();
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kMergeEach; ++j) {
+    if (j * kBlockN >= slots) break;
+    keep(key[j], [&] { return ((uint64_t)beam_of(j * kBlockN + t) << 32) | composite_index(entry[j]); });
   }
+  if (a.done && t < 64) keep(stays ? score_key((double)score) : 0, [&] { return ((uint64_t)t << 32) | (uint32_t)a.pad_id; });
   __syncthreads();
-  const uint32_t n = bad ? 0u : total;
+  const uint32_t n = bad ? 0u : held;
   const uint32_t need = min(n, (uint32_t)a.count);
-  // More than a lane each: only those at or above the count-th score are ranked.
-  const bool cut = n > (uint32_t)kMergeBlock;
-  if (cut) {
-    const SelectResult r = radix_select(
-        [&](auto f) {
-          for (uint32_t i = t; i < n; i += kMergeBlock) f(keys[i]);
-        },
-        need, hist, scratch);
-    for (uint32_t i = t; i < n; i += kMergeBlock)
-      if (selected(keys[i], r)) kept[atomicAdd(&left, 1u)] = (uint16_t)i;
-    __syncthreads();
-  }
-  const uint32_t ranked = cut ? left : n;
-  for (uint32_t i = t; i < ranked; i += kMergeBlock) {
-    const uint32_t e = cut ? kept[i] : i;
-    const uint64_t key = keys[e], tag = tags[e];
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < ranked; ++j) {
-      const uint32_t o = cut ? kept[j] : j;
-      const uint64_t k = keys[o];
-      rank += (k > key || (k == key && tags[o] < tag)) ? 1u : 0u;
-    }
-    if (rank < need) {
+  const int share = share_of(kBlockN, n);
+  for (uint32_t i = (uint32_t)t / share; i < (n + kBlockN - 1) / kBlockN * kBlockN / share; i += kBlockN / share) {
+    const uint64_t k = i < n ? keys[i] : 0, tg = i < n ? tags[i] : 0;
+    const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return keys[j] > k || (keys[j] == k && tags[j] < tg); });
+    if (i < n && rank < need && (t & (share - 1)) == 0) {
       const int64_t o = (int64_t)g * a.count + rank;
-      a.tokens[o] = (int32_t)(uint32_t)tag;
-      a.parents[o] = (int32_t)(tag >> 32);
-      a.out_scores[o] = (float)score_of(key);
+      a.tokens[o] = (int32_t)(uint32_t)tg;
+      a.parents[o] = (int32_t)(tg >> 32);
+      a.out_scores[o] = (float)score_of(k);
     }
   }
-  for (int i = (int)need + t; i < a.count; i += kMergeBlock) {
+  for (int i = (int)need + t; i < a.count; i += kBlockN) {
     const int64_t o = (int64_t)g * a.count + i;
     a.tokens[o] = -1;
     a.parents[o] = -1;
@@ -497,22 +566,36 @@ int check_beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count
 int64_t sums_bytes(int64_t lists) { return (lists * (int64_t)sizeof(RowSum) + 15) / 16 * 16; }
 
 constexpr int kCus = 256;          // an MI355X's compute units
-constexpr int kPartMin = 16384;    // a part is worth a workgroup from here on
+constexpr int kPartMin = 16384;    // a chunk to each of sixteen waves
 
 // Few rows are cut into parts, a workgroup each, until there is about one to a compute unit; a group's
 // entries have to fit the merge's LDS.
 int beam_parts(int64_t rows, int beams, int vocab, int count) {
-  int64_t parts = std::min<int64_t>({kCus / std::max<int64_t>(rows, 1), vocab / kPartMin, kPartsMax});
+  int64_t parts = std::min<int64_t>({kCus / std::max<int64_t>(rows, 1), (vocab + kPartMin - 1) / kPartMin, kPartsMax});
   parts = std::min<int64_t>(parts, kEntriesMax / (beams * count));
   return (int)std::max<int64_t>(parts, 1);
+}
+
+template <int DT, bool MASK, int NW>
+int launch_block(const BeamArgs &a, unsigned blocks, hipStream_t s) {
+  hipLaunchKernelGGL((beam_row_kernel<DT, MASK, NW>), dim3(blocks), dim3(NW * 64), 0, s, a);
+  TABBY_HIP_CHECK(hipGetLastError());
+  return TABBY_OK;
 }
 
 template <int DT, bool MASK>
 int launch_rows(const BeamArgs &a, hipStream_t s) {
   const int64_t blocks = (int64_t)a.groups * a.beams * a.parts;
-  // Up to a workgroup for each compute unit: sixteen waves each; more: eight, two to a unit at once.
-  if (blocks <= kCus) hipLaunchKernelGGL((beam_row_kernel<DT, MASK, 16>), dim3((unsigned)blocks), dim3(1024), 0, s, a);
-  else hipLaunchKernelGGL((beam_row_kernel<DT, MASK, 8>), dim3((unsigned)blocks), dim3(512), 0, s, a);
+  // Four waves where they have a chunk each. Else, up to a workgroup for each compute unit: sixteen; more:
+  // eight, two to a unit at once.
+  if (a.part_len <= 4 * kChunk) return launch_block<DT, MASK, 4>(a, (unsigned)blocks, s);
+  if (blocks <= kCus) return launch_block<DT, MASK, 16>(a, (unsigned)blocks, s);
+  return launch_block<DT, MASK, 8>(a, (unsigned)blocks, s);
+}
+
+template <int NW>
+int launch_merge(const BeamArgs &a, hipStream_t s) {
+  hipLaunchKernelGGL(beam_merge_kernel<NW>, dim3((unsigned)a.groups), dim3(NW * 64), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
@@ -571,7 +654,6 @@ extern "C" int tabby_beam_select_device(const void *logits_dev, int32_t dtype, i
     default: rc = launch_type<TABBY_BF16>(a, s); break;
   }
   if (rc) return rc;
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)groups), dim3(kMergeBlock), 0, s, a);
-  TABBY_HIP_CHECK(hipGetLastError());
-  return TABBY_OK;
+  const int lists = beams * parts;
+  return lists <= 256 && lists * count <= 256 * kMergeEach ? launch_merge<4>(a, s) : launch_merge<16>(a, s);
 }
