@@ -34,7 +34,7 @@ constexpr int kEntriesMax = 8192;             // a group's entries, all of them 
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
 constexpr int kKeyLow = 12;                   // a bound in the row need not be finer than 2^-11 of it
-constexpr int kListMax = 2048;                // entries above the bound that LDS holds
+constexpr int kListMax = 4096;                // entries above the bound that LDS holds, a share to each wave
 static_assert(kBeamsMax * kCountMax <= kEntriesMax && kBeamsMax * kPartsMax <= 1024, "a group's entries and sums");
 
 // What the first kernel leaves of a row's part, beside its entries.
@@ -67,6 +67,8 @@ __device__ __forceinline__ bool beam_reads(const BeamArgs &a, int row) {
   return a.scores[row] > -INFINITY && !(a.done && a.done[row]);
 }
 
+typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
+
 // exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
 // and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]; for 2^f the
 // polynomial of degree 7 through it at the Chebyshev nodes, within 5e-11 of it. A sum of such terms
@@ -84,9 +86,9 @@ __device__ __forceinline__ double exp_64(double d) {
   p = __builtin_fma(p, f, 0.24022651213498245);
   p = __builtin_fma(p, f, 0.6931471805568318);
   p = __builtin_fma(p, f, 0.9999999999595618);
-  const uint32_t n = (uint32_t)__double_as_longlong(shifted);
-  const uint64_t bits = (uint64_t)__double_as_longlong(p);
-  return __longlong_as_double((long long)(((uint64_t)((uint32_t)(bits >> 32) + (n << 20)) << 32) | (uint32_t)bits));
+  uint32x2 bits = __builtin_bit_cast(uint32x2, p);
+  bits.y += __builtin_bit_cast(uint32x2, shifted).x << 20;
+  return __builtin_bit_cast(double, bits);
 }
 // The same for any d <= 690: below -690 nothing is left that a sum of at least 1 would hold.
 __device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, -690.0)); }
@@ -241,12 +243,16 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   using Reader = PartReader<DT, MASK>;
   constexpr int kBlockN = NW * 64;
   __shared__ BlockScratchT<NW> scratch;
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint64_t list[kListMax];  // 0 where nothing is written yet
+  constexpr uint32_t kOwn = kListMax / NW;
+  __shared__ __align__(8) uint32_t hist[kBins];
+  __shared__ uint64_t list[kListMax];
+  __shared__ uint32_t listed[NW];  // entries of each wave, those past its share too
   __shared__ uint32_t offers[256];
-  __shared__ uint32_t listed, bad, bound;
+  __shared__ uint32_t held, bad, bound;
   __shared__ double wave_sum_[NW];
   __shared__ float wave_ref[NW], wave_max_[NW];
+  uint64_t *const packed = reinterpret_cast<uint64_t *>(hist);
+  static_assert(kBins * sizeof(uint32_t) >= kBlockN * sizeof(uint64_t), "the entries that are ranked");
   const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - row * a.parts;
   const int t = (int)threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -262,9 +268,9 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, 0, 0};
     return;
   }
-  for (int i = t; i < kListMax; i += kBlockN) list[i] = 0;
+  if (t < NW) listed[t] = 0;
   if (t == 0) {
-    listed = 0;
+    held = 0;
     bad = 0;
     bound = kNegInfKey + 1;
   }
@@ -288,49 +294,44 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
 
   double sum = 0.0;
   float ref = 0.0f, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
+  uint64_t *const own = list + wave * kOwn;
+  uint32_t mine = 0;  // entries in it
+  auto raise = [&](uint32_t k) {
+    if (k > theta) {
+      theta = k;
+      if (lane == 0) atomicMax(&bound, k);
+    }
+  };
   auto take = [&]() {
-    // Elements at or above the bound join the list; a NaN is neither.
-    float least = value_of(theta);
-    if (__ballot(!(top < least))) {
-      theta = max(theta, *(volatile uint32_t *)&bound);
-      if (__ballot(!(top < value_of(theta)))) {
-        if (!(top < INFINITY)) bad = 1;
-        if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count) {
-          // Many lanes have one: the count-th largest of the lanes' maxima is a better bound.
-          const uint32_t k = kth_largest<kKeyLow>({top == top ? key_of(top) : 0u}, a.count);
-          if (k > theta) {
-            theta = k;
-            if (lane == 0) atomicMax(&bound, k);
-          }
-        }
-        least = value_of(theta);
-        uint32_t found = 0;
+    // Elements at or above the bound join the wave's list; a NaN is neither.
+    if (__ballot(!(top < value_of(theta)))) {
+      if (!(top < INFINITY)) bad = 1;
+      // Where many lanes have one, the count-th largest of the lanes' maxima is a better bound.
+      if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count)
+        raise(kth_largest<kKeyLow>({top == top ? key_of(top) : 0u}, a.count));
+      const float least = value_of(theta);
+      const uint32_t before = mine;
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) found += (uint32_t)__popcll(__ballot(x[i] >= least));
-        uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&listed, found);
-        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-        const uint32_t from = at;
-#pragma unroll
-        for (int i = 0; i < kLane; ++i) {
-          const uint64_t who = __ballot(x[i] >= least);
-          if (who) {
-            const uint32_t to = at + lanes_before(who);
-            if (x[i] >= least && to < kListMax) list[to] = composite(key_of(x[i]), (uint32_t)reader.element(c, i));
-            at += (uint32_t)__popcll(who);
-          }
+      for (int i = 0; i < kLane; ++i) {
+        const uint64_t who = __ballot(x[i] >= least);
+        if (who) {
+          const uint32_t to = mine + lanes_before(who);
+          if (x[i] >= least && to < kOwn) own[to] = composite(key_of(x[i]), (uint32_t)reader.element(c, i));
+          mine += (uint32_t)__popcll(who);
         }
-        // Every 64 (or 256) entries the count-th largest of the last so many is a new bound.
-        const uint32_t span = a.count <= 32 ? 64 : 256;
-        if (from / span != at / span && at <= kListMax) {
-          wave_lds_sync();
-          const volatile uint32_t *high = reinterpret_cast<const volatile uint32_t *>(list + (at / span - 1) * span) + 1;
-          const uint32_t k = span == 64 ? kth_largest<kKeyLow>({high[lane * 2]}, a.count)
-                                        : kth_largest<kKeyLow>({high[lane * 2], high[128 + lane * 2], high[256 + lane * 2],
-                                                                high[384 + lane * 2]}, a.count);
-          theta = max(theta, k);
-          if (lane == 0) atomicMax(&bound, k);
-        }
+      }
+      if (lane == 0) *(volatile uint32_t *)&listed[wave] = mine;
+      // Now and then the count-th largest of all waves' last entries, 64 or 256, is a new bound.
+      constexpr uint32_t kFew = 64 / NW, kMany = 256 / NW;
+      const uint32_t span = a.count <= 32 ? kFew : kMany;
+      if (before / span != mine / span && mine <= kOwn) {
+        auto entry = [&](uint32_t i) {
+          const uint32_t w = i / span, n = min(*(volatile uint32_t *)&listed[w], kOwn);
+          const uint32_t back = i % span + 1;
+          return back <= n ? ((volatile uint32_t *)(list + w * kOwn + (n - back)))[1] : 0u;
+        };
+        raise(span == kFew ? kth_largest<kKeyLow>({entry(lane)}, a.count)
+                           : kth_largest<kKeyLow>({entry(lane), entry(64 + lane), entry(128 + lane), entry(192 + lane)}, a.count));
       }
     }
     if (__ballot(top > rise)) {
@@ -351,15 +352,16 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       sum += part_sum[0] + part_sum[1];
     }
   };
-  if (c < reader.chunks) {
+  while (c < reader.chunks) {
     take();
-    for (c += NW; c < reader.chunks; c += NW) {
-      raw = next;
-      reader.load(c + NW, next);
-      reader.widen(raw, c, x);
-      top = chunk_max();
-      take();
-    }
+    c += NW;
+    raw = next;
+    if (c >= reader.chunks) break;
+    reader.load(c + NW, next);
+    const uint32_t shared = *(volatile uint32_t *)&bound;
+    reader.widen(raw, c, x);
+    top = chunk_max();
+    theta = max(theta, shared);
   }
   largest = wave_max(largest);
   sum = wave_sum(sum);
@@ -369,7 +371,22 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     wave_max_[wave] = largest;
   }
   __syncthreads();
-  const uint32_t n = listed;
+  // The entries at or above the last bound, which at least `count` reach where there are so many.
+  bool spilled = false;
+  for (int w = 0; w < NW; ++w) spilled |= listed[w] > kOwn;
+  const uint32_t last = bound;
+  for (uint32_t i = 0; i < min(mine, kOwn); i += 64) {
+    const uint64_t v = i + lane < min(mine, kOwn) ? own[i + lane] : 0;
+    const bool in = composite_key(v) >= last;
+    const uint64_t who = __ballot(in);
+    if (!who) continue;
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&held, (uint32_t)__popcll(who));
+    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + lanes_before(who);
+    if (in && at < (uint32_t)kBlockN) packed[at] = v;
+  }
+  __syncthreads();
+  const uint32_t n = held;
   if (bad || n == 0) {
     if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, bad ? 1 : 0, 0};
     return;
@@ -383,18 +400,15 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     term = wave_sum(term);
     if (t == 0) a.sums[blockIdx.x] = RowSum{term, m, (int)need, 0, 0};
   }
-  if (n <= (uint32_t)a.count) {
-    for (uint32_t i = t; i < n; i += kBlockN) out[i] = list[i];
-    return;
-  }
-  if (n <= (uint32_t)kBlockN) {
+  if (!spilled && n <= (uint32_t)kBlockN) {
     const int share = share_of(kBlockN, n);
     const uint32_t i = (uint32_t)t / share;
-    const uint64_t v = i < n ? list[i] : 0;
-    const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return list[j] > v; });
+    const uint64_t v = i < n ? packed[i] : 0;
+    const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return packed[j] > v; });
     if (i < n && rank < need) out[rank] = v;
     return;
   }
+  __syncthreads();
   auto pick = [&](auto for_each) {
     const SelectResult r = radix_select(for_each, need, hist, scratch);
     if (t == 0) scratch.slot = 0;
@@ -403,12 +417,12 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       if (selected(v, r)) out[atomicAdd(&scratch.slot, 1u)] = v;
     });
   };
-  if (n <= (uint32_t)kListMax) {
+  if (!spilled) {
     pick([&](auto f) {
-      for (uint32_t i = t; i < n; i += kBlockN) f(list[i]);
+      for (uint32_t i = lane; i < mine; i += 64) f(own[i]);
     });
   } else {
-    // More than the list holds lie at or above every bound that the waves found: from the row again.
+    // A wave's share of the list does not hold what lies at or above its bounds: from the row again.
     const uint32_t *mask = a.allowed ? a.allowed + (int64_t)row * a.words : nullptr;
     const auto *src = Reader::start(a, row, 0);
     pick([&](auto f) {
