@@ -28,14 +28,14 @@ namespace {
 
 constexpr int kBeamsMax = 64;
 constexpr int kCountMax = 128;
-constexpr int kPartsMax = 16;
+constexpr int kPartsMax = 32;
 constexpr int kVocabMax = 1 << 28;            // a part's bytes fit a buffer resource
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
 constexpr int kKeyLow = 12;                   // a bound in the row need not be finer than 2^-11 of it
 constexpr int kListMax = 4096;                // entries above the bound that LDS holds, a share to each wave
-static_assert(kBeamsMax * kCountMax <= kEntriesMax && kBeamsMax * kPartsMax <= 1024, "a group's entries and sums");
+static_assert(kBeamsMax * kCountMax <= kEntriesMax, "a group's entries");
 
 // What the first kernel leaves of a row's part, beside its entries.
 struct RowSum {
@@ -178,18 +178,22 @@ struct PartReader {
   }
 };
 
-// The k-th largest of the wave's 64 R values, its bits below LOW taken as zero: bit by bit from the top, the
-// largest value that k of them reach. 0 where there are fewer that are not.
+// The k-th largest of the wave's 64 R values, its bits below LOW taken as zero: two bits at a time from the
+// top, the largest value that k of them reach. 0 where there are fewer that are not.
 template <int LOW, int R>
 __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[R], int k) {
+  static_assert(LOW % 2 == 0, "bits in pairs");
   uint32_t found = 0;
-#pragma unroll 4
-  for (int bit = 31; bit >= LOW; --bit) {
-    const uint32_t next = found | (1u << bit);
-    int n = 0;
+#pragma unroll 2
+  for (int bit = 30; bit >= LOW; bit -= 2) {
+    int n[4];
 #pragma unroll
-    for (int r = 0; r < R; ++r) n += (int)__popcll(__ballot(v[r] >= next));
-    if (n >= k) found = next;
+    for (uint32_t i = 1; i < 4; ++i) {
+      n[i] = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) n[i] += (int)__popcll(__ballot(v[r] >= (found | (i << bit))));
+    }
+    found |= (n[3] >= k ? 3u : n[2] >= k ? 2u : n[1] >= k ? 1u : 0u) << bit;
   }
   return found;
 }
@@ -199,23 +203,42 @@ __device__ __forceinline__ uint32_t lanes_before(uint64_t who) {
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
 }
 
-// A lower bound of the count-th largest of the keys that the workgroup's lanes hold, one each, from the
-// largest few of every wave. `offers` holds 256 words; the call meets the workgroup once.
-template <int LOW, int NW>
-__device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, uint32_t *offers) {
-  const int lane = wave_lane();
-  const int rows = count <= 16 ? 1 : count <= 64 ? 2 : 4;  // 64 offers each
-  const int each = 64 * rows / NW;
-  uint32_t *mine = offers + ((int)threadIdx.x >> 6) * each;
-  const bool in = key >= kth_largest<LOW>({key}, each);
-  const uint64_t who = __ballot(in);
-  const int at = (int)lanes_before(who);
-  if (in && at < each) mine[at] = key;
-  if (lane >= __popcll(who) && lane < each) mine[lane] = 0;
+// A lower bound of the count-th largest of the keys that the workgroup's lanes hold, one each: the keys fall
+// into 64 columns (256 where more than 32 are kept), and the count-th largest of the columns' largest,
+// found by ranking them, has as many keys at or above it. Close to the count-th largest itself where the
+// keys fall by chance; each wave's are turned by another angle so that an order among them matters less.
+template <int NW>
+struct BoundScratch {
+  uint32_t keys[NW * 64];
+  uint32_t columns[256];
+  uint32_t bound;
+};
+
+template <int NW>
+__device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, BoundScratch<NW> &s) {
+  const int lane = wave_lane(), wave = (int)threadIdx.x >> 6;
+  s.keys[wave * 64 + ((lane + 5 * wave) & 63)] = key;
+  const int waves = count <= 32 ? 1 : 4;  // those that take part
   __syncthreads();
-  if (rows == 1) return kth_largest<LOW>({offers[lane]}, count);
-  if (rows == 2) return kth_largest<LOW>({offers[lane], offers[64 + lane]}, count);
-  return kth_largest<LOW>({offers[lane], offers[64 + lane], offers[128 + lane], offers[192 + lane]}, count);
+  uint32_t mine = 0;
+  if (wave < waves) {
+    for (int w = wave; w < NW; w += waves) mine = max(mine, s.keys[w * 64 + lane]);
+    s.columns[threadIdx.x] = mine;
+  }
+  if (waves > 1) __syncthreads();
+  else wave_lds_sync();
+  if (wave < waves) {
+    int above = 0;  // columns before this one, equal ones in their order
+#pragma unroll 4
+    for (int j = 0; j < waves * 64; j += 4) {
+      const u32x4 other = *reinterpret_cast<const u32x4 *>(&s.columns[j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) above += other[i] + (j + i < (int)threadIdx.x ? 1u : 0u) > mine ? 1 : 0;
+    }
+    if (above == count - 1) s.bound = mine;
+  }
+  __syncthreads();
+  return s.bound;
 }
 
 // How many of the n things come before thing c, counted by `share` neighbouring lanes (a power of two up to
@@ -247,7 +270,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   __shared__ __align__(8) uint32_t hist[kBins];
   __shared__ uint64_t list[kListMax];
   __shared__ uint32_t listed[NW];  // entries of each wave, those past its share too
-  __shared__ uint32_t offers[256];
+  __shared__ __align__(16) BoundScratch<NW> bounds;
   __shared__ uint32_t held, bad, bound;
   __shared__ double wave_sum_[NW];
   __shared__ float wave_ref[NW], wave_max_[NW];
@@ -290,7 +313,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     top = -INFINITY;
   }
   // The first bound, from the lanes' largest of the first chunks.
-  uint32_t theta = max(bound_of<kKeyLow, NW>(top == top ? key_of(top) : 0u, a.count, offers), kNegInfKey + 1);
+  uint32_t theta = max(bound_of<NW>(top == top ? key_of(top) : 0u, a.count, bounds), kNegInfKey + 1);
 
   double sum = 0.0;
   float ref = 0.0f, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
@@ -324,7 +347,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       // Now and then the count-th largest of all waves' last entries, 64 or 256, is a new bound.
       constexpr uint32_t kFew = 64 / NW, kMany = 256 / NW;
       const uint32_t span = a.count <= 32 ? kFew : kMany;
-      if (before / span != mine / span && mine <= kOwn) {
+      if (before / span != mine / span && mine <= kOwn && c + NW < reader.chunks) {
         auto entry = [&](uint32_t i) {
           const uint32_t w = i / span, n = min(*(volatile uint32_t *)&listed[w], kOwn);
           const uint32_t back = i % span + 1;
@@ -374,7 +397,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   // The entries at or above the last bound, which at least `count` reach where there are so many.
   bool spilled = false;
   for (int w = 0; w < NW; ++w) spilled |= listed[w] > kOwn;
-  const uint32_t last = bound;
+  const uint32_t last = max(bound, theta);
   for (uint32_t i = 0; i < min(mine, kOwn); i += 64) {
     const uint64_t v = i + lane < min(mine, kOwn) ? own[i + lane] : 0;
     const bool in = composite_key(v) >= last;
@@ -444,69 +467,61 @@ __device__ __forceinline__ double score_of(uint64_t k) {
   return __longlong_as_double((long long)(k ^ (~(uint64_t)((int64_t)k >> 63) | 0x8000000000000000ull)));
 }
 
-// One workgroup of NW waves to a group of at most NW * 512 entries: its beams' entries become scores, those
-// that may be among the best `count` go to LDS, and there each is ranked by counting those that come
-// before it. Bound by the latency of its few steps.
+// One workgroup of NW waves to a group of at most NW * 512 entries and NW * 64 parts: its beams' entries
+// become scores, those that may be among the best `count` go to LDS, and there each is ranked by counting
+// those that come before it. Bound by the latency of its few steps.
 constexpr int kMergeEach = 8;  // entries to a lane
 
 template <int NW>
-__global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a) {
+__global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int width) {
   constexpr int kBlockN = NW * 64;
   constexpr int kHeld = kBlockN * kMergeEach;
   __shared__ uint64_t keys[kHeld];  // scores
   __shared__ uint64_t tags[kHeld];  // beam << 32 | token: the order of equal scores
-  __shared__ double part_term[kBlockN];
-  __shared__ float part_max[kBlockN];
   __shared__ int32_t part_count[kBlockN];
   __shared__ double base[kBeamsMax], norm[kBeamsMax];
-  __shared__ uint32_t offers[256];
+  __shared__ __align__(16) BoundScratch<NW> bounds;
   __shared__ uint32_t held, bad;
   const int g = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
   const int row0 = g * a.beams;
-  const int lists = a.beams * a.parts;  // up to kBlockN
-  const int slots = lists * a.count;
+  const int slots = a.beams * a.parts * a.count;
   uint64_t entry[kMergeEach];
 #pragma unroll
   for (int j = 0; j < kMergeEach; ++j) {
     const int i = j * kBlockN + t;
     entry[j] = i < slots ? a.entries[(int64_t)row0 * a.parts * a.count + i] : 0;
   }
+  // `width` neighbouring lanes to a beam, a power of two up to kPartsMax, one to a part.
+  const int beam = t / width, part = t & (width - 1);
   RowSum rs{0.0, -INFINITY, 0, 0, 0};
-  if (t < lists) rs = a.sums[(int64_t)row0 * a.parts + t];
   float score = 0.0f;
   int ended = 0;
-  if (t < a.beams) {
-    score = a.scores[row0 + t];
-    ended = a.done ? a.done[row0 + t] : 0;
+  if (beam < a.beams) {
+    if (part < a.parts) rs = a.sums[(int64_t)(row0 + beam) * a.parts + part];
+    score = a.scores[row0 + beam];
+    ended = a.done ? a.done[row0 + beam] : 0;
   }
   if (t == 0) held = bad = 0;
-  if (t < lists) {
-    part_max[t] = rs.max;
-    part_count[t] = rs.count;
+  if (beam < a.beams && part < a.parts) part_count[beam * a.parts + part] = rs.count;
+  float m = rs.max;
+#pragma unroll
+  for (int stride = 1; stride < kPartsMax; stride *= 2)
+    if (stride < width) m = fmaxf(m, xor_lane_by(m, stride));
+  double sum = rs.count > 0 ? rs.sum * exp_or_none((double)rs.max - (double)m) : 0.0;
+#pragma unroll
+  for (int stride = 1; stride < kPartsMax; stride *= 2)
+    if (stride < width) sum += xor_lane_by(sum, stride);
+  const bool leads = beam < a.beams && part == 0;
+  const bool stays = leads && ended && score > -INFINITY;  // as it is: one continuation
+  if (leads) {
+    base[beam] = (double)score;
+    norm[beam] = m > -INFINITY ? (double)m + log(sum) : 0.0;
   }
   __syncthreads();
   if (rs.bad || !(score < INFINITY)) bad = 1;
-  if (t < lists) {
-    const int first = t / a.parts * a.parts;
-    float m = -INFINITY;
-    for (int p = 0; p < a.parts; ++p) m = fmaxf(m, part_max[first + p]);
-    part_term[t] = rs.count > 0 ? rs.sum * exp_or_none((double)rs.max - (double)m) : 0.0;
-  }
-  __syncthreads();
-  const bool stays = t < a.beams && ended && score > -INFINITY;  // as it is: one continuation
-  if (t < a.beams) {
-    float m = -INFINITY;
-    double sum = 0.0;
-    for (int p = 0; p < a.parts; ++p) {
-      m = fmaxf(m, part_max[t * a.parts + p]);
-      sum += part_term[t * a.parts + p];
-    }
-    base[t] = (double)score;
-    norm[t] = m > -INFINITY ? (double)m + log(sum) : 0.0;
-  }
-  __syncthreads();
   // Scores; 0 is below every one.
-  auto beam_of = [&](int i) { return i / a.count / a.parts; };
+  const float per_list = 1.0f / (float)a.count, per_beam = 1.0f / (float)(a.count * a.parts);  // i + 1/2 < 2^13 has bits to spare
+  auto beam_of = [&](int i) { return (int)(((float)i + 0.5f) * per_beam); };
   uint64_t key[kMergeEach];
   uint64_t best = stays ? score_key((double)score) : 0;
 #pragma unroll
@@ -514,7 +529,7 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a) {
     const int i = j * kBlockN + t;
     key[j] = 0;
     if (i < slots) {
-      const int l = i / a.count, b = beam_of(i);
+      const int l = (int)(((float)i + 0.5f) * per_list), b = beam_of(i);
       if (i - l * a.count < part_count[l]) {
         key[j] = score_key(base[b] + ((double)value_of(composite_key(entry[j])) - norm[b]));
         best = max(best, key[j]);
@@ -523,7 +538,7 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a) {
   }
   // A bound by the upper half of the keys, where it saves more than it takes.
   uint32_t theta = 0;
-  if (slots > kBlockN / 4) theta = bound_of<0, NW>((uint32_t)(best >> 32), a.count, offers);
+  if (slots > kBlockN / 4) theta = bound_of<NW>((uint32_t)(best >> 32), a.count, bounds);
   auto keep = [&](uint64_t k, auto tag) {
     const bool in = k != 0 && (uint32_t)(k >> 32) >= theta;
     const uint64_t who = __ballot(in);
@@ -542,7 +557,7 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a) {
     if (j * kBlockN >= slots) break;
     keep(key[j], [&] { return ((uint64_t)beam_of(j * kBlockN + t) << 32) | composite_index(entry[j]); });
   }
-  if (a.done && t < 64) keep(stays ? score_key((double)score) : 0, [&] { return ((uint64_t)t << 32) | (uint32_t)a.pad_id; });
+  if (a.done) keep(stays ? score_key((double)score) : 0, [&] { return ((uint64_t)beam << 32) | (uint32_t)a.pad_id; });
   __syncthreads();
   const uint32_t n = bad ? 0u : held;
   const uint32_t need = min(n, (uint32_t)a.count);
@@ -580,10 +595,10 @@ int check_beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count
 int64_t sums_bytes(int64_t lists) { return (lists * (int64_t)sizeof(RowSum) + 15) / 16 * 16; }
 
 constexpr int kCus = 256;          // an MI355X's compute units
-constexpr int kPartMin = 16384;    // a chunk to each of sixteen waves
+constexpr int kPartMin = 8192;     // a chunk to each of eight waves
 
 // Few rows are cut into parts, a workgroup each, until there is about one to a compute unit; a group's
-// entries have to fit the merge's LDS.
+// entries have to fit its merge. (Its parts do: they are at most kCus.)
 int beam_parts(int64_t rows, int beams, int vocab, int count) {
   int64_t parts = std::min<int64_t>({kCus / std::max<int64_t>(rows, 1), (vocab + kPartMin - 1) / kPartMin, kPartsMax});
   parts = std::min<int64_t>(parts, kEntriesMax / (beams * count));
@@ -600,16 +615,16 @@ int launch_block(const BeamArgs &a, unsigned blocks, hipStream_t s) {
 template <int DT, bool MASK>
 int launch_rows(const BeamArgs &a, hipStream_t s) {
   const int64_t blocks = (int64_t)a.groups * a.beams * a.parts;
-  // Four waves where they have a chunk each. Else, up to a workgroup for each compute unit: sixteen; more:
-  // eight, two to a unit at once.
+  // Four or eight waves where they have a chunk each. Else, up to a workgroup for each compute unit: sixteen;
+  // more: eight, two to a unit at once.
   if (a.part_len <= 4 * kChunk) return launch_block<DT, MASK, 4>(a, (unsigned)blocks, s);
-  if (blocks <= kCus) return launch_block<DT, MASK, 16>(a, (unsigned)blocks, s);
+  if (blocks <= kCus && a.part_len > 8 * kChunk) return launch_block<DT, MASK, 16>(a, (unsigned)blocks, s);
   return launch_block<DT, MASK, 8>(a, (unsigned)blocks, s);
 }
 
 template <int NW>
-int launch_merge(const BeamArgs &a, hipStream_t s) {
-  hipLaunchKernelGGL(beam_merge_kernel<NW>, dim3((unsigned)a.groups), dim3(NW * 64), 0, s, a);
+int launch_merge(const BeamArgs &a, int width, hipStream_t s) {
+  hipLaunchKernelGGL(beam_merge_kernel<NW>, dim3((unsigned)a.groups), dim3(NW * 64), 0, s, a, width);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
@@ -668,6 +683,8 @@ extern "C" int tabby_beam_select_device(const void *logits_dev, int32_t dtype, i
     default: rc = launch_type<TABBY_BF16>(a, s); break;
   }
   if (rc) return rc;
-  const int lists = beams * parts;
-  return lists <= 256 && lists * count <= 256 * kMergeEach ? launch_merge<4>(a, s) : launch_merge<16>(a, s);
+  int width = 1;
+  while (width < parts) width *= 2;
+  const bool small = beams * width <= 256 && beams * parts * count <= 256 * kMergeEach;
+  return small ? launch_merge<4>(a, width, s) : launch_merge<16>(a, width, s);
 }
