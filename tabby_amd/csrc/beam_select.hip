@@ -204,13 +204,12 @@ __device__ __forceinline__ uint32_t lanes_before(uint64_t who) {
 }
 
 // A lower bound of the count-th largest of the keys that the workgroup's lanes hold, one each: the keys fall
-// into 64 columns (256 where more than 32 are kept), and the count-th largest of the columns' largest,
-// found by ranking them, has as many keys at or above it. Close to the count-th largest itself where the
-// keys fall by chance; each wave's are turned by another angle so that an order among them matters less.
+// into 64 columns (256 where more than 32 are kept), and the count-th largest of the columns' largest has
+// as many keys at or above it. Close to the count-th largest itself where the keys fall by chance; each
+// wave's are turned by another angle so that an order among them matters less.
 template <int NW>
 struct BoundScratch {
   uint32_t keys[NW * 64];
-  uint32_t columns[256];
   uint32_t bound;
 };
 
@@ -218,24 +217,19 @@ template <int NW>
 __device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, BoundScratch<NW> &s) {
   const int lane = wave_lane(), wave = (int)threadIdx.x >> 6;
   s.keys[wave * 64 + ((lane + 5 * wave) & 63)] = key;
-  const int waves = count <= 32 ? 1 : 4;  // those that take part
   __syncthreads();
-  uint32_t mine = 0;
-  if (wave < waves) {
-    for (int w = wave; w < NW; w += waves) mine = max(mine, s.keys[w * 64 + lane]);
-    s.columns[threadIdx.x] = mine;
-  }
-  if (waves > 1) __syncthreads();
-  else wave_lds_sync();
-  if (wave < waves) {
-    int above = 0;  // columns before this one, equal ones in their order
-#pragma unroll 4
-    for (int j = 0; j < waves * 64; j += 4) {
-      const u32x4 other = *reinterpret_cast<const u32x4 *>(&s.columns[j]);
+  if (wave == 0) {
+    uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) above += other[i] + (j + i < (int)threadIdx.x ? 1u : 0u) > mine ? 1 : 0;
+    for (int w = 0; w < NW; ++w) v[w & 3] = max(v[w & 3], s.keys[w * 64 + lane]);
+    if (count <= 32) {
+      uint32_t all[1] = {max(max(v[0], v[1]), max(v[2], v[3]))};
+      wave_sort_desc<1>(all);
+      if (lane == count - 1) s.bound = all[0];
+    } else {
+      wave_sort_desc<4>(v);
+      if (lane == ((count - 1) & 63)) s.bound = count > 64 ? v[1] : v[0];
     }
-    if (above == count - 1) s.bound = mine;
   }
   __syncthreads();
   return s.bound;
@@ -270,7 +264,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   __shared__ __align__(8) uint32_t hist[kBins];
   __shared__ uint64_t list[kListMax];
   __shared__ uint32_t listed[NW];  // entries of each wave, those past its share too
-  __shared__ __align__(16) BoundScratch<NW> bounds;
+  __shared__ BoundScratch<NW> bounds;
   __shared__ uint32_t held, bad, bound;
   __shared__ double wave_sum_[NW];
   __shared__ float wave_ref[NW], wave_max_[NW];
@@ -467,27 +461,25 @@ __device__ __forceinline__ double score_of(uint64_t k) {
   return __longlong_as_double((long long)(k ^ (~(uint64_t)((int64_t)k >> 63) | 0x8000000000000000ull)));
 }
 
-// One workgroup of NW waves to a group of at most NW * 512 entries and NW * 64 parts: its beams' entries
+// One workgroup of NW waves to a group of at most NW * 64 * EACH entries and NW * 64 parts: its beams' entries
 // become scores, those that may be among the best `count` go to LDS, and there each is ranked by counting
 // those that come before it. Bound by the latency of its few steps.
-constexpr int kMergeEach = 8;  // entries to a lane
-
-template <int NW>
+template <int NW, int EACH>
 __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int width) {
   constexpr int kBlockN = NW * 64;
-  constexpr int kHeld = kBlockN * kMergeEach;
+  constexpr int kHeld = kBlockN * EACH;
   __shared__ uint64_t keys[kHeld];  // scores
   __shared__ uint64_t tags[kHeld];  // beam << 32 | token: the order of equal scores
   __shared__ int32_t part_count[kBlockN];
   __shared__ double base[kBeamsMax], norm[kBeamsMax];
-  __shared__ __align__(16) BoundScratch<NW> bounds;
+  __shared__ BoundScratch<NW> bounds;
   __shared__ uint32_t held, bad;
   const int g = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
   const int row0 = g * a.beams;
   const int slots = a.beams * a.parts * a.count;
-  uint64_t entry[kMergeEach];
+  uint64_t entry[EACH];
 #pragma unroll
-  for (int j = 0; j < kMergeEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const int i = j * kBlockN + t;
     entry[j] = i < slots ? a.entries[(int64_t)row0 * a.parts * a.count + i] : 0;
   }
@@ -522,10 +514,10 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
   // Scores; 0 is below every one.
   const float per_list = 1.0f / (float)a.count, per_beam = 1.0f / (float)(a.count * a.parts);  // i + 1/2 < 2^13 has bits to spare
   auto beam_of = [&](int i) { return (int)(((float)i + 0.5f) * per_beam); };
-  uint64_t key[kMergeEach];
+  uint64_t key[EACH];
   uint64_t best = stays ? score_key((double)score) : 0;
 #pragma unroll
-  for (int j = 0; j < kMergeEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     const int i = j * kBlockN + t;
     key[j] = 0;
     if (i < slots) {
@@ -553,7 +545,7 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
     }
   };
 #pragma unroll
-  for (int j = 0; j < kMergeEach; ++j) {
+  for (int j = 0; j < EACH; ++j) {
     if (j * kBlockN >= slots) break;
     keep(key[j], [&] { return ((uint64_t)beam_of(j * kBlockN + t) << 32) | composite_index(entry[j]); });
   }
@@ -622,9 +614,9 @@ int launch_rows(const BeamArgs &a, hipStream_t s) {
   return launch_block<DT, MASK, 8>(a, (unsigned)blocks, s);
 }
 
-template <int NW>
+template <int NW, int EACH>
 int launch_merge(const BeamArgs &a, int width, hipStream_t s) {
-  hipLaunchKernelGGL(beam_merge_kernel<NW>, dim3((unsigned)a.groups), dim3(NW * 64), 0, s, a, width);
+  hipLaunchKernelGGL((beam_merge_kernel<NW, EACH>), dim3((unsigned)a.groups), dim3(NW * 64), 0, s, a, width);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
@@ -685,6 +677,9 @@ extern "C" int tabby_beam_select_device(const void *logits_dev, int32_t dtype, i
   if (rc) return rc;
   int width = 1;
   while (width < parts) width *= 2;
-  const bool small = beams * width <= 256 && beams * parts * count <= 256 * kMergeEach;
-  return small ? launch_merge<4>(a, width, s) : launch_merge<16>(a, width, s);
+  // As few waves, and as little code, as hold the entries: a launch runs most of it once.
+  const int slots = beams * parts * count;
+  if (beams * width <= 256 && slots <= 256) return launch_merge<4, 1>(a, width, s);
+  if (beams * width <= 256 && slots <= 1024) return launch_merge<4, 4>(a, width, s);
+  return slots <= 4096 ? launch_merge<16, 4>(a, width, s) : launch_merge<16, 8>(a, width, s);
 }
