@@ -33,7 +33,6 @@ constexpr int kVocabMax = 1 << 28;            // a part's bytes fit a buffer res
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
-constexpr int kKeyLow = 12;                   // a bound in the row need not be finer than 2^-11 of it
 constexpr int kListMax = 4096;                // entries above the bound that LDS holds, a share to each wave
 static_assert(kBeamsMax * kCountMax <= kEntriesMax, "a group's entries");
 
@@ -178,24 +177,12 @@ struct PartReader {
   }
 };
 
-// The k-th largest of the wave's 64 R values, its bits below LOW taken as zero: two bits at a time from the
-// top, the largest value that k of them reach. 0 where there are fewer that are not.
-template <int LOW, int R>
-__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[R], int k) {
-  static_assert(LOW % 2 == 0, "bits in pairs");
-  uint32_t found = 0;
-#pragma unroll 2
-  for (int bit = 30; bit >= LOW; bit -= 2) {
-    int n[4];
-#pragma unroll
-    for (uint32_t i = 1; i < 4; ++i) {
-      n[i] = 0;
-#pragma unroll
-      for (int r = 0; r < R; ++r) n[i] += (int)__popcll(__ballot(v[r] >= (found | (i << bit))));
-    }
-    found |= (n[3] >= k ? 3u : n[2] >= k ? 2u : n[1] >= k ? 1u : 0u) << bit;
-  }
-  return found;
+// The k-th largest of the wave's 64 R values, k up to 64 (R = 1) or 128.
+template <int R>
+__device__ __forceinline__ uint32_t kth_largest(uint32_t (&v)[R], int k) {
+  wave_sort_desc<R>(v);
+  if constexpr (R == 1) return (uint32_t)__builtin_amdgcn_readlane((int)v[0], k - 1);
+  else return (uint32_t)__builtin_amdgcn_readlane((int)(k > 64 ? v[1] : v[0]), (k - 1) & 63);
 }
 
 // The number of set lanes before this one.
@@ -222,14 +209,9 @@ __device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, BoundScrat
     uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < NW; ++w) v[w & 3] = max(v[w & 3], s.keys[w * 64 + lane]);
-    if (count <= 32) {
-      uint32_t all[1] = {max(max(v[0], v[1]), max(v[2], v[3]))};
-      wave_sort_desc<1>(all);
-      if (lane == count - 1) s.bound = all[0];
-    } else {
-      wave_sort_desc<4>(v);
-      if (lane == ((count - 1) & 63)) s.bound = count > 64 ? v[1] : v[0];
-    }
+    uint32_t all[1] = {max(max(v[0], v[1]), max(v[2], v[3]))};
+    const uint32_t k = count <= 32 ? kth_largest<1>(all, count) : kth_largest<4>(v, count);
+    if (lane == 0) s.bound = k;
   }
   __syncthreads();
   return s.bound;
@@ -324,8 +306,10 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     if (__ballot(!(top < value_of(theta)))) {
       if (!(top < INFINITY)) bad = 1;
       // Where many lanes have one, the count-th largest of the lanes' maxima is a better bound.
-      if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count)
-        raise(kth_largest<kKeyLow>({top == top ? key_of(top) : 0u}, a.count));
+      if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count) {
+        uint32_t v[1] = {top == top ? key_of(top) : 0u};
+        raise(kth_largest<1>(v, a.count));
+      }
       const float least = value_of(theta);
       const uint32_t before = mine;
 #pragma unroll
@@ -347,8 +331,13 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
           const uint32_t back = i % span + 1;
           return back <= n ? ((volatile uint32_t *)(list + w * kOwn + (n - back)))[1] : 0u;
         };
-        raise(span == kFew ? kth_largest<kKeyLow>({entry(lane)}, a.count)
-                           : kth_largest<kKeyLow>({entry(lane), entry(64 + lane), entry(128 + lane), entry(192 + lane)}, a.count));
+        if (span == kFew) {
+          uint32_t v[1] = {entry(lane)};
+          raise(kth_largest<1>(v, a.count));
+        } else {
+          uint32_t v[4] = {entry(lane), entry(64 + lane), entry(128 + lane), entry(192 + lane)};
+          raise(kth_largest<4>(v, a.count));
+        }
       }
     }
     if (__ballot(top > rise)) {
@@ -477,11 +466,13 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
   const int g = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
   const int row0 = g * a.beams;
   const int slots = a.beams * a.parts * a.count;
-  uint64_t entry[EACH];
+  const uint64_t *entries = a.entries + (int64_t)row0 * a.parts * a.count;
+  // A lane holds its entries, or reads them twice where there are many.
+  constexpr bool kHolds = EACH <= 4;
+  uint64_t entry[kHolds ? EACH : 1];
+  if constexpr (kHolds) {
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int i = j * kBlockN + t;
-    entry[j] = i < slots ? a.entries[(int64_t)row0 * a.parts * a.count + i] : 0;
+    for (int j = 0; j < EACH; ++j) entry[j] = j * kBlockN + t < slots ? entries[j * kBlockN + t] : 0;
   }
   // `width` neighbouring lanes to a beam, a power of two up to kPartsMax, one to a part.
   const int beam = t / width, part = t & (width - 1);
@@ -514,19 +505,23 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
   // Scores; 0 is below every one.
   const float per_list = 1.0f / (float)a.count, per_beam = 1.0f / (float)(a.count * a.parts);  // i + 1/2 < 2^13 has bits to spare
   auto beam_of = [&](int i) { return (int)(((float)i + 0.5f) * per_beam); };
-  uint64_t key[EACH];
+  auto key_at = [&](int i, uint64_t e) -> uint64_t {
+    if (i >= slots) return 0;
+    const int l = (int)(((float)i + 0.5f) * per_list), b = beam_of(i);
+    if (i - l * a.count >= part_count[l]) return 0;
+    return score_key(base[b] + ((double)value_of(composite_key(e)) - norm[b]));
+  };
+  uint64_t key[kHolds ? EACH : 1];
   uint64_t best = stays ? score_key((double)score) : 0;
+  if constexpr (kHolds) {
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    const int i = j * kBlockN + t;
-    key[j] = 0;
-    if (i < slots) {
-      const int l = (int)(((float)i + 0.5f) * per_list), b = beam_of(i);
-      if (i - l * a.count < part_count[l]) {
-        key[j] = score_key(base[b] + ((double)value_of(composite_key(entry[j])) - norm[b]));
-        best = max(best, key[j]);
-      }
+    for (int j = 0; j < EACH; ++j) {
+      key[j] = key_at(j * kBlockN + t, entry[j]);
+      best = max(best, key[j]);
     }
+  } else {
+#pragma unroll 1
+    for (int i = t; i < slots; i += kBlockN) best = max(best, key_at(i, entries[i]));
   }
   // A bound by the upper half of the keys, where it saves more than it takes.
   uint32_t theta = 0;
@@ -544,10 +539,19 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
       tags[at] = tag();
     }
   };
+  auto tag_at = [&](int i, uint64_t e) { return ((uint64_t)beam_of(i) << 32) | composite_index(e); };
+  if constexpr (kHolds) {
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) {
-    if (j * kBlockN >= slots) break;
-    keep(key[j], [&] { return ((uint64_t)beam_of(j * kBlockN + t) << 32) | composite_index(entry[j]); });
+    for (int j = 0; j < EACH; ++j) {
+      if (j * kBlockN >= slots) break;
+      keep(key[j], [&] { return tag_at(j * kBlockN + t, entry[j]); });
+    }
+  } else {
+#pragma unroll 1
+    for (int i = t; i - t < slots; i += kBlockN) {
+      const uint64_t e = i < slots ? entries[i] : 0;
+      keep(key_at(i, e), [&] { return tag_at(i, e); });
+    }
   }
   if (a.done) keep(stays ? score_key((double)score) : 0, [&] { return ((uint64_t)beam << 32) | (uint32_t)a.pad_id; });
   __syncthreads();
