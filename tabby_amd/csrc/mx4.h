@@ -41,11 +41,53 @@ struct Mx4Matrix {
   __host__ __device__ int col_panels() const { return (cols + kMxPanelCols - 1) / kMxPanelCols; }
 };
 
+// A block's exponent is E = floor(log2(max|x|)) - 2, the power of two that puts the largest value into [4, 8),
+// held to [-127, 127] (a block of zeros: -127). A value's code is x / 2^E rounded to the nearest of the eight
+// magnitudes, ties to the even code, and what lies above 6 becomes 6. A block with a NaN or an infinity is
+// NaN as a whole, its codes 0. The rounding is the hardware's scaled conversion; the division by a power
+// of two is exact, so there is one rounding to a value.
+
 // The block's biased exponent from the largest magnitude's bits (f32).
 __device__ __forceinline__ uint32_t block_scale(uint32_t amax_bits) {
   if (amax_bits >= 0x7f800000u) return kMxScaleNan;
   const int e = (int)(amax_bits >> 23) - 2;  // a subnormal's field is 0: below the range all the same
   return (uint32_t)max(e, 0);
+}
+
+// The codes of N = 4 or 8 values, two to a byte.
+template <int N>
+__device__ __forceinline__ uint32_t encode_values(const float *v, float scale) {
+  uint32_t word = 0;
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], scale, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], scale, 1);
+  if constexpr (N == 8) {
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], scale, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], scale, 3);
+  }
+  return word;
+}
+
+template <int N>
+__device__ __forceinline__ void decode_values(uint32_t word, uint32_t s, float *v) {
+  const float scale = __uint_as_float(s << 23);
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 0);
+  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 1);
+  v[0] = a[0];
+  v[1] = a[1];
+  v[2] = b[0];
+  v[3] = b[1];
+  if constexpr (N == 8) {
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 2);
+    const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, scale, 3);
+    v[4] = c[0];
+    v[5] = c[1];
+    v[6] = d[0];
+    v[7] = d[1];
+  }
+  if (s == kMxScaleNan) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(0x7fc00000u);
+  }
 }
 
 // The values of one row from column `col` on, widened; zero past the last column.
@@ -66,27 +108,14 @@ __device__ __forceinline__ void load_block(const typename Elem<DT>::Bits *src, i
   }
 }
 
-// A block's codes and biased exponent E + 127 from its values. E = floor(log2(max|x|)) - 2, the power of two
-// that puts the largest value into [4, 8), held to [-127, 127] (a block of zeros: -127). A value's code
-// is x / 2^E rounded to the nearest of the eight magnitudes, ties to the even code, and what lies above
-// 6 becomes 6. A block with a NaN or an infinity is NaN as a whole, its codes 0. The rounding is the
-// hardware's scaled conversion; the division by a power of two is exact, so there is one rounding to a
-// value.
+// A whole block in one lane: its codes, and its biased exponent.
 __device__ __forceinline__ uint32_t encode_block(const float (&v)[kMxBlock], u32x4 &codes) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kMxBlock; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
   const uint32_t s = block_scale(top);
-  const float scale = __uint_as_float(s << 23);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t word = 0;
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i], v[8 * i + 1], scale, 0);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 2], v[8 * i + 3], scale, 1);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 4], v[8 * i + 5], scale, 2);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * i + 6], v[8 * i + 7], scale, 3);
-    codes[i] = s != kMxScaleNan ? word : 0u;
-  }
+  for (int i = 0; i < 4; ++i) codes[i] = s != kMxScaleNan ? encode_values<8>(v + 8 * i, __uint_as_float(s << 23)) : 0u;
   return s;
 }
 

@@ -10,86 +10,138 @@
 #include "abi_internal.h"
 #include "elem.h"
 #include "mx4.h"
+#include "wave_ops.h"
 
 namespace tabby {
 namespace {
 
-constexpr int kConvertBlock = 256;  // 16 rows x 16 blocks: one tile to a wave
+constexpr int kConvertBlock = 256;
+constexpr unsigned kConvertGrid = 1u << 20;
 
-template <int DT, bool VEC>
+// Both directions take a workgroup to a panel and are bound by HBM. Memory is read and written along the
+// rows, 256 bytes (f16, bf16) or 512 at a time, 16 to a lane, and the codes change places in LDS, so that
+// either side moves whole lines; a lane that held a block of its own would touch a line in four separate
+// instructions. 151936 x 896 f16 there and back: 193 us that way, 142 so
+// (4.9 TB/s); 1531 x 4850 bf16, whose rows lie off 16-byte boundaries: 63 and 13.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));  // rows of odd strides: the hardware takes any address
+
+template <int DT>
+struct PanelWalk {
+  using E = Elem<DT>;
+  static constexpr int kRowLanes = kMxPanelCols / E::kVec;               // lanes to a row
+  static constexpr int kBlockLanes = kMxBlock / E::kVec;                 // lanes to a block
+  static constexpr int kSteps = kMxPanelRows * kRowLanes / kConvertBlock;  // rows of a thread
+  static constexpr int kRowStep = kConvertBlock / kRowLanes;
+  int row, at;  // the first row; the place in it, in lanes
+  __device__ __forceinline__ PanelWalk() : row((int)threadIdx.x / kRowLanes), at((int)threadIdx.x % kRowLanes) {}
+  __device__ __forceinline__ int col() const { return at * E::kVec; }
+  __device__ __forceinline__ int block() const { return at / kBlockLanes; }
+  // Where a row's codes of this lane lie in the panel, and their block's scale.
+  __device__ __forceinline__ int code_byte(int r) const {
+    return (r >> 4) * kMxTileBytes + ((r & 15) + 16 * block()) * 16 + at % kBlockLanes * (E::kVec / 2);
+  }
+  __device__ __forceinline__ int scale_byte(int r) const { return 4 * ((r & 15) + 16 * block()) + (r >> 4); }
+};
+
+template <int DT>
 __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typename Elem<DT>::Bits *x, int rows, int cols,
                                                                      int64_t stride, uint8_t *codes, uint8_t *scales) {
-  const int col_panels = (cols + kMxPanelCols - 1) / kMxPanelCols;
-  const int panel_col = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // one tile to a wave
-  if (panel_col >= col_panels) return;
-  const int lane = (int)threadIdx.x & 63;
-  for (int tile = (int)blockIdx.y; tile * kMxTileRows < rows; tile += (int)gridDim.y) {
-    const int row = tile * kMxTileRows + (lane & 15);
-    const int col = panel_col * kMxPanelCols + (lane >> 4) * kMxBlock;
-    if (row >= rows) continue;
-    float v[kMxBlock];
-    load_block<DT, VEC>(x + (int64_t)row * stride, col, cols, v);
-    u32x4 word;
-    const uint32_t s = encode_block(v, word);
-    const int64_t panel = (int64_t)(tile >> 2) * col_panels + panel_col;
-    *reinterpret_cast<u32x4 *>(codes + panel * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16) = word;
-    scales[panel * kMxPanelScales + lane * 4 + (tile & 3)] = (uint8_t)(col < cols ? s : kMxScaleOne);
+  using E = Elem<DT>;
+  using Walk = PanelWalk<DT>;
+  __shared__ __align__(16) uint8_t panel_codes[kMxPanelBytes];
+  __shared__ __align__(4) uint8_t panel_scales[kMxPanelScales];
+  const Walk walk;
+  const int64_t col_panels = mx_panels(cols, kMxPanelCols), panels = mx_panels(rows, kMxPanelRows) * col_panels;
+  for (int64_t panel = blockIdx.x; panel < panels; panel += gridDim.x) {
+    const int row0 = (int)(panel / col_panels) * kMxPanelRows, col0 = (int)(panel % col_panels) * kMxPanelCols;
+    const int col = col0 + walk.col();
+    u32x4 raw[Walk::kSteps];
+#pragma unroll
+    for (int i = 0; i < Walk::kSteps; ++i) {
+      const int row = row0 + walk.row + i * Walk::kRowStep;
+      raw[i] = u32x4{0, 0, 0, 0};
+      if (row >= rows) continue;
+      const typename E::Bits *from = x + (int64_t)row * stride + col;
+      if (col + E::kVec <= cols) {
+        raw[i] = *reinterpret_cast<const u32x4_any *>(from);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) {
+          if (col + j < cols) {
+            if constexpr (E::kVec == 4) raw[i][j] = from[j];
+            else raw[i][j / 2] |= (uint32_t)from[j] << (16 * (j & 1));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < Walk::kSteps; ++i) {
+      const int r = walk.row + i * Walk::kRowStep;
+      float v[E::kVec];
+      E::widen16(raw[i], v);
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < E::kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+#pragma unroll
+      for (int lanes = 1; lanes < Walk::kBlockLanes; lanes *= 2) top = max(top, xor_lane_by(top, lanes));
+      uint32_t s = block_scale(top);
+      uint32_t word = s != kMxScaleNan ? encode_values<E::kVec>(v, __uint_as_float(s << 23)) : 0u;
+      if constexpr (E::kVec == 4) *reinterpret_cast<uint16_t *>(&panel_codes[walk.code_byte(r)]) = (uint16_t)word;
+      else *reinterpret_cast<uint32_t *>(&panel_codes[walk.code_byte(r)]) = word;
+      if (col0 + walk.block() * kMxBlock >= cols) s = kMxScaleOne;
+      if (walk.at % Walk::kBlockLanes == 0) panel_scales[walk.scale_byte(r)] = (uint8_t)s;
+    }
+    __syncthreads();
+    const int t = (int)threadIdx.x;
+    reinterpret_cast<u32x4 *>(codes + panel * kMxPanelBytes)[t] = reinterpret_cast<const u32x4 *>(panel_codes)[t];
+    if (t < kMxPanelScales / 4)
+      reinterpret_cast<uint32_t *>(scales + panel * kMxPanelScales)[t] = reinterpret_cast<const uint32_t *>(panel_scales)[t];
+    __syncthreads();
   }
 }
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix m, typename Elem<DT>::Bits *out,
-                                                                       int64_t stride) {
+template <int DT>
+__global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix m, typename Elem<DT>::Bits *out, int64_t stride) {
   using E = Elem<DT>;
-  const int col_panels = m.col_panels();
-  const int panel_col = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-  if (panel_col >= col_panels) return;
-  const int lane = (int)threadIdx.x & 63;
-  for (int tile = (int)blockIdx.y; tile * kMxTileRows < m.rows; tile += (int)gridDim.y) {
-    const int row = tile * kMxTileRows + (lane & 15);
-    const int col = panel_col * kMxPanelCols + (lane >> 4) * kMxBlock;
-    if (row >= m.rows || col >= m.cols) continue;
-    const int64_t panel = (int64_t)(tile >> 2) * col_panels + panel_col;
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(m.codes + panel * kMxPanelBytes + (tile & 3) * kMxTileBytes + lane * 16);
-    const uint32_t s = m.scales[panel * kMxPanelScales + lane * 4 + (tile & 3)];
-    const float scale = s == kMxScaleNan ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23);
-    float v[kMxBlock];
+  using Walk = PanelWalk<DT>;
+  __shared__ __align__(16) uint8_t panel_codes[kMxPanelBytes];
+  __shared__ __align__(4) uint8_t panel_scales[kMxPanelScales];
+  const Walk walk;
+  const int64_t col_panels = m.col_panels(), panels = mx_panels(m.rows, kMxPanelRows) * col_panels;
+  for (int64_t panel = blockIdx.x; panel < panels; panel += gridDim.x) {
+    const int row0 = (int)(panel / col_panels) * kMxPanelRows, col0 = (int)(panel % col_panels) * kMxPanelCols;
+    const int t = (int)threadIdx.x;
+    reinterpret_cast<u32x4 *>(panel_codes)[t] = reinterpret_cast<const u32x4 *>(m.codes + panel * kMxPanelBytes)[t];
+    if (t < kMxPanelScales / 4)
+      reinterpret_cast<uint32_t *>(panel_scales)[t] = reinterpret_cast<const uint32_t *>(m.scales + panel * kMxPanelScales)[t];
+    __syncthreads();
+    const int col = col0 + walk.col();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 0);
-      const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 1);
-      const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 2);
-      const auto d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], scale, 3);
-      v[8 * i] = a[0];
-      v[8 * i + 1] = a[1];
-      v[8 * i + 2] = b[0];
-      v[8 * i + 3] = b[1];
-      v[8 * i + 4] = c[0];
-      v[8 * i + 5] = c[1];
-      v[8 * i + 6] = d[0];
-      v[8 * i + 7] = d[1];
-    }
-    if (s == kMxScaleNan) {
-#pragma unroll
-      for (int i = 0; i < kMxBlock; ++i) v[i] = scale;
-    }
-    typename E::Bits *dst = out + (int64_t)row * stride + col;
-    if (VEC && col + kMxBlock <= m.cols) {
-#pragma unroll
-      for (int i = 0; i < kMxBlock; i += E::kVec) {
+    for (int i = 0; i < Walk::kSteps; ++i) {
+      const int r = walk.row + i * Walk::kRowStep, row = row0 + r;
+      if (row >= m.rows || col >= m.cols) continue;
+      uint32_t word;
+      if constexpr (E::kVec == 4) word = *reinterpret_cast<const uint16_t *>(&panel_codes[walk.code_byte(r)]);
+      else word = *reinterpret_cast<const uint32_t *>(&panel_codes[walk.code_byte(r)]);
+      const uint32_t s = panel_scales[walk.scale_byte(r)];
+      float v[E::kVec];
+      decode_values<E::kVec>(word, s, v);
+      typename E::Bits *to = out + (int64_t)row * stride + col;
+      if (col + E::kVec <= m.cols) {
         u32x4 u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if constexpr (E::kVec == 4) u[j] = E::narrow(v[i + j]);
-          else u[j] = (uint32_t)E::narrow(v[i + 2 * j]) | ((uint32_t)E::narrow(v[i + 2 * j + 1]) << 16);
+          if constexpr (E::kVec == 4) u[j] = E::narrow(v[j]);
+          else u[j] = (uint32_t)E::narrow(v[2 * j]) | ((uint32_t)E::narrow(v[2 * j + 1]) << 16);
         }
-        *reinterpret_cast<u32x4 *>(dst + i) = u;
-      }
-    } else {
+        *reinterpret_cast<u32x4_any *>(to) = u;
+      } else {
 #pragma unroll
-      for (int i = 0; i < kMxBlock; ++i)
-        if (col + i < m.cols) dst[i] = E::narrow(v[i]);
+        for (int j = 0; j < E::kVec; ++j)
+          if (col + j < m.cols) to[j] = E::narrow(v[j]);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -130,33 +182,27 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_pack_kernel(const uint8_t *
   }
 }
 
-dim3 convert_grid(int rows, int cols) {
+dim3 pack_grid(int rows, int cols) {
   const int64_t tiles = mx_panels(rows, kMxTileRows);
   return dim3((unsigned)mx_panels(mx_panels(cols, kMxPanelCols), 4), (unsigned)std::min<int64_t>(tiles, 65535));
 }
 
+dim3 convert_grid(int rows, int cols) {
+  return dim3((unsigned)std::min<int64_t>(mx_panels(rows, kMxPanelRows) * mx_panels(cols, kMxPanelCols), kConvertGrid));
+}
+
 template <int DT>
 int launch_quantize(const void *x, int rows, int cols, int64_t stride, uint8_t *codes, uint8_t *scales, hipStream_t s) {
-  using E = Elem<DT>;
-  const auto *src = (const typename E::Bits *)x;
-  const bool vec = (uintptr_t)x % 16 == 0 && stride % E::kVec == 0;
-  const dim3 grid = convert_grid(rows, cols);
-  if (vec)
-    hipLaunchKernelGGL((mx4_quantize_kernel<DT, true>), grid, dim3(kConvertBlock), 0, s, src, rows, cols, stride, codes, scales);
-  else
-    hipLaunchKernelGGL((mx4_quantize_kernel<DT, false>), grid, dim3(kConvertBlock), 0, s, src, rows, cols, stride, codes, scales);
+  hipLaunchKernelGGL(mx4_quantize_kernel<DT>, convert_grid(rows, cols), dim3(kConvertBlock), 0, s,
+                     (const typename Elem<DT>::Bits *)x, rows, cols, stride, codes, scales);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
 
 template <int DT>
 int launch_dequantize(const Mx4Matrix &m, void *out, int64_t stride, hipStream_t s) {
-  using E = Elem<DT>;
-  auto *dst = (typename E::Bits *)out;
-  const bool vec = (uintptr_t)out % 16 == 0 && stride % E::kVec == 0;
-  const dim3 grid = convert_grid(m.rows, m.cols);
-  if (vec) hipLaunchKernelGGL((mx4_dequantize_kernel<DT, true>), grid, dim3(kConvertBlock), 0, s, m, dst, stride);
-  else hipLaunchKernelGGL((mx4_dequantize_kernel<DT, false>), grid, dim3(kConvertBlock), 0, s, m, dst, stride);
+  hipLaunchKernelGGL(mx4_dequantize_kernel<DT>, convert_grid(m.rows, m.cols), dim3(kConvertBlock), 0, s, m,
+                     (typename Elem<DT>::Bits *)out, stride);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
@@ -240,7 +286,7 @@ extern "C" int tabby_mx4_pack_device(const void *row_codes_dev, const void *row_
   if (rc) return rc;
   rc = check_mx4_shape(rows, cols);
   if (rc) return rc;
-  hipLaunchKernelGGL(mx4_pack_kernel, convert_grid(rows, cols), dim3(kConvertBlock), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(mx4_pack_kernel, pack_grid(rows, cols), dim3(kConvertBlock), 0, (hipStream_t)stream,
                      (const uint8_t *)row_codes_dev, (const uint8_t *)row_scales_dev, rows, cols, (uint8_t *)codes_dev,
                      (uint8_t *)scales_dev);
   TABBY_HIP_CHECK(hipGetLastError());
