@@ -19,8 +19,11 @@
 #include <stdint.h>
 
 #include "elem.h"
+#include "wave_ops.h"
 
 namespace tabby {
+
+typedef u32x4 u32x4_any __attribute__((aligned(1)));  // rows of odd strides: the hardware takes any address
 
 constexpr int kMxBlock = 32;           // values to a scale
 constexpr int kMxTileRows = 16;        // rows of one operand tile
@@ -90,33 +93,43 @@ __device__ __forceinline__ void decode_values(uint32_t word, uint32_t s, float *
   }
 }
 
-// The values of one row from column `col` on, widened; zero past the last column.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_block(const typename Elem<DT>::Bits *src, int col, int cols, float (&v)[kMxBlock]) {
+// 16 bytes of a row from column `col` on; zero past the last column.
+template <int DT>
+__device__ __forceinline__ u32x4 load_values(const typename Elem<DT>::Bits *row, int col, int cols) {
   using E = Elem<DT>;
-  if (VEC && col + kMxBlock <= cols) {
+  if (col + E::kVec <= cols) return *reinterpret_cast<const u32x4_any *>(row + col);
+  u32x4 raw = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < kMxBlock; i += E::kVec) {
-      float w[E::kVec];
-      E::widen16(*reinterpret_cast<const u32x4 *>(src + col + i), w);
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) v[i + j] = w[j];
+  for (int j = 0; j < E::kVec; ++j) {
+    if (col + j < cols) {
+      if constexpr (E::kVec == 4) raw[j] = row[col + j];
+      else raw[j / 2] |= (uint32_t)row[col + j] << (16 * (j & 1));
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kMxBlock; ++i) v[i] = col + i < cols ? E::widen(src[col + i]) : 0.0f;
   }
+  return raw;
 }
 
-// A whole block in one lane: its codes, and its biased exponent.
-__device__ __forceinline__ uint32_t encode_block(const float (&v)[kMxBlock], u32x4 &codes) {
+// The codes of a lane's 16 bytes, whose block lies in neighbouring lanes, and the block's biased exponent.
+template <int DT>
+__device__ __forceinline__ uint32_t encode_lane(u32x4 raw, uint32_t &codes) {
+  using E = Elem<DT>;
+  float v[E::kVec];
+  E::widen16(raw, v);
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kMxBlock; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  const uint32_t s = block_scale(top);
+  for (int j = 0; j < E::kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) codes[i] = s != kMxScaleNan ? encode_values<8>(v + 8 * i, __uint_as_float(s << 23)) : 0u;
+  for (int lanes = 1; lanes < kMxBlock / E::kVec; lanes *= 2) top = max(top, xor_lane_by(top, lanes));
+  const uint32_t s = block_scale(top);
+  codes = s != kMxScaleNan ? encode_values<E::kVec>(v, __uint_as_float(s << 23)) : 0u;
   return s;
+}
+
+// N codes, two to a byte.
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t *to, uint32_t word) {
+  if constexpr (N == 4) *reinterpret_cast<uint16_t *>(to) = (uint16_t)word;
+  else *reinterpret_cast<uint32_t *>(to) = word;
 }
 
 }  // namespace tabby

@@ -10,7 +10,6 @@
 #include "abi_internal.h"
 #include "elem.h"
 #include "mx4.h"
-#include "wave_ops.h"
 
 namespace tabby {
 namespace {
@@ -23,8 +22,6 @@ constexpr unsigned kConvertGrid = 1u << 20;
 // either side moves whole lines; a lane that held a block of its own would touch a line in four separate
 // instructions. 151936 x 896 f16 there and back: 193 us that way, 142 so
 // (4.9 TB/s); 1531 x 4850 bf16, whose rows lie off 16-byte boundaries: 63 and 13.
-typedef u32x4 u32x4_any __attribute__((aligned(1)));  // rows of odd strides: the hardware takes any address
-
 template <int DT>
 struct PanelWalk {
   using E = Elem<DT>;
@@ -59,35 +56,13 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
       const int row = row0 + walk.row + i * Walk::kRowStep;
-      raw[i] = u32x4{0, 0, 0, 0};
-      if (row >= rows) continue;
-      const typename E::Bits *from = x + (int64_t)row * stride + col;
-      if (col + E::kVec <= cols) {
-        raw[i] = *reinterpret_cast<const u32x4_any *>(from);
-      } else {
-#pragma unroll
-        for (int j = 0; j < E::kVec; ++j) {
-          if (col + j < cols) {
-            if constexpr (E::kVec == 4) raw[i][j] = from[j];
-            else raw[i][j / 2] |= (uint32_t)from[j] << (16 * (j & 1));
-          }
-        }
-      }
+      raw[i] = row < rows ? load_values<DT>(x + (int64_t)row * stride, col, cols) : u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
       const int r = walk.row + i * Walk::kRowStep;
-      float v[E::kVec];
-      E::widen16(raw[i], v);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-      for (int lanes = 1; lanes < Walk::kBlockLanes; lanes *= 2) top = max(top, xor_lane_by(top, lanes));
-      uint32_t s = block_scale(top);
-      uint32_t word = s != kMxScaleNan ? encode_values<E::kVec>(v, __uint_as_float(s << 23)) : 0u;
-      if constexpr (E::kVec == 4) *reinterpret_cast<uint16_t *>(&panel_codes[walk.code_byte(r)]) = (uint16_t)word;
-      else *reinterpret_cast<uint32_t *>(&panel_codes[walk.code_byte(r)]) = word;
+      uint32_t word, s = encode_lane<DT>(raw[i], word);
+      store_codes<E::kVec>(&panel_codes[walk.code_byte(r)], word);
       if (col0 + walk.block() * kMxBlock >= cols) s = kMxScaleOne;
       if (walk.at % Walk::kBlockLanes == 0) panel_scales[walk.scale_byte(r)] = (uint8_t)s;
     }

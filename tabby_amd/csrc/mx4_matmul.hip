@@ -10,11 +10,11 @@
 
 #include <algorithm>
 #include <string>
-#include <type_traits>
 
 #include "abi_internal.h"
 #include "elem.h"
 #include "mx4.h"
+#include "wave_ops.h"
 
 namespace tabby {
 namespace {
@@ -49,14 +49,9 @@ __device__ __forceinline__ void store4(const Mx4Product &p, int row, int col, f3
     for (int i = 0; i < 4; ++i) v[i] += col + i < n ? p.bias[col + i] : 0.0f;
   }
   Bits *dst = (Bits *)p.out + (int64_t)row * p.out_stride + col;
-  if (col + 4 <= n && (uintptr_t)dst % (4 * sizeof(Bits)) == 0) {
-    typedef Bits vec4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<vec4 *>(dst) = vec4{E::narrow(v[0]), E::narrow(v[1]), E::narrow(v[2]), E::narrow(v[3])};
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < n) dst[i] = E::narrow(v[i]);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (col + i < n) dst[i] = E::narrow(v[i]);
 }
 
 // Exchanges a's upper half of the wave with b's lower half, and a's odd quarters with b's even ones.
@@ -73,14 +68,14 @@ __device__ __forceinline__ void swap_quarters(uint32_t &a, uint32_t &b) {
 
 // A lane's 4 x 4 columns of one row of Y: tile t has columns col + 16 t + 4 q on, q the lane's quarter of
 // the wave. Inside the matrix the quarters exchange them, so that each stores 16 columns in a row: four
-// lanes fill whole lines, where 8 bytes here and there would be merged in the cache.
+// lanes fill whole lines, where 8 bytes here and there would be merged in the cache. Rows of odd strides are
+// stored as widely: the hardware takes any address (589 x 46311 f16, k = 1336: 53 us, element by element 72).
 template <int DT>
 __device__ __forceinline__ void store_panel(const Mx4Product &p, int row, int col, f32x4 t0, f32x4 t1, f32x4 t2, f32x4 t3) {
   using E = Elem<DT>;
   using Bits = typename E::Bits;
   const int q = (int)(threadIdx.x & 63) >> 4;
-  constexpr int kAlign = 16 / (int)sizeof(Bits);
-  if (col + kMxPanelRows > p.w.rows || (uintptr_t)p.out % 16 != 0 || p.out_stride % kAlign != 0) {
+  if (col + kMxPanelRows > p.w.rows) {
     store4<DT>(p, row, col + 4 * q, t0);
     store4<DT>(p, row, col + 16 + 4 * q, t1);
     store4<DT>(p, row, col + 32 + 4 * q, t2);
@@ -118,10 +113,10 @@ __device__ __forceinline__ void store_panel(const Mx4Product &p, int row, int co
   Bits *dst = (Bits *)p.out + (int64_t)row * p.out_stride + col + 16 * q;
   if constexpr (kWords == 4) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) *reinterpret_cast<u32x4 *>(dst + 4 * t) = u32x4{u[t][0], u[t][1], u[t][2], u[t][3]};
+    for (int t = 0; t < 4; ++t) *reinterpret_cast<u32x4_any *>(dst + 4 * t) = u32x4{u[t][0], u[t][1], u[t][2], u[t][3]};
   } else {
-    *reinterpret_cast<u32x4 *>(dst) = u32x4{u[0][0], u[0][1], u[1][0], u[1][1]};
-    *reinterpret_cast<u32x4 *>(dst + 8) = u32x4{u[2][0], u[2][1], u[3][0], u[3][1]};
+    *reinterpret_cast<u32x4_any *>(dst) = u32x4{u[0][0], u[0][1], u[1][0], u[1][1]};
+    *reinterpret_cast<u32x4_any *>(dst + 8) = u32x4{u[2][0], u[2][1], u[3][0], u[3][1]};
   }
 }
 
@@ -308,15 +303,18 @@ struct FewShape {
 };
 constexpr int kSlicesMax = 8;
 constexpr int kSumsMax = 16;        // slices * NT: the upper half of the slices' sums lie in LDS, 4 KB to a tile of rows
-constexpr int kFewLds = kSumsMax / 2 * 4096;
-constexpr int kStepBytes = kMxTileBytes + 64;      // codes and scales of 16 rows, 128 columns
-constexpr int kFloatPanels = kFewLds / kStepBytes;  // of k, of X quantised in the workgroup
+constexpr int kSumsLds = kSumsMax / 2 * 4096;
+constexpr int kStepBytes = kMxTileBytes + 64;  // codes and scales of 16 rows, 128 columns
+constexpr int kFloatSteps = 60;                // of them in LDS, of X quantised in the workgroup
+constexpr int kFloatPanels = 192;              // a row's panels of k, over all rows: about a microsecond's work
 
 // The tiles of X as they are held.
 template <int NT>
 struct HeldTiles {
   using Args = Mx4Matrix;
   static constexpr int kTiles = NT;
+  static constexpr bool kFills = false;
+  static constexpr int kLds = kSumsLds;
   struct Raw { u32x4 codes[NT]; uint32_t scales; };
   const uint8_t *codes, *scales;
   uint32_t shift;
@@ -340,50 +338,65 @@ struct HeldTiles {
   }
 };
 
-// Up to 16 rows of x's own values: every workgroup quantises all of them into LDS, a block of one row to a
-// thread, which costs it less than a launch before this one does. Rows past the last hold anything.
+// A few rows of x's own values: every workgroup quantises all of them into LDS, 16 bytes to a thread at a
+// time, which costs it less than a launch before this one does. Rows past the last hold anything.
 struct FloatRows {
   const void *x;
   int64_t stride;
   int rows, cols;
-  int wide;  // 16-byte loads
 };
 
-template <int XDT>
+template <int XDT, int NT>
 struct FloatTiles {
   using Args = FloatRows;
-  static constexpr int kTiles = 1;
+  static constexpr int kTiles = NT;
+  static constexpr bool kFills = true;
+  static constexpr int kLds = kFloatSteps * kStepBytes;
   struct Raw {};
   const uint8_t *codes;
-  __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int lane) : codes(lds) { (void)lane; }
+  __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int) : codes(lds) {}
   static __device__ __forceinline__ void fill(const FloatRows &a, uint8_t *lds, int kp) {
     using E = Elem<XDT>;
-    for (int i = (int)threadIdx.x; i < a.rows * kp * 4; i += (int)blockDim.x) {
-      const int r = i / (kp * 4), b = i - r * (kp * 4), col = b * kMxBlock;
-      const auto *row = (const typename E::Bits *)a.x + (int64_t)r * a.stride;
-      float v[kMxBlock];
-      u32x4 word;
-      if (a.wide) load_block<XDT, true>(row, col, a.cols, v);
-      else load_block<XDT, false>(row, col, a.cols, v);
-      const uint32_t s = encode_block(v, word);
-      uint8_t *to = lds + (b >> 2) * kStepBytes;
-      const int lane = r + 16 * (b & 3);
-      *reinterpret_cast<u32x4 *>(to + lane * 16) = word;
-      to[kMxTileBytes + lane] = (uint8_t)(col < a.cols ? s : kMxScaleOne);
+    constexpr int kBatch = 4, kBlockLanes = kMxBlock / E::kVec;
+    const int row_lanes = kp * (kMxPanelCols / E::kVec), all = a.rows * row_lanes;
+    for (int first = (int)threadIdx.x; first < all; first += kBatch * (int)blockDim.x) {
+      u32x4 raw[kBatch];
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int i = first + n * (int)blockDim.x, r = i / row_lanes, col = (i - r * row_lanes) * E::kVec;
+        raw[n] = i < all ? load_values<XDT>((const typename E::Bits *)a.x + (int64_t)r * a.stride, col, a.cols) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int i = first + n * (int)blockDim.x, r = i / row_lanes, at = i - r * row_lanes, b = at / kBlockLanes;
+        if (i >= all) break;
+        uint32_t word;
+        const uint32_t s = encode_lane<XDT>(raw[n], word);
+        uint8_t *to = lds + ((b >> 2) * NT + (r >> 4)) * kStepBytes;
+        const int lane = (r & 15) + 16 * (b & 3);
+        store_codes<E::kVec>(to + lane * 16 + at % kBlockLanes * (E::kVec / 2), word);
+        if (at % kBlockLanes == 0) to[kMxTileBytes + lane] = (uint8_t)(b * kMxBlock < a.cols ? s : kMxScaleOne);
+      }
     }
   }
   __device__ __forceinline__ void load(int, Raw &) const {}
-  __device__ __forceinline__ uint32_t tiles(const Raw &, int k, u32x4 (&c)[1]) const {
-    const uint8_t *at = codes + k * kStepBytes;
-    c[0] = *reinterpret_cast<const u32x4 *>(at + (threadIdx.x & 63) * 16);
-    return at[kMxTileBytes + (threadIdx.x & 63)];
+  __device__ __forceinline__ uint32_t tiles(const Raw &, int k, u32x4 (&c)[NT]) const {
+    const int lane = (int)threadIdx.x & 63;
+    uint32_t scales = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint8_t *at = codes + (k * NT + t) * kStepBytes;
+      c[t] = *reinterpret_cast<const u32x4 *>(at + lane * 16);
+      scales |= (uint32_t)at[kMxTileBytes + lane] << (8 * t);
+    }
+    return scales;
   }
 };
 
 template <int DT, typename Rows>
 __global__ __launch_bounds__(kSlicesMax * 64) void mx4_few_kernel(Mx4Product p, typename Rows::Args xs, FewShape shape) {
   constexpr int NT = Rows::kTiles;
-  __shared__ __align__(16) uint8_t lds[kFewLds];
+  __shared__ __align__(16) uint8_t lds[Rows::kLds > kSumsLds ? Rows::kLds : kSumsLds];
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int slice = wave & (shape.slices - 1);
@@ -421,7 +434,7 @@ __global__ __launch_bounds__(kSlicesMax * 64) void mx4_few_kernel(Mx4Product p, 
   };
   Step now, next;
   if (k < end) load(k, now);
-  if constexpr (!std::is_same<typename Rows::Args, Mx4Matrix>::value) {
+  if constexpr (Rows::kFills) {
     Rows::fill(xs, lds, kp);
     __syncthreads();
   }
@@ -434,7 +447,7 @@ __global__ __launch_bounds__(kSlicesMax * 64) void mx4_few_kernel(Mx4Product p, 
     multiply(k, now);
   }
   // The slices in halves: the upper half's sums go through LDS to the lower half's waves.
-  if constexpr (!std::is_same<typename Rows::Args, Mx4Matrix>::value) {
+  if constexpr (Rows::kFills) {
     if (shape.slices > 1) __syncthreads();
   }
   f32x4 *const sums = reinterpret_cast<f32x4 *>(lds) + lane;
@@ -497,7 +510,7 @@ template <int DT, typename Rows>
 int launch_few(const Mx4Product &p, const typename Rows::Args &xs, hipStream_t s) {
   constexpr int NT = Rows::kTiles;
   const int64_t panels = mx_panels(p.w.rows, kMxPanelRows), groups = mx_panels(p.x.rows, kMxTileRows * NT);
-  const FewShape shape = few_shape(panels * groups, p.w.col_panels(), NT, !std::is_same<typename Rows::Args, Mx4Matrix>::value);
+  const FewShape shape = few_shape(panels * groups, p.w.col_panels(), NT, Rows::kFills);
   const int64_t blocks = mx_panels(panels, shape.waves / shape.slices);
   hipLaunchKernelGGL((mx4_few_kernel<DT, Rows>), dim3((unsigned)blocks, (unsigned)groups), dim3(64 * shape.waves), 0, s, p, xs, shape);
   TABBY_HIP_CHECK(hipGetLastError());
@@ -526,12 +539,26 @@ int product(const Mx4Product &p, int32_t out_dtype, hipStream_t s) {
 }
 
 // X quantised in the product's own launch.
+bool fills(int rows, int kp) {
+  return rows <= kMxPanelRows && mx_panels(rows, kMxTileRows) * kp <= kFloatSteps && rows * kp <= kFloatPanels;
+}
+
+template <int DT, int XDT>
+int launch_linear(const Mx4Product &p, const FloatRows &x, hipStream_t s) {
+  switch (mx_panels(x.rows, kMxTileRows)) {
+    case 1: return launch_few<DT, FloatTiles<XDT, 1>>(p, x, s);
+    case 2: return launch_few<DT, FloatTiles<XDT, 2>>(p, x, s);
+    case 3: return launch_few<DT, FloatTiles<XDT, 3>>(p, x, s);
+    default: return launch_few<DT, FloatTiles<XDT, 4>>(p, x, s);
+  }
+}
+
 template <int DT>
 int launch_linear(const Mx4Product &p, const FloatRows &x, int x_dtype, hipStream_t s) {
   switch (x_dtype) {
-    case TABBY_F32: return launch_few<DT, FloatTiles<TABBY_F32>>(p, x, s);
-    case TABBY_F16: return launch_few<DT, FloatTiles<TABBY_F16>>(p, x, s);
-    default: return launch_few<DT, FloatTiles<TABBY_BF16>>(p, x, s);
+    case TABBY_F32: return launch_linear<DT, TABBY_F32>(p, x, s);
+    case TABBY_F16: return launch_linear<DT, TABBY_F16>(p, x, s);
+    default: return launch_linear<DT, TABBY_BF16>(p, x, s);
   }
 }
 
@@ -593,9 +620,8 @@ extern "C" int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64
   uint8_t *codes = (uint8_t *)workspace_dev, *scales = codes + code_bytes;
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
                      {codes, scales, rows, k}, bias_dev, out_dev, out_stride};
-  if (rows <= kMxTileRows && p.w.col_panels() <= kFloatPanels) {
-    const bool wide = (uintptr_t)x_dev % 16 == 0 && (rows == 1 || x_stride * (int64_t)dtype_size(x_dtype) % 16 == 0);
-    return linear(p, FloatRows{x_dev, x_stride, rows, k, wide}, x_dtype, out_dtype, (hipStream_t)stream);
+  if (fills(rows, p.w.col_panels())) {
+    return linear(p, FloatRows{x_dev, x_stride, rows, k}, x_dtype, out_dtype, (hipStream_t)stream);
   }
   rc = mx4_quantize(x_dev, x_dtype, rows, k, x_stride, codes, scales, (hipStream_t)stream);
   if (rc) return rc;
