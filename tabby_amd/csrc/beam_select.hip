@@ -358,8 +358,19 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       sum += part_sum[0] + part_sum[1];
     }
   };
+  // Two of these workgroups share a unit, and its waves issue the oldest first: the elder would end after 33 us
+  // of 54 and leave the other alone with half the waves. Whoever is further along yields instead: 512 rows
+  // of 151,936 f32 74 -> 67 us, f16 68 -> 61.
+  constexpr bool kYields = NW == 8;
+  const int tenth = reader.chunks / 10, late[3] = {reader.chunks - tenth, reader.chunks - 3 * tenth, reader.chunks - 6 * tenth};
+  if constexpr (kYields) __builtin_amdgcn_s_setprio(3);
   while (c < reader.chunks) {
     take();
+    if constexpr (kYields) {
+      if (c >= late[0]) __builtin_amdgcn_s_setprio(0);
+      else if (c >= late[1]) __builtin_amdgcn_s_setprio(1);
+      else if (c >= late[2]) __builtin_amdgcn_s_setprio(2);
+    }
     c += NW;
     raw = next;
     if (c >= reader.chunks) break;
