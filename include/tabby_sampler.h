@@ -271,7 +271,7 @@ TABBY_API int tabby_beam_workspace(int32_t groups, int32_t beams, int32_t vocab,
  * in 64 bits. allowed_dev (may be NULL: everything) has ceil(vocab / 32) words to a row, entry t
  * at bit t % 32 of word t / 32; what is not allowed is never looked at, NaN included.
  * done_dev [groups, beams] (may be NULL): a beam with a nonzero entry has ended, and its one
- * continuation is pad_id at its own score; its logits are not read. A beam whose score is
+ * continuation is pad_id at its own score, whatever its logits hold. A beam whose score is
  * -inf has no continuations, nor has an entry of -inf or a row in which nothing is allowed.
  * The `count` (1..128) best of each group's beams (1..64), equal scores in the order of (beam,
  * token), go to tokens_dev, parents_dev (the beam within its group) and out_scores_dev, each

@@ -102,19 +102,19 @@ def _geometry(states, rows: int, what: str):
     """(segments, capacity, unit bytes, row stride, segment stride) of states of one shape, [rows,
     positions], [rows, positions, width] or [rows, segments, positions, width], and their addresses."""
     s = states[0]
-    device, dtype, shape, strides, dims = s.device, s.dtype, s.shape, s.stride(), s.dim()
+    dtype, shape, strides, dims = s.dtype, s.shape, s.stride(), s.dim()
     if not s.is_cuda:
         raise ValueError(f"{what} must be device (cuda) tensors")
     if dims not in (2, 3, 4) or shape[0] != rows or s.numel() == 0:
         raise ValueError(f"{what} must be [rows, positions], [rows, positions, width] or [rows, segments, positions, "
                          f"width] with {rows} rows, got {tuple(shape)}")
-    addresses = []
+    index = s.get_device()
     for o in states:
-        if o.shape != shape or o.stride() != strides or o.dtype != dtype:
+        if o.shape != shape or o.stride() != strides or o.dtype is not dtype:
             raise ValueError(f"{what} must all be of one shape, layout and type")
-        if o.device != device:
-            raise ValueError(f"tensors lie on {device} and on {o.device}")
-        addresses.append(o.data_ptr())
+        if o.get_device() != index:
+            raise ValueError(f"tensors lie on {s.device} and on {o.device}")
+    addresses = [o.data_ptr() for o in states]
     size = s.element_size()
     position = 1 if dims < 4 else 2
     capacity = shape[position]

@@ -32,8 +32,10 @@ struct ReorderArgs {
   int64_t unit;      // bytes of a position
   int64_t row_stride, segment_stride;
   const int32_t *parents, *lengths;
-  int64_t chunks;  // workgroups to a segment
+  uint32_t chunks;  // columns' workgroups to a segment
+  uint32_t first;   // of all groups' segments' workgroups, this launch's first
 };
+constexpr int64_t kReorderGrid = 1 << 23;  // of 256 threads: 2^32 in a launch are too many
 
 template <int BYTES>
 struct ColumnOf;
@@ -48,11 +50,12 @@ struct ColumnOf<2> { using T = uint16_t; };
 template <>
 struct ColumnOf<1> { using T = uint8_t; };
 
-// NB: beams held at once. Grid: ((group * segments + segment) * chunks + chunk, state).
+// NB: beams held at once. Grid: ((group * segments + segment) * chunks + chunk - first, state).
 template <int BYTES, int NB, bool IN_PLACE>
-__global__ __launch_bounds__(kReorderBlock) void beam_reorder_kernel(ReorderArgs a) {
+__global__ __launch_bounds__(kReorderBlock, 4) void beam_reorder_kernel(ReorderArgs a) {
   using T = typename ColumnOf<BYTES>::T;
-  const uint32_t line = blockIdx.x / (uint32_t)a.chunks, chunk = blockIdx.x - line * (uint32_t)a.chunks;
+  const uint32_t id = a.first + blockIdx.x;
+  const uint32_t line = id / a.chunks, chunk = id - line * a.chunks;
   const int g = (int)(line / (uint32_t)a.segments), seg = (int)(line - (uint32_t)g * a.segments);
   int64_t length = a.capacity;
   if (a.lengths) length = min(length, (int64_t)max(a.lengths[g], 0));
@@ -62,39 +65,45 @@ __global__ __launch_bounds__(kReorderBlock) void beam_reorder_kernel(ReorderArgs
   const char *src = a.src[blockIdx.y] + first;
   char *dst = a.dst[blockIdx.y] + first;
   const int32_t *parents = a.parents + (int64_t)g * a.beams;
+  uint32_t parent[NB];
   T v[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    if (b >= a.beams) break;
-    const uint32_t p = (uint32_t)parents[b];
-    if (p < (uint32_t)a.beams && !(IN_PLACE && p == (uint32_t)b)) v[b] = *reinterpret_cast<const T *>(src + p * a.row_stride);
+    parent[b] = b < a.beams ? (uint32_t)__builtin_amdgcn_readfirstlane(parents[b]) : ~0u;
+    if (IN_PLACE && parent[b] == (uint32_t)b) parent[b] = ~0u;
   }
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    if (b >= a.beams) break;
-    const uint32_t p = (uint32_t)parents[b];
-    if (p < (uint32_t)a.beams && !(IN_PLACE && p == (uint32_t)b)) *reinterpret_cast<T *>(dst + b * a.row_stride) = v[b];
-  }
+  for (int b = 0; b < NB; ++b)
+    if (parent[b] < (uint32_t)a.beams) v[b] = *reinterpret_cast<const T *>(src + parent[b] * a.row_stride);
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+    if (parent[b] < (uint32_t)a.beams) *reinterpret_cast<T *>(dst + b * a.row_stride) = v[b];
 }
 
 template <int BYTES, int NB>
-int launch_width(const ReorderArgs &a, dim3 grid, bool in_place, hipStream_t s) {
-  if (in_place) hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, true>), grid, dim3(kReorderBlock), 0, s, a);
-  else hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, false>), grid, dim3(kReorderBlock), 0, s, a);
-  TABBY_HIP_CHECK(hipGetLastError());
+int launch_width(ReorderArgs &a, int groups, int states, bool in_place, hipStream_t s) {
+  const int64_t chunks = (a.capacity * a.unit + (int64_t)kReorderBlock * BYTES - 1) / ((int64_t)kReorderBlock * BYTES);
+  const int64_t rows = (int64_t)groups * a.segments;
+  if (chunks > INT32_MAX / rows) return record_failure(TABBY_EINVAL, "the states are too large for one call");
+  a.chunks = (uint32_t)chunks;
+  for (int64_t first = 0; first < chunks * rows; first += kReorderGrid) {
+    a.first = (uint32_t)first;
+    const dim3 grid((unsigned)std::min(chunks * rows - first, kReorderGrid), (unsigned)states);
+    if (in_place) hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, true>), grid, dim3(kReorderBlock), 0, s, a);
+    else hipLaunchKernelGGL((beam_reorder_kernel<BYTES, NB, false>), grid, dim3(kReorderBlock), 0, s, a);
+    TABBY_HIP_CHECK(hipGetLastError());
+  }
   return TABBY_OK;
 }
 
+// Columns of at most 256 bytes / beams: a lane holds one for each beam, 64 registers of them.
 template <int BYTES>
 int launch_reorder(ReorderArgs &a, int groups, int states, bool in_place, hipStream_t s) {
-  a.chunks = (a.capacity * a.unit + (int64_t)kReorderBlock * BYTES - 1) / ((int64_t)kReorderBlock * BYTES);
-  const int64_t rows = (int64_t)groups * a.segments;
-  if (a.chunks > INT32_MAX / rows) return record_failure(TABBY_EINVAL, "the states are too large for one launch");
-  const dim3 grid((unsigned)(a.chunks * rows), (unsigned)states);
-  if (a.beams <= 4) return launch_width<BYTES, 4>(a, grid, in_place, s);
-  if (a.beams <= 8) return launch_width<BYTES, 8>(a, grid, in_place, s);
-  if (a.beams <= 16) return launch_width<BYTES, 16>(a, grid, in_place, s);
-  return launch_width<BYTES, 64>(a, grid, in_place, s);
+  if (a.beams <= 4) return launch_width<BYTES, 4>(a, groups, states, in_place, s);
+  if (a.beams <= 8) return launch_width<BYTES, 8>(a, groups, states, in_place, s);
+  if (a.beams <= 16) return launch_width<BYTES, 16>(a, groups, states, in_place, s);
+  if (a.beams <= 32) return launch_width<(BYTES < 8 ? BYTES : 8), 32>(a, groups, states, in_place, s);
+  return launch_width<(BYTES < 4 ? BYTES : 4), 64>(a, groups, states, in_place, s);
 }
 
 }  // namespace
@@ -112,6 +121,10 @@ extern "C" int tabby_beam_reorder_device(const void *const *src_dev, void *const
   if (beams < 1 || beams > kReorderBeams)
     return record_failure(TABBY_EINVAL, "beams must be between 1 and " + std::to_string(kReorderBeams) + ", got " + std::to_string(beams));
   if (capacity > INT64_MAX / unit_bytes) return record_failure(TABBY_EINVAL, "a segment must fit 63 bits");
+  if (!lengths_dev) {  // whole segments: one position each, whose columns may be wide
+    unit_bytes *= capacity;
+    capacity = 1;
+  }
   const int64_t segment = capacity * unit_bytes;
   if (segments > 1 && segment_stride < segment)
     return record_failure(TABBY_EINVAL, "segment_stride must be at least capacity x unit_bytes");
