@@ -180,8 +180,10 @@ class BeamSearch:
         beams and appends the new tokens; returns them, int32 [groups * beams]."""
         if self.length >= self.max_tokens:
             raise ValueError(f"the search holds {self.max_tokens} tokens")
+        status = torch.empty_like(self.status)
         choice = self.select(logits, self.scores, self.beams, allowed=allowed, done=self.done, pad_id=self.pad_id,
-                             status=self.status)
+                             status=status)
+        self.status = torch.where(self.status == 0, status, self.status)  # a group's first failure
         if states:
             reorder_states(states, choice.parents, lengths=lengths)
         reorder_states([self.tokens], choice.parents)

@@ -29,7 +29,7 @@ namespace {
 constexpr int kBeamsMax = 64;
 constexpr int kCountMax = 128;
 constexpr int kPartsMax = 32;
-constexpr int kVocabMax = 1 << 28;            // a part's bytes fit a buffer resource
+constexpr int kVocabMax = 1 << 28;            // places in a row in 32 bits, with room
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
@@ -95,60 +95,65 @@ __device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, 
 // The larger of two, NaN if either is: a chunk's maximum shows that it holds a NaN.
 __device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// One part of one row, read through 16-byte loads from the boundary at or before its start:
-// position p of the part is element begin + p - lead. What lies before the part or after it is set to
-// -inf where the first or the last chunk is taken apart, and the buffer's range ends with the last
-// 16 bytes that hold an element.
+// One part of one row, 16 bytes to a lane from the part's first element on, wherever it lies (the hardware
+// takes any address): which lane takes which element, and so the order of the sum, depends on its place in
+// the row alone, and rows that are equal score alike to the last bit.
 template <int DT, bool MASK>
 struct PartReader {
   using E = Elem<DT>;
+  using Bits = typename E::Bits;
   static constexpr int kLoads = kLane / E::kVec;
-  static constexpr int kSize = (int)sizeof(typename E::Bits);
+  static constexpr int kLoad = 64 * E::kVec;  // elements of a load
   struct Raw {
     u32x4 v[kLoads];
-    uint32_t lo[MASK ? kLoads : 1], hi[MASK ? kLoads : 1];
+    uint32_t mask[MASK ? kLoads : 1];
   };
-  RowBuffer buffer;
+  const Bits *row;
   const uint32_t *mask;
-  int begin, len, lead, words, chunks;
+  int begin, len, words, chunks;
 
-  static __device__ __forceinline__ int lead_of(const typename E::Bits *at) { return (int)((uintptr_t)at % 16) / kSize; }
-
-  __device__ __forceinline__ PartReader(const BeamArgs &a, int row, int begin_, int len_)
-      : buffer(start(a, row, begin_) - lead_of(start(a, row, begin_)),
-               (uint32_t)(((uint32_t)(lead_of(start(a, row, begin_)) + len_) * kSize + 15u) & ~15u)),
-        mask(MASK ? a.allowed + (int64_t)row * a.words : nullptr),
+  __device__ __forceinline__ PartReader(const BeamArgs &a, int r, int begin_, int len_)
+      : row((const Bits *)a.logits + (int64_t)r * a.row_stride),
+        mask(MASK ? a.allowed + (int64_t)r * a.words : nullptr),
         begin(begin_),
         len(len_),
-        lead(lead_of(start(a, row, begin_))),
         words(a.words),
-        chunks((lead + len_ + kChunk - 1) / kChunk) {}
+        chunks((len_ + kChunk - 1) / kChunk) {}
 
-  static __device__ __forceinline__ const typename E::Bits *start(const BeamArgs &a, int row, int begin) {
-    return (const typename E::Bits *)a.logits + (int64_t)row * a.row_stride + begin;
-  }
-
-  // The position of the lane's first element of load u of chunk c.
-  __device__ __forceinline__ int position(int c, int u) const {
-    return c * kChunk + u * 64 * E::kVec + wave_lane() * E::kVec;
-  }
-  __device__ __forceinline__ int element(int c, int i) const {
-    return begin - lead + position(c, i / E::kVec) + i % E::kVec;
-  }
+  // The place in the part of the lane's first element of load u of chunk c.
+  __device__ __forceinline__ int position(int c, int u) const { return c * kChunk + u * kLoad + wave_lane() * E::kVec; }
+  __device__ __forceinline__ int element(int c, int i) const { return begin + position(c, i / E::kVec) + i % E::kVec; }
 
   // Past the last chunk it is the last one again, which nothing looks at.
   __device__ __forceinline__ void load(int c, Raw &r) const {
     c = min(c, chunks - 1);
-    const uint32_t at = (uint32_t)wave_lane() * 16u;
+    const Bits *from = row + begin + c * kChunk;
+    const int lane = wave_lane() * E::kVec;
+    if ((c + 1) * kChunk <= len) {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) r.v[u] = buffer.load16(at, (uint32_t)c * (kChunk * kSize) + u * 1024u);
-    if constexpr (MASK) {
+      for (int u = 0; u < kLoads; ++u) r.v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(from + lane + u * kLoad));
+    } else {
 #pragma unroll
       for (int u = 0; u < kLoads; ++u) {
-        const int w = (begin - lead + position(c, u)) >> 5;
-        r.lo[u] = mask[min(max(w, 0), words - 1)];
-        r.hi[u] = lead ? mask[min(max(w + 1, 0), words - 1)] : 0u;
+        const int left = len - position(c, u);
+        r.v[u] = u32x4{0, 0, 0, 0};
+        if (left >= E::kVec) {
+          r.v[u] = *reinterpret_cast<const u32x4_any *>(from + lane + u * kLoad);
+        } else {
+#pragma unroll
+          for (int j = 0; j < E::kVec - 1; ++j) {
+            if (j < left) {
+              const uint32_t b = from[lane + u * kLoad + j];
+              if constexpr (E::kVec == 4) r.v[u][j] = b;
+              else r.v[u][j / 2] |= b << (16 * (j & 1));
+            }
+          }
+        }
       }
+    }
+    if constexpr (MASK) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) r.mask[u] = mask[min((begin + position(c, u)) >> 5, words - 1)];
     }
   }
 
@@ -157,22 +162,15 @@ struct PartReader {
     for (int u = 0; u < kLoads; ++u) {
       float w[E::kVec];
       E::widen16(r.v[u], w);
+      uint32_t bits = 0;  // parts begin on a word of the mask, and a load lies within one
+      if constexpr (MASK) bits = r.mask[u] >> ((uint32_t)position(c, u) & 31u);
 #pragma unroll
-      for (int j = 0; j < E::kVec; ++j) x[u * E::kVec + j] = w[j];
-      if constexpr (MASK) {
-        const uint32_t shift = (uint32_t)(begin - lead + position(c, u)) & 31u;
-        const uint32_t bits = __builtin_amdgcn_alignbit(r.hi[u], r.lo[u], shift);
-#pragma unroll
-        for (int j = 0; j < E::kVec; ++j)
-          x[u * E::kVec + j] = (bits >> j) & 1u ? x[u * E::kVec + j] : -INFINITY;
-      }
+      for (int j = 0; j < E::kVec; ++j) x[u * E::kVec + j] = !MASK || (bits >> j) & 1u ? w[j] : -INFINITY;
     }
-    if (c == 0 || c == chunks - 1) {
+    if (c == chunks - 1) {
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) {
-        const int p = position(c, i / E::kVec) + i % E::kVec - lead;
-        if (p < 0 || p >= len) x[i] = -INFINITY;
-      }
+      for (int i = 0; i < kLane; ++i)
+        if (position(c, i / E::kVec) + i % E::kVec >= len) x[i] = -INFINITY;
     }
   }
 };
@@ -243,6 +241,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   constexpr int kBlockN = NW * 64;
   __shared__ BlockScratchT<NW> scratch;
   constexpr uint32_t kOwn = kListMax / NW;
+  static_assert(kOwn >= kCountMax, "a full share holds as many as are kept");
   __shared__ __align__(8) uint32_t hist[kBins];
   __shared__ uint64_t list[kListMax];
   __shared__ uint32_t listed[NW];  // entries of each wave, those past its share too
@@ -403,7 +402,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     if (in && at < (uint32_t)kBlockN) packed[at] = v;
   }
   __syncthreads();
-  const uint32_t n = held;
+  const uint32_t n = spilled ? ~0u : held;  // more than a wave's share: more than are kept
   if (bad || n == 0) {
     if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, bad ? 1 : 0, 0};
     return;
@@ -417,7 +416,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     term = wave_sum(term);
     if (t == 0) a.sums[blockIdx.x] = RowSum{term, m, (int)need, 0, 0};
   }
-  if (!spilled && n <= (uint32_t)kBlockN) {
+  if (n <= (uint32_t)kBlockN) {
     const int share = share_of(kBlockN, n);
     const uint32_t i = (uint32_t)t / share;
     const uint64_t v = i < n ? packed[i] : 0;
@@ -441,7 +440,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   } else {
     // A wave's share of the list does not hold what lies at or above its bounds: from the row again.
     const uint32_t *mask = a.allowed ? a.allowed + (int64_t)row * a.words : nullptr;
-    const auto *src = Reader::start(a, row, 0);
+    const auto *src = reader.row;
     pick([&](auto f) {
       for (int e = begin + t; e < begin + len; e += kBlockN) {
         if (mask && !((mask[e >> 5] >> (e & 31)) & 1u)) continue;
@@ -678,7 +677,7 @@ extern "C" int tabby_beam_select_device(const void *logits_dev, int32_t dtype, i
     return record_failure(TABBY_EINVAL, "workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
   const int64_t rows = (int64_t)groups * beams;
   const int parts = beam_parts(rows, beams, vocab, count);
-  // Parts begin on a mask word, and on 16 bytes where the row does.
+  // Parts begin on a word of the mask.
   const int part_len = (int)((((int64_t)vocab + parts - 1) / parts + 31) / 32 * 32);
   BeamArgs a{logits_dev, row_stride, scores_dev, allowed_dev, done_dev, groups, beams, vocab, count,
              (vocab - 1) / 32 + 1, parts, part_len, pad_id, tokens_dev, parents_dev, out_scores_dev, status_dev,

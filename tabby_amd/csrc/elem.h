@@ -10,6 +10,8 @@
 
 namespace tabby {
 
+typedef u32x4 u32x4_any __attribute__((aligned(1)));  // rows of odd strides: the hardware takes any address
+
 template <int DT>
 struct Elem;
 

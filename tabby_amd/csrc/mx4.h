@@ -23,8 +23,6 @@
 
 namespace tabby {
 
-typedef u32x4 u32x4_any __attribute__((aligned(1)));  // rows of odd strides: the hardware takes any address
-
 constexpr int kMxBlock = 32;           // values to a scale
 constexpr int kMxTileRows = 16;        // rows of one operand tile
 constexpr int kMxPanelRows = 64;       // rows of a panel

@@ -481,3 +481,91 @@ def test_search_finds_what_a_plain_search_finds():
         assert torch.equal(history[rows, :, 0], search.tokens[rows])
         assert search.done[g].tolist() == [int(l[2]) for l in live]
     assert len(search.best()) == groups
+
+
+def test_example_runs_the_product_the_selection_and_the_states_together():
+    # examples/beam_search_mx4.py against a plain search in 64 bits over the values its head stands for.
+    import os
+    import sys
+    torch = _torch()
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import beam_search_mx4 as example
+    import mx4_oracle as M
+    vocab, hidden, beams, steps = 397, 160, 3, 6
+    model = example.Model(vocab, hidden, seed=3)
+    prompt = torch.tensor([5, 77, 396], dtype=torch.int32, device="cuda")
+    best, run = example.search(model, prompt, beams, steps, end_ids=(9,))
+    weight = model.head.weight.dequantize().double().cpu().numpy()
+    embed = model.embed.cpu()
+    for g, first in enumerate(prompt.tolist()):
+        live = [(0.0, (), False, [])]
+        for _ in range(steps):
+            grown = []
+            for b, (s, ids, ended, kept) in enumerate(live):
+                h = embed[ids[-1] if ids else first]
+                if kept:
+                    h = h + torch.stack(kept).float().mean(0)
+                kept = kept + [h.to(torch.bfloat16)]
+                if ended:
+                    grown.append((-s, b, 0, True, kept))
+                    continue
+                row = M.rounded(h.double().numpy()[None])[0] @ weight.T
+                lp = row - (row.max() + np.log(np.exp(row - row.max()).sum()))
+                grown += [(-(s + lp[t]), b, t, t == 9, kept) for t in range(vocab)]
+            grown.sort(key=lambda v: v[:3])
+            live = [(float(np.float32(-v)), live[b][1] + (t,), e, kept) for v, b, t, e, kept in grown[:beams]]
+        assert run.tokens[g * beams:(g + 1) * beams].tolist() == [list(l[1]) for l in live]
+        assert np.allclose(run.scores[g].cpu().numpy(), [l[0] for l in live], rtol=0, atol=1e-3)
+        stop = next((i + 1 for i, t in enumerate(live[0][1]) if t == 9), steps)
+        assert best[g][0] == list(live[0][1])[:stop]
+
+
+def test_a_failed_group_keeps_its_first_failure():
+    torch = _torch()
+    search = _beam().BeamSearch(3, 2, 50, 4)
+    x = _logits(6, 50, "f32", 1)
+    search.step(x)
+    x[2, 7] = float("nan")
+    search.step(x)
+    search.step(_logits(6, 50, "f32", 2))
+    assert search.status.tolist() == [0, S.TABBY_EDOMAIN, 0]
+    with pytest.raises(S.SamplingError, match="group 1: a logit or score"):
+        search.best()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("groups,beams,vocab,count", [
+    (1, 1, 262143, 64), (1, 2, 151936, 40), (2, 64, 9000, 128), (1, 16, 151936, 32), (3, 33, 8193, 17), (65, 4, 12289, 65),
+    (40, 8, 40961, 33), (260, 1, 4097, 128), (9, 2, 60000, 3)])
+def test_parts_waves_and_merges(groups, beams, vocab, count, dtype):
+    # Every shape of workgroup, of parts to a row (with the last one short) and of merge.
+    _check(_logits(groups * beams, vocab, dtype, vocab + count), _scores(groups, beams, count), count)
+
+
+@pytest.mark.parametrize("count", [7, 32, 33, 64, 65, 128])
+def test_ascending_rows_fill_the_lists(count):
+    # Every chunk lies above every bound that came before it: the lists overflow and the row is read again.
+    torch = _torch()
+    rows = []
+    for step in (1e-4, 3e-3):
+        rows += [np.arange(70000) * step, np.arange(70000) // 64 * step]
+    x = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda()
+    _check(x, _scores(2, 2, count), count)
+    _check(x.repeat(80, 1), _scores(160, 2, count), count)
+
+
+def test_equal_rows_score_alike():
+    # The sums do not hang on the order in which waves and workgroups end: equal rows tie to the last bit.
+    torch = _torch()
+    x = _logits(1, 100003, "f32", 9).repeat(320, 1)
+    s = np.full((40, 8), -1.0, dtype=np.float32)
+    got = _check(x, s, 16, ctx="equal rows")
+    assert (got.scores == got.scores[:1]).all() and (got.tokens == got.tokens[:1]).all()
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("beams", [7, 15, 31, 40, 63])
+def test_reorder_many_beams_of_wide_columns(beams, in_place):
+    _check_reorder((2 * beams, 2, 19, 128), 2, beams, in_place=in_place, lengths=[19, 6], seed=beams)
+    _check_reorder((2 * beams, 5, 24), 2, beams, "int8", in_place=in_place, seed=beams)
+    _check_reorder((2 * beams, 37), 2, beams, "int32", in_place=in_place, seed=beams)

@@ -307,3 +307,63 @@ def test_refusals():
     with pytest.raises(ValueError, match="codes must have shape"):
         mx4.Mx4Matrix.from_rowmajor(torch.zeros(4, 8, dtype=torch.uint8, device="cuda"),
                                     torch.zeros(4, 1, dtype=torch.uint8, device="cuda"), 32)
+
+
+@pytest.mark.parametrize("k", [96, 256, 300, 520, 1100])
+@pytest.mark.parametrize("rows,n,out", [(300, 6001, "bf16"), (1000, 12500, "f32"), (1000, 12501, "f16")])
+def test_product_in_tiles(rows, n, k, out):
+    # More tiles of 128 x 128 than half the units: the staged kernels, small tiles and large ones, over one to
+    # nine panels of k.
+    _check_product(rows, n, k, TYPES[k % 3], out, k == 300)
+
+
+@pytest.mark.parametrize("rows,n", [(300, 6001), (1000, 12501)])
+def test_exact_sums_in_tiles(rows, n):
+    # As test_exact_sums: multiples of 1/4 far below 2^24 leave nothing to round.
+    torch = _torch()
+    k = 1000
+    rng = np.random.default_rng(rows)
+    codes = rng.integers(0, 16, (rows, 32 * 32), dtype=np.uint8)
+    ones = np.full((rows, 32), 127, dtype=np.uint8)
+    x = _mx4().Mx4Matrix.from_rowmajor(torch.from_numpy(M.packed(codes)).cuda(), torch.from_numpy(ones).cuda(), k)
+    w, wv = _weights(n, k, 3, 127, 128)
+    got = _mx4().matmul(x, w).cpu().numpy().astype(np.float64)
+    assert np.array_equal(got, M.values(codes, ones, k) @ wv.T)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 333, 7680), (2, 70, 8200), (3, 5000, 7000), (16, 200, 1536), (17, 90, 1400), (32, 150, 700),
+                                      (40, 400, 500), (48, 77, 512), (64, 130, 384), (64, 130, 385)])
+def test_quantised_in_the_product(rows, n, k):
+    # The most rows and columns that the product's own launch quantises, and the next ones.
+    for dtype in TYPES:
+        _check_product(rows, n, k, dtype, "f32", False)
+
+
+def test_infinities_and_zeros_quantised_in_the_product():
+    torch = _torch()
+    x = torch.zeros(20, 300, device="cuda")
+    x[3] = torch.linspace(-4, 4, 300, device="cuda")
+    x[17, 299] = float("-inf")
+    w, wv = _weights(90, 300, 2)
+    got = _mx4().matmul(x, w).cpu().numpy()
+    assert np.isnan(got[17]).all()
+    rest = np.delete(np.arange(20), [3, 17])
+    assert (got[rest] == 0).all()
+    want = M.rounded(x[3:4].double().cpu().numpy()) @ wv.T
+    assert (np.abs(got[3] - want[0]) <= _bound(M.rounded(x[3:4].double().cpu().numpy()), wv, want, 300, "f32")).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 8200), (63, 129), (200, 70), (64, 128), (129, 1025)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_conversion_leaves_the_surroundings(rows, cols, dtype):
+    # Buffers with a margin on either side, at addresses that are aligned to an element only.
+    torch = _torch()
+    x, exact = _values(rows, cols, dtype, cols, spread=0.5)
+    m = _mx4().Mx4Matrix.quantize(x)
+    flat = torch.full((rows * (cols + 3) + 9,), 3.0, device="cuda", dtype=_dtype(dtype))
+    view = torch.as_strided(flat, (rows, cols), (cols + 3, 1), 5)
+    m.dequantize(out=view)
+    want = torch.from_numpy(M.rounded(exact)).to(_dtype(dtype))
+    assert torch.equal(view.cpu(), want)
+    view.fill_(3.0)
+    assert (flat == 3.0).all()
