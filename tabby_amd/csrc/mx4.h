@@ -91,11 +91,14 @@ __device__ __forceinline__ void decode_values(uint32_t word, uint32_t s, float *
   }
 }
 
-// 16 bytes of a row from column `col` on; zero past the last column.
-template <int DT>
+// 16 bytes of a row from column `col` on; zero past the last column. ONCE: nothing else reads them.
+template <int DT, bool ONCE>
 __device__ __forceinline__ u32x4 load_values(const typename Elem<DT>::Bits *row, int col, int cols) {
   using E = Elem<DT>;
-  if (col + E::kVec <= cols) return *reinterpret_cast<const u32x4_any *>(row + col);
+  if (col + E::kVec <= cols) {
+    const u32x4_any *from = reinterpret_cast<const u32x4_any *>(row + col);
+    return ONCE ? __builtin_nontemporal_load(from) : *from;
+  }
   u32x4 raw = {0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < E::kVec; ++j) {

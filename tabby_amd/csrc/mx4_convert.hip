@@ -20,8 +20,9 @@ constexpr unsigned kConvertGrid = 1u << 20;
 // Both directions take a workgroup to a panel and are bound by HBM. Memory is read and written along the
 // rows, 256 bytes (f16, bf16) or 512 at a time, 16 to a lane, and the codes change places in LDS, so that
 // either side moves whole lines; a lane that held a block of its own would touch a line in four separate
-// instructions. 151936 x 896 f16 there and back: 193 us that way, 142 so
-// (4.9 TB/s); 1531 x 4850 bf16, whose rows lie off 16-byte boundaries: 63 and 13.
+// instructions. What is read or written once bypasses the caches, but for stores that start off 16 bytes, whose
+// lines two lanes fill. 151936 x 896 f16 there and back: 102 us (6.8 TB/s); cached, 142; a block to a lane, 193.
+// 1531 x 4850 bf16, whose rows lie off 16 bytes: 14 us; a block to a lane, 63.
 template <int DT>
 struct PanelWalk {
   using E = Elem<DT>;
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
       const int row = row0 + walk.row + i * Walk::kRowStep;
-      raw[i] = row < rows ? load_values<DT>(x + (int64_t)row * stride, col, cols) : u32x4{0, 0, 0, 0};
+      raw[i] = row < rows ? load_values<DT, true>(x + (int64_t)row * stride, col, cols) : u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
@@ -76,7 +77,8 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
 }
 
 template <int DT>
-__global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix m, typename Elem<DT>::Bits *out, int64_t stride) {
+__global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix m, typename Elem<DT>::Bits *out, int64_t stride,
+                                                                       int whole) {
   using E = Elem<DT>;
   using Walk = PanelWalk<DT>;
   __shared__ __align__(16) uint8_t panel_codes[kMxPanelBytes];
@@ -109,7 +111,8 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix
           if constexpr (E::kVec == 4) u[j] = E::narrow(v[j]);
           else u[j] = (uint32_t)E::narrow(v[2 * j]) | ((uint32_t)E::narrow(v[2 * j + 1]) << 16);
         }
-        *reinterpret_cast<u32x4_any *>(to) = u;
+        if (whole) __builtin_nontemporal_store(u, reinterpret_cast<u32x4 *>(to));
+        else *reinterpret_cast<u32x4_any *>(to) = u;
       } else {
 #pragma unroll
         for (int j = 0; j < E::kVec; ++j)
@@ -176,8 +179,9 @@ int launch_quantize(const void *x, int rows, int cols, int64_t stride, uint8_t *
 
 template <int DT>
 int launch_dequantize(const Mx4Matrix &m, void *out, int64_t stride, hipStream_t s) {
+  const bool whole = (uintptr_t)out % 16 == 0 && stride % Elem<DT>::kVec == 0;
   hipLaunchKernelGGL(mx4_dequantize_kernel<DT>, convert_grid(m.rows, m.cols), dim3(kConvertBlock), 0, s, m,
-                     (typename Elem<DT>::Bits *)out, stride);
+                     (typename Elem<DT>::Bits *)out, stride, whole);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }

@@ -359,16 +359,18 @@ struct FloatTiles {
     using E = Elem<XDT>;
     constexpr int kBatch = 4, kBlockLanes = kMxBlock / E::kVec;
     const int row_lanes = kp * (kMxPanelCols / E::kVec), all = a.rows * row_lanes;
+    const float per_row = 1.0f / (float)row_lanes;  // all < 2^13: (i + 1/2) / row_lanes has bits to spare
+    auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * per_row); };
     for (int first = (int)threadIdx.x; first < all; first += kBatch * (int)blockDim.x) {
       u32x4 raw[kBatch];
 #pragma unroll
       for (int n = 0; n < kBatch; ++n) {
-        const int i = first + n * (int)blockDim.x, r = i / row_lanes, col = (i - r * row_lanes) * E::kVec;
-        raw[n] = i < all ? load_values<XDT>((const typename E::Bits *)a.x + (int64_t)r * a.stride, col, a.cols) : u32x4{0, 0, 0, 0};
+        const int i = first + n * (int)blockDim.x, r = row_of(i), col = (i - r * row_lanes) * E::kVec;
+        raw[n] = i < all ? load_values<XDT, false>((const typename E::Bits *)a.x + (int64_t)r * a.stride, col, a.cols) : u32x4{0, 0, 0, 0};
       }
 #pragma unroll
       for (int n = 0; n < kBatch; ++n) {
-        const int i = first + n * (int)blockDim.x, r = i / row_lanes, at = i - r * row_lanes, b = at / kBlockLanes;
+        const int i = first + n * (int)blockDim.x, r = row_of(i), at = i - r * row_lanes, b = at / kBlockLanes;
         if (i >= all) break;
         uint32_t word;
         const uint32_t s = encode_lane<XDT>(raw[n], word);
