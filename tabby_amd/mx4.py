@@ -68,16 +68,19 @@ def _current_handle(index):
     return torch.cuda.current_stream(index).cuda_stream
 
 
-# The current stream's handle without the object around it, which takes longer to make than a launch.
+# The current stream's handle without the object around it, which takes longer to make than a launch, and the
+# device without the check that a tensor's existence has passed.
 _current_handle = getattr(torch._C, "_cuda_getCurrentRawStream", _current_handle)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def call_on(device, stream):
     """(context, stream handle) of a call on ``device``: the device is made current where it is
     not, and what the call allocates belongs to its stream."""
     if stream is None:
-        if device.index == torch.cuda.current_device():
-            return _HERE, _current_handle(device.index)
+        index = device.index
+        if index == _current_device():
+            return _HERE, _current_handle(index)
         stream = torch.cuda.current_stream(device)
     elif stream.device != device:
         raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
@@ -111,10 +114,6 @@ class Mx4Matrix:
     def scales(self):
         return self.data[self._code_bytes:]
 
-    def _addresses(self):
-        at = self.data.data_ptr()
-        return at, at + self._code_bytes
-
     @classmethod
     def quantize(cls, x, out: Optional["Mx4Matrix"] = None, stream=None) -> "Mx4Matrix":
         """``x`` ([rows, cols] or [cols], float32, float16 or bfloat16) rounded to MXFP4: a block's
@@ -123,14 +122,17 @@ class Mx4Matrix:
         x = rows_of(x, "x")
         code = dtype_code(x.dtype)
         rows, cols = x.shape
-        ctx, handle = call_on(x.device, stream)
+        device = x.device
+        if out is not None:
+            if (out.rows, out.cols) != (rows, cols):
+                raise ValueError(f"out is {out.rows} x {out.cols}, x is {rows} x {cols}")
+            on_device(device, out.data)
+        ctx, handle = call_on(device, stream)
         with ctx:
-            m = cls(rows, cols, x.device) if out is None else out
-            if (m.rows, m.cols) != (rows, cols):
-                raise ValueError(f"out is {m.rows} x {m.cols}, x is {rows} x {cols}")
-            on_device(x.device, m.data)
+            m = cls(rows, cols, device) if out is None else out
+            at = m.data.data_ptr()
             _check(load_library().tabby_mx4_quantize_device(
-                x.data_ptr(), code, rows, cols, x.stride(0), *m._addresses(), handle))
+                x.data_ptr(), code, rows, cols, x.stride(0), at, at + m._code_bytes, handle))
         return m
 
     @classmethod
@@ -151,31 +153,40 @@ class Mx4Matrix:
         ctx, handle = call_on(codes.device, stream)
         with ctx:
             m = cls(int(codes.shape[0]), int(cols), codes.device)
+            at = m.data.data_ptr()
             _check(load_library().tabby_mx4_pack_device(
-                codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, *m._addresses(), handle))
+                codes.data_ptr(), scales.data_ptr(), m.rows, m.cols, at, at + m._code_bytes, handle))
         return m
 
     def dequantize(self, dtype=None, out=None, stream=None):
         """The values that the codes stand for, [rows, cols]: exact in float32 (the default) and
         bfloat16, rounded once in float16."""
+        rows, cols, device = self.rows, self.cols, self.data.device
         if out is None:
-            code = dtype_code(dtype or torch.float32)
+            dtype = dtype or torch.float32
+            code = dtype_code(dtype)
         else:
-            if dtype is not None and out.dtype != dtype:
-                raise ValueError(f"out is {out.dtype}, asked for {dtype}")
-            code = dtype_code(out.dtype)
+            code = _result_code(out, dtype, rows, cols, device)
             out = rows_of(out, "out")
-            if tuple(out.shape) != (self.rows, self.cols):
-                raise ValueError(f"out must have shape ({self.rows}, {self.cols}), got {tuple(out.shape)}")
-            on_device(self.data.device, out)
-        ctx, handle = call_on(self.data.device, stream)
+        ctx, handle = call_on(device, stream)
         with ctx:
             if out is None:
-                out = torch.empty((self.rows, self.cols), dtype=dtype or torch.float32, device=self.data.device)
+                out = torch.empty((rows, cols), dtype=dtype, device=device)
+            at = self.data.data_ptr()
             _check(load_library().tabby_mx4_dequantize_device(
-                *self._addresses(), self.rows, self.cols, out.data_ptr(), code,
-                out.stride(0), handle))
+                at, at + self._code_bytes, rows, cols, out.data_ptr(), code, out.stride(0), handle))
         return out
+
+
+def _result_code(out, dtype, rows: int, cols: int, device) -> int:
+    """The type code of a tensor that a caller has results written to, once it is seen to fit."""
+    if dtype is not None and out.dtype != dtype:
+        raise ValueError(f"out is {out.dtype}, asked for {dtype}")
+    code = dtype_code(out.dtype)
+    if tuple(rows_of(out, "out").shape) != (rows, cols):
+        raise ValueError(f"out must have shape ({rows}, {cols}), got {tuple(out.shape)}")
+    on_device(device, out)
+    return code
 
 
 def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
@@ -193,36 +204,36 @@ def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
     rows, k = (x.rows, x.cols) if quantized else x.shape
     if k != w.cols:
         raise ValueError(f"x has {k} columns, the weights {w.cols}")
+    n = w.rows
+    bias_at = None
     if bias is not None:
         on_device(device, bias)
-        if bias.dtype != torch.float32 or not bias.is_contiguous() or tuple(bias.shape) != (w.rows,):
-            raise ValueError(f"bias must be a contiguous float32 tensor of {w.rows} entries")
+        if bias.dtype != torch.float32 or not bias.is_contiguous() or tuple(bias.shape) != (n,):
+            raise ValueError(f"bias must be a contiguous float32 tensor of {n} entries")
+        bias_at = bias.data_ptr()
     if out is None:
         dtype = dtype or torch.float32
         code = dtype_code(dtype)
     else:
-        if dtype is not None and out.dtype != dtype:
-            raise ValueError(f"out is {out.dtype}, asked for {dtype}")
-        code = dtype_code(out.dtype)
+        code = _result_code(out, dtype, rows, n, device)
         out = rows_of(out, "out")
-        if tuple(out.shape) != (rows, w.rows):
-            raise ValueError(f"out must have shape ({rows}, {w.rows}), got {tuple(out.shape)}")
-        on_device(device, out)
     lib = load_library()
-    bias_ptr = bias.data_ptr() if bias is not None else None
+    w_at = w.data.data_ptr()
     ctx, handle = call_on(device, stream)
     with ctx:
         if out is None:
-            out = torch.empty((rows, w.rows), dtype=dtype, device=device)
+            out = torch.empty((rows, n), dtype=dtype, device=device)
         if quantized:
+            x_at = x.data.data_ptr()
             _check(lib.tabby_mx4_matmul_device(
-                *x._addresses(), rows, *w._addresses(), bias_ptr,
-                w.rows, k, out.data_ptr(), code, out.stride(0), handle))
+                x_at, x_at + x._code_bytes, rows, w_at, w_at + w._code_bytes, bias_at, n, k, out.data_ptr(), code,
+                out.stride(0), handle))
         else:
-            space = torch.empty(sum(sizes(rows, k)), dtype=torch.uint8, device=device)
+            size = sum(sizes(rows, k))
+            space = torch.empty(size, dtype=torch.uint8, device=device)
             _check(lib.tabby_mx4_linear_device(
-                x.data_ptr(), x_code, x.stride(0), rows, *w._addresses(), bias_ptr,
-                w.rows, k, out.data_ptr(), code, out.stride(0), space.data_ptr(), space.numel(), handle))
+                x.data_ptr(), x_code, x.stride(0), rows, w_at, w_at + w._code_bytes, bias_at, n, k, out.data_ptr(),
+                code, out.stride(0), space.data_ptr(), size, handle))
     return out
 
 
