@@ -91,7 +91,7 @@ __device__ __forceinline__ void decode_values(uint32_t word, uint32_t s, float *
   }
 }
 
-// 16 bytes of a row from column `col` on; zero past the last column. ONCE: nothing else reads them.
+// 16 bytes of a row from column `col` on; zero past the last column. ONCE: nothing else reads their line.
 template <int DT, bool ONCE>
 __device__ __forceinline__ u32x4 load_values(const typename Elem<DT>::Bits *row, int col, int cols) {
   using E = Elem<DT>;

@@ -20,9 +20,9 @@ constexpr unsigned kConvertGrid = 1u << 20;
 // Both directions take a workgroup to a panel and are bound by HBM. Memory is read and written along the
 // rows, 256 bytes (f16, bf16) or 512 at a time, 16 to a lane, and the codes change places in LDS, so that
 // either side moves whole lines; a lane that held a block of its own would touch a line in four separate
-// instructions. What is read or written once bypasses the caches, but for stores that start off 16 bytes, whose
-// lines two lanes fill. 151936 x 896 f16 there and back: 102 us (6.8 TB/s); cached, 142; a block to a lane, 193.
-// 1531 x 4850 bf16, whose rows lie off 16 bytes: 14 us; a block to a lane, 63.
+// instructions. What is read or written once bypasses the caches, but not where rows start off 16 bytes, whose
+// lines two loads or stores share. 151936 x 896 f16 there and back: 104 us (6.6 TB/s); cached, 142; a block to a lane, 193.
+// 1531 x 4850 bf16, whose rows lie off 16 bytes: 13 us; a block to a lane, 63.
 template <int DT>
 struct PanelWalk {
   using E = Elem<DT>;
@@ -41,7 +41,7 @@ struct PanelWalk {
   __device__ __forceinline__ int scale_byte(int r) const { return 4 * ((r & 15) + 16 * block()) + (r >> 4); }
 };
 
-template <int DT>
+template <int DT, bool WHOLE>
 __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typename Elem<DT>::Bits *x, int rows, int cols,
                                                                      int64_t stride, uint8_t *codes, uint8_t *scales) {
   using E = Elem<DT>;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
       const int row = row0 + walk.row + i * Walk::kRowStep;
-      raw[i] = row < rows ? load_values<DT, true>(x + (int64_t)row * stride, col, cols) : u32x4{0, 0, 0, 0};
+      raw[i] = row < rows ? load_values<DT, WHOLE>(x + (int64_t)row * stride, col, cols) : u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int i = 0; i < Walk::kSteps; ++i) {
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kConvertBlock) void mx4_quantize_kernel(const typen
 
 template <int DT>
 __global__ __launch_bounds__(kConvertBlock) void mx4_dequantize_kernel(Mx4Matrix m, typename Elem<DT>::Bits *out, int64_t stride,
-                                                                       int whole) {
+                                                                       bool whole) {
   using E = Elem<DT>;
   using Walk = PanelWalk<DT>;
   __shared__ __align__(16) uint8_t panel_codes[kMxPanelBytes];
@@ -169,19 +169,28 @@ dim3 convert_grid(int rows, int cols) {
   return dim3((unsigned)std::min<int64_t>(mx_panels(rows, kMxPanelRows) * mx_panels(cols, kMxPanelCols), kConvertGrid));
 }
 
+// Whether no two lanes share 16 bytes of memory.
+template <int DT>
+bool whole_rows(const void *rows, int64_t stride) {
+  return (uintptr_t)rows % 16 == 0 && stride % Elem<DT>::kVec == 0;
+}
+
 template <int DT>
 int launch_quantize(const void *x, int rows, int cols, int64_t stride, uint8_t *codes, uint8_t *scales, hipStream_t s) {
-  hipLaunchKernelGGL(mx4_quantize_kernel<DT>, convert_grid(rows, cols), dim3(kConvertBlock), 0, s,
-                     (const typename Elem<DT>::Bits *)x, rows, cols, stride, codes, scales);
+  const auto *from = (const typename Elem<DT>::Bits *)x;
+  const dim3 grid = convert_grid(rows, cols);
+  if (whole_rows<DT>(x, stride))
+    hipLaunchKernelGGL((mx4_quantize_kernel<DT, true>), grid, dim3(kConvertBlock), 0, s, from, rows, cols, stride, codes, scales);
+  else
+    hipLaunchKernelGGL((mx4_quantize_kernel<DT, false>), grid, dim3(kConvertBlock), 0, s, from, rows, cols, stride, codes, scales);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
 
 template <int DT>
 int launch_dequantize(const Mx4Matrix &m, void *out, int64_t stride, hipStream_t s) {
-  const bool whole = (uintptr_t)out % 16 == 0 && stride % Elem<DT>::kVec == 0;
   hipLaunchKernelGGL(mx4_dequantize_kernel<DT>, convert_grid(m.rows, m.cols), dim3(kConvertBlock), 0, s, m,
-                     (typename Elem<DT>::Bits *)out, stride, whole);
+                     (typename Elem<DT>::Bits *)out, stride, whole_rows<DT>(out, stride));
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
