@@ -367,3 +367,23 @@ def test_conversion_leaves_the_surroundings(rows, cols, dtype):
     assert torch.equal(view.cpu(), want)
     view.fill_(3.0)
     assert (flat == 3.0).all()
+
+
+def test_weights_past_32_bits():
+    # 4.6 GB of codes: the last rows' panels lie past 2^32 bytes.
+    torch = _torch()
+    mx4 = _mx4()
+    n, k = 280_001, 32768
+    x = torch.zeros((n, k), dtype=torch.bfloat16, device="cuda")
+    x[-1] = 1.0
+    x[-130, 5] = -3.0
+    w = mx4.Mx4Matrix.quantize(x)
+    assert w.codes.numel() > 2 ** 32
+    for rows in (1, 70, 300):
+        got = mx4.matmul(torch.full((rows, k), 0.5, dtype=torch.bfloat16, device="cuda"), w)
+        assert (got[:, -1] == k / 2).all() and (got[:, -130] == -1.5).all()
+        assert int((got != 0).sum()) == 2 * rows
+        del got
+    x.zero_()
+    w.dequantize(out=x)
+    assert (x[-1] == 1.0).all() and float(x[-130, 5]) == -3.0 and int((x[-200:] != 0).sum()) == k + 1
