@@ -302,8 +302,9 @@ struct FewShape {
   int waves, slices;  // of a workgroup; powers of two
 };
 constexpr int kSlicesMax = 8;
-constexpr int kSumsMax = 16;        // slices * NT: the upper half of the slices' sums lie in LDS, 4 KB to a tile of rows
-constexpr int kSumsLds = kSumsMax / 2 * 4096;
+constexpr int kSumsMax = 16;                   // slices * NT
+// The upper half of the slices' sums lie in LDS, 4 KB to a wave's tile of rows.
+__host__ __device__ constexpr int sums_bytes(int waves, int tiles) { return waves / 2 * tiles * 4096; }
 constexpr int kStepBytes = kMxTileBytes + 64;  // codes and scales of 16 rows, 128 columns
 constexpr int kFloatSteps = 60;                // of them in LDS, of X quantised in the workgroup
 constexpr int kFloatPanels = 192;              // a row's panels of k, over all rows: about a microsecond's work
@@ -314,7 +315,9 @@ struct HeldTiles {
   using Args = Mx4Matrix;
   static constexpr int kTiles = NT;
   static constexpr bool kFills = false;
-  static constexpr int kLds = kSumsLds;
+  static constexpr int kWavesMax = kSlicesMax;
+  // Four waves, or as many as there are slices.
+  static constexpr int kLds = std::max(sums_bytes(4, NT), sums_bytes(std::min(kSlicesMax, kSumsMax / NT), NT));
   struct Raw { u32x4 codes[NT]; uint32_t scales; };
   const uint8_t *codes, *scales;
   uint32_t shift;
@@ -351,7 +354,8 @@ struct FloatTiles {
   using Args = FloatRows;
   static constexpr int kTiles = NT;
   static constexpr bool kFills = true;
-  static constexpr int kLds = kFloatSteps * kStepBytes;
+  static constexpr int kWavesMax = NT <= 2 ? 16 : 8;
+  static constexpr int kLds = std::max(kFloatSteps * kStepBytes, sums_bytes(kWavesMax, NT));
   struct Raw {};
   const uint8_t *codes;
   __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int) : codes(lds) {}
@@ -396,9 +400,9 @@ struct FloatTiles {
 };
 
 template <int DT, typename Rows>
-__global__ __launch_bounds__(kSlicesMax * 64) void mx4_few_kernel(Mx4Product p, typename Rows::Args xs, FewShape shape) {
+__global__ __launch_bounds__(Rows::kWavesMax * 64) void mx4_few_kernel(Mx4Product p, typename Rows::Args xs, FewShape shape) {
   constexpr int NT = Rows::kTiles;
-  __shared__ __align__(16) uint8_t lds[Rows::kLds > kSumsLds ? Rows::kLds : kSumsLds];
+  __shared__ __align__(16) uint8_t lds[Rows::kLds];
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int slice = wave & (shape.slices - 1);
@@ -505,18 +509,24 @@ bool large_tiles(int n, int rows) {
   return 7 * mx_panels(large, kCus) <= 2 * mx_panels(small, kCus);
 }
 
-// The slices of k: enough waves to fill the chip, eight to a unit, while every one has a panel of k.
-FewShape few_shape(int64_t panels, int kp, int tiles, bool fills) {
+// The slices of k: enough waves to fill the chip, eight to a unit, while every one has a panel of k. A
+// workgroup that quantises X does so for eight waves, or sixteen where slices make that many workgroups
+// for most units (24 x 50257, k = 800 from f32: 12.3 us in eight, 10.1 in sixteen; 16 x 200000, k = 1024, a panel
+// of W to a wave: 21.0 and 24.5).
+template <typename Rows>
+FewShape few_shape(int64_t panels, int kp) {
   int slices = 1;
-  while (slices < kSlicesMax && slices * 2 <= kp && slices * 2 * tiles <= kSumsMax && panels * slices < 8 * kCus) slices *= 2;
-  return {fills ? kSlicesMax : std::max(slices, 4), slices};
+  while (slices < kSlicesMax && slices * 2 <= kp && slices * 2 * Rows::kTiles <= kSumsMax && panels * slices < 8 * kCus) slices *= 2;
+  if (!Rows::kFills) return {std::max(slices, 4), slices};
+  const bool wide = Rows::kWavesMax == 16 && slices > 1 && panels * slices >= 16 * (kCus * 3 / 4);
+  return {wide ? 16 : 8, slices};
 }
 
 template <int DT, typename Rows>
 int launch_few(const Mx4Product &p, const typename Rows::Args &xs, hipStream_t s) {
   constexpr int NT = Rows::kTiles;
   const int64_t panels = mx_panels(p.w.rows, kMxPanelRows), groups = mx_panels(p.x.rows, kMxTileRows * NT);
-  const FewShape shape = few_shape(panels * groups, p.w.col_panels(), NT, Rows::kFills);
+  const FewShape shape = few_shape<Rows>(panels * groups, p.w.col_panels());
   const int64_t blocks = mx_panels(panels, shape.waves / shape.slices);
   hipLaunchKernelGGL((mx4_few_kernel<DT, Rows>), dim3((unsigned)blocks, (unsigned)groups), dim3(64 * shape.waves), 0, s, p, xs, shape);
   TABBY_HIP_CHECK(hipGetLastError());

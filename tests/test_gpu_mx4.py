@@ -387,3 +387,10 @@ def test_weights_past_32_bits():
     x.zero_()
     w.dequantize(out=x)
     assert (x[-1] == 1.0).all() and float(x[-130, 5]) == -3.0 and int((x[-200:] != 0).sum()) == k + 1
+
+
+@pytest.mark.parametrize("rows,n,k", [(64, 1000, 256), (64, 1000, 384), (50, 517, 300), (48, 800, 512), (33, 1300, 640), (32, 900, 768),
+                                      (17, 51000, 1000), (24, 49999, 900), (9, 50000, 1500), (3, 52000, 7000)])
+def test_sums_of_every_panel_of_a_workgroup(rows, n, k):
+    # Slices of k are added up in LDS: each of a workgroup's panels of W, its last one too, has its place there.
+    _check_product(rows, n, k, TYPES[(rows + k) % 3], "f32", False)
