@@ -89,7 +89,8 @@ class BeamSelect:
         status_at = None if status is None else _int32(status, (groups,), "status", device)
         ctx, handle = call_on(device, stream)
         with ctx:
-            tokens, parents, kept = torch.empty((3, groups, count), dtype=torch.int32, device=device).unbind()
+            tokens, parents, kept = torch.empty_strided(
+                (3, groups, count), (groups * count, count, 1), dtype=torch.int32, device=device).unbind()
             at, size = tokens.data_ptr(), 4 * groups * count
             _check(load_library().tabby_beam_select_device(
                 x.data_ptr(), code, x.stride(0), groups, beams, vocab, scores.data_ptr(), allowed_at, done_at,

@@ -171,7 +171,7 @@ class Mx4Matrix:
         ctx, handle = call_on(device, stream)
         with ctx:
             if out is None:
-                out = torch.empty((rows, cols), dtype=dtype, device=device)
+                out = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
             at = self.data.data_ptr()
             _check(load_library().tabby_mx4_dequantize_device(
                 at, at + self._code_bytes, rows, cols, out.data_ptr(), code, out.stride(0), handle))
@@ -222,7 +222,7 @@ def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
     ctx, handle = call_on(device, stream)
     with ctx:
         if out is None:
-            out = torch.empty((rows, n), dtype=dtype, device=device)
+            out = torch.empty_strided((rows, n), (n, 1), dtype=dtype, device=device)
         if quantized:
             x_at = x.data.data_ptr()
             _check(lib.tabby_mx4_matmul_device(
