@@ -30,6 +30,7 @@ constexpr int kBeamsMax = 64;
 constexpr int kCountMax = 128;
 constexpr int kPartsMax = 32;
 constexpr int kVocabMax = 1 << 28;            // places in a row in 32 bits, with room
+constexpr int kRowsMax = (1 << 23) - 1;       // of 512 threads each
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
 constexpr int kChunk = 1024;                  // elements a wave takes at a time
 constexpr int kLane = kChunk / 64;            // of them to a lane
@@ -234,7 +235,9 @@ __device__ __forceinline__ int share_of(int lanes, uint32_t n) {
   return share;
 }
 
-// One workgroup of NW waves to a part of a row. HBM-bound: every element is read once.
+// One workgroup of NW waves to a part of a row, every element read once. Many rows are bound by the issue of
+// the 64-bit terms (16 operations an element) beside HBM: 512 rows of 151,936 f32 in 62 us, 5.0 TB/s; f16 in 55.
+// Few are bound by latency: the load, the bound, the list, the ranks (four rows in 19 parts each: 7.5 us).
 template <int DT, bool MASK, int NW>
 __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   using Reader = PartReader<DT, MASK>;
@@ -594,7 +597,8 @@ int check_beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count
   if (count < 1 || count > kCountMax)
     return record_failure(TABBY_EINVAL, "count must be between 1 and " + std::to_string(kCountMax) + ", got " + std::to_string(count));
   if (vocab > kVocabMax) return record_failure(TABBY_EINVAL, "vocab must be at most " + std::to_string(kVocabMax));
-  if ((int64_t)groups * beams > INT32_MAX / kPartsMax) return record_failure(TABBY_EINVAL, "groups x beams x " + std::to_string(kPartsMax) + " must fit 32 bits");
+  if ((int64_t)groups * beams > kRowsMax)
+    return record_failure(TABBY_EINVAL, "groups x beams must be at most " + std::to_string(kRowsMax) + ": a launch's threads must fit 32 bits");
   return TABBY_OK;
 }
 

@@ -155,13 +155,14 @@ __device__ __forceinline__ void unrolled(F f) {
 typedef __attribute__((address_space(3))) void LdsVoid;
 typedef const __attribute__((address_space(1))) void GlobalVoid;
 
-// Large products, bound by the matrix cores and the LDS that feeds them: 4096 x 16384, k = 8192 in 243 us,
-// 4.5 PFLOP/s. A workgroup of WM x WN waves has a tile of WM PM x WN PN panels of Y (64 x 64), PM x PN
-// to a wave, and takes a panel of k (128) at a time. The panels of a stage lie in LDS as they do in
-// memory, W's before X's, brought there without passing through registers, three stages in turn: one
-// is in the waves' registers, one is being read into them, one or two are on their way. Eight waves of
-// 128 x 64 read 96 KB of LDS to a stage's 512 multiplications, three quarters of its rate; four of 128 x 128
-// would read 64 but need every register for the sums, which the compiler then copies about.
+// Large products, bound by the matrix cores at the card's power limit and, for a tenth of the time, by the
+// stores of Y: 4096 x 16384, k = 8192 in 227 to 243 us, one card or another, 4.5 to 4.8 PFLOP/s (zeros 176 us; random
+// operands that stay in registers run at 7.3). A workgroup of WM x WN waves has a tile of WM PM x WN PN panels
+// of Y (64 x 64), PM x PN to a wave, and takes a panel of k (128) at a time. The panels of a stage lie in
+// LDS as they do in memory, W's before X's, brought there without passing through registers, three stages in
+// turn: one is in the waves' registers, one is being read into them, one or two are on their way. Eight waves
+// of 128 x 64 leave registers for the next operands; four of 128 x 128 would read a third less of LDS but need
+// every register for the sums, which the compiler then copies about (368 us).
 template <int PM, int PN, int WM, int WN>
 struct TileShape {
   static constexpr int kWaves = WM * WN;
