@@ -352,7 +352,9 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       }
     }
     largest = fmaxf(largest, top);
-    if (rise > -INFINITY) {
+    // A chunk whose terms are all below e^-50 of one adds nothing that 64 bits of the sum would show: masks that
+    // leave little cost no exponentials.
+    if (__ballot(top >= ref - 50.0f) && rise > -INFINITY) {
       const double at = (double)ref;
       double part_sum[2] = {0.0, 0.0};
 #pragma unroll
