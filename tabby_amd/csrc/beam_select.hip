@@ -323,15 +323,17 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
           mine += (uint32_t)__popcll(who);
         }
       }
-      if (lane == 0) *(volatile uint32_t *)&listed[wave] = mine;
+      // All lanes' entries before their count: a wave that sees the count reads them.
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      if (lane == 0) __hip_atomic_store(&listed[wave], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       // Now and then the count-th largest of all waves' last entries, 64 or 256, is a new bound.
       constexpr uint32_t kFew = 64 / NW, kMany = 256 / NW;
       const uint32_t span = a.count <= 32 ? kFew : kMany;
       if (before / span != mine / span && mine <= kOwn && c + NW < reader.chunks) {
         auto entry = [&](uint32_t i) {
-          const uint32_t w = i / span, n = min(*(volatile uint32_t *)&listed[w], kOwn);
-          const uint32_t back = i % span + 1;
-          return back <= n ? ((volatile uint32_t *)(list + w * kOwn + (n - back)))[1] : 0u;
+          const uint32_t w = i / span, back = i % span + 1;
+          const uint32_t n = min(__hip_atomic_load(&listed[w], __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP), kOwn);
+          return back <= n ? composite_key(list[w * kOwn + (n - back)]) : 0u;
         };
         if (span == kFew) {
           uint32_t v[1] = {entry(lane)};
@@ -379,7 +381,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     raw = next;
     if (c >= reader.chunks) break;
     reader.load(c + NW, next);
-    const uint32_t shared = *(volatile uint32_t *)&bound;
+    const uint32_t shared = __hip_atomic_load(&bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     reader.widen(raw, c, x);
     top = chunk_max();
     theta = max(theta, shared);
