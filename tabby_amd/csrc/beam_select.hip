@@ -90,7 +90,8 @@ __device__ __forceinline__ double exp_64(double d) {
   bits.y += __builtin_bit_cast(uint32x2, shifted).x << 20;
   return __builtin_bit_cast(double, bits);
 }
-// The same for any d <= 690: below -690 nothing is left that a sum of at least 1 would hold.
+// The same for any d <= 690, -inf too: below -690 nothing is left that a sum of at least 1 would hold. Above 690 the
+// exponent's field runs over, and the result, NaN included, has nothing to do with exp.
 __device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, -690.0)); }
 
 // The larger of two, NaN if either is: a chunk's maximum shows that it holds a NaN.
@@ -294,7 +295,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   uint32_t theta = max(bound_of<NW>(top == top ? key_of(top) : 0u, a.count, bounds), kNegInfKey + 1);
 
   double sum = 0.0;
-  float ref = 0.0f, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
+  float ref = -INFINITY, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
   uint64_t *const own = list + wave * kOwn;
   uint32_t mine = 0;  // entries in it
   auto raise = [&](uint32_t k) {
