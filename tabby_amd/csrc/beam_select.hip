@@ -295,7 +295,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   uint32_t theta = max(bound_of<NW>(top == top ? key_of(top) : 0u, a.count, bounds), kNegInfKey + 1);
 
   double sum = 0.0;
-  float ref = -INFINITY, rise = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref); x > rise asks for another ref
+  float ref = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref)
   uint64_t *const own = list + wave * kOwn;
   uint32_t mine = 0;  // entries in it
   auto raise = [&](uint32_t k) {
@@ -345,19 +345,19 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
         }
       }
     }
-    if (__ballot(top > rise)) {
-      // The first chunk with an element, or one far above: another reference.
+    if (__ballot(top - ref > 600.0f)) {
+      // The first chunk with an element, or one far above: another reference. (The difference is rounded near 600
+      // only; ref + 600 would be 1,024 above a ref of 2^33.)
       const float m = wave_max(top);
       if (m < INFINITY) {
         sum *= exp_or_none((double)ref - (double)m);
         ref = m;
-        rise = m + 600.0f;
       }
     }
     largest = fmaxf(largest, top);
     // A chunk whose terms are all below e^-50 of one adds nothing that 64 bits of the sum would show: masks that
     // leave little cost no exponentials.
-    if (__ballot(top >= ref - 50.0f) && rise > -INFINITY) {
+    if (__ballot(top >= ref - 50.0f) && ref > -INFINITY) {
       const double at = (double)ref;
       double part_sum[2] = {0.0, 0.0};
 #pragma unroll

@@ -74,6 +74,22 @@ def test_stretches_of_a_finite_fill(fill, dtype):
             _check(torch.from_numpy(x).to(_dtype(dtype)).cuda(), _scores(4, 2, vocab), 9, f"fill {fill}", copies)
 
 
+@pytest.mark.parametrize("vocab", [5000, 40000])
+def test_steps_that_f32_shows_coarsely(vocab):
+    # Between 2^33 and 2^34 neighbouring logits are 1,024 apart, above it more; between 2^30 and 2^33 less.
+    torch = _torch()
+    for base in (2.0 ** 31, 2.0 ** 32, 2.0 ** 33, 2.0 ** 34, 2.0 ** 60, -2.0 ** 33, -2.0 ** 34, -2.0 ** 60):
+        step = abs(base) * 2.0 ** -23
+        x = np.full((6, vocab), base)
+        for r, at in enumerate((0, 1023, 1024, vocab // 2, vocab - 1)):
+            x[r, at] += step if base > 0 else step / 2
+        x[5] += step * (np.arange(vocab) % 4)
+        x = x.astype(np.float32)
+        scores = np.array([[-1.0], [-2.0], [-3.0], [-4.0], [-5.0], [-6.0]], dtype=np.float32)
+        for copies in (1, 44):
+            _check(torch.from_numpy(x).cuda(), scores, 3, f"about {base}", copies)
+
+
 @pytest.mark.parametrize("gap", [1e-8, 1e-9])
 @pytest.mark.parametrize("vocab", [3001, 50257])
 def test_the_order_of_beams_hangs_on_sums_in_64_bits(vocab, gap):
