@@ -204,7 +204,8 @@ TABBY_API int tabby_sampler_sample_lmhead_q4_device(tabby_sampler *sampler, cons
  * encodeQuantMatmul (src/engine/forward.ts:732-770): values of 4 bits (e2m1: 0, 1/2, 1, 3/2,
  * 2, 3, 4, 6 and a sign) in blocks of 32 along a row, each block with a power of two as a
  * biased 8-bit exponent. A matrix [rows, cols] is held as two device arrays in this
- * library's panel layout; this call gives their sizes (both multiples of 256).
+ * library's panel layout; this call gives their sizes (both multiples of 256). What the calls
+ * below write must not overlap what they read (TABBY_EINVAL), but for the product's result on x.
  */
 TABBY_API int tabby_mx4_bytes(int32_t rows, int32_t cols, int64_t *code_bytes, int64_t *scale_bytes);
 /*
@@ -249,7 +250,8 @@ TABBY_API int tabby_mx4_matmul_device(const void *x_codes_dev, const void *x_sca
  * The same from activations as the lm_head finds them (src/engine/forward.ts:408-428): x_dev
  * [rows, k] of `x_dtype`, rows x_stride elements apart, is quantised to MXFP4 in the call. The
  * caller's workspace_dev (16-byte aligned) holds at least code_bytes + scale_bytes of
- * [rows, k]; calls that may overlap need a workspace each. Asynchronous on `stream`.
+ * [rows, k]; calls that may overlap need a workspace each. out_dev may lie on x_dev, in whole or
+ * in part: x is read before any of it is written. Asynchronous on `stream`.
  */
 TABBY_API int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64_t x_stride, int32_t rows,
                                       const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,

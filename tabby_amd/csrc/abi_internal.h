@@ -3,6 +3,7 @@
 #pragma once
 
 #include <hip/hip_runtime.h>
+#include <stdint.h>
 
 #include <string>
 
@@ -37,10 +38,33 @@ int handle_view(const tabby_sampler *h, HandleView *out);
 // hidden); TABBY_EINVAL with a message otherwise.
 int check_q4_shape(int32_t vocab, int32_t hidden, int32_t block);
 
+// Rows in memory: `rows` of `row_bytes` each, `stride` bytes apart.
+struct RowSpan {
+  const void *base;
+  int64_t rows, row_bytes, stride;
+  int64_t bytes() const { return (rows - 1) * stride + row_bytes; }
+};
+
+// Rows of `cols` elements of `size` bytes, `stride` elements apart. (One row has no stride, and what lies further
+// apart than an address space is as good as that.)
+inline RowSpan row_span(const void *base, int64_t rows, int64_t cols, int64_t stride, int64_t size) {
+  const int64_t far = INT64_MAX / (8 * (rows < 1 ? 1 : rows));
+  return {base, rows, cols * size, rows > 1 ? (stride < far ? stride : far) * size : 0};
+}
+
+// Whether `bytes` at `at` meet one of the rows.
+inline bool rows_meet(const RowSpan &s, const void *at, int64_t bytes) {
+  const int64_t from = (int64_t)(uintptr_t)at - (int64_t)(uintptr_t)s.base;
+  const int64_t row = from < s.row_bytes ? 0 : s.rows > 1 ? (from - s.row_bytes) / s.stride + 1 : 1;  // the first that ends after `at`
+  return row < s.rows && row * s.stride < from + bytes;
+}
+
 // MXFP4 matrices: the sizes a matrix may have, the pointers of one, and the conversion itself
 // (arguments checked by the caller).
 int check_mx4_shape(int32_t rows, int32_t cols);
 int check_mx4_operand(const void *codes, const void *scales);
+// What a call writes must not lie on what it reads: TABBY_EINVAL if the rows meet the matrix.
+int check_mx4_apart(const RowSpan &rows, const void *codes, const void *scales, int32_t m_rows, int32_t m_cols);
 int mx4_quantize(const void *x, int32_t dtype, int32_t rows, int32_t cols, int64_t stride, uint8_t *codes,
                  uint8_t *scales, hipStream_t s);
 

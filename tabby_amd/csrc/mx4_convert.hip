@@ -211,6 +211,13 @@ int check_mx4_operand(const void *codes, const void *scales) {
   return TABBY_OK;
 }
 
+int check_mx4_apart(const RowSpan &rows, const void *codes, const void *scales, int32_t m_rows, int32_t m_cols) {
+  const int64_t panels = mx_panels(m_rows, kMxPanelRows) * mx_panels(m_cols, kMxPanelCols);
+  if (rows_meet(rows, codes, panels * kMxPanelBytes) || rows_meet(rows, scales, panels * kMxPanelScales))
+    return record_failure(TABBY_EINVAL, "what a call writes must not overlap what it reads");
+  return TABBY_OK;
+}
+
 int mx4_quantize(const void *x, int32_t dtype, int32_t rows, int32_t cols, int64_t stride, uint8_t *codes,
                  uint8_t *scales, hipStream_t s) {
   switch (dtype) {
@@ -244,6 +251,8 @@ extern "C" int tabby_mx4_quantize_device(const void *x_dev, int32_t dtype, int32
   if (!known_dtype(dtype)) return record_failure(TABBY_EINVAL, "dtype must be TABBY_F32, TABBY_F16 or TABBY_BF16");
   if (rows > 1 && row_stride < cols) return record_failure(TABBY_EINVAL, "row_stride must be at least cols");
   if ((uintptr_t)x_dev % dtype_size(dtype) != 0) return record_failure(TABBY_EINVAL, "x must be aligned to its elements");
+  rc = check_mx4_apart(row_span(x_dev, rows, cols, row_stride, dtype_size(dtype)), codes_dev, scales_dev, rows, cols);
+  if (rc) return rc;
   return mx4_quantize(x_dev, dtype, rows, cols, row_stride, (uint8_t *)codes_dev, (uint8_t *)scales_dev,
                       (hipStream_t)stream);
 }
@@ -258,6 +267,8 @@ extern "C" int tabby_mx4_dequantize_device(const void *codes_dev, const void *sc
   if (!known_dtype(dtype)) return record_failure(TABBY_EINVAL, "dtype must be TABBY_F32, TABBY_F16 or TABBY_BF16");
   if (rows > 1 && row_stride < cols) return record_failure(TABBY_EINVAL, "row_stride must be at least cols");
   if ((uintptr_t)out_dev % dtype_size(dtype) != 0) return record_failure(TABBY_EINVAL, "out must be aligned to its elements");
+  rc = check_mx4_apart(row_span(out_dev, rows, cols, row_stride, dtype_size(dtype)), codes_dev, scales_dev, rows, cols);
+  if (rc) return rc;
   const Mx4Matrix m{(const uint8_t *)codes_dev, (const uint8_t *)scales_dev, rows, cols};
   const hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
@@ -273,6 +284,10 @@ extern "C" int tabby_mx4_pack_device(const void *row_codes_dev, const void *row_
   int rc = check_mx4_operand(codes_dev, scales_dev);
   if (rc) return rc;
   rc = check_mx4_shape(rows, cols);
+  if (rc) return rc;
+  const int64_t blocks = mx_panels(cols, kMxBlock);
+  rc = check_mx4_apart(row_span(row_codes_dev, 1, rows * blocks * (kMxBlock / 2), 0, 1), codes_dev, scales_dev, rows, cols);
+  if (!rc) rc = check_mx4_apart(row_span(row_scales_dev, 1, rows * blocks, 0, 1), codes_dev, scales_dev, rows, cols);
   if (rc) return rc;
   hipLaunchKernelGGL(mx4_pack_kernel, pack_grid(rows, cols), dim3(kConvertBlock), 0, (hipStream_t)stream,
                      (const uint8_t *)row_codes_dev, (const uint8_t *)row_scales_dev, rows, cols, (uint8_t *)codes_dev,

@@ -595,6 +595,15 @@ int check_output(const void *out, int32_t dtype, int32_t rows, int32_t n, int64_
   return TABBY_OK;
 }
 
+// The rows apart from the weights and the bias.
+int check_apart(const RowSpan &rows, const Mx4Product &p) {
+  const int rc = check_mx4_apart(rows, p.w.codes, p.w.scales, p.w.rows, p.w.cols);
+  if (rc) return rc;
+  if (p.bias && rows_meet(rows, p.bias, (int64_t)p.w.rows * (int64_t)sizeof(float)))
+    return record_failure(TABBY_EINVAL, "what a call writes must not overlap its bias");
+  return TABBY_OK;
+}
+
 }  // namespace
 }  // namespace tabby
 
@@ -613,6 +622,10 @@ extern "C" int tabby_mx4_matmul_device(const void *x_codes_dev, const void *x_sc
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
                      {(const uint8_t *)x_codes_dev, (const uint8_t *)x_scales_dev, rows, k},
                      bias_dev, out_dev, out_stride};
+  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
+  rc = check_apart(out, p);
+  if (!rc) rc = check_mx4_apart(out, x_codes_dev, x_scales_dev, rows, k);
+  if (rc) return rc;
   return product(p, out_dtype, (hipStream_t)stream);
 }
 
@@ -637,7 +650,17 @@ extern "C" int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64
   uint8_t *codes = (uint8_t *)workspace_dev, *scales = codes + code_bytes;
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
                      {codes, scales, rows, k}, bias_dev, out_dev, out_stride};
-  if (fills(rows, p.w.col_panels())) {
+  const RowSpan x = row_span(x_dev, rows, k, x_stride, dtype_size(x_dtype));
+  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
+  rc = check_apart(out, p);
+  if (!rc) rc = check_apart(row_span(workspace_dev, 1, code_bytes + scale_bytes, 0, 1), p);
+  if (rc) return rc;
+  if (rows_meet(out, workspace_dev, code_bytes + scale_bytes) || rows_meet(x, workspace_dev, code_bytes + scale_bytes))
+    return record_failure(TABBY_EINVAL, "workspace must not overlap x or out");
+  // A result that lies on x (a layer whose input and output share a buffer) is written after a launch that has read
+  // all of x; in the product's own launch some workgroups would read what others have written.
+  const bool apart = !rows_meet({out_dev, 1, out.bytes(), 0}, x_dev, x.bytes());
+  if (apart && fills(rows, p.w.col_panels())) {
     return linear(p, FloatRows{x_dev, x_stride, rows, k}, x_dtype, out_dtype, (hipStream_t)stream);
   }
   rc = mx4_quantize(x_dev, x_dtype, rows, k, x_stride, codes, scales, (hipStream_t)stream);

@@ -191,8 +191,8 @@ def _result_code(out, dtype, rows: int, cols: int, device) -> int:
 
 def matmul(x, w: Mx4Matrix, bias=None, dtype=None, out=None, stream=None):
     """x W^T (+ bias), [rows, w.rows] of ``dtype`` (float32 by default): ``x`` is an ``Mx4Matrix``
-    or a float tensor ([rows, k] or [k]), which is quantised in the call. Products of codes are
-    exact, their sums float32, rounded once to ``dtype``."""
+    or a float tensor ([rows, k] or [k]), which is quantised in the call and may share memory with
+    ``out``. Products of codes are exact, their sums float32, rounded once to ``dtype``."""
     device = w.data.device
     quantized = isinstance(x, Mx4Matrix)
     if not quantized:

@@ -394,3 +394,38 @@ def test_weights_past_32_bits():
 def test_sums_of_every_panel_of_a_workgroup(rows, n, k):
     # Slices of k are added up in LDS: each of a workgroup's panels of W, its last one too, has its place there.
     _check_product(rows, n, k, TYPES[(rows + k) % 3], "f32", False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k,n,at", [(1, 896, 896, 0), (8, 1024, 1024, 0), (24, 800, 800, 0), (64, 384, 384, 0), (16, 512, 700, 40),
+                                         (3, 700, 512, -90), (40, 2000, 2000, 0), (200, 300, 300, 0), (300, 6001, 6001, 0)])
+def test_result_on_its_own_input(rows, k, n, at, dtype):
+    # The product into the buffer that holds x: the same rows, or columns that lie across them. Whatever a row's
+    # workgroups write, all of them have read x before.
+    torch = _torch()
+    w, _ = _weights(n, k, n + at)
+    x, _ = _values(rows, k, dtype, rows + k)
+    want = _mx4().matmul(x, w, dtype=_dtype(dtype))
+    wide = torch.full((rows, max(k, n) + 2 * abs(at)), 3.0, device="cuda", dtype=_dtype(dtype))
+    for _ in range(3):
+        first = abs(at)
+        held = wide[:, first:first + k]
+        held.copy_(x)
+        got = _mx4().matmul(held, w, out=wide[:, first + at:first + at + n])
+        assert torch.equal(got, want)
+
+
+def test_result_beside_its_input_and_bias():
+    # Views of one buffer that share none of its elements.
+    torch = _torch()
+    w, _ = _weights(96, 160, 3)
+    x, _ = _values(9, 160, "f32", 4)
+    bias = torch.randn(96, device="cuda")
+    want = _mx4().matmul(x, w, bias=bias)
+    wide = torch.zeros((9, 160 + 96 + 96), device="cuda")
+    wide[:, :160] = x
+    wide[4, 256:] = bias
+    got = _mx4().matmul(wide[:, :160], w, bias=wide[4, 256:], out=wide[:, 160:256])
+    assert torch.equal(got, want) and torch.equal(wide[:, :160], x)
+    held = _mx4().Mx4Matrix.quantize(x)
+    assert torch.equal(_mx4().matmul(held, w, bias=wide[4, 256:], out=wide[:, 160:256]), want)

@@ -107,3 +107,26 @@ def test_beam_reorder_arguments(lib):
     _refused(lib, call(dst=(A, 4 * A)), "in place")
     _refused(lib, call(dst=(A + 4096, 4 * A)), "overlap")
     _refused(lib, call(groups=2 ** 20, segments=2 ** 20), "32 bits")
+
+
+def test_mx4_results_apart_from_operands(lib):
+    # 1 x 32 and 64 x 128: one panel, 4,096 bytes of codes and 256 of scales. B, C, ... lie 1 MiB apart.
+    B, C, D, E = (A * i for i in (2, 3, 4, 5))
+    q, d, p = lib.tabby_mx4_quantize_device, lib.tabby_mx4_dequantize_device, lib.tabby_mx4_pack_device
+    m, f = lib.tabby_mx4_matmul_device, lib.tabby_mx4_linear_device
+    _refused(lib, q(A, 0, 1, 32, 32, A, B, None), "overlap")
+    _refused(lib, q(A, 0, 1, 32, 32, A - 4080, B, None), "overlap")
+    _refused(lib, q(A, 0, 1, 32, 32, B, A + 124, None), "overlap")
+    _refused(lib, q(A, 0, 3, 32, 2 ** 20, A + 8 * 2 ** 20 + 112, 64 * A, None), "overlap")  # the last row
+    _refused(lib, d(A, B, 1, 32, A + 4092, 0, 32, None), "overlap")
+    _refused(lib, d(A, B, 1, 32, B, 0, 32, None), "overlap")
+    _refused(lib, p(A, B, 1, 32, A, C, None), "overlap")
+    _refused(lib, p(A, B, 1, 32, C, B, None), "overlap")
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, A, 0, 64, None), "overlap")
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, D + 252, 0, 64, None), "overlap")
+    _refused(lib, m(A, B, 1, C, D, E, 64, 128, E + 252, 0, 64, None), "overlap")
+    _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, C, 0, 64, E, 4352, None), "overlap")
+    _refused(lib, f(A, 0, 128, 1, C, D, B, 64, 128, B, 0, 64, E, 4352, None), "overlap")
+    _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, E + 4348, 0, 64, E, 4352, None), "workspace")
+    _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, B, 0, 64, A, 4352, None), "workspace")
+    _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, B, 0, 64, C, 4352, None), "overlap")
