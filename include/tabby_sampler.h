@@ -297,8 +297,9 @@ TABBY_API int tabby_beam_select_device(const void *logits_dev, int32_t dtype, in
  * each. In every segment the first lengths_dev[g] positions (NULL: all; held to
  * [0, capacity]) of row (g, b) of dst become those of row (g, parents_dev[g, b]) of src; the rest
  * of dst stays. parents_dev [groups, beams]; a row whose parent is not within [0, beams) stays
- * as it is. Every state's dst is its src (in place, any parents), or none is, and then they do
- * not overlap. beams 1..64. Asynchronous on `stream`; no scratch.
+ * as it is. Every state's dst is its src (in place, any parents), or none is; nothing that is
+ * written may overlap another state (TABBY_EINVAL), while states may lie side by side in one
+ * buffer. beams 1..64. Asynchronous on `stream`; no scratch.
  */
 TABBY_API int tabby_beam_reorder_device(const void *const *src_dev, void *const *dst_dev, int32_t states,
                                         int32_t groups, int32_t beams, int32_t segments, int64_t capacity,

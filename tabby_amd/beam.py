@@ -131,7 +131,8 @@ def reorder_states(states: Sequence, parents, lengths=None, out: Optional[Sequen
     (all, without ``lengths``); a row whose parent is outside the group (-1) stays. ``states`` are
     tensors of one shape and layout, [groups * beams, positions], [rows, positions, width] or
     [rows, segments, positions, width]; they are moved in place, or into ``out``, whose rest
-    stays. Returns the tensors written."""
+    stays. What is written must not overlap another of the tensors: a cache that layers share is
+    listed once. Returns the tensors written."""
     states = list(states)
     out = states if out is None else list(out)
     n = len(states)

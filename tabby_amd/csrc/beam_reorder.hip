@@ -14,6 +14,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <memory>
+#include <new>
 #include <string>
 
 #include "abi_internal.h"
@@ -109,6 +111,70 @@ int launch_reorder(ReorderArgs &a, int groups, int states, bool in_place, hipStr
   return launch_width<(BYTES < 4 ? BYTES : 4), 64>(a, groups, states, in_place, s);
 }
 
+// What one state takes of memory.
+struct StateShape {
+  int64_t rows, row_stride;
+  int64_t segments, segment_stride, segment;
+  int64_t extent() const { return (segments - 1) * segment_stride + segment; }  // of a row
+  int64_t span() const { return (rows - 1) * row_stride + extent(); }
+};
+
+// Whether a state and one `apart` bytes after it share any byte; apart < span. Rows do not interleave, and segments
+// do not, so that of either only the two nearest can meet.
+bool states_meet(const StateShape &s, int64_t apart) {
+  const int64_t row = s.rows > 1 ? apart / s.row_stride : 0;
+  for (int64_t r = row; r < std::min(row + 2, s.rows); ++r) {
+    const int64_t rest = std::abs(apart - r * s.row_stride);
+    const int64_t segment = s.segments > 1 ? rest / s.segment_stride : 0;
+    for (int64_t i = segment; i < std::min(segment + 2, s.segments); ++i)
+      if (std::abs(rest - i * s.segment_stride) < s.segment) return true;
+  }
+  return false;
+}
+
+struct StateAt {
+  int64_t address;
+  bool read_only;  // two of these may share memory
+};
+
+// Whether any two states share memory that one of them has written to. Sorts them.
+bool any_meet(StateAt *at, size_t n, const StateShape &s) {
+  const auto before = [](const StateAt &a, const StateAt &b) { return a.address < b.address; };
+  if (!std::is_sorted(at, at + n, before)) std::sort(at, at + n, before);
+  // Nearly always states lie one after another, or side by side within a row's stride (layers in one tensor).
+  const int64_t extent = s.extent(), span = s.span();
+  size_t first = 0, i = 1;  // `first`: of those side by side
+  for (; i < n; ++i) {
+    const int64_t from_first = at[i].address - at[first].address;
+    if (first + 1 == i ? from_first >= span : from_first / s.row_stride >= s.rows) first = i;
+    else if (s.rows < 2 || at[i].address - at[i - 1].address < extent || from_first + extent > s.row_stride) break;
+  }
+  if (i >= n) return false;
+  for (i = 0; i < n; ++i)
+    for (size_t j = i + 1; j < n && at[j].address - at[i].address < span; ++j)
+      if (!(at[i].read_only && at[j].read_only) && states_meet(s, at[j].address - at[i].address)) return true;
+  return false;
+}
+
+int check_states_apart(const void *const *src, void *const *dst, int states, bool in_place, const StateShape &s) {
+  const size_t n = (size_t)states * (in_place ? 1 : 2);
+  StateAt few[256];
+  std::unique_ptr<StateAt[]> many;
+  if (n > sizeof(few) / sizeof(few[0])) {
+    many.reset(new (std::nothrow) StateAt[n]);
+    if (!many) return record_failure(TABBY_EINVAL, "no memory to look at that many states");
+  }
+  StateAt *at = many ? many.get() : few;
+  for (int i = 0; i < states; ++i) {
+    at[i] = {(int64_t)(uintptr_t)dst[i], false};
+    if (!in_place) at[states + i] = {(int64_t)(uintptr_t)src[i], true};
+  }
+  if (any_meet(at, n, s))
+    return record_failure(TABBY_EINVAL, in_place ? "states moved in place must not overlap each other"
+                                                 : "destinations must not overlap sources or each other");
+  return TABBY_OK;
+}
+
 }  // namespace
 }  // namespace tabby
 
@@ -135,7 +201,6 @@ extern "C" int tabby_beam_reorder_device(const void *const *src_dev, void *const
   const int64_t rows = (int64_t)groups * beams;
   const int64_t last = (segments - 1) * segment_stride;  // where a row's last segment starts
   if (rows > 1 && row_stride < last + segment) return record_failure(TABBY_EINVAL, "rows must not overlap: row_stride is too small");
-  const int64_t span = (rows - 1) * row_stride + last + segment;
   // The widest column that every address is a multiple of.
   uint64_t bits = (uint64_t)unit_bytes | (rows > 1 ? (uint64_t)row_stride : 0) | (segments > 1 ? (uint64_t)segment_stride : 0);
   const bool in_place = src_dev[0] == dst_dev[0];
@@ -143,10 +208,12 @@ extern "C" int tabby_beam_reorder_device(const void *const *src_dev, void *const
     const char *from = (const char *)src_dev[i], *to = (const char *)dst_dev[i];
     if (!from || !to) return record_failure(TABBY_EINVAL, "null pointer");
     if ((from == to) != in_place) return record_failure(TABBY_EINVAL, "either every state or none is moved in place");
-    if (from != to && from < to + span && to < from + span)
-      return record_failure(TABBY_EINVAL, "a state's source and destination must be the same or not overlap");
     bits |= (uint64_t)(uintptr_t)from | (uint64_t)(uintptr_t)to;
   }
+  // The move reads and writes each state on its own: what two share would be moved twice, or half.
+  const int rc = check_states_apart(src_dev, dst_dev, states, in_place,
+                                    {rows, rows > 1 ? row_stride : 0, segments, segments > 1 ? segment_stride : 0, segment});
+  if (rc) return rc;
   const hipStream_t s = (hipStream_t)stream;
   for (int i0 = 0; i0 < states; i0 += kStatesPerLaunch) {
     const int n = std::min(kStatesPerLaunch, states - i0);

@@ -569,3 +569,54 @@ def test_reorder_many_beams_of_wide_columns(beams, in_place):
     _check_reorder((2 * beams, 2, 19, 128), 2, beams, in_place=in_place, lengths=[19, 6], seed=beams)
     _check_reorder((2 * beams, 5, 24), 2, beams, "int8", in_place=in_place, seed=beams)
     _check_reorder((2 * beams, 37), 2, beams, "int32", in_place=in_place, seed=beams)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_reorder_states_in_one_buffer(seed):
+    # Views of one buffer, side by side or across each other: refused if they share an element that is written, and
+    # moved like states of their own if not.
+    torch = _torch()
+    rng = np.random.default_rng(seed)
+    moved = refused = 0
+    for trial in range(60):
+        groups, beams = int(rng.integers(1, 3)), int(rng.integers(1, 4))
+        rows, segments, positions, width = groups * beams, int(rng.integers(1, 4)), int(rng.integers(1, 4)), int(rng.integers(1, 5))
+        segment = positions * width
+        segment_stride = segment * int(rng.integers(1, 4))
+        extent = (segments - 1) * segment_stride + segment
+        row_stride = extent + int(rng.choice([0, 0, segment, extent, 2 * extent]))
+        span = (rows - 1) * row_stride + extent
+        n, in_place = int(rng.integers(2, 5)), bool(rng.integers(0, 2))
+        step = int(rng.choice([segment, extent, row_stride, span]))
+        count = n if in_place else 2 * n
+        offsets = rng.permutation(count * 2)[:count] * step
+        if trial % 3 == 0:
+            offsets = offsets + rng.integers(-1, 2, count) * (rng.random(count) < 0.3)
+        offsets = offsets - offsets.min()
+        base = rng.integers(0, 30000, int(offsets.max()) + span + 8, dtype=np.int16)
+        shape, strides = (rows, segments, positions, width), (row_stride, segment_stride, width, 1)
+        at = np.zeros(shape, dtype=np.int64)
+        for axis, stride in enumerate(strides):
+            at += (np.arange(shape[axis]) * stride).reshape([-1 if i == axis else 1 for i in range(4)])
+        buffer = torch.from_numpy(base).cuda()
+        views = [torch.as_strided(buffer, shape, strides, int(o)) for o in offsets]
+        parents = rng.integers(-1, beams, (groups, beams)).astype(np.int32)
+        src, out = (views, None) if in_place else (views[:n], views[n:])
+        owners = np.zeros(base.size, dtype=np.int64)
+        for o in offsets if in_place else offsets[n:]:
+            owners[at + o] += 1
+        clash = (owners > 1).any() or (not in_place and any((owners[at + o] > 0).any() for o in offsets[:n]))
+        print(f"one buffer {shape} {strides} at {offsets.tolist()} in_place={in_place} clash={clash}", flush=True)
+        if clash:
+            refused += 1
+            with pytest.raises(S.SamplingError, match="overlap"):
+                _beam().reorder_states(src, torch.from_numpy(parents).cuda(), out=out)
+            continue
+        moved += 1
+        _beam().reorder_states(src, torch.from_numpy(parents).cuda(), out=out)
+        want = base.copy()
+        for i in range(n):
+            to = at + (offsets[i] if in_place else offsets[n + i])
+            want[to] = _moved(base[at + offsets[i]], base[to], parents, None, 2)
+        assert np.array_equal(buffer.cpu().numpy(), want)
+    assert moved > 5 and refused > 5

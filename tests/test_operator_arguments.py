@@ -130,3 +130,28 @@ def test_mx4_results_apart_from_operands(lib):
     _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, E + 4348, 0, 64, E, 4352, None), "workspace")
     _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, B, 0, 64, A, 4352, None), "workspace")
     _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, B, 0, 64, C, 4352, None), "overlap")
+
+
+def test_beam_reorder_states_apart(lib):
+    def call(src, dst=None, groups=2, beams=4, segments=2, capacity=16, unit=128, row=4096, segment=2048):
+        dst = src if dst is None else dst
+        n = len(src)
+        arr = ctypes.c_void_p * n
+        return lib.tabby_beam_reorder_device(arr(*src), arr(*dst), n, groups, beams, segments, capacity, unit, row, segment, A,
+                                             None, None)
+    span = 8 * 4096
+    far = [A * (i + 2) for i in range(200)]
+    for src, dst in (((A, A), None),                                      # a cache listed twice
+                     ((A, 2 * A, 3 * A, 2 * A), None),
+                     ((A, A + span - 16), None),
+                     ((2 * A + 4096, 2 * A), None),
+                     ((A, 2 * A), (3 * A, A)),                            # one's destination is another's source
+                     ((A, 2 * A), (3 * A, 2 * A + 2048)),
+                     ((A, 2 * A), (3 * A, 3 * A)),                        # two destinations
+                     (tuple(far) + (far[77],), None),
+                     (tuple(far), tuple(a + 200 * A for a in far[:-1]) + (far[3],))):
+        _refused(lib, call(src, dst), "overlap")
+    # Between the segments and rows of one another, but for one byte.
+    _refused(lib, call((A, A + 1023), segments=3, capacity=1024, unit=1, row=16384, segment=2048), "overlap")
+    _refused(lib, call((A, A + 16384 * 2 + 3 * 2048 - 1), segments=4, capacity=2048, unit=1, row=16384, segment=4096), "overlap")
+    _refused(lib, call((A, A + 63), beams=1, groups=1, segments=9, capacity=64, unit=1, segment=128, row=0), "overlap")
