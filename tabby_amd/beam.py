@@ -7,7 +7,8 @@ searched keeps ``beams`` sequences and their cache rows (src/engine/kvcache.ts:1
 holds ``groups`` of them, and row ``g * beams + b`` is beam ``b`` of group ``g``.
 
 Every call is asynchronous on the given stream (default: torch's current one) and checks its
-arguments before any GPU work.
+arguments before any GPU work; what reads back (``BeamSearch.finished``, ``best``) does so on the
+current one.
 """
 from __future__ import annotations
 
@@ -177,24 +178,30 @@ class BeamSearch:
         self.end_ids = torch.tensor(list(end_ids), dtype=torch.int32, device=device)
         self.length = 0
 
-    def step(self, logits, states: Sequence = (), lengths=None, allowed=None):
+    def step(self, logits, states: Sequence = (), lengths=None, allowed=None, stream=None):
         """One step from the beams' logits: chooses, moves ``states`` and the tokens to the surviving
         beams and appends the new tokens; returns them, int32 [groups * beams]."""
         if self.length >= self.max_tokens:
             raise ValueError(f"the search holds {self.max_tokens} tokens")
-        status = torch.empty_like(self.status)
-        choice = self.select(logits, self.scores, self.beams, allowed=allowed, done=self.done, pad_id=self.pad_id,
-                             status=status)
-        self.status = torch.where(self.status == 0, status, self.status)  # a group's first failure
-        if states:
-            reorder_states(states, choice.parents, lengths=lengths)
-        reorder_states([self.tokens], choice.parents)
-        reorder_states([self.done.view(-1, 1)], choice.parents)
-        new = torch.where(choice.tokens < 0, self.pad_id, choice.tokens)
-        self.tokens[:, self.length] = new.view(-1)
-        if self.end_ids.numel():
-            self.done |= torch.isin(new, self.end_ids).to(torch.int32)
-        self.scores = choice.scores.contiguous()
+        ctx, _ = call_on(self.scores.device, stream)
+        with ctx:
+            # What is replaced below may be an earlier stream's: it is not to be used again before this one is done.
+            here = torch.cuda.current_stream(self.scores.device)
+            self.scores.record_stream(here)
+            self.status.record_stream(here)
+            status = torch.empty_like(self.status)
+            choice = self.select(logits, self.scores, self.beams, allowed=allowed, done=self.done, pad_id=self.pad_id,
+                                 status=status)
+            self.status = torch.where(self.status == 0, status, self.status)  # a group's first failure
+            if states:
+                reorder_states(states, choice.parents, lengths=lengths)
+            reorder_states([self.tokens], choice.parents)
+            reorder_states([self.done.view(-1, 1)], choice.parents)
+            new = torch.where(choice.tokens < 0, self.pad_id, choice.tokens)
+            self.tokens[:, self.length] = new.view(-1)
+            if self.end_ids.numel():
+                self.done |= torch.isin(new, self.end_ids).to(torch.int32)
+            self.scores = choice.scores.contiguous()
         self.length += 1
         return new.view(-1)
 

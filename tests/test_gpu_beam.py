@@ -620,3 +620,27 @@ def test_reorder_states_in_one_buffer(seed):
             want[to] = _moved(base[at + offsets[i]], base[to], parents, None, 2)
         assert np.array_equal(buffer.cpu().numpy(), want)
     assert moved > 5 and refused > 5
+
+
+def test_a_search_on_another_stream():
+    # Step by step on the current stream and on one of its own, which ends while the current one is busy.
+    torch = _torch()
+    beam = _beam()
+    steps = [_logits(6, 4001, "f32", 40 + i) for i in range(5)]
+    plain, other = (beam.BeamSearch(2, 3, 4001, 5, end_ids=(7,)) for _ in range(2))
+    caches = [torch.arange(6, dtype=torch.int32, device="cuda")[:, None].repeat(1, 9) for _ in range(2)]
+    wanted = [plain.step(x, states=[caches[0]]).cpu() for x in steps]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(2_000_000_000)  # about a second
+    busy.record()
+    got = [other.step(x, states=[caches[1]], stream=side) for x in steps]
+    side.synchronize()
+    assert not busy.query()
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a.cpu(), b) for a, b in zip(got, wanted))
+    torch.cuda.synchronize()
+    assert torch.equal(caches[0], caches[1]) and torch.equal(plain.tokens, other.tokens)
+    assert torch.equal(plain.scores, other.scores) and torch.equal(plain.done, other.done)
+    assert plain.best() == other.best()
