@@ -209,17 +209,19 @@ class BeamSearch:
         """Whether every beam that has a score has ended (reads back)."""
         return bool(((self.done != 0) | (self.scores == float("-inf"))).all())
 
-    def best(self):
-        """Each group's best sequence and its score: a list of (token ids, score) (reads back)."""
+    def best(self, strict: bool = True):
+        """Each group's best sequence and its score: a list of (token ids, score) (reads back). A group that
+        failed raises its SamplingError, or is None in the list where not ``strict``."""
         status = self.status.tolist()
-        for g, code in enumerate(status):
-            if code in (TABBY_EEMPTY, TABBY_EDOMAIN):
+        failed = {g: code for g, code in enumerate(status) if code in (TABBY_EEMPTY, TABBY_EDOMAIN)}
+        if strict:
+            for g, code in failed.items():
                 raise SamplingError(code, f"group {g}: " + ("no continuation" if code == TABBY_EEMPTY else
                                                             "a logit or score is NaN or +inf"))
         tokens = self.tokens.view(self.groups, self.beams, -1)[:, 0, :self.length].tolist()
         ends = set(self.end_ids.tolist())
         out = []
-        for ids, score in zip(tokens, self.scores[:, 0].tolist()):
+        for g, (ids, score) in enumerate(zip(tokens, self.scores[:, 0].tolist())):
             stop = next((i + 1 for i, t in enumerate(ids) if t in ends), len(ids))
-            out.append((ids[:stop], score))
+            out.append(None if g in failed else (ids[:stop], score))
         return out

@@ -1,0 +1,24 @@
+"""BeamSearch's own state, without a GPU: what it reads back."""
+import pytest
+import torch
+
+from tabby_amd import beam
+from tabby_amd import sampler as S
+
+
+def _search(groups=3, beams=2):
+    run = beam.BeamSearch(groups, beams, 50, 4, end_ids=(9,), device="cpu")
+    run.length = 3
+    run.tokens[::beams] = torch.tensor([[1, 2, 3, 0], [4, 9, 0, 0], [5, 6, 7, 0]], dtype=torch.int32)[:groups]
+    run.scores[:, 0] = torch.tensor([-1.0, -2.0, -3.0])[:groups]
+    return run
+
+
+@pytest.mark.parametrize("code,text", [(S.TABBY_EEMPTY, "no continuation"), (S.TABBY_EDOMAIN, "NaN")])
+def test_the_other_groups_results_when_one_failed(code, text):
+    run = _search()
+    assert run.best() == [([1, 2, 3], -1.0), ([4, 9], -2.0), ([5, 6, 7], -3.0)] == run.best(strict=False)
+    run.status[1] = code
+    with pytest.raises(S.SamplingError, match=f"group 1: .*{text}"):
+        run.best()
+    assert run.best(strict=False) == [([1, 2, 3], -1.0), None, ([5, 6, 7], -3.0)]
