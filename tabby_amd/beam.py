@@ -180,11 +180,14 @@ class BeamSearch:
 
     def step(self, logits, states: Sequence = (), lengths=None, allowed=None, stream=None):
         """One step from the beams' logits: chooses, moves ``states`` and the tokens to the surviving
-        beams and appends the new tokens; returns them, int32 [groups * beams]."""
+        beams and appends the new tokens; returns them, int32 [groups * beams]. A step is not captured
+        into a graph, where it would stay the same step: ``BeamSelect`` and ``reorder_states`` are."""
         if self.length >= self.max_tokens:
             raise ValueError(f"the search holds {self.max_tokens} tokens")
         ctx, _ = call_on(self.scores.device, stream)
         with ctx:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("a step of a search cannot be captured: the next one has other scores and another place")
             # What is replaced below may be an earlier stream's: it is not to be used again before this one is done.
             here = torch.cuda.current_stream(self.scores.device)
             self.scores.record_stream(here)

@@ -22,3 +22,14 @@ def test_the_other_groups_results_when_one_failed(code, text):
     with pytest.raises(S.SamplingError, match=f"group 1: .*{text}"):
         run.best()
     assert run.best(strict=False) == [([1, 2, 3], -1.0), None, ([5, 6, 7], -3.0)]
+
+
+def test_a_step_is_not_captured(monkeypatch):
+    # A replay would read the scores of the step that was captured and write its tokens into the same column again.
+    import contextlib
+    run = _search()
+    monkeypatch.setattr(beam, "call_on", lambda device, stream: (contextlib.nullcontext(), 0))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError, match="captured"):
+        run.step(torch.zeros(6, 50))
+    assert run.length == 3

@@ -644,3 +644,24 @@ def test_a_search_on_another_stream():
     assert torch.equal(caches[0], caches[1]) and torch.equal(plain.tokens, other.tokens)
     assert torch.equal(plain.scores, other.scores) and torch.equal(plain.done, other.done)
     assert plain.best() == other.best()
+
+
+def test_a_search_refuses_to_be_captured():
+    torch = _torch()
+    x = [_logits(6, 900, "f32", 60 + i) for i in range(3)]
+    plain, run = (_beam().BeamSearch(2, 3, 900, 3) for _ in range(2))
+    run.step(x[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x[1] + 1.0
+        with pytest.raises(ValueError, match="captured"):
+            run.step(x[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, x[1] + 1.0)
+    run.step(x[1])
+    run.step(x[2])
+    for v in x:
+        plain.step(v)
+    assert torch.equal(run.tokens, plain.tokens) and torch.equal(run.scores, plain.scores)
