@@ -17,7 +17,7 @@ from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 
-from .mx4 import call_on, dtype_code, on_device, rows_of
+from .mx4 import INT32_MAX, call_on, dtype_code, on_device, rows_of
 from .sampler import SamplingError, TABBY_EDOMAIN, TABBY_EEMPTY, _check, load_library
 
 BEAMS_MAX = 64
@@ -56,6 +56,8 @@ class BeamSelect:
     overlap need an object each."""
 
     def __init__(self, vocab_max: int, groups_max: int = 1, beams_max: int = 4, count_max: int = 8, device="cuda"):
+        if max(groups_max, beams_max, vocab_max, count_max) > INT32_MAX:
+            raise ValueError("groups_max, beams_max, vocab_max and count_max must fit 32 bits")
         size = ctypes.c_int64()
         _check(load_library().tabby_beam_workspace(groups_max, beams_max, vocab_max, count_max, ctypes.byref(size)))
         self.vocab_max, self.groups_max = int(vocab_max), int(groups_max)
@@ -84,6 +86,8 @@ class BeamSelect:
                              f"{self.groups_max} x {self.beams_max} x {self.vocab_max}, {self.count_max}")
         if count < 1:
             raise ValueError(f"count must be between 1 and {self.count_max}, got {count}")
+        if pad_id > INT32_MAX:
+            raise ValueError(f"pad_id must fit 32 bits, got {pad_id}")
         on_device(device, scores, self.workspace)
         allowed_at = None if allowed is None else _int32(allowed, (rows, -(-vocab // 32)), "allowed", device)
         done_at = None if done is None else _int32(done, (groups, beams), "done", device)
@@ -124,6 +128,8 @@ def _geometry(states, rows: int, what: str):
     if (dims > 2 and width > 1 and strides[-1] != 1) or (capacity > 1 and strides[position] != width):
         raise ValueError(f"{what}: a segment's positions must lie one after another")
     segments = shape[1] if dims == 4 else 1
+    if segments > INT32_MAX or rows > INT32_MAX:
+        raise ValueError(f"{what}'s rows and segments must fit 32 bits, got {tuple(shape)}")
     return (segments, capacity, width * size, strides[0] * size, strides[1] * size if dims == 4 else 0), addresses
 
 

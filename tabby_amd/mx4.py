@@ -32,6 +32,9 @@ def dtype_code(dtype) -> int:
     return code
 
 
+INT32_MAX = 2 ** 31 - 1  # of the C entries' sizes; ctypes would take larger ones modulo 2^32
+
+
 def rows_of(x, what: str):
     """A CUDA tensor as rows: 1-D becomes one row; a row's elements must be adjacent."""
     if not x.is_cuda:
@@ -43,6 +46,8 @@ def rows_of(x, what: str):
     rows, cols = x.shape
     if rows < 1 or cols < 1:
         raise ValueError(f"{what} must not be empty, got {tuple(x.shape)}")
+    if rows > INT32_MAX or cols > INT32_MAX:
+        raise ValueError(f"{what}'s rows and columns must fit 32 bits, got {tuple(x.shape)}")
     row_stride, stride = x.stride()
     if (cols > 1 and stride != 1) or (rows > 1 and row_stride < cols):
         raise ValueError(f"{what} must hold its rows' elements adjacent and its rows apart")
@@ -92,6 +97,8 @@ def sizes(rows: int, cols: int):
     if rows < 2 ** 20 and cols < 2 ** 20 and rows > 0 and cols > 0:
         panels = -(-rows // PANEL_ROWS) * -(-cols // PANEL_COLS)
         return panels * 4096, panels * 256
+    if rows > INT32_MAX or cols > INT32_MAX:
+        raise ValueError(f"rows and columns must fit 32 bits, got {rows} x {cols}")
     code, scale = ctypes.c_int64(), ctypes.c_int64()
     _check(load_library().tabby_mx4_bytes(rows, cols, ctypes.byref(code), ctypes.byref(scale)))
     return code.value, scale.value

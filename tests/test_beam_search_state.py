@@ -1,4 +1,4 @@
-"""BeamSearch's own state, without a GPU: what it reads back."""
+"""BeamSearch's own state and the objects' sizes, without a GPU."""
 import pytest
 import torch
 
@@ -33,3 +33,15 @@ def test_a_step_is_not_captured(monkeypatch):
     with pytest.raises(ValueError, match="captured"):
         run.step(torch.zeros(6, 50))
     assert run.length == 3
+
+
+def test_sizes_past_32_bits_are_refused():
+    # The C entries take 32-bit sizes: what does not fit would be taken modulo 2^32.
+    from tabby_amd import mx4
+    for rows, cols in ((2 ** 32 + 1, 5), (5, 2 ** 32 + 1), (2 ** 31, 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            mx4.Mx4Matrix(rows, cols, device="cpu")
+    for sizes in ({"vocab_max": 2 ** 32 + 100}, {"vocab_max": 100, "groups_max": 2 ** 32 + 1},
+                  {"vocab_max": 100, "beams_max": 2 ** 32 + 4}, {"vocab_max": 100, "count_max": 2 ** 32 + 8}):
+        with pytest.raises(ValueError, match="32 bits"):
+            beam.BeamSelect(**sizes, device="cpu")

@@ -429,3 +429,25 @@ def test_result_beside_its_input_and_bias():
     assert torch.equal(got, want) and torch.equal(wide[:, :160], x)
     held = _mx4().Mx4Matrix.quantize(x)
     assert torch.equal(_mx4().matmul(held, w, bias=wide[4, 256:], out=wide[:, 160:256]), want)
+
+
+def test_tensors_past_32_bits_are_refused():
+    # More rows or columns than the C entries' 32-bit sizes hold, which would be taken modulo 2^32.
+    torch = _torch()
+    from tabby_amd import beam
+    mx4 = _mx4()
+    flat = torch.empty(2 ** 32 + 3, dtype=torch.float16, device="cuda")
+    for x in (flat.view(-1, 1), flat):
+        with pytest.raises(ValueError, match="32 bits"):
+            mx4.Mx4Matrix.quantize(x)
+    w, _ = _weights(4, 3, 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        mx4.matmul(flat.view(1, -1), w)
+    scores = torch.zeros((1, 1), device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.BeamSelect(vocab_max=3)(flat.view(1, -1), scores, 1)
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.BeamSelect(vocab_max=3)(flat[:3].view(1, -1), scores, 1, pad_id=2 ** 32)
+    parents = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        beam.reorder_states([flat.view(1, -1, 1, 1)], parents)
