@@ -24,6 +24,15 @@ BEAMS_MAX = 64
 COUNT_MAX = 128
 
 
+def _used_here(seen, device, handle, *tensors):
+    """Tells the allocator that an object's own tensors are used on the current stream (`handle`; once for each in
+    `seen`): the object may be dropped while the stream still works with them."""
+    if handle not in seen:
+        seen.add(handle)
+        for t in tensors:
+            t.record_stream(torch.cuda.current_stream(device))
+
+
 class BeamChoice(NamedTuple):
     """The continuations kept, best first, [groups, count] each; -1, -1 and -inf where there are
     fewer."""
@@ -64,6 +73,7 @@ class BeamSelect:
         self.beams_max, self.count_max = int(beams_max), int(count_max)
         self.workspace_bytes = size.value
         self.workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+        self._streams = set()
 
     def __call__(self, logits, scores, count: int, allowed=None, done=None, pad_id: int = 0, status=None,
                  stream=None) -> BeamChoice:
@@ -94,6 +104,7 @@ class BeamSelect:
         status_at = None if status is None else _int32(status, (groups,), "status", device)
         ctx, handle = call_on(device, stream)
         with ctx:
+            _used_here(self._streams, device, handle, self.workspace)
             tokens, parents, kept = torch.empty_strided(
                 (3, groups, count), (groups * count, count, 1), dtype=torch.int32, device=device).unbind()
             at, size = tokens.data_ptr(), 4 * groups * count
@@ -183,21 +194,25 @@ class BeamSearch:
         self.status = torch.zeros(groups, dtype=torch.int32, device=device)
         self.end_ids = torch.tensor(list(end_ids), dtype=torch.int32, device=device)
         self.length = 0
+        self._streams = set()
 
     def step(self, logits, states: Sequence = (), lengths=None, allowed=None, stream=None):
         """One step from the beams' logits: chooses, moves ``states`` and the tokens to the surviving
         beams and appends the new tokens; returns them, int32 [groups * beams]. A step is not captured
-        into a graph, where it would stay the same step: ``BeamSelect`` and ``reorder_states`` are."""
+        into a graph, where it would stay the same step: ``BeamSelect`` and ``reorder_states`` are. The
+        caller orders a stream's steps after those of another, and after the object's making."""
         if self.length >= self.max_tokens:
             raise ValueError(f"the search holds {self.max_tokens} tokens")
-        ctx, _ = call_on(self.scores.device, stream)
+        device = self.scores.device
+        ctx, handle = call_on(device, stream)
         with ctx:
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError("a step of a search cannot be captured: the next one has other scores and another place")
-            # What is replaced below may be an earlier stream's: it is not to be used again before this one is done.
-            here = torch.cuda.current_stream(self.scores.device)
+            # Scores and status are replaced below, and may be an earlier stream's.
+            here = torch.cuda.current_stream(device)
             self.scores.record_stream(here)
             self.status.record_stream(here)
+            _used_here(self._streams, device, handle, self.tokens, self.done, self.end_ids)
             status = torch.empty_like(self.status)
             choice = self.select(logits, self.scores, self.beams, allowed=allowed, done=self.done, pad_id=self.pad_id,
                                  status=status)

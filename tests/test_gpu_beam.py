@@ -665,3 +665,33 @@ def test_a_search_refuses_to_be_captured():
     for v in x:
         plain.step(v)
     assert torch.equal(run.tokens, plain.tokens) and torch.equal(run.scores, plain.scores)
+
+
+def test_an_object_dropped_while_another_stream_works():
+    # Its workspace and state are not handed out again before the stream that uses them is done.
+    torch = _torch()
+    beam = _beam()
+    side = torch.cuda.Stream()
+    x, s = _logits(6, 5000, "f32", 7), torch.from_numpy(_scores(2, 3, 1)).cuda()
+    want = beam.BeamSelect(5000, 2, 3, 4)(x, s, 4)
+    run = beam.BeamSearch(2, 3, 5000, 64)
+    wanted = run.step(x).cpu()
+    del run
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)  # about half a second
+    select, run = beam.BeamSelect(5000, 2, 3, 4), beam.BeamSearch(2, 3, 5000, 64)
+    side.wait_stream(torch.cuda.current_stream())  # the search's first contents
+    mine = [select.workspace, run.select.workspace, run.tokens, run.done, run.scores, run.status]
+    sizes, at = [t.numel() * t.element_size() for t in mine], {t.data_ptr() for t in mine}
+    del mine
+    got = select(x, s, 4, stream=side)
+    new = run.step(x, stream=side)
+    del select, run
+    others = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(3)]
+    assert not side.query()
+    assert not at & {t.data_ptr() for t in others}
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(new.cpu(), wanted)
