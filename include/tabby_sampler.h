@@ -270,18 +270,20 @@ TABBY_API int tabby_beam_workspace(int32_t groups, int32_t beams, int32_t vocab,
  * row_stride elements apart) holds the logits of beam b of group g, whose score so far is
  * scores_dev [groups, beams] (f32). A continuation by token t scores
  *   scores[g, b] + (x_t - log sum over the row's allowed entries of exp(x)),
- * in 64 bits. allowed_dev (may be NULL: everything) has ceil(vocab / 32) words to a row, entry t
+ * in 64 bits, the logarithm within 1e-10. allowed_dev (may be NULL: everything) has ceil(vocab / 32) words to a row, entry t
  * at bit t % 32 of word t / 32; what is not allowed is never looked at, NaN included.
  * done_dev [groups, beams] (may be NULL): a beam with a nonzero entry has ended, and its one
  * continuation is pad_id at its own score, whatever its logits hold. A beam whose score is
  * -inf has no continuations, nor has an entry of -inf or a row in which nothing is allowed.
  * The `count` (1..128) best of each group's beams (1..64), equal scores in the order of (beam,
- * token), go to tokens_dev, parents_dev (the beam within its group) and out_scores_dev, each
+ * token) -- of each beam only its first `count` entries by (logit, token) are looked at, which
+ * matters where 64 bits do not tell their scores apart -- go to tokens_dev, parents_dev (the beam within its group) and out_scores_dev, each
  * [groups, count]; where there are fewer the rest is -1, -1 and -inf. status_dev [groups] (may
  * be NULL) receives TABBY_OK, TABBY_EEMPTY (no continuation at all) or TABBY_EDOMAIN (an
  * allowed entry of a row that is read is NaN or +inf, or a score is NaN or +inf; the group's
- * outputs are as if it had none). workspace_dev: 16-byte aligned, of the size given above;
- * calls that may overlap need one each. Asynchronous on `stream`.
+ * outputs are as if it had none). The outputs lie apart from the inputs and from each other, but
+ * out_scores_dev may be scores_dev where count is beams. workspace_dev: 16-byte aligned, of the
+ * size given above; calls that may overlap need one each. Asynchronous on `stream`.
  */
 TABBY_API int tabby_beam_select_device(const void *logits_dev, int32_t dtype, int64_t row_stride, int32_t groups,
                                        int32_t beams, int32_t vocab, const float *scores_dev,

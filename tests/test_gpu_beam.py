@@ -695,3 +695,21 @@ def test_an_object_dropped_while_another_stream_works():
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert torch.equal(new.cpu(), wanted)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_written_over_the_ones_before(dtype):
+    # The C entry's promise where as many are kept as there are beams.
+    torch = _torch()
+    lib = S.load_library()
+    x, s = _logits(40 * 5, 3001, dtype, 12), torch.from_numpy(_scores(40, 5, 3)).cuda()
+    sel = _beam().BeamSelect(3001, 40, 5, 5)
+    want = sel(x, s, 5)
+    held = s.clone()
+    tokens, parents = (torch.empty((40, 5), dtype=torch.int32, device="cuda") for _ in range(2))
+    code = {"f32": S.TABBY_F32, "f16": S.TABBY_F16, "bf16": S.TABBY_BF16}[dtype]
+    rc = lib.tabby_beam_select_device(x.data_ptr(), code, x.stride(0), 40, 5, 3001, held.data_ptr(), None, None, 0, 5,
+                                      tokens.data_ptr(), parents.data_ptr(), held.data_ptr(), None, sel.workspace.data_ptr(),
+                                      sel.workspace_bytes, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert torch.equal(held, want.scores) and torch.equal(tokens, want.tokens) and torch.equal(parents, want.parents)
