@@ -8,7 +8,8 @@
 // Two kernels. The first reads the logits and leaves, for each row (or each part of one, where rows
 // are few), its largest logit M, the sum S of exp(x - M), and its first `count` entries by (logit,
 // index) -- adding s and subtracting the row's logarithm keeps their order, so no entry after those
-// can be among the group's. The second adds M, log S and s to each group's entries and takes the
+// can be among the group's (where rounding makes scores of one beam equal that its logits tell apart, the logits
+// have decided). The second adds M, log S and s to each group's entries and takes the
 // best. Sums and scores are in 64 bits: whether a continuation of one beam comes before another
 // beam's hangs on the difference of two logarithms.
 
@@ -71,7 +72,7 @@ typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
 
 // exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
 // and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]; for 2^f the
-// polynomial of degree 7 through it at the Chebyshev nodes, within 5e-11 of it. A sum of such terms
+// polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it. A sum of such terms
 // decides the order of two beams' continuations only where their scores are that close.
 __device__ __forceinline__ double exp_64(double d) {
   constexpr double kLog2e = 1.4426950408889634;
@@ -237,8 +238,10 @@ __device__ __forceinline__ int share_of(int lanes, uint32_t n) {
 }
 
 // One workgroup of NW waves to a part of a row, every element read once. Many rows are bound by the issue of
-// the 64-bit terms (16 operations an element) beside HBM: 512 rows of 151,936 f32 in 62 us, 5.0 TB/s; f16 in 55.
-// Few are bound by latency: the load, the bound, the list, the ranks (four rows in 19 parts each: 7.5 us).
+// the 64-bit terms (16 operations an element) and by HBM, which one wave does not overlap: it asks for its next
+// chunk before it looks at this one, but waits for it at the loop's end, and the unit's other waves cover that.
+// 512 rows of 151,936 f32 in 65 us, 4.8 TB/s; the whole call 66, from f16 63, from bf16 59. Few rows are bound by
+// latency: the load, the bound, the list, the ranks (four rows in 19 parts each: 7.7 us).
 template <int DT, bool MASK, int NW>
 __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   using Reader = PartReader<DT, MASK>;
@@ -355,8 +358,9 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       }
     }
     largest = fmaxf(largest, top);
-    // A chunk whose terms are all below e^-50 of one adds nothing that 64 bits of the sum would show: masks that
-    // leave little cost no exponentials.
+    // A chunk whose terms are all below e^-50 is left out: it would add 2e-22 an element to a sum of at least one,
+    // 3e-17 over 151,936 and 5e-14 over the longest row, less than the terms' own error. Masks that leave little
+    // cost no exponentials.
     if (__ballot(top >= ref - 50.0f) && ref > -INFINITY) {
       const double at = (double)ref;
       double part_sum[2] = {0.0, 0.0};
@@ -366,8 +370,8 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     }
   };
   // Two of these workgroups share a unit, and its waves issue the oldest first: the elder would end after 33 us
-  // of 54 and leave the other alone with half the waves. Whoever is further along yields instead: 512 rows
-  // of 151,936 f32 74 -> 67 us, f16 68 -> 61.
+  // of 54 and leave the other alone with half the waves. Whoever is further along yields instead: the whole call of
+  // 512 rows of 151,936 f32 74 -> 67 us, f16 68 -> 61.
   constexpr bool kYields = NW == 8;
   const int tenth = reader.chunks / 10, late[3] = {reader.chunks - tenth, reader.chunks - 3 * tenth, reader.chunks - 6 * tenth};
   if constexpr (kYields) __builtin_amdgcn_s_setprio(3);

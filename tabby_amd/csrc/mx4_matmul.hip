@@ -155,9 +155,11 @@ __device__ __forceinline__ void unrolled(F f) {
 typedef __attribute__((address_space(3))) void LdsVoid;
 typedef const __attribute__((address_space(1))) void GlobalVoid;
 
-// Large products, bound by the matrix cores at the card's power limit and, for a tenth of the time, by the
-// stores of Y: 4096 x 16384, k = 8192 in 227 to 243 us, one card or another, 4.5 to 4.8 PFLOP/s (zeros 176 us; random
-// operands that stay in registers run at 7.3). A workgroup of WM x WN waves has a tile of WM PM x WN PN panels
+// Large products: 4096 x 16384, k = 8192 in 227 to 243 us, one card or another, 4.5 to 4.8 PFLOP/s (random operands
+// that stay in registers run at 7.3). Bound by the schedule and the clock. The matrix cores are busy in 59 % of
+// 446,000 cycles; the rest is each step's wait for LDS and for the slowest wave, and a tenth the stores of Y. Zeros
+// take as many cycles (435,000) at 2.47 GHz, 176 us; random operands draw more power and the card runs them at 1.86.
+// A workgroup of WM x WN waves has a tile of WM PM x WN PN panels
 // of Y (64 x 64), PM x PN to a wave, and takes a panel of k (128) at a time. The panels of a stage lie in
 // LDS as they do in memory, W's before X's, brought there without passing through registers, three stages in
 // turn: one is in the waves' registers, one is being read into them, one or two are on their way. Eight waves
@@ -296,7 +298,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mx4_tile_kernel(Mx4Product p, 
 }
 
 // Few rows: W is streamed from memory straight into registers, a wave to a panel of 64 columns of Y and
-// NT tiles of 16 rows. Bound by HBM where W is large (1 x 151936, k = 896: 12 us, 5.9 TB/s); where it is
+// NT tiles of 16 rows. Bound by HBM where W is large (1 x 151936, k = 896: 13 us, 5.6 TB/s); where it is
 // small, by how long a wave takes for its share of k, so `slices` waves of the workgroup take a part of
 // k each and add up through LDS.
 struct FewShape {
@@ -439,7 +441,8 @@ __global__ __launch_bounds__(Rows::kWavesMax * 64) void mx4_few_kernel(Mx4Produc
       });
     });
   };
-  // Two steps ahead: 128 x 4864, k = 4096 in 8.2 us, one ahead in 9.7.
+  // Three steps in registers: 128 x 4864, k = 4096 in 8.2 us, with two in 9.7. (The compiled copies between them wait
+  // for the next step before the one after it is asked for: one is on its way during a step's products.)
   Step now, next, after;
   if (k < end) load(k, now);
   if (k + 1 < end) load(k + 1, next);
