@@ -22,7 +22,7 @@ constexpr unsigned kConvertGrid = 1u << 20;
 // either side moves whole lines; a lane that held a block of its own would touch a line in four separate
 // instructions. What is read or written once bypasses the caches, but not where rows start off 16 bytes, whose
 // lines two loads or stores share. 151936 x 896 f16 there and back: 104 us (6.6 TB/s); cached, 142; a block to a lane, 193.
-// 1531 x 4850 bf16, whose rows lie off 16 bytes: 13 us; a block to a lane, 63.
+// 1531 x 4850 bf16, whose rows lie off 16 bytes: 14 us; a block to a lane, 63.
 template <int DT>
 struct PanelWalk {
   using E = Elem<DT>;
