@@ -8,7 +8,8 @@
 // several children is fetched from memory once, its further reads close behind in the cache. Bound by
 // HBM: every surviving row read once, every moved row written once. Stores bypass the caches, which leaves
 // these to the parents' further reads: 48 states of [64, 2, 1024, 64] bf16, 16 groups of different lengths,
-// 136 to 142 us, one card or another (5.0 to 5.2 TB/s; through the caches 146); 12 beams of 24 states of [48, 2, 1024, 128], 98 us (6.7 TB/s; 130).
+// 136 to 142 us, one card or another (5.0 to 5.2 TB/s; through the caches 146); 12 beams of 24 states of
+// [48, 2, 1024, 128], 98 us (6.7 TB/s; 130).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
