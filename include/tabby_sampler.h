@@ -307,6 +307,64 @@ TABBY_API int tabby_beam_reorder_device(const void *const *src_dev, void *const 
                                         int32_t groups, int32_t beams, int32_t segments, int64_t capacity,
                                         int64_t unit_bytes, int64_t row_stride, int64_t segment_stride,
                                         const int32_t *parents_dev, const int32_t *lengths_dev, void *stream);
+/*
+ * 8-bit floating point (FP8: e4m3, largest value 448, no infinities) beside the int4 weights of the
+ * reference's encodeQuantMatmul (src/engine/forward.ts:732-770): a matrix [rows, cols] in blocks of
+ * `block_rows` x 128, each with an f32 that its codes are multiplied by. block_rows is 128 for weights
+ * and 1 for activations. A matrix is held as two device arrays in this library's panel layout;
+ * this call gives their sizes (both multiples of 256). What the calls below write must not overlap what they
+ * read (TABBY_EINVAL), but for the product's result on x.
+ */
+TABBY_API int tabby_fp8_bytes(int32_t rows, int32_t cols, int32_t block_rows, int64_t *code_bytes, int64_t *scale_bytes);
+/*
+ * x_dev [rows, cols] of `dtype` (TABBY_F32, TABBY_F16 or TABBY_BF16; rows row_stride elements
+ * apart) to FP8, as a loader would convert weights for encodeQuantMatmul
+ * (src/engine/forward.ts:732-770). A block's scale is the smallest power of two, 2^-126 or more, with
+ * max |x| <= 448 times it (1 for zeros); a value is divided by it and rounded to the nearest code (ties to the
+ * even one). A block that holds a NaN or an infinity is NaN as a whole. codes_dev is 16-byte
+ * aligned, scales_dev 4-byte. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_fp8_quantize_device(const void *x_dev, int32_t dtype, int32_t rows, int32_t cols,
+                                        int64_t row_stride, int32_t block_rows, void *codes_dev, void *scales_dev,
+                                        void *stream);
+/*
+ * The way back: out_dev [rows, cols] of `dtype` receives code times scale, as encodeQuantMatmul's
+ * shader expands its codes (src/engine/forward.ts:732-770): the f32 product (above f32's range: infinity), rounded
+ * to nearest even in f16 and bf16. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_fp8_dequantize_device(const void *codes_dev, const void *scales_dev, int32_t rows, int32_t cols,
+                                          int32_t block_rows, void *out_dev, int32_t dtype, int64_t row_stride,
+                                          void *stream);
+/*
+ * A checkpoint's FP8 weights, repacked once as the int4 ones are for encodeQuantMatmul
+ * (src/engine/forward.ts:732-770). Input: row_codes_dev [rows][cols] and block_scales_dev
+ * [ceil(rows / 128)][ceil(cols / 128)] f32, of any value. Output: a matrix with block_rows 128.
+ * Asynchronous on `stream`.
+ */
+TABBY_API int tabby_fp8_pack_device(const void *row_codes_dev, const float *block_scales_dev, int32_t rows, int32_t cols,
+                                    void *codes_dev, void *scales_dev, void *stream);
+/*
+ * The product that stands in encodeQuantMatmul's place (src/engine/forward.ts:732-770) where
+ * both sides are FP8: out_dev [rows, n] of `out_dtype` (rows out_stride elements apart) =
+ * x [rows, k] (block_rows 1) times the transpose of w [n, k] (block_rows 128), plus bias_dev [n] (f32, may be
+ * NULL). Products of codes are exact, their sums and the scales' application f32, rounded once to
+ * out_dtype. Asynchronous on `stream`; no scratch.
+ */
+TABBY_API int tabby_fp8_matmul_device(const void *x_codes_dev, const void *x_scales_dev, int32_t rows,
+                                      const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,
+                                      int32_t n, int32_t k, void *out_dev, int32_t out_dtype, int64_t out_stride,
+                                      void *stream);
+/*
+ * The same from activations as the lm_head finds them (src/engine/forward.ts:408-428): x_dev
+ * [rows, k] of `x_dtype`, rows x_stride elements apart, is quantised (block_rows 1) in the call. The
+ * caller's workspace_dev (16-byte aligned) holds at least code_bytes + scale_bytes of
+ * [rows, k]; calls that may overlap need a workspace each. out_dev may lie on x_dev, in whole or
+ * in part: x is read before any of it is written. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64_t x_stride, int32_t rows,
+                                      const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,
+                                      int32_t n, int32_t k, void *out_dev, int32_t out_dtype, int64_t out_stride,
+                                      void *workspace_dev, int64_t workspace_bytes, void *stream);
 /* Message of the calling thread's last failure ("" if none). */
 TABBY_API const char *tabby_last_error(void);
 

@@ -68,6 +68,14 @@ int check_mx4_apart(const RowSpan &rows, const void *codes, const void *scales, 
 int mx4_quantize(const void *x, int32_t dtype, int32_t rows, int32_t cols, int64_t stride, uint8_t *codes,
                  uint8_t *scales, hipStream_t s);
 
+// FP8 matrices, likewise; block_rows 1 or 128.
+int check_fp8_shape(int32_t rows, int32_t cols, int32_t block_rows);
+void fp8_sizes(int32_t rows, int32_t cols, int32_t block_rows, int64_t *code_bytes, int64_t *scale_bytes);
+int check_fp8_operand(const void *codes, const void *scales);
+int check_fp8_apart(const RowSpan &rows, const void *codes, const void *scales, int32_t m_rows, int32_t m_cols, int32_t block_rows);
+int fp8_quantize(const void *x, int32_t dtype, int32_t rows, int32_t cols, int64_t stride, int32_t block_rows, uint8_t *codes,
+                 float *scales, hipStream_t s);
+
 }  // namespace tabby
 
 #define TABBY_HIP_CHECK(expr)                                            \

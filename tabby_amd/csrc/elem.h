@@ -49,6 +49,25 @@ struct Elem<TABBY_BF16> {
   }
 };
 
+// 16 bytes of a row from column `col` on; zero past the last column. ONCE: nothing else reads their line.
+template <int DT, bool ONCE>
+__device__ __forceinline__ u32x4 load_values(const typename Elem<DT>::Bits *row, int col, int cols) {
+  using E = Elem<DT>;
+  if (col + E::kVec <= cols) {
+    const u32x4_any *from = reinterpret_cast<const u32x4_any *>(row + col);
+    return ONCE ? __builtin_nontemporal_load(from) : *from;
+  }
+  u32x4 raw = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < E::kVec; ++j) {
+    if (col + j < cols) {
+      if constexpr (E::kVec == 4) raw[j] = row[col + j];
+      else raw[j / 2] |= (uint32_t)row[col + j] << (16 * (j & 1));
+    }
+  }
+  return raw;
+}
+
 inline size_t dtype_size(int dtype) { return dtype == TABBY_F32 ? 4 : 2; }
 
 inline bool known_dtype(int dtype) { return dtype == TABBY_F32 || dtype == TABBY_F16 || dtype == TABBY_BF16; }

@@ -14,6 +14,7 @@
 #include "abi_internal.h"
 #include "elem.h"
 #include "mx4.h"
+#include "product_ops.h"
 #include "wave_ops.h"
 
 namespace tabby {
@@ -32,128 +33,8 @@ __device__ __forceinline__ f32x4 mx4_mfma(u32x4 w, u32x4 x, f32x4 acc, uint32_t 
 
 struct Mx4Product {
   Mx4Matrix w, x;
-  const float *bias;  // [n] or null
-  void *out;
-  int64_t out_stride;
+  ProductOut y;
 };
-
-// Four consecutive columns of one row of Y.
-template <int DT>
-__device__ __forceinline__ void store4(const Mx4Product &p, int row, int col, f32x4 v) {
-  using E = Elem<DT>;
-  using Bits = typename E::Bits;
-  const int n = p.w.rows;
-  if (row >= p.x.rows || col >= n) return;
-  if (p.bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += col + i < n ? p.bias[col + i] : 0.0f;
-  }
-  Bits *dst = (Bits *)p.out + (int64_t)row * p.out_stride + col;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < n) dst[i] = E::narrow(v[i]);
-}
-
-// Exchanges a's upper half of the wave with b's lower half, and a's odd quarters with b's even ones.
-__device__ __forceinline__ void swap_halves(uint32_t &a, uint32_t &b) {
-  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-  a = r[0];
-  b = r[1];
-}
-__device__ __forceinline__ void swap_quarters(uint32_t &a, uint32_t &b) {
-  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-  a = r[0];
-  b = r[1];
-}
-
-// A lane's 4 x 4 columns of one row of Y: tile t has columns col + 16 t + 4 q on, q the lane's quarter of
-// the wave. Inside the matrix the quarters exchange them, so that each stores 16 columns in a row: four
-// lanes fill whole lines, where 8 bytes here and there would be merged in the cache. Rows of odd strides are
-// stored as widely: the hardware takes any address (589 x 46311 f16, k = 1336: 53 us, element by element 72).
-template <int DT>
-__device__ __forceinline__ void store_panel(const Mx4Product &p, int row, int col, f32x4 t0, f32x4 t1, f32x4 t2, f32x4 t3) {
-  using E = Elem<DT>;
-  using Bits = typename E::Bits;
-  const int q = (int)(threadIdx.x & 63) >> 4;
-  if (col + kMxPanelRows > p.w.rows) {
-    store4<DT>(p, row, col + 4 * q, t0);
-    store4<DT>(p, row, col + 16 + 4 * q, t1);
-    store4<DT>(p, row, col + 32 + 4 * q, t2);
-    store4<DT>(p, row, col + 48 + 4 * q, t3);
-    return;
-  }
-  f32x4 v[4] = {t0, t1, t2, t3};
-  if (p.bias) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[t][i] += p.bias[col + 16 * t + 4 * q + i];
-    }
-  }
-  constexpr int kWords = (int)sizeof(Bits);  // 32-bit words of four columns
-  uint32_t u[4][kWords];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    if constexpr (kWords == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[t][i] = E::narrow(v[t][i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) u[t][i] = (uint32_t)E::narrow(v[t][2 * i]) | ((uint32_t)E::narrow(v[t][2 * i + 1]) << 16);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    swap_halves(u[0][i], u[2][i]);
-    swap_halves(u[1][i], u[3][i]);
-    swap_quarters(u[0][i], u[1][i]);
-    swap_quarters(u[2][i], u[3][i]);
-  }
-  if (row >= p.x.rows) return;
-  Bits *dst = (Bits *)p.out + (int64_t)row * p.out_stride + col + 16 * q;
-  if constexpr (kWords == 4) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) *reinterpret_cast<u32x4_any *>(dst + 4 * t) = u32x4{u[t][0], u[t][1], u[t][2], u[t][3]};
-  } else {
-    *reinterpret_cast<u32x4_any *>(dst) = u32x4{u[0][0], u[0][1], u[1][0], u[1][1]};
-    *reinterpret_cast<u32x4_any *>(dst + 8) = u32x4{u[2][0], u[2][1], u[3][0], u[3][1]};
-  }
-}
-
-// Where a workgroup's tile lies. Workgroups go to the eight dies in turn, so each die is given a run of
-// tiles that lie together: bands of eight tiles of X, along W, whose panels its cache then holds.
-struct TilePlace { int w, x; };
-__device__ __forceinline__ TilePlace tile_place(int id, int tiles_w, int tiles_x) {
-  constexpr int kDies = 8, kBand = 8;
-  const int total = tiles_w * tiles_x;
-  const int die = id % kDies, each = total / kDies, more = total % kDies;
-  const int at = die * each + min(die, more) + id / kDies;
-  const int band = at / (kBand * tiles_w);
-  const int in_band = at - band * kBand * tiles_w;
-  const int wide = min(kBand, tiles_x - band * kBand);
-  return {in_band / wide, band * kBand + in_band % wide};
-}
-
-// Waits until at most N of this wave's loads from memory are on their way and its reads of LDS are done,
-// then for the workgroup's other waves. The memory clobbers keep the compiler from moving reads over it.
-template <int N>
-__device__ __forceinline__ void wait_and_meet() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
-// A constant that a lambda's body can use in constant expressions.
-template <int V>
-struct Const { static constexpr int value = V; };
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void unrolled(F f) {
-  if constexpr (I < N) {
-    f(Const<I>{});
-    unrolled<N, I + 1>(f);
-  }
-}
-
-typedef __attribute__((address_space(3))) void LdsVoid;
-typedef const __attribute__((address_space(1))) void GlobalVoid;
 
 // Large products: 4096 x 16384, k = 8192 in 227 to 243 us, one card or another, 4.5 to 4.8 PFLOP/s (random operands
 // that stay in registers run at 7.3). Bound by the schedule and the clock. The matrix cores are busy in 59 % of
@@ -292,7 +173,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void mx4_tile_kernel(Mx4Product p, 
     for (int j = 0; j < kX; ++j) {
       const int row = (place.x * WN + wn) * PN * kMxPanelRows + j * kMxTileRows + (lane & 15);
       const int col = ((place.w * WM + wm) * PM + i) * kMxPanelRows;
-      store_panel<DT>(p, row, col, acc[i * 4][j], acc[i * 4 + 1][j], acc[i * 4 + 2][j], acc[i * 4 + 3][j]);
+      store_panel<DT>(p.y, row, col, acc[i * 4][j], acc[i * 4 + 1][j], acc[i * 4 + 2][j], acc[i * 4 + 3][j]);
     }
   }
 }
@@ -481,7 +362,7 @@ __global__ __launch_bounds__(Rows::kWavesMax * 64) void mx4_few_kernel(Mx4Produc
   if (!works || slice != 0) return;
 #pragma unroll
   for (int u = 0; u < NT; ++u)
-    store_panel<DT>(p, (tile + u) * kMxTileRows + (lane & 15), panel * kMxPanelRows, acc[0][u], acc[1][u], acc[2][u], acc[3][u]);
+    store_panel<DT>(p.y, (tile + u) * kMxTileRows + (lane & 15), panel * kMxPanelRows, acc[0][u], acc[1][u], acc[2][u], acc[3][u]);
 }
 
 constexpr int kCus = 256;             // an MI355X's compute units
@@ -590,19 +471,11 @@ int linear(const Mx4Product &p, const FloatRows &x, int x_dtype, int32_t out_dty
   }
 }
 
-int check_output(const void *out, int32_t dtype, int32_t rows, int32_t n, int64_t stride) {
-  if (!out) return record_failure(TABBY_EINVAL, "null pointer");
-  if (!known_dtype(dtype)) return record_failure(TABBY_EINVAL, "dtype must be TABBY_F32, TABBY_F16 or TABBY_BF16");
-  if (rows > 1 && stride < n) return record_failure(TABBY_EINVAL, "out_stride must be at least n");
-  if ((uintptr_t)out % dtype_size(dtype) != 0) return record_failure(TABBY_EINVAL, "out must be aligned to its elements");
-  return TABBY_OK;
-}
-
 // The rows apart from the weights and the bias.
 int check_apart(const RowSpan &rows, const Mx4Product &p) {
   const int rc = check_mx4_apart(rows, p.w.codes, p.w.scales, p.w.rows, p.w.cols);
   if (rc) return rc;
-  if (p.bias && rows_meet(rows, p.bias, (int64_t)p.w.rows * (int64_t)sizeof(float)))
+  if (p.y.bias && rows_meet(rows, p.y.bias, (int64_t)p.w.rows * (int64_t)sizeof(float)))
     return record_failure(TABBY_EINVAL, "what a call writes must not overlap its bias");
   return TABBY_OK;
 }
@@ -624,7 +497,7 @@ extern "C" int tabby_mx4_matmul_device(const void *x_codes_dev, const void *x_sc
   if (rc) return rc;
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
                      {(const uint8_t *)x_codes_dev, (const uint8_t *)x_scales_dev, rows, k},
-                     bias_dev, out_dev, out_stride};
+                     {rows, n, bias_dev, out_dev, out_stride}};
   const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
   rc = check_apart(out, p);
   if (!rc) rc = check_mx4_apart(out, x_codes_dev, x_scales_dev, rows, k);
@@ -652,7 +525,7 @@ extern "C" int tabby_mx4_linear_device(const void *x_dev, int32_t x_dtype, int64
     return record_failure(TABBY_EINVAL, "workspace must be 16-byte aligned and hold the quantised x (tabby_mx4_bytes)");
   uint8_t *codes = (uint8_t *)workspace_dev, *scales = codes + code_bytes;
   const Mx4Product p{{(const uint8_t *)w_codes_dev, (const uint8_t *)w_scales_dev, n, k},
-                     {codes, scales, rows, k}, bias_dev, out_dev, out_stride};
+                     {codes, scales, rows, k}, {rows, n, bias_dev, out_dev, out_stride}};
   const RowSpan x = row_span(x_dev, rows, k, x_stride, dtype_size(x_dtype));
   const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
   rc = check_apart(out, p);

@@ -53,6 +53,8 @@ EXPORTED_SYMBOLS = (
     "tabby_mx4_bytes", "tabby_mx4_quantize_device", "tabby_mx4_dequantize_device", "tabby_mx4_pack_device",
     "tabby_mx4_matmul_device", "tabby_mx4_linear_device", "tabby_beam_workspace", "tabby_beam_select_device",
     "tabby_beam_reorder_device",
+    "tabby_fp8_bytes", "tabby_fp8_quantize_device", "tabby_fp8_dequantize_device", "tabby_fp8_pack_device",
+    "tabby_fp8_matmul_device", "tabby_fp8_linear_device",
 )
 
 
@@ -103,7 +105,13 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     L.tabby_beam_workspace.argtypes = [i32, i32, i32, i32, pi64]
     L.tabby_beam_select_device.argtypes = [vp, i32, i64, i32, i32, i32, vp, vp, vp, i32, i32, vp, vp, vp, vp, vp, i64, vp]
     L.tabby_beam_reorder_device.argtypes = [vp, vp, i32, i32, i32, i32, i64, i64, i64, i64, vp, vp, vp]
-    for name in EXPORTED_SYMBOLS[-9:]:
+    L.tabby_fp8_bytes.argtypes = [i32, i32, i32, pi64, pi64]
+    L.tabby_fp8_quantize_device.argtypes = [vp, i32, i32, i32, i64, i32, vp, vp, vp]
+    L.tabby_fp8_dequantize_device.argtypes = [vp, vp, i32, i32, i32, vp, i32, i64, vp]
+    L.tabby_fp8_pack_device.argtypes = [vp, vp, i32, i32, vp, vp, vp]
+    L.tabby_fp8_matmul_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp]
+    L.tabby_fp8_linear_device.argtypes = [vp, i32, i64, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp, i64, vp]
+    for name in EXPORTED_SYMBOLS[EXPORTED_SYMBOLS.index("tabby_mx4_bytes"):]:
         getattr(L, name).restype = ctypes.c_int
     for name in ("tabby_sampler_create", "tabby_sampler_destroy", "tabby_sampler_sample_device",
                  "tabby_sampler_sample", "tabby_debug_exp", "tabby_debug_seq_sum",
