@@ -365,6 +365,45 @@ TABBY_API int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64_
                                       const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,
                                       int32_t n, int32_t k, void *out_dev, int32_t out_dtype, int64_t out_stride,
                                       void *workspace_dev, int64_t workspace_bytes, void *stream);
+/*
+ * Bytes of the workspace of the verification declared next, which stands where a decode step has
+ * drafted tokens to check in the place of sampleFromTopK's one token (src/engine/sampler.ts:147-212).
+ */
+TABBY_API int tabby_draft_workspace(int32_t requests, int32_t drafts_max, int32_t vocab, int64_t *bytes);
+/*
+ * Verification of drafted tokens, in the place of encodeSampling and sampleFromTopK
+ * (src/engine/forward.ts:522-601, src/engine/sampler.ts:147-212) where a smaller model, or a lookup,
+ * has proposed a request's next tokens. Request r's rows of logits_dev [rows, vocab] (`dtype`
+ * TABBY_F32, TABBY_F16 or TABBY_BF16, rows row_stride elements apart) are offsets_dev[r] to
+ * offsets_dev[r + 1] - 1 (NULL: drafts_max + 1 rows to each): row j after j of its drafted tokens. It has one
+ * drafted token less than rows, at most drafts_max (0..63); they, their uniforms (uniforms_dev, in [0, 1))
+ * and, with draft_logits_dev, the rows they were drawn from lie one request after another, [rows - requests]. Without
+ * draft_logits_dev (NULL) the tokens were certain. params_dev [requests] holds each request's
+ * settings, those of the target and of the draft, and the uniform of its last draw.
+ * P and Q are what sampleFromTopK draws from for a row of the target and of the draft: the first top_k
+ * entries by (logit, lower index), weights exp((x - max) / temperature), those up to and with the first at
+ * which their running sum reaches top_p of the total, divided by their sum; temperature <= 0: the first
+ * entry. A drafted token d is accepted while uniform * Q(d) < P(d), Q(d) being 1 where the tokens were certain and where
+ * temperature <= 0. The next token is drawn from max(P - Q, 0) at the first refusal (from P without d where d was
+ * certain), from the last row's P if there is none: the first token in the vocabulary's order at which the
+ * running sum exceeds params' uniform times the total.
+ * tokens_dev [requests, drafts_max + 1] receives the accepted tokens, the drawn one and -1s, accepted_dev
+ * [requests] how many were accepted, status_dev [requests] (may be NULL) TABBY_OK, TABBY_EINVAL
+ * (settings as tabby_sampler_sample_device refuses them, offsets that do not ascend within the rows, a
+ * drafted token outside the vocabulary) or TABBY_EDOMAIN (a row with a NaN, +inf or nothing above -inf);
+ * such a request's tokens are -1, none accepted. Rows after the first refusal do not matter.
+ * `flags`: TABBY_FLAG_FULL_VOCAB must be set if a request may have temperature > 0 and top_k 0, or above 128, with a
+ * vocabulary of more than 128 (such a request is refused without it). vocab is at most 2^24. What is written lies apart from
+ * what is read. workspace_dev: 16-byte aligned, of the size given above; calls that may overlap need one
+ * each. Asynchronous on `stream`.
+ */
+TABBY_API int tabby_draft_verify_device(const void *logits_dev, int32_t dtype, int64_t row_stride, int32_t rows,
+                                        const void *draft_logits_dev, int64_t draft_row_stride,
+                                        const int32_t *drafts_dev, const double *uniforms_dev,
+                                        const int32_t *offsets_dev, int32_t requests, int32_t drafts_max, int32_t vocab,
+                                        const tabby_row_params *params_dev, int32_t *tokens_dev, int32_t *accepted_dev,
+                                        int32_t *status_dev, void *workspace_dev, int64_t workspace_bytes,
+                                        uint32_t flags, void *stream);
 /* Message of the calling thread's last failure ("" if none). */
 TABBY_API const char *tabby_last_error(void);
 

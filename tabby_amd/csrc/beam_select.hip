@@ -23,6 +23,7 @@
 #include "block_ops.h"
 #include "device_math.h"
 #include "elem.h"
+#include "row_scan.h"
 
 namespace tabby {
 namespace {
@@ -30,13 +31,10 @@ namespace {
 constexpr int kBeamsMax = 64;
 constexpr int kCountMax = 128;
 constexpr int kPartsMax = 32;
-constexpr int kVocabMax = 1 << 28;            // places in a row in 32 bits, with room
 constexpr int kRowsMax = (1 << 23) - 1;       // of 512 threads each
 constexpr int kEntriesMax = 8192;             // a group's entries, all of them in LDS
-constexpr int kChunk = 1024;                  // elements a wave takes at a time
-constexpr int kLane = kChunk / 64;            // of them to a lane
-constexpr int kListMax = 4096;                // entries above the bound that LDS holds, a share to each wave
 static_assert(kBeamsMax * kCountMax <= kEntriesMax, "a group's entries");
+static_assert(kCountMax == kListCountMax, "what a list keeps");
 
 // What the first kernel leaves of a row's part, beside its entries.
 struct RowSum {
@@ -68,175 +66,6 @@ __device__ __forceinline__ bool beam_reads(const BeamArgs &a, int row) {
   return a.scores[row] > -INFINITY && !(a.done && a.done[row]);
 }
 
-typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
-
-// exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
-// and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]; for 2^f the
-// polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it. A sum of such terms
-// decides the order of two beams' continuations only where their scores are that close.
-__device__ __forceinline__ double exp_64(double d) {
-  constexpr double kLog2e = 1.4426950408889634;
-  const double magic = 6755399441055744.0;
-  const double shifted = __builtin_fma(d, kLog2e, magic);
-  const double f = __builtin_fma(d, kLog2e, -(shifted - magic));
-  double p = 1.530370102315244e-05;
-  p = __builtin_fma(p, f, 0.0001546972921563772);
-  p = __builtin_fma(p, f, 0.0013333478472326247);
-  p = __builtin_fma(p, f, 0.009618025613309008);
-  p = __builtin_fma(p, f, 0.055504109063275894);
-  p = __builtin_fma(p, f, 0.24022651213498245);
-  p = __builtin_fma(p, f, 0.6931471805568318);
-  p = __builtin_fma(p, f, 0.9999999999595618);
-  uint32x2 bits = __builtin_bit_cast(uint32x2, p);
-  bits.y += __builtin_bit_cast(uint32x2, shifted).x << 20;
-  return __builtin_bit_cast(double, bits);
-}
-// The same for any d <= 690, -inf too: below -690 nothing is left that a sum of at least 1 would hold. Above 690 the
-// exponent's field runs over, and the result, NaN included, has nothing to do with exp.
-__device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, -690.0)); }
-
-// The larger of two, NaN if either is: a chunk's maximum shows that it holds a NaN.
-__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
-// One part of one row, 16 bytes to a lane from the part's first element on, wherever it lies (the hardware
-// takes any address): which lane takes which element, and so the order of the sum, depends on its place in
-// the row alone, and rows that are equal score alike to the last bit.
-template <int DT, bool MASK>
-struct PartReader {
-  using E = Elem<DT>;
-  using Bits = typename E::Bits;
-  static constexpr int kLoads = kLane / E::kVec;
-  static constexpr int kLoad = 64 * E::kVec;  // elements of a load
-  struct Raw {
-    u32x4 v[kLoads];
-    uint32_t mask[MASK ? kLoads : 1];
-  };
-  const Bits *row;
-  const uint32_t *mask;
-  int begin, len, words, chunks;
-
-  __device__ __forceinline__ PartReader(const BeamArgs &a, int r, int begin_, int len_)
-      : row((const Bits *)a.logits + (int64_t)r * a.row_stride),
-        mask(MASK ? a.allowed + (int64_t)r * a.words : nullptr),
-        begin(begin_),
-        len(len_),
-        words(a.words),
-        chunks((len_ + kChunk - 1) / kChunk) {}
-
-  // The place in the part of the lane's first element of load u of chunk c.
-  __device__ __forceinline__ int position(int c, int u) const { return c * kChunk + u * kLoad + wave_lane() * E::kVec; }
-  __device__ __forceinline__ int element(int c, int i) const { return begin + position(c, i / E::kVec) + i % E::kVec; }
-
-  // Past the last chunk it is the last one again, which nothing looks at.
-  __device__ __forceinline__ void load(int c, Raw &r) const {
-    c = min(c, chunks - 1);
-    const Bits *from = row + begin + c * kChunk;
-    const int lane = wave_lane() * E::kVec;
-    if ((c + 1) * kChunk <= len) {
-#pragma unroll
-      for (int u = 0; u < kLoads; ++u) r.v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any *>(from + lane + u * kLoad));
-    } else {
-#pragma unroll
-      for (int u = 0; u < kLoads; ++u) {
-        const int left = len - position(c, u);
-        r.v[u] = u32x4{0, 0, 0, 0};
-        if (left >= E::kVec) {
-          r.v[u] = *reinterpret_cast<const u32x4_any *>(from + lane + u * kLoad);
-        } else {
-#pragma unroll
-          for (int j = 0; j < E::kVec - 1; ++j) {
-            if (j < left) {
-              const uint32_t b = from[lane + u * kLoad + j];
-              if constexpr (E::kVec == 4) r.v[u][j] = b;
-              else r.v[u][j / 2] |= b << (16 * (j & 1));
-            }
-          }
-        }
-      }
-    }
-    if constexpr (MASK) {
-#pragma unroll
-      for (int u = 0; u < kLoads; ++u) r.mask[u] = mask[min((begin + position(c, u)) >> 5, words - 1)];
-    }
-  }
-
-  __device__ __forceinline__ void widen(const Raw &r, int c, float (&x)[kLane]) const {
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      float w[E::kVec];
-      E::widen16(r.v[u], w);
-      uint32_t bits = 0;  // parts begin on a word of the mask, and a load lies within one
-      if constexpr (MASK) bits = r.mask[u] >> ((uint32_t)position(c, u) & 31u);
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) x[u * E::kVec + j] = !MASK || (bits >> j) & 1u ? w[j] : -INFINITY;
-    }
-    if (c == chunks - 1) {
-#pragma unroll
-      for (int i = 0; i < kLane; ++i)
-        if (position(c, i / E::kVec) + i % E::kVec >= len) x[i] = -INFINITY;
-    }
-  }
-};
-
-// The k-th largest of the wave's 64 R values, k up to 64 (R = 1) or 128.
-template <int R>
-__device__ __forceinline__ uint32_t kth_largest(uint32_t (&v)[R], int k) {
-  wave_sort_desc<R>(v);
-  if constexpr (R == 1) return (uint32_t)__builtin_amdgcn_readlane((int)v[0], k - 1);
-  else return (uint32_t)__builtin_amdgcn_readlane((int)(k > 64 ? v[1] : v[0]), (k - 1) & 63);
-}
-
-// The number of set lanes before this one.
-__device__ __forceinline__ uint32_t lanes_before(uint64_t who) {
-  return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-}
-
-// A lower bound of the count-th largest of the keys that the workgroup's lanes hold, one each: the keys fall
-// into 64 columns (256 where more than 32 are kept), and the count-th largest of the columns' largest has
-// as many keys at or above it. Close to the count-th largest itself where the keys fall by chance; each
-// wave's are turned by another angle so that an order among them matters less.
-template <int NW>
-struct BoundScratch {
-  uint32_t keys[NW * 64];
-  uint32_t bound;
-};
-
-template <int NW>
-__device__ __forceinline__ uint32_t bound_of(uint32_t key, int count, BoundScratch<NW> &s) {
-  const int lane = wave_lane(), wave = (int)threadIdx.x >> 6;
-  s.keys[wave * 64 + ((lane + 5 * wave) & 63)] = key;
-  __syncthreads();
-  if (wave == 0) {
-    uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < NW; ++w) v[w & 3] = max(v[w & 3], s.keys[w * 64 + lane]);
-    uint32_t all[1] = {max(max(v[0], v[1]), max(v[2], v[3]))};
-    const uint32_t k = count <= 32 ? kth_largest<1>(all, count) : kth_largest<4>(v, count);
-    if (lane == 0) s.bound = k;
-  }
-  __syncthreads();
-  return s.bound;
-}
-
-// How many of the n things come before thing c, counted by `share` neighbouring lanes (a power of two up to
-// 64), every one of which returns it.
-template <class Before>
-__device__ __forceinline__ uint32_t rank_of(int share, uint32_t n, Before before) {
-  uint32_t rank = 0;
-#pragma unroll 4
-  for (uint32_t j = threadIdx.x & (share - 1); j < n; j += share) rank += before(j) ? 1u : 0u;
-#pragma unroll
-  for (int stride = 1; stride < 64; stride *= 2)
-    if (stride < share) rank += xor_lane_by(rank, stride);
-  return rank;
-}
-// The lanes to a thing where `lanes` of them rank n.
-__device__ __forceinline__ int share_of(int lanes, uint32_t n) {
-  int share = 1;
-  while (share < 64 && n * share * 2 <= (uint32_t)lanes) share *= 2;
-  return share;
-}
-
 // One workgroup of NW waves to a part of a row, every element read once. Many rows are bound by the issue of
 // the 64-bit terms (16 operations an element) and by HBM, which one wave does not overlap: it asks for its next
 // chunk before it looks at this one, but waits for it at the loop's end, and the unit's other waves cover that.
@@ -246,23 +75,15 @@ template <int DT, bool MASK, int NW>
 __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   using Reader = PartReader<DT, MASK>;
   constexpr int kBlockN = NW * 64;
-  __shared__ BlockScratchT<NW> scratch;
-  constexpr uint32_t kOwn = kListMax / NW;
-  static_assert(kOwn >= kCountMax, "a full share holds as many as are kept");
-  __shared__ __align__(8) uint32_t hist[kBins];
-  __shared__ uint64_t list[kListMax];
-  __shared__ uint32_t listed[NW];  // entries of each wave, those past its share too
-  __shared__ BoundScratch<NW> bounds;
-  __shared__ uint32_t held, bad, bound;
+  __shared__ ListScratch<NW> scratch;
   __shared__ double wave_sum_[NW];
   __shared__ float wave_ref[NW], wave_max_[NW];
-  uint64_t *const packed = reinterpret_cast<uint64_t *>(hist);
-  static_assert(kBins * sizeof(uint32_t) >= kBlockN * sizeof(uint64_t), "the entries that are ranked");
   const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - row * a.parts;
   const int t = (int)threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int begin = part * a.part_len, len = min(a.part_len, a.vocab - begin);
-  const Reader reader(a, row, begin, len);
+  const uint32_t *const mask = a.allowed ? a.allowed + (int64_t)row * a.words : nullptr;
+  const Reader reader((const typename Reader::Bits *)a.logits + (int64_t)row * a.row_stride, MASK ? mask : nullptr, a.words, begin, len);
   typename Reader::Raw raw, next;
   float x[kLane];
   int c = wave;
@@ -273,81 +94,21 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, 0, 0};
     return;
   }
-  if (t < NW) listed[t] = 0;
-  if (t == 0) {
-    held = 0;
-    bad = 0;
-    bound = kNegInfKey + 1;
-  }
-  auto chunk_max = [&]() {
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < kLane; ++i) m = max_or_nan(m, x[i]);
-    return m;
-  };
   float top;  // of the lane's elements of the chunk; NaN if one of them is
   if (c < reader.chunks) {
     reader.widen(raw, c, x);
-    top = chunk_max();
+    top = chunk_max(x);
   } else {
 #pragma unroll
     for (int i = 0; i < kLane; ++i) x[i] = -INFINITY;
     top = -INFINITY;
   }
-  // The first bound, from the lanes' largest of the first chunks.
-  uint32_t theta = max(bound_of<NW>(top == top ? key_of(top) : 0u, a.count, bounds), kNegInfKey + 1);
+  RowList<NW> list(scratch, a.count, wave, top);
 
   double sum = 0.0;
   float ref = -INFINITY, largest = -INFINITY;  // terms are exp(x - ref)
-  uint64_t *const own = list + wave * kOwn;
-  uint32_t mine = 0;  // entries in it
-  auto raise = [&](uint32_t k) {
-    if (k > theta) {
-      theta = k;
-      if (lane == 0) atomicMax(&bound, k);
-    }
-  };
   auto take = [&]() {
-    // Elements at or above the bound join the wave's list; a NaN is neither.
-    if (__ballot(!(top < value_of(theta)))) {
-      if (!(top < INFINITY)) bad = 1;
-      // Where many lanes have one, the count-th largest of the lanes' maxima is a better bound.
-      if (a.count <= 64 && __popcll(__ballot(top >= value_of(theta))) > a.count) {
-        uint32_t v[1] = {top == top ? key_of(top) : 0u};
-        raise(kth_largest<1>(v, a.count));
-      }
-      const float least = value_of(theta);
-      const uint32_t before = mine;
-#pragma unroll
-      for (int i = 0; i < kLane; ++i) {
-        const uint64_t who = __ballot(x[i] >= least);
-        if (who) {
-          const uint32_t to = mine + lanes_before(who);
-          if (x[i] >= least && to < kOwn) own[to] = composite(key_of(x[i]), (uint32_t)reader.element(c, i));
-          mine += (uint32_t)__popcll(who);
-        }
-      }
-      // All lanes' entries before their count: a wave that sees the count reads them.
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-      if (lane == 0) __hip_atomic_store(&listed[wave], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-      // Now and then the count-th largest of all waves' last entries, 64 or 256, is a new bound.
-      constexpr uint32_t kFew = 64 / NW, kMany = 256 / NW;
-      const uint32_t span = a.count <= 32 ? kFew : kMany;
-      if (before / span != mine / span && mine <= kOwn && c + NW < reader.chunks) {
-        auto entry = [&](uint32_t i) {
-          const uint32_t w = i / span, back = i % span + 1;
-          const uint32_t n = min(__hip_atomic_load(&listed[w], __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP), kOwn);
-          return back <= n ? composite_key(list[w * kOwn + (n - back)]) : 0u;
-        };
-        if (span == kFew) {
-          uint32_t v[1] = {entry(lane)};
-          raise(kth_largest<1>(v, a.count));
-        } else {
-          uint32_t v[4] = {entry(lane), entry(64 + lane), entry(128 + lane), entry(192 + lane)};
-          raise(kth_largest<4>(v, a.count));
-        }
-      }
-    }
+    list.take(reader, c, x, top);
     if (__ballot(top - ref > 600.0f)) {
       // The first chunk with an element, or one far above: another reference. (The difference is rounded near 600
       // only; ref + 600 would be 1,024 above a ref of 2^33.)
@@ -386,10 +147,10 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     raw = next;
     if (c >= reader.chunks) break;
     reader.load(c + NW, next);
-    const uint32_t shared = __hip_atomic_load(&bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    const uint32_t shared = list.shared_bound();
     reader.widen(raw, c, x);
-    top = chunk_max();
-    theta = max(theta, shared);
+    top = chunk_max(x);
+    list.theta = max(list.theta, shared);
   }
   largest = wave_max(largest);
   sum = wave_sum(sum);
@@ -399,28 +160,12 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     wave_max_[wave] = largest;
   }
   __syncthreads();
-  // The entries at or above the last bound, which at least `count` reach where there are so many.
-  bool spilled = false;
-  for (int w = 0; w < NW; ++w) spilled |= listed[w] > kOwn;
-  const uint32_t last = max(bound, theta);
-  for (uint32_t i = 0; i < min(mine, kOwn); i += 64) {
-    const uint64_t v = i + lane < min(mine, kOwn) ? own[i + lane] : 0;
-    const bool in = composite_key(v) >= last;
-    const uint64_t who = __ballot(in);
-    if (!who) continue;
-    uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&held, (uint32_t)__popcll(who));
-    at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + lanes_before(who);
-    if (in && at < (uint32_t)kBlockN) packed[at] = v;
-  }
-  __syncthreads();
-  const uint32_t n = spilled ? ~0u : held;  // more than a wave's share: more than are kept
-  if (bad || n == 0) {
-    if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, bad ? 1 : 0, 0};
+  const uint32_t n = list.pack();
+  if (scratch.bad || n == 0) {
+    if (t == 0) a.sums[blockIdx.x] = RowSum{0.0, -INFINITY, 0, scratch.bad ? 1 : 0, 0};
     return;
   }
   const uint32_t need = min(n, (uint32_t)a.count);
-  uint64_t *out = a.entries + (int64_t)blockIdx.x * a.count;
   if (wave == 0) {
     const float m = wave_max(lane < NW ? wave_max_[lane] : -INFINITY);
     double term = lane < NW ? wave_sum_[lane] : 0.0;
@@ -428,39 +173,14 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
     term = wave_sum(term);
     if (t == 0) a.sums[blockIdx.x] = RowSum{term, m, (int)need, 0, 0};
   }
-  if (n <= (uint32_t)kBlockN) {
-    const int share = share_of(kBlockN, n);
-    const uint32_t i = (uint32_t)t / share;
-    const uint64_t v = i < n ? packed[i] : 0;
-    const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return packed[j] > v; });
-    if (i < n && rank < need) out[rank] = v;
-    return;
-  }
-  __syncthreads();
-  auto pick = [&](auto for_each) {
-    const SelectResult r = radix_select(for_each, need, hist, scratch);
-    if (t == 0) scratch.slot = 0;
-    __syncthreads();
-    for_each([&](uint64_t v) {
-      if (selected(v, r)) out[atomicAdd(&scratch.slot, 1u)] = v;
-    });
-  };
-  if (!spilled) {
-    pick([&](auto f) {
-      for (uint32_t i = lane; i < mine; i += 64) f(own[i]);
-    });
-  } else {
-    // A wave's share of the list does not hold what lies at or above its bounds: from the row again.
-    const uint32_t *mask = a.allowed ? a.allowed + (int64_t)row * a.words : nullptr;
-    const auto *src = reader.row;
-    pick([&](auto f) {
-      for (int e = begin + t; e < begin + len; e += kBlockN) {
-        if (mask && !((mask[e >> 5] >> (e & 31)) & 1u)) continue;
-        const float v = Reader::E::widen(src[e]);
-        if (v > -INFINITY) f(composite(key_of(v), (uint32_t)e));
-      }
-    });
-  }
+  // A wave's share of the list that does not hold what lies at or above its bounds: from the row again.
+  list.select(n, need, a.entries + (int64_t)blockIdx.x * a.count, [&](auto f) {
+    for (int e = begin + t; e < begin + len; e += kBlockN) {
+      if (mask && !((mask[e >> 5] >> (e & 31)) & 1u)) continue;
+      const float v = Reader::E::widen(reader.row[e]);
+      if (v > -INFINITY) f(composite(key_of(v), (uint32_t)e));
+    }
+  });
 }
 
 // Order-preserving 64-bit key of a score that is no NaN.

@@ -29,7 +29,7 @@ import numpy as np
 from .build import LIB_PATH
 
 TABBY_OK, TABBY_EINVAL, TABBY_EHIP, TABBY_EEMPTY, TABBY_EDOMAIN, TABBY_ECAPACITY = range(6)
-TABBY_F32, TABBY_F16, TABBY_BF16 = 0, 1, 2  # bf16: the MXFP4 and beam operators only
+TABBY_F32, TABBY_F16, TABBY_BF16 = 0, 1, 2  # bf16: the MXFP4, FP8, beam and draft operators only
 TABBY_FLAG_FULL_VOCAB = 1
 
 PARAMS_DTYPE = np.dtype([
@@ -55,6 +55,7 @@ EXPORTED_SYMBOLS = (
     "tabby_beam_reorder_device",
     "tabby_fp8_bytes", "tabby_fp8_quantize_device", "tabby_fp8_dequantize_device", "tabby_fp8_pack_device",
     "tabby_fp8_matmul_device", "tabby_fp8_linear_device",
+    "tabby_draft_workspace", "tabby_draft_verify_device",
 )
 
 
@@ -111,6 +112,8 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     L.tabby_fp8_pack_device.argtypes = [vp, vp, i32, i32, vp, vp, vp]
     L.tabby_fp8_matmul_device.argtypes = [vp, vp, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp]
     L.tabby_fp8_linear_device.argtypes = [vp, i32, i64, i32, vp, vp, vp, i32, i32, vp, i32, i64, vp, i64, vp]
+    L.tabby_draft_workspace.argtypes = [i32, i32, i32, pi64]
+    L.tabby_draft_verify_device.argtypes = [vp, i32, i64, i32, vp, i64, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, i64, u32, vp]
     for name in EXPORTED_SYMBOLS[EXPORTED_SYMBOLS.index("tabby_mx4_bytes"):]:
         getattr(L, name).restype = ctypes.c_int
     for name in ("tabby_sampler_create", "tabby_sampler_destroy", "tabby_sampler_sample_device",
