@@ -51,7 +51,7 @@ struct PartSum {
   float max;
   int32_t count;  // entries written
   int32_t bad;    // a NaN or +inf
-  int32_t reserved;
+  int32_t far;    // an entry so far above the reference that the bins do not hold it
 };
 
 // A row's distribution.
@@ -62,14 +62,20 @@ struct RowDist {
   float max;
   int32_t count;       // a pool's entries that are left
   int32_t bad;         // a NaN, +inf, or nothing above -inf
-  int32_t reserved;
+  int32_t far;         // its bins do not hold all of it
 };
 
 enum Draw : int32_t { kDone = 0, kFromTarget, kFromRest, kWithoutToken };
 
+// What a request's last token is drawn from, where that is not a pool.
 struct Decision {
-  int32_t accepted;
-  int32_t draw;
+  int64_t target, draft;         // the rows' first elements
+  uint64_t threshold, draft_threshold;
+  double inverse, of_target, of_draft;  // of the temperature and of the totals
+  double uniform;
+  float max, draft_max;
+  int32_t draw, token;           // the token that is left out, or -1
+  int64_t out;                   // its place among the tokens
 };
 
 struct VerifyArgs {
@@ -86,7 +92,8 @@ struct VerifyArgs {
   PartSum *sums;         // [requests][slots][parts]
   uint64_t *entries;     // [requests][slots][parts][kPoolMax]
   RowDist *dists;        // [requests][slots]
-  uint64_t *pools;       // [requests][slots][kPoolMax]
+  uint64_t *bins;        // [requests][slots][parts][kBins], or null
+  uint64_t *pools;       // [requests][slots][kPoolMax], where a workgroup's LDS does not keep them
   Decision *decisions;   // [requests]
   double2 *segment_sums;  // [requests][segments]: of max(P - Q, 0) and of P
 };
@@ -95,6 +102,8 @@ struct Setting {
   Kind kind;
   int k;
   double inverse, top_p;
+  // Whether a whole vocabulary's distribution ends before its last entry.
+  __device__ __forceinline__ bool cut(int vocab) const { return kind == kWhole && (top_p < 1.0 || k < vocab); }
 };
 
 __device__ __forceinline__ Setting setting_of(const VerifyArgs &a, int request) {
@@ -110,6 +119,15 @@ __device__ __forceinline__ Setting setting_of(const VerifyArgs &a, int request) 
   s.inverse = 1.0 / fmax(p.temperature, 1e-290);
   s.kind = s.k <= kPoolMax ? kPool : a.whole ? kWhole : kInvalid;
   return s;
+}
+
+// The parts that a row is cut into: what a wave holds of their lists has to fit.
+constexpr int kWaveHeld = 1024;
+struct Parts { int count, len; };
+__device__ __forceinline__ Parts parts_of(const VerifyArgs &a, const Setting &set) {
+  if (set.kind == kWhole || a.parts * set.k <= kWaveHeld) return {a.parts, a.part_len};
+  const int most = kWaveHeld / set.k, len = ((a.vocab + most - 1) / most + 31) / 32 * 32;
+  return {(a.vocab + len - 1) / len, len};
 }
 
 // Where a request's rows lie; drafts < 0: nowhere.
@@ -146,10 +164,62 @@ __device__ __forceinline__ SlotRow row_of(const VerifyArgs &a, const Place &p, K
   return {true, j < p.drafts ? p.first_draft + j : -1, base};
 }
 
+// The bins of a row whose distribution is cut: 16 to each power of two of exp((x - reference) / T), from 2^-96 to 2^32 on.
+// A bin holds the sum of its entries' weights in units of its power, 2^-kBinBits of them, or their number: whole numbers, so
+// that no order matters. The reference is the largest of 256 loads spread over the row, which all of its parts find alike.
+constexpr int kOctavesBelow = 96, kOctavesAbove = 32;
+static_assert((kOctavesBelow + kOctavesAbove) * 16 == kBins, "sixteen to a power");
+__device__ __forceinline__ int bin_bits(int vocab) { return min(60 - (32 - __clz(vocab)), 48); }
+
+struct RowBins {
+  double reference, scale;
+  __device__ __forceinline__ RowBins(float reference_, const Setting &set) : reference(reference_), scale(set.inverse * 1.4426950408889634) {}
+  __device__ __forceinline__ double octaves(float x) const { return ((double)x - reference) * scale; }
+  // The place of the octave n and of f, what is left of it, in [-1/2, 1/2]; no lower for a larger logit.
+  __device__ __forceinline__ int place(double octaves, double &f, int &n) const {
+    const double magic = 6755399441055744.0;  // as in exp_64
+    const double shifted = octaves + magic;
+    n = (int)__builtin_bit_cast(uint32x2, shifted).x;
+    f = octaves - (shifted - magic);
+    const int part = (int)__builtin_bit_cast(uint32x2, __builtin_fma(f, 16.0, magic + 8.0)).x;
+    return ((n + kOctavesBelow) << 4) + max(min(part, 15), 0);
+  }
+  // For any logit: below the bins or above them where they do not hold it.
+  __device__ __forceinline__ int bin(float x) const {
+    double f;
+    int n;
+    return place(fmin(fmax(octaves(x), -(double)kOctavesBelow - 1.0), (double)kOctavesAbove), f, n);
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ float reference_of(const void *base, int vocab) {
+  using E = Elem<DT>;
+  const int loads = (vocab + E::kVec - 1) / E::kVec;
+  u32x4 raw[4];
+  int at[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    at[u] = (int)((int64_t)(u * 64 + wave_lane()) * loads >> 8) * E::kVec;
+    raw[u] = load_values<DT, false>((const typename E::Bits *)base, at[u], vocab);
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    float v[E::kVec];
+    E::widen16(raw[u], v);
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) top = at[u] + j < vocab ? fmaxf(top, v[j]) : top;
+  }
+  top = wave_max(top);
+  return top > -INFINITY && top < INFINITY ? top : 0.0f;
+}
+
 template <int DT, int NW>
 __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   using Reader = PartReader<DT, false>;
-  __shared__ ListScratch<NW> scratch;
+  __shared__ union { ListScratch<NW> list; uint64_t bins[kBins]; } lds;
+  ListScratch<NW> &scratch = lds.list;
   __shared__ double wave_sums[NW];
   __shared__ float wave_refs[NW], wave_tops[NW];
   const int row = (int)blockIdx.x / a.parts, part = (int)blockIdx.x - row * a.parts;
@@ -158,8 +228,9 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Setting set = setting_of(a, request);
   const SlotRow source = row_of<DT>(a, place_of(a, request), set.kind, slot);
-  if (!source.used) return;
-  const int begin = part * a.part_len, len = min(a.part_len, a.vocab - begin);
+  const Parts parts = parts_of(a, set);
+  if (!source.used || part >= parts.count) return;
+  const int begin = part * parts.len, len = min(parts.len, a.vocab - begin);
   PartSum *const out = a.sums + blockIdx.x;
   const Reader reader((const typename Reader::Bits *)source.base, nullptr, 0, begin, len);
   typename Reader::Raw raw, next;
@@ -221,6 +292,47 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   double sum = 0.0;
   float ref = -INFINITY, largest = -INFINITY;  // terms are exp((x - ref) / T)
   bool bad = false;
+  if (set.cut(a.vocab) && a.bins) {
+    const RowBins bins(reference_of<DT>(source.base, a.vocab), set);
+    const bool masses = set.k == a.vocab;  // else numbers
+    const double unit = __builtin_ldexp(1.0, bin_bits(a.vocab));
+    for (int b = t; b < kBins; b += NW * 64) lds.bins[b] = 0;
+    __syncthreads();
+    bool far = false;
+    if (c < reader.chunks) {
+      do {
+        bad |= !(top < INFINITY);
+        far |= bins.octaves(top) > (double)kOctavesAbove - 1.0;
+        largest = fmaxf(largest, top);
+        if (__ballot(far) != 0) continue;
+#pragma unroll
+        for (int i = 0; i < kLane; ++i) {
+          const double octaves = bins.octaves(x[i]);
+          if (!(octaves > -(double)kOctavesBelow)) continue;  // nothing of it is left in a sum
+          double f;
+          int n;
+          const int at = bins.place(octaves, f, n);
+          uint64_t add = 1;
+          if (masses) add = (uint64_t)__double_as_longlong(__builtin_fma(exp2_64(f), unit, 0x1p52)) & ((1ull << 52) - 1);
+          atomicAdd((unsigned long long *)&lds.bins[max(at, 0)], (unsigned long long)add);
+        }
+      } while (advance());
+    }
+    bad = __ballot(bad) != 0;
+    far = __ballot(far) != 0;
+    largest = wave_max(largest);
+    if (lane == 0) wave_tops[wave] = bad ? INFINITY : largest;
+    if (lane == 0) wave_refs[wave] = far ? 1.0f : 0.0f;
+    __syncthreads();
+    uint64_t *const to = a.bins + (int64_t)blockIdx.x * kBins;
+    for (int b = t; b < kBins; b += NW * 64) to[b] = lds.bins[b];
+    if (wave == 0) {
+      const float m = wave_max(lane < NW ? wave_tops[lane] : -INFINITY);
+      far = __ballot(lane < NW && wave_refs[lane] != 0.0f) != 0;
+      if (t == 0) *out = m < INFINITY ? PartSum{0.0, m, 0, 0, far ? 1 : 0} : PartSum{0.0, -INFINITY, 0, 1, 0};
+    }
+    return;
+  }
   if (c < reader.chunks) {
     do {
       bad |= !(top < INFINITY);
@@ -261,20 +373,47 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   }
 }
 
+// A whole row's distribution, not cut, from its parts; by a wave.
+__device__ __forceinline__ RowDist whole_row(const VerifyArgs &a, int row, const Setting &set) {
+  const int lane = wave_lane();
+  const bool has = lane < a.parts;
+  PartSum own{0.0, -INFINITY, 0, 0, 0};
+  if (has) own = a.sums[(int64_t)row * a.parts + lane];
+  const float m = wave_max(own.max);
+  const bool bad = __ballot(own.bad) != 0 || !(m > -INFINITY);
+  const bool far = __ballot(own.far) != 0;
+  const double total = wave_sum(own.max > -INFINITY ? own.sum * exp_or_none(((double)own.max - (double)m) * set.inverse) : 0.0);
+  return {total, 0.0, 0, m, 0, bad ? 1 : 0, far ? 1 : 0};
+}
+
 // A pool's weights run off by 1e-15 from the sampler's own exponential; a whole vocabulary's as its sums do.
 __device__ __forceinline__ double weight_of(float x, float max, double inverse) {
   return exp_nonpos(((double)x - (double)max) * inverse);
 }
 
-// Inclusive prefix sum over the wave's lanes, always in the same order.
+// What a lane gets from another: CTRL and the rows of 16 lanes that it is for; 0 elsewhere.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T from_lane(T v) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, ROWS == 0xF));
+  } else {
+    uint32x2 u = __builtin_bit_cast(uint32x2, v);
+    u.x = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, CTRL, ROWS, 0xF, ROWS == 0xF);
+    u.y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, CTRL, ROWS, 0xF, ROWS == 0xF);
+    return __builtin_bit_cast(T, u);
+  }
+}
+
+// Inclusive prefix sum over the wave's lanes, always in the same order (the steps of wave_inclusive_scan_u32).
 template <typename T>
 __device__ __forceinline__ T wave_prefix(T v) {
-  const int lane = wave_lane();
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const T o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v += from_lane<0x111, 0xF>(v);
+  v += from_lane<0x112, 0xF>(v);
+  v += from_lane<0x114, 0xF>(v);
+  v += from_lane<0x118, 0xF>(v);
+  v += from_lane<0x142, 0xA>(v);
+  v += from_lane<0x143, 0xC>(v);
   return v;
 }
 
@@ -299,382 +438,499 @@ __device__ __forceinline__ T block_prefix(T v, T *scratch, T &total) {
 
 constexpr int kSettleWaves = 16;
 constexpr int kSettleThreads = kSettleWaves * 64;
-constexpr int kHeldMax = kPartsMax * kPoolMax;  // entries that a settling workgroup holds
-static_assert(kHeldMax == 4096, "a power of two: they are sorted");
+constexpr int kHeldMax = 1024;         // entries that are ranked at once
+constexpr int kCandidatesMax = 14336;  // entries of a row that may be left after its cut, in LDS
 
 // Masses of a row's entries are whole multiples of 2^-shift: their sums are exact and do not depend on an order.
-__device__ __forceinline__ int mass_shift(int vocab) { return 62 - (32 - __clz(vocab)); }
+__device__ __forceinline__ int mass_shift(int vocab) { return min(62 - (32 - __clz(vocab)), 51); }
 __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, double unit) {
-  return (uint64_t)(exp_or_none(((double)x - (double)max) * inverse) * unit + 0.5);
+  // At most 2^51: added to 2^52 it is rounded to a whole number, in the low bits.
+  const double whole = __builtin_fma(exp_or_none(((double)x - (double)max) * inverse), unit, 0x1p52);
+  return (uint64_t)__double_as_longlong(whole) & ((1ull << 52) - 1);
 }
 
 // The bin of an entry `below` the row's maximum, in temperatures: 128 to a doubling of 1 + below, the largest
 // entries in the highest. Equal logits share one, and a larger logit has none below a smaller one's.
-__device__ __forceinline__ uint32_t bin_of(float x, float max, float inverse) {
-  const float below = (max - x) * inverse + 1.0f;
-  const uint32_t at = (__float_as_uint(below) - 0x3f800000u) >> 16;
+__device__ __forceinline__ uint32_t bin_below(float below_and_one) {
+  const uint32_t at = (__float_as_uint(below_and_one) - 0x3f800000u) >> 16;
   return (uint32_t)(kBins - 1) - min(at, (uint32_t)(kBins - 1));
 }
+__device__ __forceinline__ uint32_t bin_of(float x, float max, float inverse) { return bin_below((max - x) * inverse + 1.0f); }
 
 struct SettleScratch {
-  __attribute__((aligned(16))) uint64_t held[kHeldMax];
+  uint64_t candidates[kCandidatesMax];
+  uint64_t held[kHeldMax + 8], sorted[kHeldMax];
   uint64_t masses[kBins];
   uint32_t counts[kBins];
-  BlockScratchT<kSettleWaves> block;
-  BoundScratch<kSettleWaves> bounds;
-  uint64_t wave64[kSettleWaves];
-  uint64_t found_mass, found_entry;
-  uint32_t found_bin, found_above, taken;
+  uint64_t wave64[kSettleWaves], wave64_mass[kSettleWaves];
+  double wave_f64[kSettleWaves], found_above;
+  uint64_t found_measure, found_mass, found_entry;
+  uint32_t found_bin, taken, gathered;
 };
 
-// Every element of a row above -inf, and its place.
-template <int DT, class F>
-__device__ __forceinline__ void each_element(const void *base, int vocab, F f) {
+// A row's entries at or above `least` (and above -inf) and below `most`, by the whole workgroup. They are gathered in LDS first, so that
+// what is done with them is done by full waves.
+template <int DT>
+struct Candidates {
   using E = Elem<DT>;
-  const typename E::Bits *row = (const typename E::Bits *)base;
-  constexpr int kAhead = 4;
-  const int whole = vocab / E::kVec;
-  for (int i = (int)threadIdx.x; i < whole; i += kAhead * kSettleThreads) {
+  using Bits = typename E::Bits;
+  static constexpr int kLoad = kSettleThreads * E::kVec;  // elements of a load
+  static_assert(kLoad <= kCandidatesMax, "a load's entries find room");
+  const Bits *row;
+  int vocab;
+  float least, most;
+  SettleScratch &s;
+  bool resident = false;  // all of them lie in s.candidates, s.gathered of them
+
+  __device__ __forceinline__ Candidates(const void *base, int vocab_, float least_, float most_, SettleScratch &s_)
+      : row((const Bits *)base), vocab(vocab_), least(least_), most(most_), s(s_) {}
+  __device__ __forceinline__ int place(int load) const { return load * kLoad + (int)threadIdx.x * E::kVec; }
+  __device__ __forceinline__ u32x4 read(int load) const {
+    const int at = place(load);
+    return at < vocab ? load_values<DT, false>(row, at, vocab) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ bool in(float v, int e) const { return e < vocab && v >= least && v < most && v > -INFINITY; }
+  // The entries of a load behind those that are there already.
+  __device__ __forceinline__ void append(u32x4 raw, int load) const {
+    float v[E::kVec];
+    E::widen16(raw, v);
+    const int at = place(load);
+    uint32_t own = 0;
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) own += in(v[j], at + j) ? 1u : 0u;
+    if (!__ballot(own != 0)) return;
+    const uint32_t upto = wave_inclusive_scan_u32(own);
+    uint32_t to = 0;
+    if (wave_lane() == 63) to = atomicAdd(&s.gathered, upto);
+    to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) {
+      if (!in(v[j], at + j)) continue;
+      if (to < (uint32_t)kCandidatesMax) s.candidates[to] = composite(key_of(v[j]), (uint32_t)(at + j));
+      ++to;
+    }
+  }
+  // All of them, if they are as few as LDS holds.
+  __device__ __forceinline__ void fill() {
+    constexpr int kAhead = 4;
+    if (threadIdx.x == 0) s.gathered = 0;
     u32x4 raw[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      raw[u] = *reinterpret_cast<const u32x4_any *>(row + (int64_t)min(i + u * kSettleThreads, whole - 1) * E::kVec);
+    for (int u = 0; u < kAhead; ++u) raw[u] = read(u);
+    __syncthreads();
+    const int loads = (vocab + kLoad - 1) / kLoad;
+#pragma unroll 1
+    for (int first = 0; first < loads; first += kAhead) {
+      u32x4 next[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (i + u * kSettleThreads >= whole) break;
-      float v[E::kVec];
-      E::widen16(raw[u], v);
+      for (int u = 0; u < kAhead; ++u) next[u] = read(first + kAhead + u);
 #pragma unroll
-      for (int j = 0; j < E::kVec; ++j)
-        if (v[j] > -INFINITY) f(v[j], (uint32_t)((i + u * kSettleThreads) * E::kVec + j));
+      for (int u = 0; u < kAhead; ++u) append(raw[u], first + u);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
+    }
+    __syncthreads();
+    resident = s.gathered <= (uint32_t)kCandidatesMax;
+  }
+  // f(logit, composite) of every one of them. More than LDS holds: the row again, as much of it as fits at a time.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int loads = resident ? 1 : (vocab + kLoad - 1) / kLoad;
+    if (!resident) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.gathered = 0;
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (int load = 0; load < loads; ++load) {
+      if (!resident) append(read(load), load);
+      __syncthreads();
+      const uint32_t n = s.gathered;
+      const bool full = load + 1 == loads || n + (uint32_t)kLoad > (uint32_t)kCandidatesMax;
+      if (full) {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < n; i += kSettleThreads) f(value_of(composite_key(s.candidates[i])), s.candidates[i]);
+      }
+      __syncthreads();
+      if (full && !resident) {
+        if (threadIdx.x == 0) s.gathered = 0;
+        __syncthreads();
+      }
     }
   }
-  for (int e = whole * E::kVec + (int)threadIdx.x; e < vocab; e += kSettleThreads) {
-    const float v = E::widen(row[e]);
-    if (v > -INFINITY) f(v, (uint32_t)e);
-  }
-}
-
-// The highest bin at which the running count, or mass, from the highest on reaches `need`: its place, and what lies above
-// it. (A need that no bin reaches: the lowest one that holds anything.)
-template <typename T>
-__device__ __forceinline__ void find_reached(const T *bins, T need, T *wave_space, SettleScratch &s, T *above) {
-  constexpr int kPer = kBins / kSettleThreads;
-  const int t = (int)threadIdx.x, high = kBins - 1 - t * kPer;
-  T own[kPer], sum = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    own[i] = bins[high - i];
-    sum += own[i];
-  }
-  T total;
-  T before = block_prefix<kSettleWaves>(sum, wave_space, total) - sum;
-  const T goal = need < total ? need : total;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    // The first at which the sum reaches the goal: bins that hold nothing do not change it.
-    if (own[i] > 0 && before < goal && before + own[i] >= goal) {
-      s.found_bin = (uint32_t)(high - i);
-      *above = before;
-    }
-    before += own[i];
-  }
-  __syncthreads();
-}
-
-// The entries of one bin, or of a part of one: those whose composite begins with `prefix` down to bit `done`.
-struct Cell {
-  uint32_t bin;
-  int done;  // 64: all of the bin
-  uint64_t prefix;
-  __device__ __forceinline__ bool holds(uint64_t c) const { return done == 64 || (c >> done) == (prefix >> done); }
 };
 
-// What a row's cut has come to: entries down to and with `entry`, and their mass.
-struct Cut {
-  uint64_t entry;
-  uint64_t mass;
-};
-
-// The row cut after its k-th entry (BY_MASS: after the first at which the running mass reaches `goal`), given the bins'
-// counts and masses, and no further than `last`.
-template <int DT, bool BY_MASS>
-__device__ __forceinline__ Cut cut_row(const VerifyArgs &a, const void *base, const Setting &set, float max, uint32_t k, uint64_t goal,
-                                       uint64_t last, SettleScratch &s) {
-  const int t = (int)threadIdx.x;
-  const float inverse = fminf((float)set.inverse, 3.0e38f);
-  const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
-  uint64_t above_mass = 0;  // of what lies above the cell
-  uint32_t above = 0;
-  Cell cell{0, 64, 0};
-  uint32_t in_cell;
-  auto descend = [&]() {
-    // Where the goal is reached among the bins of s, and what lies above it.
-    if constexpr (BY_MASS) {
-      const uint64_t left = goal > above_mass ? goal - above_mass : 1;
-      find_reached<uint64_t>(s.masses, left, s.wave64, s, &s.found_mass);
-      above_mass += s.found_mass;
-    } else {
-      find_reached<uint32_t>(s.counts, k - above, s.block.u, s, &s.found_above);
-      above += s.found_above;
-      // Their mass: of the bins above.
-      uint64_t mass = 0, total;
-      for (int b = kBins - 1 - t; b > (int)s.found_bin; b -= kSettleThreads) mass += s.masses[b];
-      block_prefix<kSettleWaves>(mass, s.wave64, total);
-      above_mass += total;
-    }
-    in_cell = s.counts[s.found_bin];
-    const uint32_t found = s.found_bin;
-    __syncthreads();
-    return found;
-  };
-  cell.bin = descend();
-  // More entries than LDS holds: the next eleven bits of their composites.
-  while (in_cell > (uint32_t)kHeldMax && cell.done > 0) {
-    const int shift = cell.done >= 11 ? cell.done - 11 : 0;
-    const uint32_t digits = (1u << (cell.done - shift)) - 1;
-    for (int b = t; b < kBins; b += kSettleThreads) {
-      s.counts[b] = 0;
-      s.masses[b] = 0;
-    }
-    __syncthreads();
-    each_element<DT>(base, a.vocab, [&](float x, uint32_t e) {
-      if (bin_of(x, max, inverse) != cell.bin) return;
-      const uint64_t c = composite(key_of(x), e);
-      if (c < last || !cell.holds(c)) return;
-      const uint32_t digit = (uint32_t)(c >> shift) & digits;
-      atomicAdd(&s.counts[digit], 1u);
-      atomicAdd((unsigned long long *)&s.masses[digit], (unsigned long long)mass_of(x, max, set.inverse, unit));
-    });
-    __syncthreads();
-    const uint32_t digit = descend();
-    cell.prefix |= (uint64_t)digit << shift;
-    cell.done = shift;
+// The smallest logit that lies in bin b or above, by a wave: 64 probes at a time among the keys.
+__device__ __forceinline__ float bin_begin(const RowBins &bins, int b) {
+  if (b >= kBins) return INFINITY;
+  uint32_t low = kNegInfKey, high = key_of(INFINITY);  // low lies below, high does not
+#pragma unroll 1
+  while (high - low > 1) {
+    const uint32_t step = (high - low + 63) / 64;
+    const uint32_t probe = low + (uint32_t)(wave_lane() + 1) * step;
+    const bool in = probe >= high || bins.bin(value_of(probe)) >= b;
+    const int first = __builtin_ctzll(__ballot(in));  // the last lane's probe is high or beyond
+    const uint32_t next_high = min(low + (uint32_t)(first + 1) * step, high);
+    low += (uint32_t)first * step;
+    high = next_high;
   }
-  if (t == 0) s.taken = 0;
-  __syncthreads();
-  each_element<DT>(base, a.vocab, [&](float x, uint32_t e) {
-    if (bin_of(x, max, inverse) != cell.bin) return;
-    const uint64_t c = composite(key_of(x), e);
-    if (c < last || !cell.holds(c)) return;
-    const uint32_t at = atomicAdd(&s.taken, 1u);
-    if (at < (uint32_t)kHeldMax) s.held[at] = c;
-  });
-  __syncthreads();
-  const int n = (int)min(s.taken, (uint32_t)kHeldMax), room = next_pow2(n);
-  for (int i = n + t; i < room; i += kSettleThreads) s.held[i] = 0;
-  __syncthreads();
-  bitonic_sort_desc<kSettleWaves>(s.held, room);
-  if (room <= 1) __syncthreads();
-  // In order, four to a thread: the first that reaches the goal, or the last there is.
-  constexpr int kPer = kHeldMax / kSettleThreads;
-  uint64_t mass[kPer], sum = 0, total;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int at = t * kPer + i;
-    mass[i] = at < n ? mass_of(value_of(composite_key(s.held[at])), max, set.inverse, unit) : 0;
-    sum += mass[i];
-  }
-  uint64_t before = block_prefix<kSettleWaves>(sum, s.wave64, total) - sum + above_mass;
-  const uint64_t reach = BY_MASS ? (goal < above_mass + total ? goal : above_mass + total) : 0;
-  bool reached = BY_MASS && t > 0 && before >= reach;  // by an entry of a thread before this one
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int at = t * kPer + i;
-    before += mass[i];
-    const bool here = at < n && (BY_MASS ? !reached && before >= reach : above + at + 1 == k || (at == n - 1 && above + n < k));
-    if (here) {
-      s.found_entry = s.held[at];
-      s.found_mass = before;
-      reached = true;
-    }
-  }
-  __syncthreads();
-  return {s.found_entry, s.found_mass};
+  return value_of(high);
 }
 
+// The rows whose distribution is cut by more than a list: after the k-th entry, and where top_p is reached. The bins that
+// the row's parts have left say in which of them the row is cut, and its entries (of k, those above it as well) go to LDS
+// as the row passes. Among them the cut is found: by the counts and masses of finer bins, of parts of a bin (eleven bits of
+// the composites at a time) where it has more than are ranked at once, then among the ranked entries of one cell. Where
+// there are no bins, or a row's do not hold it, all entries that may be left are gone through.
 template <int DT>
 __global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArgs a) {
   using E = Elem<DT>;
   __shared__ SettleScratch s;
   const int row = (int)blockIdx.x;
   const int request = row / a.slots, slot = row - request * a.slots;
-  const int t = (int)threadIdx.x, lane = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int t = (int)threadIdx.x;
   const Setting set = setting_of(a, request);
   const SlotRow source = row_of<DT>(a, place_of(a, request), set.kind, slot);
-  if (!source.used) return;
-  const PartSum *sums = a.sums + (int64_t)row * a.parts;
-  RowDist dist{0.0, 0.0, 0, -INFINITY, 0, 0, 0};
-  float m = -INFINITY;
-  int bad = 0;
-  for (int p = 0; p < a.parts; ++p) {
-    m = fmaxf(m, sums[p].max);
-    bad |= sums[p].bad;
-  }
-  bad |= !(m > -INFINITY);
-  dist.max = m;
-  dist.bad = bad;
-  if (bad) {
-    if (t == 0) a.dists[row] = dist;
+  if (!source.used || !set.cut(a.vocab)) return;
+  const RowDist whole = whole_row(a, row, set);
+  if (whole.bad) {
+    if (t == 0) a.dists[row] = whole;
     return;
   }
-  if (set.kind == kWhole) {
-    double total = 0.0;
-    for (int p = 0; p < a.parts; ++p)
-      if (sums[p].max > -INFINITY) total += sums[p].sum * exp_or_none(((double)sums[p].max - (double)m) * set.inverse);
-    dist.total = total;
-    const bool cut = set.top_p < 1.0;
-    if (cut || set.k < a.vocab) {
-      const float inverse = fminf((float)set.inverse, 3.0e38f);
-      const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
-      for (int b = t; b < kBins; b += kSettleThreads) {
-        s.counts[b] = 0;
-        s.masses[b] = 0;
+  const float m = whole.max, inverse = fminf((float)set.inverse, 3.0e38f);  // of the bins in LDS
+  const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
+  const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
+  // The smallest whole number of units that is top_p of the total, within the rounding of sums and masses (so that
+  // 900 of 1,000 equal entries are 0.9 of them); at least one.
+  auto goal_of = [&](double all) { return (uint64_t)fmax(ceil(set.top_p * all * (1.0 - 1e-12 - 1.0 / unit)), 1.0); };
+  auto clear = [&]() {
+    for (int b = t; b < kBins; b += kSettleThreads) {
+      s.counts[b] = 0;
+      s.masses[b] = 0;
+    }
+    __syncthreads();
+  };
+  // The highest bin at which the running count (or mass) from the highest on reaches `need` -- where none does, the lowest
+  // that holds anything -- to s.found_bin, and the count (or mass) and the mass above it. Returns the sum of all bins.
+  auto find = [&](uint64_t need, bool masses) {
+    constexpr int kPer = kBins / kSettleThreads;
+    const int high = kBins - 1 - t * kPer;
+    uint64_t own[kPer], mass[kPer], sum = 0, sum_mass = 0, total, total_mass;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      mass[i] = s.masses[high - i];
+      own[i] = masses ? mass[i] : s.counts[high - i];
+      sum += own[i];
+      sum_mass += mass[i];
+    }
+    uint64_t before = block_prefix<kSettleWaves>(sum, s.wave64, total) - sum;
+    uint64_t before_mass = block_prefix<kSettleWaves>(sum_mass, s.wave64_mass, total_mass) - sum_mass;
+    const uint64_t goal = need < total ? need : total;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      // The first at which the sum reaches the goal: bins that hold nothing do not change it.
+      if (own[i] > 0 && before < goal && before + own[i] >= goal) {
+        s.found_bin = (uint32_t)(high - i);
+        s.found_measure = before;
+        s.found_mass = before_mass;
       }
-      __syncthreads();
-      each_element<DT>(source.base, a.vocab, [&](float x, uint32_t) {
-        const uint32_t b = bin_of(x, m, inverse);
-        atomicAdd(&s.counts[b], 1u);
-        atomicAdd((unsigned long long *)&s.masses[b], (unsigned long long)mass_of(x, m, set.inverse, unit));
-      });
-      __syncthreads();
-      uint64_t mass = 0, all;
-      for (int b = t; b < kBins; b += kSettleThreads) mass += s.masses[b];
-      block_prefix<kSettleWaves>(mass, s.wave64, all);
-      Cut c{0, all};
-      if (set.k < a.vocab) {
-        c = cut_row<DT, false>(a, source.base, set, m, (uint32_t)set.k, 0, 0, s);
-        if (cut) {
-          // The bins again, of what is left.
-          __syncthreads();
-          for (int b = t; b < kBins; b += kSettleThreads) {
-            s.counts[b] = 0;
-            s.masses[b] = 0;
-          }
-          __syncthreads();
-          each_element<DT>(source.base, a.vocab, [&](float x, uint32_t e) {
-            if (composite(key_of(x), e) < c.entry) return;
-            const uint32_t b = bin_of(x, m, inverse);
-            atomicAdd(&s.counts[b], 1u);
-            atomicAdd((unsigned long long *)&s.masses[b], (unsigned long long)mass_of(x, m, set.inverse, unit));
-          });
-          __syncthreads();
+      before += own[i];
+      before_mass += mass[i];
+    }
+    __syncthreads();
+    return total;
+  };
+  float least = -INFINITY, most = INFINITY;  // where what may be the last entry lies
+  uint64_t from = 0;                         // mass above that
+  double total = whole.total * unit;         // of what top_p is a share of, in units; 0: not known
+  const RowBins bins(a.bins ? reference_of<DT>(source.base, a.vocab) : 0.0f, set);
+  const double raised = bins.octaves(m);  // the maximum above the bins' reference
+  if (a.bins && !whole.far && raised > -16.0) {
+    // The bins of the row, left by its parts: sixteen to a power of two of the weights.
+    constexpr int kPer = kBins / kSettleThreads;
+    const int high = kBins - 1 - t * kPer;
+    const uint64_t *const parts = a.bins + (int64_t)row * a.parts * kBins;
+    uint64_t own[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) own[i] = 0;
+#pragma unroll 1
+    for (int p = 0; p < a.parts; ++p) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) own[i] += parts[(int64_t)p * kBins + high - i];
+    }
+    // Counts, or weights relative to the maximum's.
+    double v[kPer], sum = 0.0, all;
+    const double share = exp2(-raised) / __builtin_ldexp(1.0, bin_bits(a.vocab));
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      v[i] = (double)own[i];
+      if (!by_count) v[i] = __builtin_ldexp(v[i], ((high - i) >> 4) - kOctavesBelow) * share;
+      sum += v[i];
+    }
+    if (t == 0) s.found_bin = kBins;
+    double before = block_prefix<kSettleWaves>(sum, s.wave_f64, all) - sum;
+    const double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - 1e-12);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (v[i] > 0.0 && before + v[i] >= goal && (before < goal || !(before > 0.0))) {
+        s.found_bin = (uint32_t)(high - i);
+        s.found_above = before;
+      }
+      before += v[i];
+    }
+    __syncthreads();
+    const int found = (int)s.found_bin;
+    if (found < kBins) {
+      least = bin_begin(bins, found);
+      if (!by_count) {
+        most = bin_begin(bins, found + 1);
+        total = all * unit;
+        from = (uint64_t)(s.found_above * unit + 0.5);
+      }
+    }
+    __syncthreads();
+  } else if (!by_count && total > 0.0) {
+    // Entries below (1 - top_p) total / vocab hold less than 1 - top_p together. (A margin for roundings.)
+    const double low = (1.0 - set.top_p) * whole.total / (double)a.vocab * (1.0 - 1e-6);
+    const double bound = (double)m - fmax(-log(low), 0.0) / set.inverse - fabs((double)m) * 1e-6;
+    least = bound > -3.4e38 ? (float)bound : -INFINITY;
+  }
+  Candidates<DT> left(source.base, a.vocab, least, most, s);
+  left.fill();
+  uint64_t entry = 0;      // the last entry that is left
+  uint64_t left_mass = 0;  // of what is left
+#pragma unroll 1
+  for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
+    const bool masses = stage == 1;
+    uint64_t goal = (uint64_t)set.k;
+    uint64_t above_mass = masses ? from : 0, above = above_mass;  // what lies above the cell
+    uint64_t prefix = 0;                             // how the cell's composites begin
+    uint32_t bin = 0;                                // the cell's bin
+    int done = 64, shift = 0;                        // its entries begin with prefix >> done
+    enum { kByBin, kByDigit, kTakeBin, kTakeAll } step = kByBin;
+    // Few enough to be ranked at once: no bins. (The first stage's bins count them all.)
+    if (left.resident && s.gathered <= (uint32_t)kHeldMax && (!masses || total > 0.0)) step = kTakeAll;
+#pragma unroll 1
+    for (;;) {
+      const bool takes = step >= kTakeBin;
+      if (masses && (takes || total > 0.0)) goal = goal_of(total);
+      if (!takes) clear();
+      else if (t == 0) s.taken = 0;
+      if (takes) __syncthreads();
+      left.each([&](float x, uint64_t c) {
+        if (c < entry) return;
+        uint32_t to = bin_of(x, m, inverse);
+        if ((step == kByDigit || step == kTakeBin) && (to != bin || (done < 64 && (c >> done) != (prefix >> done)))) return;
+        if (takes) {
+          const uint32_t at = atomicAdd(&s.taken, 1u);
+          if (at < (uint32_t)kHeldMax) s.held[at] = c;
+          return;
         }
+        if (step == kByDigit) to = (uint32_t)(c >> shift) & ((1u << (done - shift)) - 1);
+        atomicAdd(&s.counts[to], 1u);
+        atomicAdd((unsigned long long *)&s.masses[to], (unsigned long long)mass_of(x, m, set.inverse, unit));
+      });
+      if (takes) break;
+      if (masses && !(total > 0.0)) {
+        // The bins hold all of the row.
+        uint64_t mass = 0, all;
+        for (int b = t; b < kBins; b += kSettleThreads) mass += s.masses[b];
+        block_prefix<kSettleWaves>(mass, s.wave64, all);
+        total = (double)all;
+        goal = goal_of(total);
       }
-      if (cut) {
-        // The smallest whole number of units that is top_p of the total, within the rounding of that product (so that
-        // 900 of 1,000 equal entries are 0.9 of them); at least one.
-        const double share = fmax(ceil(set.top_p * (double)c.mass * (1.0 - 0x1p-51)), 1.0);
-        c = cut_row<DT, true>(a, source.base, set, m, 0, (uint64_t)share, c.entry, s);
+      find(goal > above ? goal - above : 1, masses);
+      above += s.found_measure;
+      above_mass += s.found_mass;
+      const uint32_t found = s.found_bin, in_cell = s.counts[found];
+      __syncthreads();
+      if (step == kByBin) {
+        bin = found;
+      } else {
+        prefix |= (uint64_t)found << shift;
+        done = shift;
       }
-      dist.threshold = c.entry;
-      dist.total = (double)c.mass / unit;
+      if (in_cell > (uint32_t)kHeldMax && done > 0) {
+        step = kByDigit;
+        shift = done >= 11 ? done - 11 : 0;
+      } else {
+        step = kTakeBin;
+      }
     }
-  } else {
-    // The parts' entries: those at or above a bound are ranked by counting.
-    const uint64_t *entries = a.entries + (int64_t)row * a.parts * kPoolMax;
-    const int slots = a.parts * kPoolMax;
-    constexpr int kEach = kHeldMax / kSettleThreads;
-    uint64_t entry[kEach], best = 0;
+    // In order, by counting; one to a thread: the first that reaches the goal, or the last there is.
+    const uint32_t n = min(s.taken, (uint32_t)kHeldMax);
+    if ((uint32_t)t < 8) s.held[n + (uint32_t)t] = 0;  // whole rounds
+    __syncthreads();
+    if ((uint32_t)t < n) {
+      const uint64_t own = s.held[t];
+      uint32_t rank = 0;
+#pragma unroll 1
+      for (uint32_t j = 0; j < n; j += 8) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int at = i * kSettleThreads + t;
-      entry[i] = at < slots && at % kPoolMax < sums[at / kPoolMax].count ? entries[at] : 0;
-      best = max(best, entry[i]);
-    }
-    if (t == 0) s.taken = 0;
-    uint32_t theta = 0;
-    if (a.parts > 1) theta = bound_of<kSettleWaves>((uint32_t)(best >> 32), set.k, s.bounds);
-    else __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const bool in = entry[i] != 0 && composite_key(entry[i]) >= theta;
-      const uint64_t who = __ballot(in);
-      if (!who) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&s.taken, (uint32_t)__popcll(who));
-      at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + lanes_before(who);
-      if (in) s.held[at] = entry[i];
+        for (uint32_t u = 0; u < 8; ++u) rank += s.held[j + u] > own ? 1u : 0u;
+      }
+      s.sorted[rank] = own;
     }
     __syncthreads();
-    const uint32_t n = s.taken, need = min(n, (uint32_t)set.k);
-    uint64_t *const pool = s.masses;  // in order
-    const int share = share_of(kSettleThreads, n);
-    for (uint32_t i = (uint32_t)t / share; i < (n + kSettleThreads - 1) / kSettleThreads * kSettleThreads / share; i += kSettleThreads / share) {
-      const uint64_t v = i < n ? s.held[i] : 0;
-      const uint32_t rank = rank_of(share, n, [&](uint32_t j) { return s.held[j] > v; });
-      if (i < n && rank < need && (t & (share - 1)) == 0) pool[rank] = v;
+    const uint64_t mine = (uint32_t)t < n ? s.sorted[t] : 0;
+    const uint64_t mass = (uint32_t)t < n ? mass_of(value_of(composite_key(mine)), m, set.inverse, unit) : 0;
+    uint64_t all;
+    const uint64_t upto = block_prefix<kSettleWaves>(mass, s.wave64, all) + above_mass;
+    // (Of masses, `above` is above_mass.)
+    const uint64_t reach = masses ? (goal < above_mass + all ? goal : above_mass + all) : (goal < above + n ? goal : above + n);
+    if ((uint32_t)t < n && (masses ? upto >= reach && (t == 0 || upto - mass < reach) : above + t + 1 == reach)) {
+      s.found_entry = mine;
+      s.found_mass = upto;
     }
     __syncthreads();
-    if (wave == 0) {
-      double w[2], sum[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t i = (uint32_t)(lane + 64 * h);
-        w[h] = i >= need ? 0.0 : set.kind == kGreedy ? 1.0 : weight_of(value_of(composite_key(pool[i])), m, set.inverse);
-        sum[h] = wave_prefix(w[h]);
-      }
-      sum[1] += __shfl(sum[0], 63);
-      const double total = __shfl(sum[1], 63);
-      uint32_t left = need;
-      if (set.top_p < 1.0) {
-        const uint64_t low = __ballot(sum[0] >= set.top_p * total), high = __ballot(sum[1] >= set.top_p * total);
-        const uint32_t first = low ? (uint32_t)__builtin_ctzll(low) : high ? 64u + (uint32_t)__builtin_ctzll(high) : need - 1;
-        left = min(first + 1, need);
-      }
-      const int at = (int)left - 1;
-      const double low = __shfl(sum[0], at & 63), high = __shfl(sum[1], at & 63);
-      dist.total = at < 64 ? low : high;
-      dist.threshold = pool[at];
-      dist.count = (int)left;
-      uint64_t *out = a.pools + (int64_t)row * kPoolMax;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t i = (uint32_t)(lane + 64 * h);
-        if (i < left) out[i] = pool[i];
-      }
-    }
+    entry = s.found_entry;
+    left_mass = s.found_mass;
+    total = (double)left_mass;
+    __syncthreads();
   }
   if (t != 0) return;
-  if (source.drafted >= 0) {
-    const int token = a.drafts[source.drafted];
-    if (token < 0 || token >= a.vocab) {
-      dist.drafted = -1.0;
-    } else {
-      const float x = E::widen(((const typename E::Bits *)source.base)[token]);
-      if (x > -INFINITY && composite(key_of(x), (uint32_t)token) >= dist.threshold)
-        dist.drafted = (set.kind == kGreedy ? 1.0 : weight_of(x, m, set.inverse)) / dist.total;
-    }
-  }
+  RowDist dist = whole;
+  dist.threshold = entry;
+  dist.total = (double)left_mass / unit;
   a.dists[row] = dist;
 }
 
-// One workgroup of two waves to a request.
-constexpr int kDecideThreads = 128;
+// A wave's work on a row whose distribution is a list: its parts' entries together in `held`, those at or above a
+// bound ranked by counting, and cut. The entries that are left go to `pool`, in order.
+__device__ __forceinline__ RowDist pool_row(const VerifyArgs &a, int row, const Setting &set, uint64_t *held, uint64_t *pool) {
+  const int lane = wave_lane();
+  const int parts = parts_of(a, set).count;
+  const PartSum *sums = a.sums + (int64_t)row * a.parts;
+  const uint64_t *entries = a.entries + (int64_t)row * a.parts * kPoolMax;
+  // A lane to a part.
+  PartSum own{0.0, -INFINITY, 0, 0, 0};
+  if (lane < parts) own = sums[lane];
+  const float m = wave_max(own.max);
+  RowDist dist{0.0, 0.0, 0, m, 0, 0, 0};
+  dist.bad = __ballot(own.bad) != 0 || !(m > -INFINITY);
+  if (dist.bad) return dist;
+  // The parts' entries one after another, a part's turned by five places from the one before: each of the 64 lanes' four
+  // columns has entries of different ranks.
+  const int slots = parts * set.k;
+  const float per = 1.0f / (float)set.k;  // slots <= 2^10: (i + 1/2) / k has bits to spare
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int first = 0; first < slots; first += 8 * 64) {
+    uint64_t e[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = first + u * 64 + lane, p = (int)(((float)i + 0.5f) * per), turned = i - p * set.k + 5 * p;
+      const int at = turned - (int)(((float)turned + 0.5f) * per) * set.k;
+      const bool here = i < slots && at < __shfl(own.count, p & 63);
+      e[u] = here ? entries[p * kPoolMax + at] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (first + u * 64 + lane < slots) held[first + u * 64 + lane] = e[u];
+      v[u & 3] = max(v[u & 3], composite_key(e[u]));
+    }
+  }
+  uint32_t theta = 0;
+  if (parts > 1) {
+    uint32_t all[1] = {max(max(v[0], v[1]), max(v[2], v[3]))};
+    theta = set.k <= 32 ? kth_largest<1>(all, set.k) : kth_largest<4>(v, set.k);
+  }
+  wave_lds_sync();
+  uint32_t n = 0;
+#pragma unroll 1
+  for (int first = 0; first < slots; first += 64) {
+    // To the front: what is written was read before.
+    const uint64_t e = first + lane < slots ? held[first + lane] : 0;
+    const bool in = e != 0 && composite_key(e) >= theta;
+    const uint64_t who = __ballot(in);
+    if (in) held[n + lanes_before(who)] = e;
+    n += (uint32_t)__popcll(who);
+    wave_lds_sync();
+  }
+  const uint32_t need = min(n, (uint32_t)set.k);
+#pragma unroll 1
+  for (uint32_t i = (uint32_t)lane; i < n; i += 64) {
+    const uint64_t e = held[i];
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) rank += held[j] > e ? 1u : 0u;
+    if (rank < need) pool[rank] = e;
+  }
+  wave_lds_sync();
+  double sum[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t i = (uint32_t)(lane + 64 * h);
+    const double w = i >= need ? 0.0 : set.kind == kGreedy ? 1.0 : weight_of(value_of(composite_key(pool[i])), m, set.inverse);
+    sum[h] = wave_prefix(w);
+  }
+  sum[1] += __shfl(sum[0], 63);
+  const double total = __shfl(sum[1], 63);
+  uint32_t left = need;
+  if (set.top_p < 1.0) {
+    const uint64_t low = __ballot(sum[0] >= set.top_p * total), high = __ballot(sum[1] >= set.top_p * total);
+    const uint32_t first = low ? (uint32_t)__builtin_ctzll(low) : high ? 64u + (uint32_t)__builtin_ctzll(high) : need - 1;
+    left = min(first + 1, need);
+  }
+  const int at = (int)left - 1;
+  const double low = __shfl(sum[0], at & 63), high = __shfl(sum[1], at & 63);
+  dist.total = at < 64 ? low : high;
+  dist.threshold = pool[at];
+  dist.count = (int)left;
+  return dist;
+}
 
-__global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArgs a) {
-  __shared__ uint64_t target[kPoolMax], draft[kPoolMax];
-  __shared__ double rest[kPoolMax], all[kPoolMax], wave_space[2];
+// A workgroup of NW waves to a request: a wave to a row gives its distribution and the probability of its drafted token;
+// then the first refusal; then, for pools, the draw.
+template <int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void verify_decide_kernel(VerifyArgs a) {
+  using E = Elem<DT>;
+  constexpr int kKept = NW;  // rows whose entries stay in LDS
+  __shared__ uint64_t held[NW][kWaveHeld], pools[kKept][kPoolMax];
+  __shared__ RowDist dists[2 * kDraftsMax + 1];
+  __shared__ double rest[kPoolMax], all[kPoolMax];
   __shared__ int accepted_, status_;
   __shared__ uint32_t ids[kPoolMax];
-  __shared__ uint64_t overs[2], somes[2];
-  const int request = (int)blockIdx.x, t = (int)threadIdx.x;
+  const int request = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const Setting set = setting_of(a, request);
   const Place place = place_of(a, request);
-  const RowDist *dists = a.dists + (int64_t)request * a.slots;
+  for (int slot = wave; slot < a.slots; slot += NW) {
+    const SlotRow source = row_of<DT>(a, place, set.kind, slot);
+    if (!source.used) continue;
+    // The drafted token's logit, on its way while the row's parts are.
+    int token = -1;
+    float x = -INFINITY;
+    if (source.drafted >= 0) {
+      token = a.drafts[source.drafted];
+      if (token >= 0 && token < a.vocab) x = E::widen(((const typename E::Bits *)source.base)[token]);
+    }
+    const int row = request * a.slots + slot;
+    RowDist d;
+    if (set.kind != kWhole) d = pool_row(a, row, set, held[wave], pools[a.slots > kKept ? wave : slot]);
+    else d = set.cut(a.vocab) ? a.dists[row] : whole_row(a, row, set);
+    if (source.drafted >= 0 && !d.bad) {
+      if (token < 0 || token >= a.vocab) d.drafted = -1.0;
+      else if (x > -INFINITY && composite(key_of(x), (uint32_t)token) >= d.threshold)
+        d.drafted = (set.kind == kGreedy ? 1.0 : weight_of(x, d.max, set.inverse)) / d.total;
+    }
+    if (lane == 0) dists[slot] = d;
+    if (set.kind == kPool && a.slots > kKept) {
+      for (int i = lane; i < d.count; i += 64) a.pools[(int64_t)row * kPoolMax + i] = pools[wave][i];
+    }
+  }
+  __syncthreads();
   const bool drawn = a.draft_logits != nullptr && set.kind != kGreedy;  // else the drafted tokens were certain
-  if (t < 64) {
-    const bool asked = place.drafts >= 0 && t < place.drafts && set.kind != kInvalid;
+  const int first_draft = a.drafts_max + 1;                             // slot of the draft's rows
+  if (wave == 0) {
+    const bool asked = place.drafts >= 0 && lane < place.drafts && set.kind != kInvalid;
     bool good = false, broken = false, unknown = false;
     if (asked) {
-      const RowDist &p = dists[t];
-      const double claim = drawn ? dists[a.drafts_max + 1 + t].drafted : 1.0;
-      broken = p.bad || (drawn && dists[a.drafts_max + 1 + t].bad);
-      unknown = !broken && p.drafted < 0.0;
-      good = !broken && !unknown && a.uniforms[place.first_draft + t] * claim < p.drafted;
+      const double share = dists[lane].drafted, claim = drawn ? dists[first_draft + lane].drafted : 1.0;
+      broken = dists[lane].bad || (drawn && dists[first_draft + lane].bad);
+      unknown = !broken && share < 0.0;
+      good = !broken && !unknown && a.uniforms[place.first_draft + lane] * claim < share;
     }
-    // Of the greedy settings the draft's distribution is not asked: a token is accepted if it is the largest's.
     const uint64_t goods = __ballot(good), brokens = __ballot(broken), unknowns = __ballot(unknown);
     if (t == 0) {
       int n = 0, status = TABBY_EINVAL;
@@ -697,134 +953,133 @@ __global__ __launch_bounds__(kDecideThreads) void verify_decide_kernel(VerifyArg
   }
   const bool refused = n < place.drafts;
   const Draw draw = !refused || set.kind == kGreedy ? kFromTarget : drawn ? kFromRest : kWithoutToken;
-  if (t == 0 && a.whole) a.decisions[request] = {n, status == TABBY_OK && set.kind == kWhole ? draw : kDone};
+  if (t == 0 && a.whole) {
+    Decision d{};
+    if (status == TABBY_OK && set.kind == kWhole) {
+      const RowDist &p = dists[n], &q = dists[draw == kFromRest ? first_draft + n : n];
+      d = {(int64_t)(place.first + n) * a.stride, (int64_t)(place.first_draft + n) * a.draft_stride,
+           p.threshold, q.threshold, set.inverse, 1.0 / p.total, 1.0 / q.total, a.params[request].uniform, p.max, q.max, draw,
+           draw == kWithoutToken ? a.drafts[place.first_draft + n] : -1, (int64_t)request * (a.drafts_max + 1) + n};
+    }
+    a.decisions[request] = d;
+  }
   if (status != TABBY_OK || set.kind == kWhole) return;
   // A pool: what is left of the target's entries, in the vocabulary's order.
-  const RowDist p = dists[n];
+  const RowDist p = dists[n], q = draw == kFromRest ? dists[first_draft + n] : p;
   if (set.kind == kGreedy) {
     if (t == 0) tokens[n] = (int32_t)composite_index(p.threshold);
     return;
   }
-  const RowDist q = draw == kFromRest ? dists[a.drafts_max + 1 + n] : p;
-  const uint64_t own = t < p.count ? a.pools[((int64_t)request * a.slots + n) * kPoolMax + t] : 0;
-  target[t] = own;
-  if (draw == kFromRest) draft[t] = t < q.count ? a.pools[((int64_t)request * a.slots + a.drafts_max + 1 + n) * kPoolMax + t] : 0;
-  __syncthreads();
-  const uint32_t id = composite_index(own);
-  double share = 0.0, left = 0.0;
-  uint32_t before = 0;
-  if (t < p.count) {
-    share = weight_of(value_of(composite_key(own)), p.max, set.inverse) / p.total;
-    left = share;
+  uint64_t *target = pools[n % kKept], *draft = pools[(first_draft + n) % kKept];
+  if (a.slots > kKept) {
+    // More rows than LDS keeps.
+    target = held[0];
+    draft = held[1];
+    const int64_t at = (int64_t)request * a.slots;
+    if (t < p.count) target[t] = a.pools[(at + n) * kPoolMax + t];
+    if (draw == kFromRest && t < q.count) draft[t] = a.pools[(at + first_draft + n) * kPoolMax + t];
+    __syncthreads();
+  }
+  // Some threads to an entry: how many tokens come before its own, and what the draft takes of it.
+  constexpr int kShare = NW * 64 / kPoolMax;
+  const int i = t / kShare, part = t % kShare;
+  if (i < p.count) {
+    const uint64_t own = target[i];
+    const uint32_t id = composite_index(own);
+    uint32_t before = 0, found = 0;  // the place in the draft's list, from 1
+#pragma unroll 1
+    for (int j = part; j < p.count; j += kShare) before += composite_index(target[j]) < id ? 1u : 0u;
     if (draw == kFromRest) {
-      for (int j = 0; j < q.count; ++j)
-        if (composite_index(draft[j]) == id) left = fmax(share - weight_of(value_of(composite_key(draft[j])), q.max, set.inverse) / q.total, 0.0);
-    } else if (draw == kWithoutToken && (int)id == a.drafts[place.first_draft + n]) {
-      left = 0.0;
+#pragma unroll 1
+      for (int j = part; j < q.count; j += kShare)
+        if (composite_index(draft[j]) == id) found = (uint32_t)j + 1;
     }
-    for (int j = 0; j < p.count; ++j) before += composite_index(target[j]) < id ? 1u : 0u;
-    rest[before] = left;
-    all[before] = share;
-    ids[before] = id;
+#pragma unroll
+    for (int stride = 1; stride < kShare; stride *= 2) {
+      before += xor_lane_by(before, stride);
+      found = max(found, xor_lane_by(found, stride));
+    }
+    if (part == 0) {
+      const double share = weight_of(value_of(composite_key(own)), p.max, set.inverse) / p.total;
+      double left = share;
+      if (found) left = fmax(share - weight_of(value_of(composite_key(draft[found - 1])), q.max, set.inverse) / q.total, 0.0);
+      if (draw == kWithoutToken && (int)id == a.drafts[place.first_draft + n]) left = 0.0;
+      rest[before] = left;
+      all[before] = share;
+      ids[before] = id;
+    }
   }
   __syncthreads();
-  double total;
-  double v = t < p.count ? rest[t] : 0.0;
-  double sum = block_prefix<2>(v, wave_space, total);
-  if (!(total > 0.0)) {  // nothing left: P is Q, but for roundings
-    v = t < p.count ? all[t] : 0.0;
-    sum = block_prefix<2>(v, wave_space, total);
-  }
+  if (wave != 0) return;
   // The first whose running sum exceeds the share; the last with a weight where none does.
+  double w[2], sum[2], total = 0.0;
+#pragma unroll 1
+  for (int tries = 0; tries < 2; ++tries) {
+    const double *const of = tries == 0 ? rest : all;  // nothing left: P is Q, but for roundings
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      w[h] = lane + 64 * h < p.count ? of[lane + 64 * h] : 0.0;
+      sum[h] = wave_prefix(w[h]);
+    }
+    sum[1] += __shfl(sum[0], 63);
+    total = __shfl(sum[1], 63);
+    if (total > 0.0) break;
+  }
   const double goal = a.params[request].uniform * total;
-  const uint64_t over = __ballot(v > 0.0 && sum > goal), some = __ballot(v > 0.0);
-  if ((t & 63) == 0) {
-    overs[t >> 6] = over;
-    somes[t >> 6] = some;
-  }
-  __syncthreads();
-  if (t == 0) {
-    int at = 0;
-    if (overs[0]) at = __builtin_ctzll(overs[0]);
-    else if (overs[1]) at = 64 + __builtin_ctzll(overs[1]);
-    else if (somes[1]) at = 127 - __builtin_clzll(somes[1]);
-    else if (somes[0]) at = 63 - __builtin_clzll(somes[0]);
-    tokens[n] = (int32_t)ids[at];
-  }
+  const uint64_t over[2] = {__ballot(w[0] > 0.0 && sum[0] > goal), __ballot(w[1] > 0.0 && sum[1] > goal)};
+  const uint64_t some[2] = {__ballot(w[0] > 0.0), __ballot(w[1] > 0.0)};
+  int at = 0;
+  if (over[0]) at = __builtin_ctzll(over[0]);
+  else if (over[1]) at = 64 + __builtin_ctzll(over[1]);
+  else if (some[1]) at = 127 - __builtin_clzll(some[1]);
+  else if (some[0]) at = 63 - __builtin_clzll(some[0]);
+  if (lane == 0) tokens[n] = (int32_t)ids[at];
 }
 
-// What a request draws from, over the whole vocabulary.
+// What a thread's elements of a segment weigh in a request's draw: `rest` of them is drawn from, or `all` where nothing rests.
 template <int DT>
 struct RestOf {
   using E = Elem<DT>;
   using Bits = typename E::Bits;
-  const Bits *target, *draft;
-  RowDist p, q;
-  double inverse, of_p, of_q;
-  Draw draw;
-  int token;
-  __device__ __forceinline__ RestOf(const VerifyArgs &a, int request, const Decision &d) {
-    const Setting set = setting_of(a, request);
-    const Place place = place_of(a, request);
-    const RowDist *dists = a.dists + (int64_t)request * a.slots;
-    draw = (Draw)d.draw;
-    inverse = set.inverse;
-    p = dists[d.accepted];
-    target = (const Bits *)a.logits + (int64_t)(place.first + d.accepted) * a.stride;
-    of_p = 1.0 / p.total;
-    q = p;
-    draft = target;
-    of_q = 0.0;
-    token = -1;
-    if (draw == kFromRest) {
-      q = dists[a.drafts_max + 1 + d.accepted];
-      draft = (const Bits *)a.draft_logits + (int64_t)(place.first_draft + d.accepted) * a.draft_stride;
-      of_q = 1.0 / q.total;
-    } else if (draw == kWithoutToken) {
-      token = a.drafts[place.first_draft + d.accepted];
-    }
+  static constexpr int kThreads = kSegment / E::kVec;  // 16 bytes to a thread
+  double rest[E::kVec], all[E::kVec];
+  static __device__ __forceinline__ double share(uint64_t threshold, float max, double inverse, double scale, float x, int e) {
+    if (!(x > -INFINITY) || composite(key_of(x), (uint32_t)e) < threshold) return 0.0;
+    return exp_or_none(((double)x - (double)max) * inverse) * scale;
   }
-  static __device__ __forceinline__ double share(const RowDist &d, double inverse, double scale, float x, int e) {
-    if (!(x > -INFINITY) || composite(key_of(x), (uint32_t)e) < d.threshold) return 0.0;
-    return exp_or_none(((double)x - (double)d.max) * inverse) * scale;
-  }
-  // The sums over this thread's 16 elements of a segment; each(element, rest, share).
-  template <class F>
-  __device__ __forceinline__ void each(int first, int vocab, F f) const {
-    constexpr int kOwn = kSegment / 256;
-    const int at = first + (int)threadIdx.x * kOwn;
+  __device__ __forceinline__ RestOf(const VerifyArgs &a, const Decision &d, int first) {
+    const int vocab = a.vocab;
+    float x[E::kVec], y[E::kVec];
+    const bool both = d.draw == kFromRest;
+    const u32x4 none = {0, 0, 0, 0};
+    const u32x4 p = first < vocab ? load_values<DT, false>((const Bits *)a.logits + d.target, first, vocab) : none;
+    const u32x4 q = both && first < vocab ? load_values<DT, false>((const Bits *)a.draft_logits + d.draft, first, vocab) : none;
+    E::widen16(p, x);
+    E::widen16(q, y);
 #pragma unroll
-    for (int g = 0; g < kOwn / E::kVec; ++g) {
-      const int e = at + g * E::kVec;
-      if (e >= vocab) break;
-      float x[E::kVec], y[E::kVec];
-      E::widen16(load_values<DT, false>(target, e, vocab), x);
-      if (draw == kFromRest) E::widen16(load_values<DT, false>(draft, e, vocab), y);
-#pragma unroll
-      for (int j = 0; j < E::kVec; ++j) {
-        if (e + j >= vocab) break;
-        const double v = share(p, inverse, of_p, x[j], e + j);
-        double left = v;
-        if (draw == kFromRest) left = fmax(v - share(q, inverse, of_q, y[j], e + j), 0.0);
-        else if (e + j == token) left = 0.0;
-        f(e + j, left, v);
-      }
+    for (int j = 0; j < E::kVec; ++j) {
+      const bool in = first + j < vocab;
+      all[j] = in ? share(d.threshold, d.max, d.inverse, d.of_target, x[j], first + j) : 0.0;
+      rest[j] = both ? fmax(all[j] - (in ? share(d.draft_threshold, d.draft_max, d.inverse, d.of_draft, y[j], first + j) : 0.0), 0.0)
+                     : first + j == d.token ? 0.0 : all[j];
     }
   }
 };
 
 template <int DT>
-__global__ __launch_bounds__(256) void verify_weigh_kernel(VerifyArgs a) {
-  __shared__ double wave_space[2][4];
+__global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_weigh_kernel(VerifyArgs a) {
+  constexpr int kWavesN = RestOf<DT>::kThreads / 64;
+  __shared__ double wave_space[2][kWavesN];
   const int request = (int)blockIdx.y, segment = (int)blockIdx.x, t = (int)threadIdx.x;
   const Decision d = a.decisions[request];
   if (d.draw == kDone) return;
-  const RestOf<DT> rest(a, request, d);
+  const RestOf<DT> own(a, d, segment * kSegment + t * RestOf<DT>::E::kVec);
   double left = 0.0, all = 0.0;
-  rest.each(segment * kSegment, a.vocab, [&](int, double r, double v) {
-    left += r;
-    all += v;
-  });
+#pragma unroll
+  for (int j = 0; j < RestOf<DT>::E::kVec; ++j) {
+    left += own.rest[j];
+    all += own.all[j];
+  }
   left = wave_sum(left);
   all = wave_sum(all);
   if ((t & 63) == 0) {
@@ -832,46 +1087,38 @@ __global__ __launch_bounds__(256) void verify_weigh_kernel(VerifyArgs a) {
     wave_space[1][t >> 6] = all;
   }
   __syncthreads();
-  if (t == 0) {
-    double2 sums{0.0, 0.0};
-    for (int w = 0; w < 4; ++w) {
-      sums.x += wave_space[0][w];
-      sums.y += wave_space[1][w];
-    }
-    a.segment_sums[(int64_t)request * a.segments + segment] = sums;
-  }
+  if (t >= 64) return;
+  left = wave_sum(t < kWavesN ? wave_space[0][t] : 0.0);
+  all = wave_sum(t < kWavesN ? wave_space[1][t] : 0.0);
+  if (t == 0) a.segment_sums[(int64_t)request * a.segments + segment] = double2{left, all};
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double wave_space[4], before_;
-  __shared__ int segment_, last_, token_;
+__global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_pick_kernel(VerifyArgs a) {
+  constexpr int kThreads = RestOf<DT>::kThreads, kWavesN = kThreads / 64;
+  __shared__ double wave_space[kWavesN], before_;
+  __shared__ int segment_, last_, token_, last_token_;
   const int request = (int)blockIdx.x, t = (int)threadIdx.x;
   const Decision d = a.decisions[request];
   if (d.draw == kDone) return;
-  const RestOf<DT> rest(a, request, d);
   const double2 *sums = a.segment_sums + (int64_t)request * a.segments;
   // A run of segments to a thread.
-  const int per = (a.segments + 255) / 256, begin = min(t * per, a.segments), end = min(begin + per, a.segments);
-  double own = 0.0, own_all = 0.0, total, total_all;
+  const int per = (a.segments + kThreads - 1) / kThreads, begin = min(t * per, a.segments), end = min(begin + per, a.segments);
+  double own = 0.0, own_all = 0.0, total;
   for (int i = begin; i < end; ++i) {
     own += sums[i].x;
     own_all += sums[i].y;
   }
-  double before = block_prefix<4>(own, wave_space, total) - own;
-  const double before_all = block_prefix<4>(own_all, wave_space, total_all) - own_all;
-  const bool plain = !(total > 0.0);  // nothing left: P is Q, but for roundings
-  if (plain) {
-    total = total_all;
-    before = before_all;
-  }
-  const double goal = a.params[request].uniform * total;
   if (t == 0) {
     segment_ = a.segments;
     last_ = -1;
     token_ = a.vocab;
+    last_token_ = -1;
   }
-  __syncthreads();
+  double before = block_prefix<kWavesN>(own, wave_space, total) - own;
+  const bool plain = !(total > 0.0);  // nothing left: P is Q, but for roundings
+  if (plain) before = block_prefix<kWavesN>(own_all, wave_space, total) - own_all;
+  const double goal = d.uniform * total;
   // The first segment whose running sum exceeds the share; the last with a weight where none does.
   double at = before;
   int found = a.segments, last = -1;
@@ -891,29 +1138,29 @@ __global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
   if (found < a.segments) atomicMin(&segment_, found);
   if (last >= 0) atomicMax(&last_, last);
   __syncthreads();
-  const int chosen = segment_ < a.segments ? segment_ : max(last_, 0);
-  if (found == chosen && segment_ < a.segments) before_ = found_before;
-  else if (last == chosen && segment_ == a.segments) before_ = last_before;
-  __syncthreads();
-  const double base = before_;
-  if (t == 0) last_ = -1;
-  __syncthreads();
+  const bool reached = segment_ < a.segments;
+  const int chosen = reached ? segment_ : max(last_, 0);
+  if ((reached ? found : last) == chosen) before_ = reached ? found_before : last_before;
+  const int first = chosen * kSegment + t * RestOf<DT>::E::kVec;
+  const RestOf<DT> weights(a, d, first);
   double sum = 0.0, all;
-  rest.each(chosen * kSegment, a.vocab, [&](int, double r, double v) { sum += plain ? v : r; });
-  double run = block_prefix<4>(sum, wave_space, all) - sum + base;
-  int first = a.vocab, some = -1;
-  rest.each(chosen * kSegment, a.vocab, [&](int e, double r, double v) {
-    const double w = plain ? v : r;
+#pragma unroll
+  for (int j = 0; j < RestOf<DT>::E::kVec; ++j) sum += plain ? weights.all[j] : weights.rest[j];
+  double run = block_prefix<kWavesN>(sum, wave_space, all) - sum + before_;
+  int token = a.vocab, some = -1;
+#pragma unroll
+  for (int j = 0; j < RestOf<DT>::E::kVec; ++j) {
+    const double w = plain ? weights.all[j] : weights.rest[j];
     run += w;
     if (w > 0.0) {
-      some = e;
-      if (first == a.vocab && run > goal) first = e;
+      some = first + j;
+      if (token == a.vocab && run > goal) token = first + j;
     }
-  });
-  if (first < a.vocab) atomicMin(&token_, first);
-  if (some >= 0) atomicMax(&last_, some);
+  }
+  if (token < a.vocab) atomicMin(&token_, token);
+  if (some >= 0) atomicMax(&last_token_, some);
   __syncthreads();
-  if (t == 0) a.tokens[(int64_t)request * (a.drafts_max + 1) + d.accepted] = token_ < a.vocab ? token_ : max(last_, 0);
+  if (t == 0) a.tokens[d.out] = token_ < a.vocab ? token_ : max(last_token_, 0);
 }
 
 int check_verify_shape(int32_t requests, int32_t drafts_max, int32_t vocab) {
@@ -938,13 +1185,15 @@ int verify_parts(int64_t rows, int vocab) {
 int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The workspace's arrays: where each begins, and the end.
-struct Space { int64_t sums, entries, dists, pools, decisions, segments, end; };
+struct Space { int64_t sums, entries, dists, bins, pools, decisions, segments, end; };
+constexpr int64_t kBinnedMax = 4096;  // lists (parts of rows) that have bins, 16 KB each
 Space space_of(int64_t requests, int64_t slots, int64_t lists, int64_t segments) {
   Space s;
   s.sums = 0;
   s.entries = s.sums + aligned(lists * (int64_t)sizeof(PartSum));
   s.dists = s.entries + aligned(lists * kPoolMax * 8);
-  s.pools = s.dists + aligned(requests * slots * (int64_t)sizeof(RowDist));
+  s.bins = s.dists + aligned(requests * slots * (int64_t)sizeof(RowDist));
+  s.pools = s.bins + std::min(lists, kBinnedMax) * kBins * 8;
   s.decisions = s.pools + aligned(requests * slots * kPoolMax * 8);
   s.segments = s.decisions + aligned(requests * (int64_t)sizeof(Decision));
   s.end = s.segments + aligned(requests * segments * (int64_t)sizeof(double2));
@@ -959,14 +1208,17 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   else if (blocks <= (unsigned)kCus && a.part_len > 8 * kChunk) hipLaunchKernelGGL((verify_rows_kernel<DT, 16>), dim3(blocks), dim3(1024), 0, s, a);
   else hipLaunchKernelGGL((verify_rows_kernel<DT, 8>), dim3(blocks), dim3(512), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3(rows), dim3(kSettleThreads), 0, s, a);
-  TABBY_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL(verify_decide_kernel, dim3((unsigned)a.requests), dim3(kDecideThreads), 0, s, a);
+  if (a.whole) {
+    hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3(rows), dim3(kSettleThreads), 0, s, a);
+    TABBY_HIP_CHECK(hipGetLastError());
+  }
+  if (a.slots <= 4) hipLaunchKernelGGL((verify_decide_kernel<DT, 4>), dim3((unsigned)a.requests), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((verify_decide_kernel<DT, 16>), dim3((unsigned)a.requests), dim3(1024), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   if (!a.whole) return TABBY_OK;
-  hipLaunchKernelGGL(verify_weigh_kernel<DT>, dim3((unsigned)a.segments, (unsigned)a.requests), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(verify_weigh_kernel<DT>, dim3((unsigned)a.segments, (unsigned)a.requests), dim3(RestOf<DT>::kThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL(verify_pick_kernel<DT>, dim3((unsigned)a.requests), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(verify_pick_kernel<DT>, dim3((unsigned)a.requests), dim3(RestOf<DT>::kThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
@@ -1023,13 +1275,14 @@ extern "C" int tabby_draft_verify_device(const void *logits_dev, int32_t dtype, 
   const int part_len = (int)((((int64_t)vocab + fit - 1) / fit + 31) / 32 * 32);
   const int used = (int)(((int64_t)vocab + part_len - 1) / part_len);
   const int segments = (vocab + kSegment - 1) / kSegment;
-  const Space space = space_of(requests, slots, (int64_t)requests * slots * used, segments);
+  const int64_t lists = (int64_t)requests * slots * used;
+  const Space space = space_of(requests, slots, lists, segments);
   char *w = (char *)workspace_dev;
   VerifyArgs a{logits_dev, draft_logits_dev, row_stride, draft_row_stride, drafts_dev, uniforms_dev, offsets_dev, params_dev,
                rows, requests, drafts_max, vocab, slots, (flags & TABBY_FLAG_FULL_VOCAB) != 0, used, part_len, segments,
                tokens_dev, accepted_dev, status_dev, (PartSum *)(w + space.sums), (uint64_t *)(w + space.entries),
-               (RowDist *)(w + space.dists), (uint64_t *)(w + space.pools), (Decision *)(w + space.decisions),
-               (double2 *)(w + space.segments)};
+               (RowDist *)(w + space.dists), lists <= kBinnedMax ? (uint64_t *)(w + space.bins) : nullptr,
+               (uint64_t *)(w + space.pools), (Decision *)(w + space.decisions), (double2 *)(w + space.segments)};
   // What is written lies apart from what is read.
   const RowSpan outputs[] = {row_span(tokens_dev, 1, (int64_t)requests * (drafts_max + 1), 0, 4), row_span(accepted_dev, 1, requests, 0, 4),
                              row_span(status_dev, 1, status_dev ? requests : 0, 0, 4), row_span(workspace_dev, 1, need, 0, 1)};

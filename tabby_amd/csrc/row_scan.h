@@ -20,15 +20,8 @@ constexpr int kListMax = 4096;                // entries above the bound that LD
 
 typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
 
-// exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
-// and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]; for 2^f the
-// polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it. A sum of such terms
-// decides the order of two beams' continuations only where their scores are that close.
-__device__ __forceinline__ double exp_64(double d) {
-  constexpr double kLog2e = 1.4426950408889634;
-  const double magic = 6755399441055744.0;
-  const double shifted = __builtin_fma(d, kLog2e, magic);
-  const double f = __builtin_fma(d, kLog2e, -(shifted - magic));
+// 2^f in 64 bits for f in [-1/2, 1/2]: the polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it.
+__device__ __forceinline__ double exp2_64(double f) {
   double p = 1.530370102315244e-05;
   p = __builtin_fma(p, f, 0.0001546972921563772);
   p = __builtin_fma(p, f, 0.0013333478472326247);
@@ -36,8 +29,17 @@ __device__ __forceinline__ double exp_64(double d) {
   p = __builtin_fma(p, f, 0.055504109063275894);
   p = __builtin_fma(p, f, 0.24022651213498245);
   p = __builtin_fma(p, f, 0.6931471805568318);
-  p = __builtin_fma(p, f, 0.9999999999595618);
-  uint32x2 bits = __builtin_bit_cast(uint32x2, p);
+  return __builtin_fma(p, f, 0.9999999999595618);
+}
+
+// exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
+// and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]. A sum of such terms
+// decides the order of two beams' continuations only where their scores are that close.
+__device__ __forceinline__ double exp_64(double d) {
+  constexpr double kLog2e = 1.4426950408889634;
+  const double magic = 6755399441055744.0;
+  const double shifted = __builtin_fma(d, kLog2e, magic);
+  uint32x2 bits = __builtin_bit_cast(uint32x2, exp2_64(__builtin_fma(d, kLog2e, -(shifted - magic))));
   bits.y += __builtin_bit_cast(uint32x2, shifted).x << 20;
   return __builtin_bit_cast(double, bits);
 }
