@@ -41,6 +41,7 @@ constexpr int kDraftsMax = 63;                // of a request: one wave decides
 constexpr int kVerifyVocabMax = 1 << 24;      // masses of a row's entries are added up as whole multiples of 2^-38 or less
 constexpr int64_t kBlocksMax = (1 << 22) - 1;  // of 1,024 threads each
 constexpr int kPartsMax = 32;
+constexpr int kBlocksAimed = 512;
 constexpr int kSegment = 4096;                // elements of a segment
 
 enum Kind : int32_t { kInvalid = 0, kGreedy, kPool, kWhole };
@@ -181,7 +182,7 @@ struct RowBins {
     const double shifted = octaves + magic;
     n = (int)__builtin_bit_cast(uint32x2, shifted).x;
     f = octaves - (shifted - magic);
-    const int part = (int)__builtin_bit_cast(uint32x2, __builtin_fma(f, 16.0, magic + 8.0)).x;
+    const int part = (int)__builtin_bit_cast(uint32x2, fma_const(f, 16.0, magic + 8.0)).x;
     return ((n + kOctavesBelow) << 4) + max(min(part, 15), 0);
   }
   // For any logit: below the bins or above them where they do not hold it.
@@ -305,16 +306,24 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
         far |= bins.octaves(top) > (double)kOctavesAbove - 1.0;
         largest = fmaxf(largest, top);
         if (__ballot(far) != 0) continue;
+        // Entries below the bins are no number of theirs, and far less than a sum tells: they count as the lowest bin's.
+        if (masses) {
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) {
-          const double octaves = bins.octaves(x[i]);
-          if (!(octaves > -(double)kOctavesBelow)) continue;  // nothing of it is left in a sum
-          double f;
-          int n;
-          const int at = bins.place(octaves, f, n);
-          uint64_t add = 1;
-          if (masses) add = (uint64_t)__double_as_longlong(__builtin_fma(exp2_64(f), unit, 0x1p52)) & ((1ull << 52) - 1);
-          atomicAdd((unsigned long long *)&lds.bins[max(at, 0)], (unsigned long long)add);
+          for (int i = 0; i < kLane; ++i) {
+            double f;
+            int n;
+            const int at = bins.place(fmax(bins.octaves(x[i]), -(double)kOctavesBelow), f, n);
+            const uint64_t add = (uint64_t)__double_as_longlong(fma_const(exp2_64(f), unit, 0x1p52)) & ((1ull << 52) - 1);
+            atomicAdd((unsigned long long *)&lds.bins[at], (unsigned long long)add);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLane; ++i) {
+            double f;
+            int n;
+            const int at = bins.place(fmax(bins.octaves(x[i]), -(double)kOctavesBelow), f, n);
+            atomicAdd((unsigned long long *)&lds.bins[at], 1ull);
+          }
         }
       } while (advance());
     }
@@ -680,7 +689,7 @@ __global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArg
     }
     __syncthreads();
     const int found = (int)s.found_bin;
-    if (found < kBins) {
+    if (found < kBins && found > 0) {  // the lowest bin counts what lies below it as well
       least = bin_begin(bins, found);
       if (!by_count) {
         most = bin_begin(bins, found + 1);
@@ -1173,12 +1182,11 @@ int check_verify_shape(int32_t requests, int32_t drafts_max, int32_t vocab) {
   return TABBY_OK;
 }
 
-constexpr int kCus = 256;       // an MI355X's compute units
 constexpr int kPartMin = 8192;  // a chunk to each of eight waves
 
-// Few rows are cut into parts, a workgroup each, until there is about one to a compute unit.
+// Rows are cut into parts, a workgroup each, until there are some to a compute unit.
 int verify_parts(int64_t rows, int vocab) {
-  const int64_t parts = std::min<int64_t>({kCus / std::max<int64_t>(rows, 1), (vocab + kPartMin - 1) / kPartMin, kPartsMax});
+  const int64_t parts = std::min<int64_t>({kBlocksAimed / std::max<int64_t>(rows, 1), (vocab + kPartMin - 1) / kPartMin, kPartsMax});
   return (int)std::max<int64_t>(parts, 1);
 }
 
@@ -1205,7 +1213,7 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   const unsigned rows = (unsigned)(a.requests * a.slots), blocks = rows * (unsigned)a.parts;
   // Four or eight waves where they have a chunk each. Else, up to a workgroup for each compute unit, sixteen.
   if (a.part_len <= 4 * kChunk) hipLaunchKernelGGL((verify_rows_kernel<DT, 4>), dim3(blocks), dim3(256), 0, s, a);
-  else if (blocks <= (unsigned)kCus && a.part_len > 8 * kChunk) hipLaunchKernelGGL((verify_rows_kernel<DT, 16>), dim3(blocks), dim3(1024), 0, s, a);
+  else if (blocks <= 256u && a.part_len > 8 * kChunk) hipLaunchKernelGGL((verify_rows_kernel<DT, 16>), dim3(blocks), dim3(1024), 0, s, a);
   else hipLaunchKernelGGL((verify_rows_kernel<DT, 8>), dim3(blocks), dim3(512), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   if (a.whole) {
@@ -1232,8 +1240,8 @@ extern "C" int tabby_draft_workspace(int32_t requests, int32_t drafts_max, int32
   if (!bytes) return record_failure(TABBY_EINVAL, "null pointer");
   const int rc = check_verify_shape(requests, drafts_max, vocab);
   if (rc) return rc;
-  // For these sizes and every smaller one: rows that are cut make at most kCus parts.
-  const int64_t slots = 2 * drafts_max + 1, lists = std::max<int64_t>(requests * slots, kCus);
+  // For these sizes and every smaller one: rows that are cut make at most kBlocksAimed parts.
+  const int64_t slots = 2 * drafts_max + 1, lists = std::max<int64_t>(requests * slots, kBlocksAimed);
   *bytes = space_of(requests, slots, lists, ((int64_t)vocab + kSegment - 1) / kSegment).end;
   return TABBY_OK;
 }
@@ -1271,7 +1279,7 @@ extern "C" int tabby_draft_verify_device(const void *logits_dev, int32_t dtype, 
   const int slots = drafts_max + 1 + (draft_logits_dev ? drafts_max : 0);
   const int parts = verify_parts(rows + (draft_logits_dev ? total : 0), vocab);
   // Slots that no row fills take parts as well, which the workspace has to hold.
-  const int fit = (int)std::max<int64_t>(1, std::min<int64_t>(parts, std::max<int64_t>((int64_t)requests * (2 * drafts_max + 1), kCus) / ((int64_t)requests * slots)));
+  const int fit = (int)std::max<int64_t>(1, std::min<int64_t>(parts, std::max<int64_t>((int64_t)requests * (2 * drafts_max + 1), kBlocksAimed) / ((int64_t)requests * slots)));
   const int part_len = (int)((((int64_t)vocab + fit - 1) / fit + 31) / 32 * 32);
   const int used = (int)(((int64_t)vocab + part_len - 1) / part_len);
   const int segments = (vocab + kSegment - 1) / kSegment;

@@ -20,16 +20,22 @@ constexpr int kListMax = 4096;                // entries above the bound that LD
 
 typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
 
+// a b + c, c a constant: written out, because the compiler copies c to registers first to add to it there.
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+}
+
 // 2^f in 64 bits for f in [-1/2, 1/2]: the polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it.
 __device__ __forceinline__ double exp2_64(double f) {
-  double p = 1.530370102315244e-05;
-  p = __builtin_fma(p, f, 0.0001546972921563772);
-  p = __builtin_fma(p, f, 0.0013333478472326247);
-  p = __builtin_fma(p, f, 0.009618025613309008);
-  p = __builtin_fma(p, f, 0.055504109063275894);
-  p = __builtin_fma(p, f, 0.24022651213498245);
-  p = __builtin_fma(p, f, 0.6931471805568318);
-  return __builtin_fma(p, f, 0.9999999999595618);
+  double p = fma_const(f, 1.530370102315244e-05, 0.0001546972921563772);
+  p = fma_const(p, f, 0.0013333478472326247);
+  p = fma_const(p, f, 0.009618025613309008);
+  p = fma_const(p, f, 0.055504109063275894);
+  p = fma_const(p, f, 0.24022651213498245);
+  p = fma_const(p, f, 0.6931471805568318);
+  return fma_const(p, f, 0.9999999999595618);
 }
 
 // exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
