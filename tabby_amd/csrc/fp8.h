@@ -75,6 +75,34 @@ __device__ __forceinline__ void f8_decode4(uint32_t word, float *v) {
   v[3] = b[1];
 }
 
+// The largest magnitude of 16 bytes, as f32 bits; what is no number is larger than any.
+template <int DT>
+__device__ __forceinline__ uint32_t f8_largest(u32x4 raw) {
+  using E = Elem<DT>;
+  float v[E::kVec];
+  E::widen16(raw, v);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < E::kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  return top;
+}
+
+// The codes of 16 bytes, to LDS.
+template <int DT>
+__device__ __forceinline__ void f8_encode(uint8_t *to, u32x4 raw, float inverse) {
+  using E = Elem<DT>;
+  float v[E::kVec];
+  E::widen16(raw, v);
+  uint32_t word[E::kVec / 4];
+#pragma unroll
+  for (int i = 0; i < E::kVec / 4; ++i) {
+    word[i] = f8_encode4(v[4 * i] * inverse, v[4 * i + 1] * inverse, v[4 * i + 2] * inverse, v[4 * i + 3] * inverse);
+    if (inverse == 0.0f) word[i] = 0;  // a block that is NaN as a whole
+  }
+  if constexpr (E::kVec == 4) *reinterpret_cast<uint32_t *>(to) = word[0];
+  else *reinterpret_cast<uint64_t *>(to) = word[0] | ((uint64_t)word[1] << 32);
+}
+
 // Where the code of row r, column c of a panel lies in it.
 __device__ __forceinline__ int f8_code_byte(int r, int c) {
   return (r >> 4) * kF8TileBytes + ((c >> 4) & 1) * (kF8TileBytes / 2) + ((r & 15) + 16 * (c >> 5)) * 16 + (c & 15);

@@ -32,34 +32,6 @@ struct BlockWalk {
       : row((int)threadIdx.x / kRowLanes), col((int)threadIdx.x % kRowLanes * E::kVec) {}
 };
 
-// The largest magnitude of 16 bytes, as f32 bits; what is no number is larger than any.
-template <int DT>
-__device__ __forceinline__ uint32_t largest_bits(u32x4 raw) {
-  using E = Elem<DT>;
-  float v[E::kVec];
-  E::widen16(raw, v);
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < E::kVec; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  return top;
-}
-
-// The codes of 16 bytes, to LDS.
-template <int DT>
-__device__ __forceinline__ void encode_to(uint8_t *to, u32x4 raw, float inverse) {
-  using E = Elem<DT>;
-  float v[E::kVec];
-  E::widen16(raw, v);
-  uint32_t word[E::kVec / 4];
-#pragma unroll
-  for (int i = 0; i < E::kVec / 4; ++i) {
-    word[i] = f8_encode4(v[4 * i] * inverse, v[4 * i + 1] * inverse, v[4 * i + 2] * inverse, v[4 * i + 3] * inverse);
-    if (inverse == 0.0f) word[i] = 0;  // a block that is NaN as a whole
-  }
-  if constexpr (E::kVec == 4) *reinterpret_cast<uint32_t *>(to) = word[0];
-  else *reinterpret_cast<uint64_t *>(to) = word[0] | ((uint64_t)word[1] << 32);
-}
-
 template <int DT, int BR, bool WHOLE>
 __global__ __launch_bounds__(BR == 1 ? 256 : 512) void fp8_quantize_kernel(const typename Elem<DT>::Bits *x, int rows, int cols,
                                                                            int64_t stride, uint8_t *codes, float *scales) {
@@ -86,18 +58,18 @@ __global__ __launch_bounds__(BR == 1 ? 256 : 512) void fp8_quantize_kernel(const
 #pragma unroll
       for (int i = 0; i < Walk::kSteps; ++i) {
         const int r = walk.row + i * Walk::kRowStep;
-        uint32_t top = largest_bits<DT>(raw[i]);
+        uint32_t top = f8_largest<DT>(raw[i]);
 #pragma unroll
         for (int lanes = 1; lanes < Walk::kRowLanes; lanes *= 2) top = max(top, xor_lane_by(top, lanes));
         float scale, inverse;
         f8_scale(top, scale, inverse);
-        encode_to<DT>(&held[f8_code_byte(r, walk.col)], raw[i], inverse);
+        f8_encode<DT>(&held[f8_code_byte(r, walk.col)], raw[i], inverse);
         if (walk.col == 0) row_scales[r] = scale;
       }
     } else {
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < Walk::kSteps; ++i) top = max(top, largest_bits<DT>(raw[i]));
+      for (int i = 0; i < Walk::kSteps; ++i) top = max(top, f8_largest<DT>(raw[i]));
       top = wave_max_u32(top);
       if ((t & 63) == 0) wave_top[t >> 6] = top;
       __syncthreads();
@@ -108,7 +80,7 @@ __global__ __launch_bounds__(BR == 1 ? 256 : 512) void fp8_quantize_kernel(const
 #pragma unroll
       for (int i = 0; i < Walk::kSteps; ++i) {
         const int r = walk.row + i * Walk::kRowStep;
-        encode_to<DT>(&held[r / kF8PanelRows * kF8PanelBytes + f8_code_byte(r % kF8PanelRows, walk.col)], raw[i], inverse);
+        f8_encode<DT>(&held[r / kF8PanelRows * kF8PanelBytes + f8_code_byte(r % kF8PanelRows, walk.col)], raw[i], inverse);
       }
       if (t == 0) scales[block] = scale;
     }

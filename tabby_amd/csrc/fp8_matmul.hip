@@ -85,6 +85,12 @@ __device__ __forceinline__ void add_scaled(f32x4 &acc, f32x4 t, float s) {
   for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(t[i], s, acc[i]);
 }
 
+// A square block's scale, the same for the whole wave: by the scalar unit, whose loads no wait for the vector ones holds up.
+__device__ __forceinline__ float block_scale_at(const float *scales, int64_t at) {
+  typedef const __attribute__((address_space(4))) float Constant;
+  return ((Constant *)(uintptr_t)scales)[at];
+}
+
 struct Fp8Product {
   Fp8Matrix w, x;  // square blocks; blocks of one row
   ProductOut y;
@@ -93,8 +99,9 @@ struct Fp8Product {
 // A workgroup of WM x WN waves has a tile of WM PM x WN PN panels of Y (64 x 64), PM x PN to a wave, and takes a
 // panel of k (128) at a time. The panels of a stage lie in LDS as they do in memory, W's before X's, then X's scales,
 // brought there without passing through registers, a stage ahead. A wave holds the tiles of X and goes through those
-// of W; a tile's results are added while the next one's products run.
-template <int PM, int PN, int WM, int WN>
+// of W; a tile's results are added while the next one's products run. Where there are few tiles, KG groups of such waves
+// take every KG-th panel of k, each with stages of its own, and add up through LDS.
+template <int PM, int PN, int WM, int WN, int KG>
 struct TileShape {
   static constexpr int kWaves = WM * WN;
   static constexpr int kPanels = WM * PM + WN * PN;
@@ -104,7 +111,8 @@ struct TileShape {
   static constexpr int kTiles = 4 * kPanels / kWaves;  // tiles that a wave brings to a stage
   static_assert(4 * kPanels % kWaves == 0, "every wave brings as much");
   static_assert(PM <= 2, "a wave's panels of W lie in one square block");
-  static constexpr int kLoads = 2 * kTiles + 1;
+  static constexpr int kLds = KG * kStages * kStage;
+  static_assert(KG == 1 || (KG == 2 && kWaves * PM * PN * 16 * 1024 <= kLds), "a group's sums find room");
 };
 
 __device__ __forceinline__ void bring_tile(const uint8_t *from, uint8_t *to) {
@@ -116,15 +124,17 @@ __device__ __forceinline__ void bring_scales(const uint8_t *from, uint8_t *to) {
   __builtin_amdgcn_global_load_lds((GlobalVoid *)from, (LdsVoid *)to, 4, 0, 0);
 }
 
-template <int DT, int PM, int PN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, int tiles_w, int tiles_x) {
-  using S = TileShape<PM, PN, WM, WN>;
+template <int DT, int PM, int PN, int WM, int WN, int KG>
+__global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, int tiles_w, int tiles_x) {
+  using S = TileShape<PM, PN, WM, WN, KG>;
   using Operand = typename std::conditional<DT == TABBY_F32, HalfOperand, CodeOperand>::type;
-  __shared__ __align__(1024) uint8_t lds[S::kStages][S::kStage];
+  __shared__ __align__(1024) uint8_t all_lds[S::kLds];
   const int lane = (int)threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int all_waves = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int group = all_waves / S::kWaves, wave = all_waves % S::kWaves;
   const int wm = wave % WM, wn = wave / WM;
   const int kp = p.w.col_panels();
+  uint8_t(*const lds)[S::kStage] = reinterpret_cast<uint8_t(*)[S::kStage]>(all_lds + group * S::kStages * S::kStage);
   const TilePlace place = tile_place((int)blockIdx.x, tiles_w, tiles_x);
 
   // Panels past the last are the last again; what they give is not stored.
@@ -141,17 +151,20 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, 
   }
   const int scales_of = wave % (WN * PN);  // twice or more where there are more waves
   const uint8_t *x_scales = (const uint8_t *)p.x.scales + panel_at(WM * PM + scales_of) * kF8PanelScales + lane * 4;
-  int brought = 0;
-  auto bring = [&](uint8_t *stage) {
-    // Past the last panel of k it is the last one again, which nothing reads: every stage has as many loads.
-    const int step = ++brought < kp ? 1 : 0;
+  int at = 0;  // the panel of k that comes next
+  auto advance = [&](int to) {
+    // Past the last panel of k it is the last one again, which nothing uses: every stage has as many loads.
+    const int step = min(to, kp - 1) - at;
+    at += step;
 #pragma unroll
-    for (int h = 0; h < S::kTiles; ++h) {
-      bring_tile(codes[h], stage + (wave * S::kTiles + h) * kF8TileBytes);
-      codes[h] += step * kF8PanelBytes;
-    }
-    bring_scales(x_scales, stage + S::kCodes + scales_of * kF8PanelScales);
+    for (int h = 0; h < S::kTiles; ++h) codes[h] += step * kF8PanelBytes;
     x_scales += step * kF8PanelScales;
+  };
+  advance(group);
+  auto bring = [&](uint8_t *stage) {
+#pragma unroll
+    for (int h = 0; h < S::kTiles; ++h) bring_tile(codes[h], stage + (wave * S::kTiles + h) * kF8TileBytes);
+    bring_scales(x_scales, stage + S::kCodes + scales_of * kF8PanelScales);
   };
   // The wave's panels of W lie in one square block.
   const float *w_scales = p.w.scales + (int64_t)(min((place.w * WM + wm) * PM, w_panels - 1) >> 1) * kp;
@@ -162,37 +175,57 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, 
   const int sx_from = S::kCodes + wn * PN * kF8PanelScales + (lane & 15) * 4;
   bring(lds[0]);
   int now = 0;
-  for (int k = 0; k < kp; ++k) {
+  float sw = block_scale_at(w_scales, at);
+  for (int first = 0; first < kp; first += KG) {
+    const bool works = first + group < kp;  // the last group may have a panel less
     wait_and_meet<0>();
     const uint8_t *stage = lds[now];
     now ^= 1;
+    advance(first + group + KG);
     bring(lds[now]);
-    const float sw = w_scales[k];
+    const float sw_next = block_scale_at(w_scales, at);
+    if (KG > 1 && !works) continue;
     Operand x[kX];
-    TileCodes w[2];
+    TileCodes w[3];
     float s[kX];
     w[0] = read_tile(stage + w_from);
 #pragma unroll
-    for (int c = 0; c < kX; ++c) {
-      x[c] = Operand(read_tile(stage + x_from + c * kF8TileBytes));
-      s[c] = *reinterpret_cast<const float *>(stage + sx_from + c * 64) * sw;
-    }
+    for (int c = 0; c < kX; ++c) x[c] = Operand(read_tile(stage + x_from + c * kF8TileBytes));
+    w[1] = read_tile(stage + w_from + kF8TileBytes);
+#pragma unroll
+    for (int c = 0; c < kX; ++c) s[c] = *reinterpret_cast<const float *>(stage + sx_from + c * 64) * sw;
     f32x4 t[2][kX];
 #pragma unroll
     for (int r = 0; r < kW; ++r) {
-      if (r + 1 < kW) w[(r + 1) & 1] = read_tile(stage + w_from + (r + 1) * kF8TileBytes);
-      const Operand of_w(w[r & 1]);
+      // Two tiles ahead of the products.
+      if (r + 2 < kW) w[(r + 2) % 3] = read_tile(stage + w_from + (r + 2) * kF8TileBytes);
+      __builtin_amdgcn_sched_barrier(0);
+      const Operand of_w(w[r % 3]);
 #pragma unroll
-      for (int c = 0; c < kX; ++c) t[r & 1][c] = tile_product(of_w, x[c]);
-      if (r > 0) {
-#pragma unroll
-        for (int c = 0; c < kX; ++c) add_scaled(acc[r - 1][c], t[(r - 1) & 1][c], s[c]);
+      for (int c = 0; c < kX; ++c) {
+        // A product is on its way while an earlier one's results are added: in this order, or they would be waited for.
+        t[r & 1][c] = tile_product(of_w, x[c]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (r > 0) add_scaled(acc[r - 1][c], t[(r - 1) & 1][c], s[c]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 #pragma unroll
     for (int c = 0; c < kX; ++c) add_scaled(acc[kW - 1][c], t[(kW - 1) & 1][c], s[c]);
+    sw = sw_next;
   }
   wait_and_meet<0>();
+  if constexpr (KG > 1) {
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(all_lds) + wave * kW * kX * 64 + lane;
+    if (group == 1) {
+#pragma unroll
+      for (int i = 0; i < kW * kX; ++i) sums[i * 64] = acc[i / kX][i % kX];
+    }
+    __syncthreads();
+    if (group == 1) return;
+#pragma unroll
+    for (int i = 0; i < kW * kX; ++i) acc[i / kX][i % kX] += sums[i * 64];
+  }
 #pragma unroll
   for (int i = 0; i < PM; ++i) {
 #pragma unroll
@@ -206,73 +239,192 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, 
 
 // Few rows: W is streamed from memory straight into registers, a wave to a panel of 64 columns of Y and
 // NT tiles of 16 rows; where there are few panels, `slices` waves of the workgroup take a part of k each and add up
-// through LDS.
+// through LDS. The registers of a tile of W take the next panel's as soon as the tile is read, so a panel is on its way
+// all the time (two for one tile of rows, which leaves the registers). Workgroups of four waves where the slices allow:
+// one token, W of 151,936 x 896: 27 us, of which the weights' 136 MB need 21 to 26; workgroups of eight took 30 us.
 struct FewShape {
   int waves, slices;  // of a workgroup; powers of two
 };
 constexpr int kSlicesMax = 8;
 constexpr int kSumsMax = 16;  // slices * NT
+constexpr int kFewWaves = 8;
+constexpr int kFewWavesMin = 4;
 // The upper half of the slices' sums lie in LDS, 4 KB to a wave's tile of rows.
 __host__ __device__ constexpr int sums_bytes(int waves, int tiles) { return waves / 2 * tiles * 4096; }
+constexpr int kStepBytes = kF8TileBytes + 64;  // codes and scales of 16 rows, 128 columns
 
-template <int DT, int NT>
-__global__ __launch_bounds__(kSlicesMax * 64) void fp8_few_kernel(Fp8Product p, FewShape shape) {
-  __shared__ __align__(16) uint8_t lds[std::max(sums_bytes(4, NT), sums_bytes(std::min(kSlicesMax, kSumsMax / NT), NT))];
+// The tiles of X as they are held.
+template <int NT>
+struct HeldTiles {
+  using Args = Fp8Matrix;
+  static constexpr int kTiles = NT;
+  static constexpr bool kFills = false;
+  static constexpr int kAhead = NT == 1 ? 2 : 1;
+  static constexpr int kLds = sums_bytes(kFewWaves, NT);
+  struct Raw {
+    TileCodes x[NT];
+    float scale[NT];
+  };
+  const uint8_t *codes;
+  const float *scales;
+  __device__ __forceinline__ HeldTiles(const Fp8Matrix &m, const uint8_t *, int tile, int lane) {
+    // NT tiles from `tile` on lie in one panel.
+    const int64_t panel = (int64_t)(tile >> 2) * m.col_panels();
+    codes = m.codes + panel * kF8PanelBytes + (tile & 3) * kF8TileBytes + lane * 16;
+    scales = m.scales + panel * kF8PanelRows + (tile & 3) * kF8TileRows + (lane & 15);
+  }
+  static __device__ __forceinline__ void fill(const Fp8Matrix &, uint8_t *, int) {}
+  __device__ __forceinline__ void load(int k, Raw &r) const {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      r.x[u] = read_tile(codes + (int64_t)k * kF8PanelBytes + u * kF8TileBytes);
+      r.scale[u] = scales[(int64_t)k * kF8PanelRows + u * kF8TileRows];
+    }
+  }
+  __device__ __forceinline__ HalfOperand tile(const Raw &r, int, int u, float &scale) const {
+    scale = r.scale[u];
+    return HalfOperand(r.x[u]);
+  }
+};
+
+// Up to 16 rows of x's own values, kFillPanels blocks at most: every workgroup quantises all of them into LDS while its
+// first panels of W are on their way. Rows past the last hold anything.
+constexpr int kFillPanels = 32;
+
+struct FloatRows {
+  const void *x;
+  int64_t stride;
+  int rows, cols;
+};
+
+template <int XDT>
+struct FloatTiles {
+  using E = Elem<XDT>;
+  using Args = FloatRows;
+  static constexpr int kTiles = 1;
+  static constexpr bool kFills = true;
+  static constexpr int kAhead = 2;
+  static constexpr int kBlockLanes = kF8Block / E::kVec;  // they lie together: the workgroup's threads are a multiple
+  static constexpr int kLoads = kFillPanels * kBlockLanes / (kFewWavesMin * 64);  // of a thread, 16 bytes each
+  static constexpr int kLds = kFillPanels * kStepBytes;
+  static_assert(kLds >= sums_bytes(kFewWaves, 1), "the slices' sums find room");
+  struct Raw {};
+  const uint8_t *codes;
+  __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int lane) : codes(lds + lane * 16) {}
+  static __device__ __forceinline__ void fill(const FloatRows &a, uint8_t *lds, int kp) {
+    const int row_lanes = kp * kBlockLanes, all = a.rows * row_lanes;
+    const float per_row = 1.0f / (float)row_lanes;  // all <= 2^10: (i + 1/2) / row_lanes has bits to spare
+    u32x4 raw[kLoads];
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int i = n * (int)blockDim.x + (int)threadIdx.x, r = (int)(((float)i + 0.5f) * per_row);
+      raw[n] = i < all ? load_values<XDT, false>((const typename E::Bits *)a.x + (int64_t)r * a.stride, (i - r * row_lanes) * E::kVec, a.cols) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int i = n * (int)blockDim.x + (int)threadIdx.x, r = (int)(((float)i + 0.5f) * per_row);
+      const int at = i - r * row_lanes;
+      uint32_t top = f8_largest<XDT>(raw[n]);
+#pragma unroll
+      for (int lanes = 1; lanes < kBlockLanes; lanes *= 2) top = max(top, xor_lane_by(top, lanes));
+      float scale, inverse;
+      f8_scale(top, scale, inverse);
+      if (i >= all) break;
+      uint8_t *to = lds + at / kBlockLanes * kStepBytes;
+      f8_encode<XDT>(to + f8_code_byte(r, at % kBlockLanes * E::kVec), raw[n], inverse);
+      if (at % kBlockLanes == 0) reinterpret_cast<float *>(to + kF8TileBytes)[r] = scale;
+    }
+  }
+  __device__ __forceinline__ void load(int, Raw &) const {}
+  __device__ __forceinline__ HalfOperand tile(const Raw &, int k, int, float &scale) const {
+    const uint8_t *at = codes + k * kStepBytes;
+    scale = *reinterpret_cast<const float *>(at - (int)(threadIdx.x & 63) * 16 + kF8TileBytes + (threadIdx.x & 15) * 4);
+    return HalfOperand(read_tile(at));
+  }
+};
+
+template <int DT, typename Rows>
+__global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p, typename Rows::Args xs, FewShape shape) {
+  constexpr int NT = Rows::kTiles;
+  __shared__ __align__(16) uint8_t lds[Rows::kLds];
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int slice = wave & (shape.slices - 1);
   const int panel = (int)blockIdx.x * (shape.waves / shape.slices) + wave / shape.slices;
   const int kp = p.w.col_panels();
   const int tile = (int)blockIdx.y * NT;
-  f32x4 acc[4][NT] = {};
-  struct Step {
-    TileCodes w[4], x[NT];
-    float sx[NT], sw;
-  };
   // A wave past the last panel has nothing to do but to meet the others.
   const bool works = panel * kF8PanelRows < p.w.rows;
+  const Rows rows(xs, lds, tile, lane);
   const uint8_t *wc = p.w.codes + (int64_t)panel * kp * kF8PanelBytes + lane * 16;
   const float *ws = p.w.scales + (int64_t)(panel >> 1) * kp;
-  // NT tiles from `tile` on lie in one panel.
-  const int64_t x_panel = (int64_t)(tile >> 2) * kp;
-  const uint8_t *xc = p.x.codes + x_panel * kF8PanelBytes + (tile & 3) * kF8TileBytes + lane * 16;
-  const float *xs = p.x.scales + x_panel * kF8PanelRows + (tile & 3) * kF8TileRows + (lane & 15);
   int k = (int)((int64_t)kp * slice / shape.slices);
   const int end = works ? (int)((int64_t)kp * (slice + 1) / shape.slices) : k;
-  auto load = [&](int at, Step &s) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) s.w[t] = read_tile(wc + (int64_t)at * kF8PanelBytes + t * kF8TileBytes);
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      s.x[u] = read_tile(xc + (int64_t)at * kF8PanelBytes + u * kF8TileBytes);
-      s.sx[u] = xs[(int64_t)at * kF8PanelRows + u * kF8TileRows];
-    }
-    s.sw = ws[at];
-  };
-  auto multiply = [&](const Step &s) {
+  // The panels of W that come next, two or one; a tile's registers take the one after as soon as it is read.
+  constexpr int kAhead = Rows::kAhead;
+  struct Step {
+    TileCodes w[4];
+    float scale;
+  } steps[kAhead];
+  auto bring = [&](int at, Step &s, int t) { s.w[t] = read_tile(wc + (int64_t)at * kF8PanelBytes + t * kF8TileBytes); };
+  typename Rows::Raw raw;
+  f32x4 acc[4][NT] = {};
+  auto multiply = [&](int at, Step &s, auto more) {
+    constexpr bool kMore = decltype(more)::value != 0;
     HalfOperand x[NT];
     float both[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      x[u] = HalfOperand(s.x[u]);
-      both[u] = s.sx[u] * s.sw;
+      x[u] = rows.tile(raw, at, u, both[u]);
+      both[u] *= s.scale;
     }
+    rows.load(min(at + 1, end - 1), raw);
+    if constexpr (kMore) s.scale = block_scale_at(ws, at + kAhead);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const HalfOperand w(s.w[t]);
+      if constexpr (kMore) bring(at + kAhead, s, t);
 #pragma unroll
       for (int u = 0; u < NT; ++u) add_scaled(acc[t][u], tile_product(w, x[u]), both[u]);
     }
   };
-  Step now, next;
-  if (k < end) load(k, now);
-  for (; k + 1 < end; ++k) {
-    load(k + 1, next);
-    multiply(now);
-    now = next;
+  if (k < end) {
+    rows.load(k, raw);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int at = min(k + a, end - 1);
+      steps[a].scale = block_scale_at(ws, at);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) bring(at, steps[a], t);
+    }
   }
-  if (k < end) multiply(now);
+  if constexpr (Rows::kFills) {
+    Rows::fill(xs, lds, kp);
+    __syncthreads();
+  }
+  constexpr Const<1> kWith;
+  constexpr Const<0> kWithout;
+  if constexpr (kAhead == 1) {
+    for (; k + 1 < end; ++k) multiply(k, steps[0], kWith);
+    if (k < end) multiply(k, steps[0], kWithout);
+  } else {
+    for (; k + 3 < end; k += 2) {
+      multiply(k, steps[0], kWith);
+      multiply(k + 1, steps[1], kWith);
+    }
+    if (k + 2 < end) {
+      multiply(k, steps[0], kWith);
+      multiply(k + 1, steps[1], kWithout);
+      multiply(k + 2, steps[0], kWithout);
+    } else {
+      if (k < end) multiply(k, steps[0], kWithout);
+      if (k + 1 < end) multiply(k + 1, steps[1], kWithout);
+    }
+  }
   // The slices in halves: the upper half's sums go through LDS to the lower half's waves.
+  if constexpr (Rows::kFills) {
+    if (shape.slices > 1) __syncthreads();
+  }
   f32x4 *const sums = reinterpret_cast<f32x4 *>(lds) + lane;
   for (int half = shape.slices / 2; half > 0; half /= 2) {
     const int at = (wave / shape.slices * half + (slice & (half - 1))) * NT * 4;
@@ -296,17 +448,19 @@ __global__ __launch_bounds__(kSlicesMax * 64) void fp8_few_kernel(Fp8Product p, 
 constexpr int kCus = 256;               // an MI355X's compute units
 constexpr int64_t kTilesMax = 1 << 22;  // of a launch: 2^32 threads are too many
 
-// Whether W is streamed into registers: up to 64 rows, which one wave takes, and where tiles of 128 x 128
-// would leave half the units idle.
-bool few_rows(int n, int rows) {
-  return rows <= kF8PanelRows || f8_parts(n, 128) * f8_parts(rows, 128) <= kCus / 2;
-}
+// Tiles of 128 x 128.
+int64_t small_tiles(int n, int rows) { return f8_parts(n, 128) * f8_parts(rows, 128); }
 
-template <int DT, int PM, int PN, int WM, int WN>
+// Whether W is streamed into registers: up to 64 rows, which one wave takes, and where tiles of 128 x 128 would leave half
+// of the units idle (300 rows, W of 4,864 x 4,096: 25 us, in tiles 26 us to bf16 and 41 us to f32; 512 rows: 36 us, in
+// tiles 27 us to bf16).
+bool few_rows(int n, int rows) { return rows <= kF8PanelRows || small_tiles(n, rows) < kCus / 2; }
+
+template <int DT, int PM, int PN, int WM, int WN, int KG>
 int launch_tiles(const Fp8Product &p, hipStream_t s) {
   const int64_t tiles_w = f8_parts(p.w.rows, kF8PanelRows * PM * WM), tiles_x = f8_parts(p.x.rows, kF8PanelRows * PN * WN);
   if (tiles_w * tiles_x > kTilesMax) return record_failure(TABBY_EINVAL, "the product is too large for one launch");
-  hipLaunchKernelGGL((fp8_tile_kernel<DT, PM, PN, WM, WN>), dim3((unsigned)(tiles_w * tiles_x)), dim3(WM * WN * 64), 0, s, p,
+  hipLaunchKernelGGL((fp8_tile_kernel<DT, PM, PN, WM, WN, KG>), dim3((unsigned)(tiles_w * tiles_x)), dim3(KG * WM * WN * 64), 0, s, p,
                      (int)tiles_w, (int)tiles_x);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
@@ -315,30 +469,40 @@ int launch_tiles(const Fp8Product &p, hipStream_t s) {
 // Whether tiles of 256 x 256 are the better choice, else 128 x 128: a last round of them that few units take part in
 // costs as much as a full one.
 bool large_tiles(int n, int rows) {
-  const int64_t large = f8_parts(n, 256) * f8_parts(rows, 256), small = f8_parts(n, 128) * f8_parts(rows, 128);
-  return 7 * f8_parts(large, kCus) <= 2 * f8_parts(small, kCus);
+  const int64_t large = f8_parts(n, 256) * f8_parts(rows, 256);
+  return 7 * f8_parts(large, kCus) <= 2 * f8_parts(small_tiles(n, rows), kCus);
 }
 
-template <int DT, int NT>
-int launch_few(const Fp8Product &p, hipStream_t s) {
+template <int DT, typename Rows>
+int launch_few(const Fp8Product &p, const typename Rows::Args &xs, hipStream_t s) {
+  constexpr int NT = Rows::kTiles;
   const int64_t panels = f8_parts(p.w.rows, kF8PanelRows), groups = f8_parts(p.x.rows, kF8TileRows * NT);
-  // Enough waves to fill the chip, eight to a unit, while every one has a panel of k.
+  // As many waves as the chip holds at once, eight to a unit, while every one has a panel of k.
   int slices = 1;
-  while (slices < kSlicesMax && slices * 2 <= p.w.col_panels() && slices * 2 * NT <= kSumsMax && panels * groups * slices < 8 * kCus) slices *= 2;
-  const FewShape shape{std::max(slices, 4), slices};
+  while (slices < kSlicesMax && slices * 2 <= p.w.col_panels() && slices * 2 * NT <= kSumsMax && panels * groups * slices * 2 <= kFewWaves * kCus) slices *= 2;
+  const FewShape shape{std::max(slices, kFewWavesMin), slices};
   const int64_t blocks = f8_parts(panels, shape.waves / shape.slices);
-  hipLaunchKernelGGL((fp8_few_kernel<DT, NT>), dim3((unsigned)blocks, (unsigned)groups), dim3(64 * shape.waves), 0, s, p, shape);
+  hipLaunchKernelGGL((fp8_few_kernel<DT, Rows>), dim3((unsigned)blocks, (unsigned)groups), dim3(64 * shape.waves), 0, s, p, xs, shape);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
 }
 
+// X as it is held.
 template <int DT>
 int launch_product(const Fp8Product &p, hipStream_t s) {
-  if (!few_rows(p.w.rows, p.x.rows)) return large_tiles(p.w.rows, p.x.rows) ? launch_tiles<DT, 2, 1, 2, 4>(p, s) : launch_tiles<DT, 1, 1, 2, 2>(p, s);
+  if (!few_rows(p.w.rows, p.x.rows)) {
+    // (As f16, X's tiles take twice the registers: the large ones do not fit.)
+    if constexpr (DT != TABBY_F32) {
+      if (large_tiles(p.w.rows, p.x.rows)) return launch_tiles<DT, 2, 1, 2, 4, 1>(p, s);
+    }
+    // (512 rows, W of 4,864 x 4,096: 27 us with two groups of waves, 31 us with one.)
+    return small_tiles(p.w.rows, p.x.rows) <= kCus ? launch_tiles<DT, 1, 1, 2, 2, 2>(p, s) : launch_tiles<DT, 1, 1, 2, 2, 1>(p, s);
+  }
   switch (f8_parts(p.x.rows, kF8TileRows)) {
-    case 1: return launch_few<DT, 1>(p, s);
-    case 2: return launch_few<DT, 2>(p, s);
-    default: return launch_few<DT, 4>(p, s);
+    case 1: return launch_few<DT, HeldTiles<1>>(p, p.x, s);
+    case 2: return launch_few<DT, HeldTiles<2>>(p, p.x, s);
+    case 3: return launch_few<DT, HeldTiles<3>>(p, p.x, s);
+    default: return launch_few<DT, HeldTiles<4>>(p, p.x, s);
   }
 }
 
@@ -347,6 +511,26 @@ int product(const Fp8Product &p, int32_t out_dtype, hipStream_t s) {
     case TABBY_F32: return launch_product<TABBY_F32>(p, s);
     case TABBY_F16: return launch_product<TABBY_F16>(p, s);
     default: return launch_product<TABBY_BF16>(p, s);
+  }
+}
+
+// X quantised in the product's own launch.
+bool fills(int rows, int kp) { return rows <= kF8TileRows && kp <= kFillPanels / rows; }
+
+template <int DT>
+int launch_linear(const Fp8Product &p, const FloatRows &x, int x_dtype, hipStream_t s) {
+  switch (x_dtype) {
+    case TABBY_F32: return launch_few<DT, FloatTiles<TABBY_F32>>(p, x, s);
+    case TABBY_F16: return launch_few<DT, FloatTiles<TABBY_F16>>(p, x, s);
+    default: return launch_few<DT, FloatTiles<TABBY_BF16>>(p, x, s);
+  }
+}
+
+int linear(const Fp8Product &p, const FloatRows &x, int x_dtype, int32_t out_dtype, hipStream_t s) {
+  switch (out_dtype) {
+    case TABBY_F32: return launch_linear<TABBY_F32>(p, x, x_dtype, s);
+    case TABBY_F16: return launch_linear<TABBY_F16>(p, x, x_dtype, s);
+    default: return launch_linear<TABBY_BF16>(p, x, x_dtype, s);
   }
 }
 
@@ -420,6 +604,11 @@ extern "C" int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64
   if (rc) return rc;
   if (rows_meet(out, workspace_dev, need) || rows_meet(x, workspace_dev, need))
     return record_failure(TABBY_EINVAL, "workspace must not overlap x or out");
+  // A result that lies on x (a layer whose input and output share a buffer) is written after a launch that has read
+  // all of x; in the product's own launch some workgroups would read what others have written.
+  const bool apart = !rows_meet({out_dev, 1, out.bytes(), 0}, x_dev, x.bytes());
+  if (apart && fills(rows, p.w.col_panels()))
+    return linear(p, FloatRows{x_dev, x_stride, rows, k}, x_dtype, out_dtype, (hipStream_t)stream);
   rc = fp8_quantize(x_dev, x_dtype, rows, k, x_stride, 1, codes, scales, (hipStream_t)stream);
   if (rc) return rc;
   return product(p, out_dtype, (hipStream_t)stream);
