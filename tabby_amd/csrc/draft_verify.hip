@@ -14,9 +14,13 @@
 // Kernels, in order:
 //   rows    a workgroup to a part of a row: the list of its first entries (top_k up to 128), or its maximum and the sum of
 //           exp((x - max) / T) (the whole vocabulary, or larger pools)
-//   settle  a workgroup to a row: its parts together, the cut, and the probability of its drafted token. A distribution
-//           is then a maximum, a total and a threshold: an entry is in it if its (logit, index) is at or above that
-//   decide  a workgroup to a request: how many are accepted; pools are drawn from here
+//   decide  a workgroup to a request: its rows' parts together; how many tokens are accepted; pools are drawn from here. A
+//           distribution is a maximum, a total and a threshold: an entry is in it if its (logit, index) is at or above that.
+//           Of a whole vocabulary's that is cut, the parts' bins say between which bounds its probabilities lie: most
+//           comparisons need no more
+//   gather  (whole vocabularies that are cut) workgroups to a request: of the rows for which that is not enough, and of those
+//           that the last token is drawn from, the entries among which the cut lies
+//   settle  a workgroup to a request: the exact cuts of these rows, then the decision
 //   weigh   (whole vocabularies) a workgroup to a segment of a deciding row: the sum of what is drawn from
 //   pick    (whole vocabularies) a workgroup to a request: the draw, among segments, then within one
 // Sums are in 64 bits, and exponentials within 5.5e-11: which token comes out hangs on comparisons of sums.
@@ -26,6 +30,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "abi_internal.h"
 #include "block_ops.h"
@@ -42,7 +47,8 @@ constexpr int kVerifyVocabMax = 1 << 24;      // masses of a row's entries are a
 constexpr int64_t kBlocksMax = (1 << 22) - 1;  // of 1,024 threads each
 constexpr int kPartsMax = 32;
 constexpr int kBlocksAimed = 512;
-constexpr int kSegment = 4096;                // elements of a segment
+constexpr int kSharesMax = 32;
+constexpr int kSegment = 1024;                // elements of a segment
 
 enum Kind : int32_t { kInvalid = 0, kGreedy, kPool, kWhole };
 
@@ -53,6 +59,7 @@ struct PartSum {
   int32_t count;  // entries written
   int32_t bad;    // a NaN or +inf
   int32_t far;    // an entry so far above the reference that the bins do not hold it
+  float reference;  // of the bins
 };
 
 // A row's distribution.
@@ -66,6 +73,12 @@ struct RowDist {
   int32_t far;         // its bins do not hold all of it
 };
 
+// Where the cut of a whole vocabulary's distribution lies, as its row's bins tell.
+struct RowCut {
+  double from, total;  // the mass above the window; what top_p is a share of, or 0: not known
+  float least, most;   // the window: logits at or above `least` and below `most`
+};
+
 enum Draw : int32_t { kDone = 0, kFromTarget, kFromRest, kWithoutToken };
 
 // What a request's last token is drawn from, where that is not a pool.
@@ -77,6 +90,12 @@ struct Decision {
   float max, draft_max;
   int32_t draw, token;           // the token that is left out, or -1
   int64_t out;                   // its place among the tokens
+};
+
+// The rows of a request that have to be settled, by slots, and the workgroups that have settled theirs.
+struct Needed {
+  uint64_t slots[2];
+  uint32_t settled;
 };
 
 struct VerifyArgs {
@@ -97,6 +116,11 @@ struct VerifyArgs {
   uint64_t *pools;       // [requests][slots][kPoolMax], where a workgroup's LDS does not keep them
   Decision *decisions;   // [requests]
   double2 *segment_sums;  // [requests][segments]: of max(P - Q, 0) and of P
+  RowCut *cuts;           // [requests][slots]
+  Needed *needed;         // [requests]
+  double2 *groups;        // [requests][slots][parts][64]: number and mass of the bins, 32 at a time
+  uint32_t *gathered;     // [requests][slots][kSharesMax]: entries of the row's window, which lie where its bins did
+  int shares;             // workgroups that gather a row
 };
 
 struct Setting {
@@ -165,31 +189,56 @@ __device__ __forceinline__ SlotRow row_of(const VerifyArgs &a, const Place &p, K
   return {true, j < p.drafts ? p.first_draft + j : -1, base};
 }
 
-// The bins of a row whose distribution is cut: 16 to each power of two of exp((x - reference) / T), from 2^-96 to 2^32 on.
-// A bin holds the sum of its entries' weights in units of its power, 2^-kBinBits of them, or their number: whole numbers, so
-// that no order matters. The reference is the largest of 256 loads spread over the row, which all of its parts find alike.
-constexpr int kOctavesBelow = 96, kOctavesAbove = 32;
-static_assert((kOctavesBelow + kOctavesAbove) * 16 == kBins, "sixteen to a power");
-__device__ __forceinline__ int bin_bits(int vocab) { return min(60 - (32 - __clz(vocab)), 48); }
+// The bins of a row whose distribution is cut: 16 to each power of two of exp((x - reference) / T), from 2^-96 to 2^32 on,
+// each around its 2^(n/16). A bin holds the sum of its entries' weights in units of 2^(n/16) 2^-38, or their number and the
+// sum in units of 2^(n/16) 2^-14: whole numbers, so that no order matters. The reference is the largest of 256 loads spread
+// over the row, which all of its parts find alike.
+constexpr int kPerOctave = 16, kBinsBelow = 96 * kPerOctave, kBinsAbove = kBins - kBinsBelow;
+constexpr int kMassBits = 38, kSmallBits = 14, kCountShift = 40;
+static_assert((int64_t)kVerifyVocabMax << (kMassBits + 1) <= INT64_MAX && (int64_t)kVerifyVocabMax << (kSmallBits + 1) < (1ll << kCountShift),
+              "all of a row in one bin");
+
+constexpr int kGroups = 64, kGroupBins = kBins / kGroups;  // the highest bins' group first
 
 struct RowBins {
   double reference, scale;
-  __device__ __forceinline__ RowBins(float reference_, const Setting &set) : reference(reference_), scale(set.inverse * 1.4426950408889634) {}
-  __device__ __forceinline__ double octaves(float x) const { return ((double)x - reference) * scale; }
-  // The place of the octave n and of f, what is left of it, in [-1/2, 1/2]; no lower for a larger logit.
-  __device__ __forceinline__ int place(double octaves, double &f, int &n) const {
+  __device__ __forceinline__ RowBins(float reference_, const Setting &set) : reference(reference_), scale(set.inverse * (kPerOctave * 1.4426950408889634)) {}
+  // In bins, above the reference's.
+  __device__ __forceinline__ double height(float x) const { return ((double)x - reference) * scale; }
+  // The bin of a height, no lower for a larger one, and what is left of it, in [-1/2, 1/2].
+  static __device__ __forceinline__ int place(double height, double &f) {
     const double magic = 6755399441055744.0;  // as in exp_64
-    const double shifted = octaves + magic;
-    n = (int)__builtin_bit_cast(uint32x2, shifted).x;
-    f = octaves - (shifted - magic);
-    const int part = (int)__builtin_bit_cast(uint32x2, fma_const(f, 16.0, magic + 8.0)).x;
-    return ((n + kOctavesBelow) << 4) + max(min(part, 15), 0);
+    const double shifted = height + magic;
+    f = height - (shifted - magic);
+    return (int)__builtin_bit_cast(uint32x2, shifted).x + kBinsBelow;
   }
-  // For any logit: below the bins or above them where they do not hold it.
+  // For any logit: the lowest or the highest bin where they do not hold it.
   __device__ __forceinline__ int bin(float x) const {
     double f;
-    int n;
-    return place(fmin(fmax(octaves(x), -(double)kOctavesBelow - 1.0), (double)kOctavesAbove), f, n);
+    return place(fmin(fmax(height(x), -(double)kBinsBelow), (double)(kBinsAbove - 1)), f);
+  }
+  // 2^(f/16) in units of 2^-38, rounded: the polynomial of degree 4 through it at the Chebyshev nodes, within 2.5e-12 of it,
+  // plus 2^52, which leaves the whole number in the low bits.
+  static __device__ __forceinline__ uint64_t mass(double f) {
+    constexpr double kUnit = 274877906944.0;
+    static_assert(kUnit == (double)(1ll << kMassBits), "the unit");
+    double p = fma_const(f, 1.4676387238435006e-07 * kUnit, 1.3551205154935067e-05 * kUnit);
+    p = fma_const(p, f, 0.0009383847926296646 * kUnit);
+    p = fma_const(p, f, 0.043321698760160544 * kUnit);
+    return (uint64_t)__double_as_longlong(fma_const(p, f, kUnit + 0x1p52)) & ((1ull << 52) - 1);
+  }
+  // What a bin holds: its number, if it has one, and its mass, relative to the reference's.
+  static __device__ __forceinline__ double2 worth(uint64_t v, int bin, bool counts) {
+    const double number = counts ? (double)(uint32_t)(v >> kCountShift) : 0.0;
+    if (counts) v &= (1ull << kCountShift) - 1;
+    const double power = (double)(bin - kBinsBelow) * (1.0 / kPerOctave), whole = rint(power);
+    return {number, __builtin_ldexp((double)v * exp2_64(power - whole), (int)whole - (counts ? kSmallBits : kMassBits))};
+  }
+  // One entry and its mass, within 2^-14 of it.
+  static __device__ __forceinline__ uint64_t one_and_mass(double f) {
+    const float g = (float)f;
+    const float w = __builtin_fmaf(__builtin_fmaf(g, 0.000938385f, 0.0433217f), g, 1.0f);
+    return 1ull << kCountShift | (uint64_t)(uint32_t)(w * (float)(1 << kSmallBits) + 0.5f);
   }
 };
 
@@ -274,13 +323,13 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
     __syncthreads();
     const uint32_t n = list.pack();
     if (scratch.bad || n == 0) {
-      if (t == 0) *out = PartSum{0.0, -INFINITY, 0, scratch.bad ? 1 : 0, 0};
+      if (t == 0) *out = PartSum{0.0, -INFINITY, 0, scratch.bad ? 1 : 0, 0, 0.0f};
       return;
     }
     const uint32_t need = min(n, (uint32_t)set.k);
     if (wave == 0) {
       const float m = wave_max(lane < NW ? wave_tops[lane] : -INFINITY);
-      if (t == 0) *out = PartSum{0.0, m, (int)need, 0, 0};
+      if (t == 0) *out = PartSum{0.0, m, (int)need, 0, 0, 0.0f};
     }
     list.select(n, need, a.entries + (int64_t)blockIdx.x * kPoolMax, [&](auto f) {
       for (int e = begin + t; e < begin + len; e += NW * 64) {
@@ -295,15 +344,14 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   bool bad = false;
   if (set.cut(a.vocab) && a.bins) {
     const RowBins bins(reference_of<DT>(source.base, a.vocab), set);
-    const bool masses = set.k == a.vocab;  // else numbers
-    const double unit = __builtin_ldexp(1.0, bin_bits(a.vocab));
+    const bool masses = set.k == a.vocab;  // else numbers as well
     for (int b = t; b < kBins; b += NW * 64) lds.bins[b] = 0;
     __syncthreads();
     bool far = false;
     if (c < reader.chunks) {
       do {
         bad |= !(top < INFINITY);
-        far |= bins.octaves(top) > (double)kOctavesAbove - 1.0;
+        far |= bins.height(top) > (double)(kBinsAbove - 1);
         largest = fmaxf(largest, top);
         if (__ballot(far) != 0) continue;
         // Entries below the bins are no number of theirs, and far less than a sum tells: they count as the lowest bin's.
@@ -311,18 +359,15 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
           for (int i = 0; i < kLane; ++i) {
             double f;
-            int n;
-            const int at = bins.place(fmax(bins.octaves(x[i]), -(double)kOctavesBelow), f, n);
-            const uint64_t add = (uint64_t)__double_as_longlong(fma_const(exp2_64(f), unit, 0x1p52)) & ((1ull << 52) - 1);
-            atomicAdd((unsigned long long *)&lds.bins[at], (unsigned long long)add);
+            const int at = bins.place(fmax(bins.height(x[i]), -(double)kBinsBelow), f);
+            atomicAdd((unsigned long long *)&lds.bins[at], (unsigned long long)bins.mass(f));
           }
         } else {
 #pragma unroll
           for (int i = 0; i < kLane; ++i) {
             double f;
-            int n;
-            const int at = bins.place(fmax(bins.octaves(x[i]), -(double)kOctavesBelow), f, n);
-            atomicAdd((unsigned long long *)&lds.bins[at], 1ull);
+            const int at = bins.place(fmax(bins.height(x[i]), -(double)kBinsBelow), f);
+            atomicAdd((unsigned long long *)&lds.bins[at], (unsigned long long)bins.one_and_mass(f));
           }
         }
       } while (advance());
@@ -334,11 +379,28 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
     if (lane == 0) wave_refs[wave] = far ? 1.0f : 0.0f;
     __syncthreads();
     uint64_t *const to = a.bins + (int64_t)blockIdx.x * kBins;
-    for (int b = t; b < kBins; b += NW * 64) to[b] = lds.bins[b];
+    // A group of 32 bins lies in some neighbouring threads.
+    constexpr int kPer = kBins / (NW * 64), kGroup = kGroupBins / kPer;
+    double2 group{0.0, 0.0};
+#pragma unroll 1
+    for (int i = 0; i < kPer; ++i) {
+      const int b = t * kPer + i;
+      const uint64_t v = lds.bins[b];
+      to[b] = v;
+      const double2 w = RowBins::worth(v, b, !masses);
+      group.x += w.x;
+      group.y += w.y;
+    }
+#pragma unroll
+    for (int d = 1; d < kGroup; d *= 2) {
+      group.x += __shfl_xor(group.x, d);
+      group.y += __shfl_xor(group.y, d);
+    }
+    if (t % kGroup == 0) a.groups[(int64_t)blockIdx.x * kGroups + (kGroups - 1 - t / kGroup)] = group;
     if (wave == 0) {
       const float m = wave_max(lane < NW ? wave_tops[lane] : -INFINITY);
       far = __ballot(lane < NW && wave_refs[lane] != 0.0f) != 0;
-      if (t == 0) *out = m < INFINITY ? PartSum{0.0, m, 0, 0, far ? 1 : 0} : PartSum{0.0, -INFINITY, 0, 1, 0};
+      if (t == 0) *out = m < INFINITY ? PartSum{0.0, m, 0, 0, far ? 1 : 0, (float)bins.reference} : PartSum{0.0, -INFINITY, 0, 1, 0, 0.0f};
     }
     return;
   }
@@ -378,7 +440,7 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
     double term = lane < NW ? wave_sums[lane] : 0.0;
     if (term > 0.0) term *= exp_or_none(((double)wave_refs[lane] - (double)m) * set.inverse);
     term = wave_sum(term);
-    if (t == 0) *out = m < INFINITY ? PartSum{term, m, 0, 0, 0} : PartSum{0.0, -INFINITY, 0, 1, 0};
+    if (t == 0) *out = m < INFINITY ? PartSum{term, m, 0, 0, 0, 0.0f} : PartSum{0.0, -INFINITY, 0, 1, 0, 0.0f};
   }
 }
 
@@ -386,7 +448,7 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
 __device__ __forceinline__ RowDist whole_row(const VerifyArgs &a, int row, const Setting &set) {
   const int lane = wave_lane();
   const bool has = lane < a.parts;
-  PartSum own{0.0, -INFINITY, 0, 0, 0};
+  PartSum own{0.0, -INFINITY, 0, 0, 0, 0.0f};
   if (has) own = a.sums[(int64_t)row * a.parts + lane];
   const float m = wave_max(own.max);
   const bool bad = __ballot(own.bad) != 0 || !(m > -INFINITY);
@@ -445,11 +507,6 @@ __device__ __forceinline__ T block_prefix(T v, T *scratch, T &total) {
   return before + v;
 }
 
-constexpr int kSettleWaves = 16;
-constexpr int kSettleThreads = kSettleWaves * 64;
-constexpr int kHeldMax = 1024;         // entries that are ranked at once
-constexpr int kCandidatesMax = 14336;  // entries of a row that may be left after its cut, in LDS
-
 // Masses of a row's entries are whole multiples of 2^-shift: their sums are exact and do not depend on an order.
 __device__ __forceinline__ int mass_shift(int vocab) { return min(62 - (32 - __clz(vocab)), 51); }
 __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, double unit) {
@@ -457,117 +514,6 @@ __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, 
   const double whole = __builtin_fma(exp_or_none(((double)x - (double)max) * inverse), unit, 0x1p52);
   return (uint64_t)__double_as_longlong(whole) & ((1ull << 52) - 1);
 }
-
-// The bin of an entry `below` the row's maximum, in temperatures: 128 to a doubling of 1 + below, the largest
-// entries in the highest. Equal logits share one, and a larger logit has none below a smaller one's.
-__device__ __forceinline__ uint32_t bin_below(float below_and_one) {
-  const uint32_t at = (__float_as_uint(below_and_one) - 0x3f800000u) >> 16;
-  return (uint32_t)(kBins - 1) - min(at, (uint32_t)(kBins - 1));
-}
-__device__ __forceinline__ uint32_t bin_of(float x, float max, float inverse) { return bin_below((max - x) * inverse + 1.0f); }
-
-struct SettleScratch {
-  uint64_t candidates[kCandidatesMax];
-  uint64_t held[kHeldMax + 8], sorted[kHeldMax];
-  uint64_t masses[kBins];
-  uint32_t counts[kBins];
-  uint64_t wave64[kSettleWaves], wave64_mass[kSettleWaves];
-  double wave_f64[kSettleWaves], found_above;
-  uint64_t found_measure, found_mass, found_entry;
-  uint32_t found_bin, taken, gathered;
-};
-
-// A row's entries at or above `least` (and above -inf) and below `most`, by the whole workgroup. They are gathered in LDS first, so that
-// what is done with them is done by full waves.
-template <int DT>
-struct Candidates {
-  using E = Elem<DT>;
-  using Bits = typename E::Bits;
-  static constexpr int kLoad = kSettleThreads * E::kVec;  // elements of a load
-  static_assert(kLoad <= kCandidatesMax, "a load's entries find room");
-  const Bits *row;
-  int vocab;
-  float least, most;
-  SettleScratch &s;
-  bool resident = false;  // all of them lie in s.candidates, s.gathered of them
-
-  __device__ __forceinline__ Candidates(const void *base, int vocab_, float least_, float most_, SettleScratch &s_)
-      : row((const Bits *)base), vocab(vocab_), least(least_), most(most_), s(s_) {}
-  __device__ __forceinline__ int place(int load) const { return load * kLoad + (int)threadIdx.x * E::kVec; }
-  __device__ __forceinline__ u32x4 read(int load) const {
-    const int at = place(load);
-    return at < vocab ? load_values<DT, false>(row, at, vocab) : u32x4{0, 0, 0, 0};
-  }
-  __device__ __forceinline__ bool in(float v, int e) const { return e < vocab && v >= least && v < most && v > -INFINITY; }
-  // The entries of a load behind those that are there already.
-  __device__ __forceinline__ void append(u32x4 raw, int load) const {
-    float v[E::kVec];
-    E::widen16(raw, v);
-    const int at = place(load);
-    uint32_t own = 0;
-#pragma unroll
-    for (int j = 0; j < E::kVec; ++j) own += in(v[j], at + j) ? 1u : 0u;
-    if (!__ballot(own != 0)) return;
-    const uint32_t upto = wave_inclusive_scan_u32(own);
-    uint32_t to = 0;
-    if (wave_lane() == 63) to = atomicAdd(&s.gathered, upto);
-    to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
-#pragma unroll
-    for (int j = 0; j < E::kVec; ++j) {
-      if (!in(v[j], at + j)) continue;
-      if (to < (uint32_t)kCandidatesMax) s.candidates[to] = composite(key_of(v[j]), (uint32_t)(at + j));
-      ++to;
-    }
-  }
-  // All of them, if they are as few as LDS holds.
-  __device__ __forceinline__ void fill() {
-    constexpr int kAhead = 4;
-    if (threadIdx.x == 0) s.gathered = 0;
-    u32x4 raw[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) raw[u] = read(u);
-    __syncthreads();
-    const int loads = (vocab + kLoad - 1) / kLoad;
-#pragma unroll 1
-    for (int first = 0; first < loads; first += kAhead) {
-      u32x4 next[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) next[u] = read(first + kAhead + u);
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) append(raw[u], first + u);
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
-    }
-    __syncthreads();
-    resident = s.gathered <= (uint32_t)kCandidatesMax;
-  }
-  // f(logit, composite) of every one of them. More than LDS holds: the row again, as much of it as fits at a time.
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    const int loads = resident ? 1 : (vocab + kLoad - 1) / kLoad;
-    if (!resident) {
-      __syncthreads();
-      if (threadIdx.x == 0) s.gathered = 0;
-      __syncthreads();
-    }
-#pragma unroll 1
-    for (int load = 0; load < loads; ++load) {
-      if (!resident) append(read(load), load);
-      __syncthreads();
-      const uint32_t n = s.gathered;
-      const bool full = load + 1 == loads || n + (uint32_t)kLoad > (uint32_t)kCandidatesMax;
-      if (full) {
-#pragma unroll 1
-        for (uint32_t i = threadIdx.x; i < n; i += kSettleThreads) f(value_of(composite_key(s.candidates[i])), s.candidates[i]);
-      }
-      __syncthreads();
-      if (full && !resident) {
-        if (threadIdx.x == 0) s.gathered = 0;
-        __syncthreads();
-      }
-    }
-  }
-};
 
 // The smallest logit that lies in bin b or above, by a wave: 64 probes at a time among the keys.
 __device__ __forceinline__ float bin_begin(const RowBins &bins, int b) {
@@ -586,222 +532,116 @@ __device__ __forceinline__ float bin_begin(const RowBins &bins, int b) {
   return value_of(high);
 }
 
-// The rows whose distribution is cut by more than a list: after the k-th entry, and where top_p is reached. The bins that
-// the row's parts have left say in which of them the row is cut, and its entries (of k, those above it as well) go to LDS
-// as the row passes. Among them the cut is found: by the counts and masses of finer bins, of parts of a bin (eleven bits of
-// the composites at a time) where it has more than are ranked at once, then among the ranked entries of one cell. Where
-// there are no bins, or a row's do not hold it, all entries that may be left are gone through.
-template <int DT>
-__global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArgs a) {
-  using E = Elem<DT>;
-  __shared__ SettleScratch s;
-  const int row = (int)blockIdx.x;
-  const int request = row / a.slots, slot = row - request * a.slots;
-  const int t = (int)threadIdx.x;
-  const Setting set = setting_of(a, request);
-  const SlotRow source = row_of<DT>(a, place_of(a, request), set.kind, slot);
-  if (!source.used || !set.cut(a.vocab)) return;
-  const RowDist whole = whole_row(a, row, set);
-  if (whole.bad) {
-    if (t == 0) a.dists[row] = whole;
-    return;
+// A row's bins, its parts' together, by a wave: a lane to a group of them. Masses are relative to the reference's.
+struct BinSums {
+  const uint64_t *bins;  // [parts][kBins]
+  int parts;
+  bool counts;           // numbers and masses, else masses
+  double count = 0.0, mass = 0.0, count_before, mass_before;  // the lane's, and what lies above
+  double all_count, all_mass;
+
+  __device__ __forceinline__ BinSums(const VerifyArgs &a, int row, bool counts_)
+      : bins(a.bins + (int64_t)row * a.parts * kBins), parts(a.parts), counts(counts_) {
+    const double2 *const groups = a.groups + (int64_t)row * a.parts * kGroups + wave_lane();
+#pragma unroll 1
+    for (int first = 0; first < parts; first += 4) {
+      double2 v[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) v[p] = first + p < parts ? groups[(first + p) * kGroups] : double2{0.0, 0.0};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        count += v[p].x;
+        mass += v[p].y;
+      }
+    }
+    count_before = wave_prefix(count);
+    mass_before = wave_prefix(mass);
+    all_count = __shfl(count_before, 63);
+    all_mass = __shfl(mass_before, 63);
+    count_before -= count;
+    mass_before -= mass;
   }
-  const float m = whole.max, inverse = fminf((float)set.inverse, 3.0e38f);  // of the bins in LDS
+  struct Found { int bin; double above, mass; };  // the mass above the bin, and its own
+  // The highest bin at which the number (or the mass) from the highest on reaches `goal`; 0: there is none.
+  __device__ __forceinline__ Found find(double goal, bool by_count) const {
+    const double own = by_count ? count : mass, before = by_count ? count_before : mass_before;
+    uint64_t who = __ballot(own > 0.0 && before + own >= goal);
+    if (!who) return {0, 0.0, 0.0};
+    const int owner = __builtin_ctzll(who);
+    const double above = __shfl(mass_before, owner), above_own = __shfl(before, owner);
+    // The owner's bins, a lane to each.
+    const int b = kBins - kGroupBins * owner - 1 - (wave_lane() & (kGroupBins - 1));
+    uint64_t v = 0;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) v += bins[(int64_t)p * kBins + b];
+    double2 w = RowBins::worth(v, b, counts);
+    if (wave_lane() >= kGroupBins) w = double2{0.0, 0.0};
+    const double upto_mass = wave_prefix(w.y) + above, upto = by_count ? wave_prefix(w.x) + above_own : upto_mass;
+    const bool some = (by_count ? w.x : w.y) > 0.0;
+    who = __ballot(some && upto >= goal);
+    // (By roundings none: the last that holds anything.)
+    const int lane = who ? __builtin_ctzll(who) : 63 - __builtin_clzll(__ballot(some) | 1);
+    return {__builtin_amdgcn_readlane(b, lane), __shfl(upto_mass - w.y, lane), __shfl(w.y, lane)};
+  }
+};
+
+// What is known of a row whose distribution is cut, by a wave: its window, and the bounds of its drafted token's
+// probability, x its logit. The distribution that is given lies between the bounds too.
+__device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, const Setting &set, float x, RowCut &window, double &least_share,
+                                              double &most_share) {
+  RowDist dist = whole_row(a, row, set);
+  const float m = dist.max;
   const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
   const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
-  // The smallest whole number of units that is top_p of the total, within the rounding of sums and masses (so that
-  // 900 of 1,000 equal entries are 0.9 of them); at least one.
-  auto goal_of = [&](double all) { return (uint64_t)fmax(ceil(set.top_p * all * (1.0 - 1e-12 - 1.0 / unit)), 1.0); };
-  auto clear = [&]() {
-    for (int b = t; b < kBins; b += kSettleThreads) {
-      s.counts[b] = 0;
-      s.masses[b] = 0;
-    }
-    __syncthreads();
-  };
-  // The highest bin at which the running count (or mass) from the highest on reaches `need` -- where none does, the lowest
-  // that holds anything -- to s.found_bin, and the count (or mass) and the mass above it. Returns the sum of all bins.
-  auto find = [&](uint64_t need, bool masses) {
-    constexpr int kPer = kBins / kSettleThreads;
-    const int high = kBins - 1 - t * kPer;
-    uint64_t own[kPer], mass[kPer], sum = 0, sum_mass = 0, total, total_mass;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      mass[i] = s.masses[high - i];
-      own[i] = masses ? mass[i] : s.counts[high - i];
-      sum += own[i];
-      sum_mass += mass[i];
-    }
-    uint64_t before = block_prefix<kSettleWaves>(sum, s.wave64, total) - sum;
-    uint64_t before_mass = block_prefix<kSettleWaves>(sum_mass, s.wave64_mass, total_mass) - sum_mass;
-    const uint64_t goal = need < total ? need : total;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      // The first at which the sum reaches the goal: bins that hold nothing do not change it.
-      if (own[i] > 0 && before < goal && before + own[i] >= goal) {
-        s.found_bin = (uint32_t)(high - i);
-        s.found_measure = before;
-        s.found_mass = before_mass;
-      }
-      before += own[i];
-      before_mass += mass[i];
-    }
-    __syncthreads();
-    return total;
-  };
-  float least = -INFINITY, most = INFINITY;  // where what may be the last entry lies
-  uint64_t from = 0;                         // mass above that
-  double total = whole.total * unit;         // of what top_p is a share of, in units; 0: not known
-  const RowBins bins(a.bins ? reference_of<DT>(source.base, a.vocab) : 0.0f, set);
-  const double raised = bins.octaves(m);  // the maximum above the bins' reference
-  if (a.bins && !whole.far && raised > -16.0) {
-    // The bins of the row, left by its parts: sixteen to a power of two of the weights.
-    constexpr int kPer = kBins / kSettleThreads;
-    const int high = kBins - 1 - t * kPer;
-    const uint64_t *const parts = a.bins + (int64_t)row * a.parts * kBins;
-    uint64_t own[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) own[i] = 0;
+  window = {0.0, dist.total * unit, -INFINITY, INFINITY};
+  least_share = 0.0;
+  most_share = INFINITY;
+  if (dist.bad) return dist;
+  const RowBins bins(a.sums[(int64_t)row * a.parts].reference, set);
+  const double raised = bins.height(m);  // the row's maximum above the reference
+  if (a.bins && !dist.far && raised > -256.0) {
+    const BinSums sums(a, row, by_count);
+    const double scale = exp2(raised * (-1.0 / kPerOctave));
+    // What the sums may be off by: masses beside numbers are held in few bits.
+    const double off = by_count ? 1e-4 : 1e-9, less = 1.0 - off, more = 1.0 + off;
+    const double all = sums.all_mass;
+    // The cut lies in the bins from `low` to `high`; `last` is the one of the k-th entry. (One loop: the code of one search.)
+    BinSums::Found low{0, 0.0, 0.0}, high = low, last = low;
+    double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - 1e-12);
 #pragma unroll 1
-    for (int p = 0; p < a.parts; ++p) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) own[i] += parts[(int64_t)p * kBins + high - i];
+    for (int search = 0; search < (by_count && by_mass ? 3 : 1); ++search) {
+      const BinSums::Found found = sums.find(goal, by_count && search == 0);
+      if (search == 0) last = high = low = found;
+      else if (found.bin >= last.bin) (search == 1 ? low : high) = found;
+      if (search == 0 && by_mass && by_count) goal = set.top_p * (last.above + last.mass) * more;
+      if (search == 1) goal = set.top_p * last.above * less;
     }
-    // Counts, or weights relative to the maximum's.
-    double v[kPer], sum = 0.0, all;
-    const double share = exp2(-raised) / __builtin_ldexp(1.0, bin_bits(a.vocab));
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      v[i] = (double)own[i];
-      if (!by_count) v[i] = __builtin_ldexp(v[i], ((high - i) >> 4) - kOctavesBelow) * share;
-      sum += v[i];
-    }
-    if (t == 0) s.found_bin = kBins;
-    double before = block_prefix<kSettleWaves>(sum, s.wave_f64, all) - sum;
-    const double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - 1e-12);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (v[i] > 0.0 && before + v[i] >= goal && (before < goal || !(before > 0.0))) {
-        s.found_bin = (uint32_t)(high - i);
-        s.found_above = before;
+    if (by_count && !by_mass) goal = last.above;
+    if (by_count) window.least = bin_begin(bins, last.bin);
+    if (low.bin > 0) {  // (the lowest bin holds what lies below it as well)
+      const float least = bin_begin(bins, low.bin);
+      if (!by_count) window = {high.above * scale * unit, all * scale * unit, least, bin_begin(bins, high.bin + 1)};
+      const double total_least = fmax(high.above, goal) * scale * less, total_most = (low.above + low.mass) * scale * more;
+      dist.total = 0.5 * (total_least + total_most);
+      dist.threshold = (uint64_t)key_of(least) << 32;
+      if (!(x > -INFINITY)) {
+        most_share = 0.0;
+      } else {
+        const int b = bins.bin(x);
+        const double w = exp_or_none(((double)x - (double)m) * set.inverse);
+        if (b > high.bin) least_share = w / total_most * (1.0 - 1e-9);
+        most_share = b < low.bin ? 0.0 : w / total_least * (1.0 + 1e-9);
       }
-      before += v[i];
+      return dist;
     }
-    __syncthreads();
-    const int found = (int)s.found_bin;
-    if (found < kBins && found > 0) {  // the lowest bin counts what lies below it as well
-      least = bin_begin(bins, found);
-      if (!by_count) {
-        most = bin_begin(bins, found + 1);
-        total = all * unit;
-        from = (uint64_t)(s.found_above * unit + 0.5);
-      }
-    }
-    __syncthreads();
-  } else if (!by_count && total > 0.0) {
+    window = {0.0, 0.0, -INFINITY, INFINITY};
+  } else if (!by_count && window.total > 0.0) {
     // Entries below (1 - top_p) total / vocab hold less than 1 - top_p together. (A margin for roundings.)
-    const double low = (1.0 - set.top_p) * whole.total / (double)a.vocab * (1.0 - 1e-6);
+    const double low = (1.0 - set.top_p) * dist.total / (double)a.vocab * (1.0 - 1e-6);
     const double bound = (double)m - fmax(-log(low), 0.0) / set.inverse - fabs((double)m) * 1e-6;
-    least = bound > -3.4e38 ? (float)bound : -INFINITY;
+    window.least = bound > -3.4e38 ? (float)bound : -INFINITY;
   }
-  Candidates<DT> left(source.base, a.vocab, least, most, s);
-  left.fill();
-  uint64_t entry = 0;      // the last entry that is left
-  uint64_t left_mass = 0;  // of what is left
-#pragma unroll 1
-  for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
-    const bool masses = stage == 1;
-    uint64_t goal = (uint64_t)set.k;
-    uint64_t above_mass = masses ? from : 0, above = above_mass;  // what lies above the cell
-    uint64_t prefix = 0;                             // how the cell's composites begin
-    uint32_t bin = 0;                                // the cell's bin
-    int done = 64, shift = 0;                        // its entries begin with prefix >> done
-    enum { kByBin, kByDigit, kTakeBin, kTakeAll } step = kByBin;
-    // Few enough to be ranked at once: no bins. (The first stage's bins count them all.)
-    if (left.resident && s.gathered <= (uint32_t)kHeldMax && (!masses || total > 0.0)) step = kTakeAll;
-#pragma unroll 1
-    for (;;) {
-      const bool takes = step >= kTakeBin;
-      if (masses && (takes || total > 0.0)) goal = goal_of(total);
-      if (!takes) clear();
-      else if (t == 0) s.taken = 0;
-      if (takes) __syncthreads();
-      left.each([&](float x, uint64_t c) {
-        if (c < entry) return;
-        uint32_t to = bin_of(x, m, inverse);
-        if ((step == kByDigit || step == kTakeBin) && (to != bin || (done < 64 && (c >> done) != (prefix >> done)))) return;
-        if (takes) {
-          const uint32_t at = atomicAdd(&s.taken, 1u);
-          if (at < (uint32_t)kHeldMax) s.held[at] = c;
-          return;
-        }
-        if (step == kByDigit) to = (uint32_t)(c >> shift) & ((1u << (done - shift)) - 1);
-        atomicAdd(&s.counts[to], 1u);
-        atomicAdd((unsigned long long *)&s.masses[to], (unsigned long long)mass_of(x, m, set.inverse, unit));
-      });
-      if (takes) break;
-      if (masses && !(total > 0.0)) {
-        // The bins hold all of the row.
-        uint64_t mass = 0, all;
-        for (int b = t; b < kBins; b += kSettleThreads) mass += s.masses[b];
-        block_prefix<kSettleWaves>(mass, s.wave64, all);
-        total = (double)all;
-        goal = goal_of(total);
-      }
-      find(goal > above ? goal - above : 1, masses);
-      above += s.found_measure;
-      above_mass += s.found_mass;
-      const uint32_t found = s.found_bin, in_cell = s.counts[found];
-      __syncthreads();
-      if (step == kByBin) {
-        bin = found;
-      } else {
-        prefix |= (uint64_t)found << shift;
-        done = shift;
-      }
-      if (in_cell > (uint32_t)kHeldMax && done > 0) {
-        step = kByDigit;
-        shift = done >= 11 ? done - 11 : 0;
-      } else {
-        step = kTakeBin;
-      }
-    }
-    // In order, by counting; one to a thread: the first that reaches the goal, or the last there is.
-    const uint32_t n = min(s.taken, (uint32_t)kHeldMax);
-    if ((uint32_t)t < 8) s.held[n + (uint32_t)t] = 0;  // whole rounds
-    __syncthreads();
-    if ((uint32_t)t < n) {
-      const uint64_t own = s.held[t];
-      uint32_t rank = 0;
-#pragma unroll 1
-      for (uint32_t j = 0; j < n; j += 8) {
-#pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) rank += s.held[j + u] > own ? 1u : 0u;
-      }
-      s.sorted[rank] = own;
-    }
-    __syncthreads();
-    const uint64_t mine = (uint32_t)t < n ? s.sorted[t] : 0;
-    const uint64_t mass = (uint32_t)t < n ? mass_of(value_of(composite_key(mine)), m, set.inverse, unit) : 0;
-    uint64_t all;
-    const uint64_t upto = block_prefix<kSettleWaves>(mass, s.wave64, all) + above_mass;
-    // (Of masses, `above` is above_mass.)
-    const uint64_t reach = masses ? (goal < above_mass + all ? goal : above_mass + all) : (goal < above + n ? goal : above + n);
-    if ((uint32_t)t < n && (masses ? upto >= reach && (t == 0 || upto - mass < reach) : above + t + 1 == reach)) {
-      s.found_entry = mine;
-      s.found_mass = upto;
-    }
-    __syncthreads();
-    entry = s.found_entry;
-    left_mass = s.found_mass;
-    total = (double)left_mass;
-    __syncthreads();
-  }
-  if (t != 0) return;
-  RowDist dist = whole;
-  dist.threshold = entry;
-  dist.total = (double)left_mass / unit;
-  a.dists[row] = dist;
+  return dist;
 }
 
 // A wave's work on a row whose distribution is a list: its parts' entries together in `held`, those at or above a
@@ -812,7 +652,7 @@ __device__ __forceinline__ RowDist pool_row(const VerifyArgs &a, int row, const 
   const PartSum *sums = a.sums + (int64_t)row * a.parts;
   const uint64_t *entries = a.entries + (int64_t)row * a.parts * kPoolMax;
   // A lane to a part.
-  PartSum own{0.0, -INFINITY, 0, 0, 0};
+  PartSum own{0.0, -INFINITY, 0, 0, 0, 0.0f};
   if (lane < parts) own = sums[lane];
   const float m = wave_max(own.max);
   RowDist dist{0.0, 0.0, 0, m, 0, 0, 0};
@@ -889,16 +729,107 @@ __device__ __forceinline__ RowDist pool_row(const VerifyArgs &a, int row, const 
   return dist;
 }
 
+// The probability of a row's drafted token, x its logit.
+__device__ __forceinline__ double share_of(const RowDist &d, const Setting &set, int token, int vocab, float x) {
+  if (token < 0 || token >= vocab) return -1.0;
+  if (!(x > -INFINITY) || composite(key_of(x), (uint32_t)token) < d.threshold) return 0.0;
+  return (set.kind == kGreedy ? 1.0 : weight_of(x, d.max, set.inverse)) / d.total;
+}
+
+// How many of a request's tokens are accepted, by its workgroup, whose first wave compares.
+struct Verdict { int accepted, status; };
+__device__ __forceinline__ Verdict verdict_of(const VerifyArgs &a, int request, const Setting &set, const Place &place, const RowDist *dists, Verdict &shared) {
+  const int t = (int)threadIdx.x, first_draft = a.drafts_max + 1;
+  const bool drawn = a.draft_logits != nullptr && set.kind != kGreedy;  // else the drafted tokens were certain
+  if (t < 64) {
+    const bool asked = place.drafts >= 0 && t < place.drafts && set.kind != kInvalid;
+    bool good = false, broken = false, unknown = false;
+    if (asked) {
+      const double share = dists[t].drafted, claim = drawn ? dists[first_draft + t].drafted : 1.0;
+      broken = dists[t].bad || (drawn && dists[first_draft + t].bad);
+      unknown = !broken && share < 0.0;
+      good = !broken && !unknown && a.uniforms[place.first_draft + t] * claim < share;
+    }
+    const uint64_t goods = __ballot(good), brokens = __ballot(broken), unknowns = __ballot(unknown);
+    if (t == 0) {
+      int n = 0, status = TABBY_EINVAL;
+      if (place.drafts >= 0 && set.kind != kInvalid) {
+        n = min((int)__builtin_ctzll(~goods), place.drafts);  // lane 63 never has a token
+        const uint64_t here = 1ull << n;
+        status = (brokens & here) || (n == place.drafts && dists[n].bad) ? TABBY_EDOMAIN : (unknowns & here) ? TABBY_EINVAL : TABBY_OK;
+      }
+      shared = {n, status};
+    }
+  }
+  __syncthreads();
+  const int n = shared.accepted, status = shared.status;
+  int32_t *tokens = a.tokens + (int64_t)request * (a.drafts_max + 1);
+  if (t <= a.drafts_max && (status != TABBY_OK || t != n)) tokens[t] = status == TABBY_OK && t < n ? a.drafts[place.first_draft + t] : -1;
+  if (t == 0) {
+    a.accepted[request] = status == TABBY_OK ? n : 0;
+    if (a.status) a.status[request] = status;
+  }
+  return {n, status};
+}
+
+__device__ __forceinline__ Draw draw_of(const VerifyArgs &a, const Setting &set, const Place &place, int accepted) {
+  if (accepted >= place.drafts || set.kind == kGreedy) return kFromTarget;
+  return a.draft_logits ? kFromRest : kWithoutToken;
+}
+
+// What the last token of a whole vocabulary is drawn from.
+__device__ __forceinline__ Decision decision_of(const VerifyArgs &a, int request, const Setting &set, const Place &place, const RowDist *dists, Verdict v) {
+  const int n = v.accepted, first_draft = a.drafts_max + 1;
+  if (v.status != TABBY_OK || set.kind != kWhole) return Decision{};
+  const Draw draw = draw_of(a, set, place, n);
+  const RowDist &p = dists[n], &q = dists[draw == kFromRest ? first_draft + n : n];
+  return {(int64_t)(place.first + n) * a.stride, (int64_t)(place.first_draft + n) * a.draft_stride,
+          p.threshold, q.threshold, set.inverse, 1.0 / p.total, 1.0 / q.total, a.params[request].uniform, p.max, q.max, draw,
+          draw == kWithoutToken ? a.drafts[place.first_draft + n] : -1, (int64_t)request * (a.drafts_max + 1) + n};
+}
+
+// Which rows have to be settled, by the first wave, from the bounds of the drafted tokens' probabilities: [slot][least, most].
+// Up to the first token that is refused for certain, both rows of each that is neither refused nor accepted for certain, and
+// the rows that the last token is drawn from then.
+__device__ __forceinline__ Needed needed_of(const VerifyArgs &a, const Place &place, const RowDist *dists, const double (*bounds)[2]) {
+  const int lane = wave_lane(), first_draft = a.drafts_max + 1;
+  const bool drawn = a.draft_logits != nullptr, asked = lane < place.drafts;
+  bool stops = false, refused = false, open = false;
+  if (asked) {
+    const double u = a.uniforms[place.first_draft + lane];
+    const double claim_least = drawn ? bounds[first_draft + lane][0] : 1.0, claim_most = drawn ? bounds[first_draft + lane][1] : 1.0;
+    stops = dists[lane].bad || (drawn && dists[first_draft + lane].bad) || dists[lane].drafted < 0.0;
+    const bool plain = u >= 0.0 && u <= 1.0;
+    refused = !stops && plain && !(u * claim_least < bounds[lane][1]);
+    open = !stops && !refused && !(plain && u * claim_most < bounds[lane][0]);
+  }
+  const uint64_t ends = __ballot(stops || refused), refusals = __ballot(refused), opens = __ballot(open);
+  const int last = ends ? __builtin_ctzll(ends) : place.drafts;  // at most 63
+  uint64_t target = opens & ((1ull << last) - 1), draft = drawn ? target : 0;
+  if (last == place.drafts) {
+    if (!dists[last].bad) target |= 1ull << last;
+  } else if (refusals >> last & 1) {
+    target |= 1ull << last;
+    if (drawn) draft |= 1ull << last;
+  }
+  Needed needed{{target, 0}, 0};
+  needed.slots[0] |= first_draft < 64 ? draft << first_draft : 0;
+  needed.slots[1] = first_draft < 64 ? draft >> 1 >> (63 - first_draft) : draft << (first_draft - 64);
+  return needed;
+}
+
 // A workgroup of NW waves to a request: a wave to a row gives its distribution and the probability of its drafted token;
 // then the first refusal; then, for pools, the draw.
-template <int DT, int NW>
+template <int DT, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64) void verify_decide_kernel(VerifyArgs a) {
   using E = Elem<DT>;
   constexpr int kKept = NW;  // rows whose entries stay in LDS
   __shared__ uint64_t held[NW][kWaveHeld], pools[kKept][kPoolMax];
   __shared__ RowDist dists[2 * kDraftsMax + 1];
   __shared__ double rest[kPoolMax], all[kPoolMax];
-  __shared__ int accepted_, status_;
+  __shared__ double bounds[FULL ? 2 * kDraftsMax + 1 : 1][2];
+  __shared__ Verdict shared;
+  __shared__ bool waits;
   __shared__ uint32_t ids[kPoolMax];
   const int request = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -916,64 +847,49 @@ __global__ __launch_bounds__(NW * 64) void verify_decide_kernel(VerifyArgs a) {
     }
     const int row = request * a.slots + slot;
     RowDist d;
-    if (set.kind != kWhole) d = pool_row(a, row, set, held[wave], pools[a.slots > kKept ? wave : slot]);
-    else d = set.cut(a.vocab) ? a.dists[row] : whole_row(a, row, set);
-    if (source.drafted >= 0 && !d.bad) {
-      if (token < 0 || token >= a.vocab) d.drafted = -1.0;
-      else if (x > -INFINITY && composite(key_of(x), (uint32_t)token) >= d.threshold)
-        d.drafted = (set.kind == kGreedy ? 1.0 : weight_of(x, d.max, set.inverse)) / d.total;
+    if (!FULL || set.kind != kWhole) {
+      d = pool_row(a, row, set, held[wave], pools[a.slots > kKept ? wave : slot]);
+    } else if (!set.cut(a.vocab)) {
+      d = whole_row(a, row, set);
+    } else {
+      RowCut window;
+      double least, most;
+      d = screen_row(a, row, set, x, window, least, most);
+      if (lane == 0) {
+        bounds[slot][0] = least;
+        bounds[slot][1] = most;
+        a.cuts[row] = window;
+      }
     }
+    if (source.drafted >= 0 && !d.bad) d.drafted = share_of(d, set, token, a.vocab, x);
+    if (FULL && lane == 0) a.dists[row] = d;
     if (lane == 0) dists[slot] = d;
     if (set.kind == kPool && a.slots > kKept) {
       for (int i = lane; i < d.count; i += 64) a.pools[(int64_t)row * kPoolMax + i] = pools[wave][i];
     }
   }
   __syncthreads();
-  const bool drawn = a.draft_logits != nullptr && set.kind != kGreedy;  // else the drafted tokens were certain
-  const int first_draft = a.drafts_max + 1;                             // slot of the draft's rows
-  if (wave == 0) {
-    const bool asked = place.drafts >= 0 && lane < place.drafts && set.kind != kInvalid;
-    bool good = false, broken = false, unknown = false;
-    if (asked) {
-      const double share = dists[lane].drafted, claim = drawn ? dists[first_draft + lane].drafted : 1.0;
-      broken = dists[lane].bad || (drawn && dists[first_draft + lane].bad);
-      unknown = !broken && share < 0.0;
-      good = !broken && !unknown && a.uniforms[place.first_draft + lane] * claim < share;
-    }
-    const uint64_t goods = __ballot(good), brokens = __ballot(broken), unknowns = __ballot(unknown);
-    if (t == 0) {
-      int n = 0, status = TABBY_EINVAL;
-      if (place.drafts >= 0 && set.kind != kInvalid) {
-        n = min((int)__builtin_ctzll(~goods), place.drafts);  // lane 63 never has a token
-        const uint64_t here = 1ull << n;
-        status = (brokens & here) || (n == place.drafts && dists[n].bad) ? TABBY_EDOMAIN : (unknowns & here) ? TABBY_EINVAL : TABBY_OK;
+  if constexpr (FULL) {
+    if (wave == 0) {
+      Needed needed{};
+      if (place.drafts >= 0 && set.cut(a.vocab)) needed = needed_of(a, place, dists, bounds);
+      if (t == 0) {
+        a.needed[request] = needed;
+        waits = (needed.slots[0] | needed.slots[1]) != 0;
+        if (waits) a.decisions[request] = Decision{};
       }
-      accepted_ = n;
-      status_ = status;
     }
+    __syncthreads();
+    if (waits) return;
   }
-  __syncthreads();
-  const int n = accepted_, status = status_;
+  const int first_draft = a.drafts_max + 1;  // slot of the draft's rows
+  const Verdict verdict = verdict_of(a, request, set, place, dists, shared);
+  const int n = verdict.accepted, status = verdict.status;
   int32_t *tokens = a.tokens + (int64_t)request * (a.drafts_max + 1);
-  if (t <= a.drafts_max && (status != TABBY_OK || t != n)) tokens[t] = status == TABBY_OK && t < n ? a.drafts[place.first_draft + t] : -1;
-  if (t == 0) {
-    a.accepted[request] = status == TABBY_OK ? n : 0;
-    if (a.status) a.status[request] = status;
-  }
-  const bool refused = n < place.drafts;
-  const Draw draw = !refused || set.kind == kGreedy ? kFromTarget : drawn ? kFromRest : kWithoutToken;
-  if (t == 0 && a.whole) {
-    Decision d{};
-    if (status == TABBY_OK && set.kind == kWhole) {
-      const RowDist &p = dists[n], &q = dists[draw == kFromRest ? first_draft + n : n];
-      d = {(int64_t)(place.first + n) * a.stride, (int64_t)(place.first_draft + n) * a.draft_stride,
-           p.threshold, q.threshold, set.inverse, 1.0 / p.total, 1.0 / q.total, a.params[request].uniform, p.max, q.max, draw,
-           draw == kWithoutToken ? a.drafts[place.first_draft + n] : -1, (int64_t)request * (a.drafts_max + 1) + n};
-    }
-    a.decisions[request] = d;
-  }
+  if (FULL && t == 0) a.decisions[request] = decision_of(a, request, set, place, dists, verdict);
   if (status != TABBY_OK || set.kind == kWhole) return;
   // A pool: what is left of the target's entries, in the vocabulary's order.
+  const Draw draw = draw_of(a, set, place, n);
   const RowDist p = dists[n], q = draw == kFromRest ? dists[first_draft + n] : p;
   if (set.kind == kGreedy) {
     if (t == 0) tokens[n] = (int32_t)composite_index(p.threshold);
@@ -1045,6 +961,361 @@ __global__ __launch_bounds__(NW * 64) void verify_decide_kernel(VerifyArgs a) {
   if (lane == 0) tokens[n] = (int32_t)ids[at];
 }
 
+constexpr int kSettleWaves = 8;
+constexpr int kSettleThreads = kSettleWaves * 64;
+constexpr int kHeldMax = 64;          // entries that are ranked at once, by a wave
+constexpr int kCells = kSettleThreads;
+constexpr int kCandidatesMax = 5632;  // entries of a row's window, in LDS
+
+struct SettleScratch {
+  uint64_t candidates[kCandidatesMax];
+  uint64_t masses[kCells];
+  uint32_t counts[kCells];
+  RowDist dists[2 * kDraftsMax + 1];
+  uint64_t held[kHeldMax], sorted[kHeldMax];
+  uint64_t wave64[kSettleWaves], wave64_mass[kSettleWaves];
+  uint64_t found_measure, found_mass, found_entry;
+  uint32_t found_bin, taken, gathered, begins[kSharesMax + 1];
+  Verdict shared;
+  bool last;
+};
+
+// The entries of a row at or above `least` (and above -inf) and below `most`, by the whole workgroup. They are gathered in LDS
+// first, so that what is done with them is done by full waves.
+template <int DT>
+struct Candidates {
+  using E = Elem<DT>;
+  using Bits = typename E::Bits;
+  static constexpr int kLoad = kSettleThreads * E::kVec;  // elements of a load
+  static_assert(kLoad <= kCandidatesMax, "a load's entries find room");
+  const Bits *row;
+  int vocab;
+  float least, most;
+  SettleScratch &s;
+  bool resident = false;  // all of them lie in s.candidates, s.gathered of them
+
+  __device__ __forceinline__ Candidates(const void *base, int vocab_, const RowCut &window, SettleScratch &s_)
+      : row((const Bits *)base), vocab(vocab_), least(window.least), most(window.most), s(s_) {}
+  __device__ __forceinline__ int place(int load) const { return load * kLoad + (int)threadIdx.x * E::kVec; }
+  __device__ __forceinline__ int loads() const { return (vocab + kLoad - 1) / kLoad; }
+  __device__ __forceinline__ u32x4 read(int load) const {
+    const int at = place(load);
+    return at < vocab ? load_values<DT, false>(row, at, vocab) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ bool in(float v, int e) const { return e < vocab && v >= least && v < most && v > -INFINITY; }
+  // The entries of a load behind those that are there already.
+  __device__ __forceinline__ void append(u32x4 raw, int load) const {
+    float v[E::kVec];
+    E::widen16(raw, v);
+    const int at = place(load);
+    uint32_t own = 0;
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) own += in(v[j], at + j) ? 1u : 0u;
+    if (!__ballot(own != 0)) return;
+    const uint32_t upto = wave_inclusive_scan_u32(own);
+    uint32_t to = 0;
+    if (wave_lane() == 63) to = atomicAdd(&s.gathered, upto);
+    to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) {
+      if (!in(v[j], at + j)) continue;
+      if (to < (uint32_t)kCandidatesMax) s.candidates[to] = composite(key_of(v[j]), (uint32_t)(at + j));
+      ++to;
+    }
+  }
+  // All of them, if they are as few as LDS holds.
+  __device__ __forceinline__ void fill() {
+    constexpr int kAhead = 4;
+    __syncthreads();
+    if (threadIdx.x == 0) s.gathered = 0;
+    u32x4 raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) raw[u] = read(u);
+    __syncthreads();
+#pragma unroll 1
+    for (int first = 0; first < loads(); first += kAhead) {
+      u32x4 next[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next[u] = read(first + kAhead + u);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) append(raw[u], first + u);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
+    }
+    __syncthreads();
+    resident = s.gathered <= (uint32_t)kCandidatesMax;
+  }
+  // Those that were gathered, if they all were and are as few as LDS holds.
+  __device__ __forceinline__ void take(const uint64_t *list, const uint32_t *counts, int shares, uint32_t room) {
+    static_assert(kSharesMax * 16 == kSettleThreads, "sixteen threads to a share");
+    const int share = (int)threadIdx.x >> 4;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const uint32_t own = (int)threadIdx.x < shares ? counts[threadIdx.x] : 0, upto = wave_inclusive_scan_u32(own);
+      if (threadIdx.x < kSharesMax) s.begins[threadIdx.x] = upto - own;
+      const bool fits = __ballot(own > room) == 0;
+      if (threadIdx.x == 63) s.gathered = fits ? upto : ~0u;
+      if (threadIdx.x == kSharesMax - 1) s.begins[kSharesMax] = upto;
+    }
+    __syncthreads();
+    resident = s.gathered <= (uint32_t)kCandidatesMax;
+    if (resident) {
+      const uint32_t begin = s.begins[share], n = s.begins[share + 1] - begin;
+      for (uint32_t i = threadIdx.x & 15; i < n; i += 16) s.candidates[begin + i] = list[(int64_t)share * room + i];
+    }
+    __syncthreads();
+  }
+  // f(logit, composite) of every one of them. More than LDS holds: the row again, as much of it as fits at a time.
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int all = resident ? 1 : loads();
+    if (!resident) {
+      __syncthreads();
+      if (threadIdx.x == 0) s.gathered = 0;
+      __syncthreads();
+    }
+#pragma unroll 1
+    for (int load = 0; load < all; ++load) {
+      if (!resident) append(read(load), load);
+      __syncthreads();
+      const uint32_t n = s.gathered;
+      const bool full = load + 1 == all || n + (uint32_t)kLoad > (uint32_t)kCandidatesMax;
+      if (full) {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < n; i += kSettleThreads) f(value_of(composite_key(s.candidates[i])), s.candidates[i]);
+      }
+      __syncthreads();
+      if (full && !resident) {
+        if (threadIdx.x == 0) s.gathered = 0;
+        __syncthreads();
+      }
+    }
+  }
+};
+
+// The cut of a row, exactly: after the k-th entry, and where top_p is reached. It lies in a cell of composites, which is
+// narrowed by the counts and masses of 512 equal parts of it until it holds as few as a wave ranks.
+template <int DT>
+__device__ __forceinline__ void settle_row(const VerifyArgs &a, const Setting &set, const RowCut &window, const Candidates<DT> &left, RowDist &dist, SettleScratch &s) {
+  const int t = (int)threadIdx.x;
+  const float m = dist.max;
+  const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
+  const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
+  double total = window.total;  // of what top_p is a share of, in units; 0: not known
+  uint64_t goal = 0, entry = 0, left_mass = 0;  // the last entry that is left; of what is left
+  // The smallest whole number of units that is top_p of the total, within the rounding of sums and masses (so that
+  // 900 of 1,000 equal entries are 0.9 of them); at least one.
+  auto aim = [&]() { goal = (uint64_t)fmax(ceil(set.top_p * total * (1.0 - 1e-12 - 1.0 / unit)), 1.0); };
+#pragma unroll 1
+  for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
+    const bool masses = stage == 1;
+    // The cell: from low to high.
+    uint64_t low = masses && by_count ? entry : window.least > -INFINITY ? (uint64_t)key_of(window.least) << 32 : 0;
+    uint64_t high = ((uint64_t)key_of(fminf(m, window.most)) << 32 | 0xffffffffu) - (window.most <= m ? 1ull << 32 : 0);
+    uint64_t above_mass = masses && !by_count ? (uint64_t)(window.from + 0.5) : 0, above = above_mass;  // what lies above it
+    if (!masses) goal = (uint64_t)set.k;
+    else if (total > 0.0) aim();
+    uint32_t in_cell = left.resident && (!masses || total > 0.0) && !(masses && by_count) ? s.gathered : ~0u;
+    // (A cell of one composite holds one entry. One whose masses are all zero ends the search with none.)
+#pragma unroll 1
+    while (in_cell > (uint32_t)kHeldMax) {
+      const int shift = max(55 - (int)__clzll(high - low), 0);
+      static_assert(kCells == 512, "nine bits");
+      s.counts[t] = 0;
+      s.masses[t] = 0;
+      if (t == 0) {
+        s.found_bin = s.taken = 0;
+        s.found_measure = s.found_mass = 0;
+      }
+      __syncthreads();
+      left.each([&](float x, uint64_t c) {
+        if (c < low || c > high) return;
+        const uint32_t to = (uint32_t)((c - low) >> shift);
+        atomicAdd(&s.counts[to], 1u);
+        atomicAdd((unsigned long long *)&s.masses[to], (unsigned long long)mass_of(x, m, set.inverse, unit));
+      });
+      // The highest part at which the running count (or mass) from the highest on reaches the goal -- where none does, the
+      // lowest that holds anything.
+      const int cell = kCells - 1 - t;
+      const uint64_t mass = s.masses[cell], own = masses ? mass : s.counts[cell];
+      uint64_t all, all_mass;
+      const uint64_t before = block_prefix<kSettleWaves>(own, s.wave64, all) - own;
+      const uint64_t before_mass = masses ? before : block_prefix<kSettleWaves>(mass, s.wave64_mass, all_mass) - mass;
+      if (masses && !(total > 0.0)) {
+        // The first time, with all of the row in the cell.
+        total = (double)all;
+        aim();
+      }
+      const uint64_t want = goal <= above ? 1 : goal - above < all ? goal - above : all;
+      if (own > 0 && before < want && before + own >= want) {
+        s.found_bin = (uint32_t)cell;
+        s.found_measure = before;
+        s.found_mass = before_mass;
+        s.taken = s.counts[cell];
+      }
+      __syncthreads();
+      above += s.found_measure;
+      above_mass += s.found_mass;
+      in_cell = s.taken;
+      low += (uint64_t)s.found_bin << shift;
+      const uint64_t end = low + ((1ull << shift) - 1);
+      high = end < high ? end : high;
+      __syncthreads();
+    }
+    __syncthreads();
+    if (t == 0) s.taken = 0;
+    __syncthreads();
+    left.each([&](float, uint64_t c) {
+      if (c < low || c > high || in_cell == 0) return;
+      const uint32_t at = atomicAdd(&s.taken, 1u);
+      if (at < (uint32_t)kHeldMax) s.held[at] = c;
+    });
+    // In order: the first that reaches the goal, or the last there is.
+    if (t < 64) {
+      const uint32_t n = min(s.taken, (uint32_t)kHeldMax);
+      const uint64_t own = (uint32_t)t < n ? s.held[t] : 0;
+      uint32_t rank = 0;
+#pragma unroll 4
+      for (uint32_t j = 0; j < n; ++j) rank += s.held[j] > own ? 1u : 0u;
+      if ((uint32_t)t < n) s.sorted[rank] = own;
+      wave_lds_sync();
+      const uint64_t mine = (uint32_t)t < n ? s.sorted[t] : 0;
+      const uint64_t mass = (uint32_t)t < n ? mass_of(value_of(composite_key(mine)), m, set.inverse, unit) : 0;
+      const uint64_t upto = wave_prefix(mass) + above_mass;
+      // (Of masses, `above` is above_mass.)
+      const uint64_t who = __ballot((uint32_t)t < n && (masses ? upto >= goal : above + (uint64_t)t + 1 >= goal));
+      const int at = who ? __builtin_ctzll(who) : (int)max(n, 1u) - 1;
+      if (t == at) {
+        s.found_entry = n ? mine : low;
+        s.found_mass = upto;
+      }
+    }
+    __syncthreads();
+    entry = s.found_entry;
+    left_mass = s.found_mass;
+    total = (double)left_mass;
+    __syncthreads();
+  }
+  dist.threshold = entry;
+  dist.total = (double)left_mass / unit;
+}
+
+// f(slot) of the rows that have to be settled, from the `first` on, every `step`-th.
+template <class F>
+__device__ __forceinline__ void each_needed(const Needed &needed, int first, int step, F f) {
+  int n = 0;
+#pragma unroll 1
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+    for (uint64_t rest = needed.slots[h]; rest; rest &= rest - 1, ++n)
+      if (n % step == first) f(h * 64 + (int)__builtin_ctzll(rest));
+  }
+}
+
+// The entries that a share of a row's gathering has room for: they lie where its bins did.
+__device__ __forceinline__ uint32_t share_room(const VerifyArgs &a) { return (uint32_t)(a.parts * kBins / a.shares); }
+
+// A row's entries in its window, to the row's lists, a workgroup to a share: loads far apart, so that no order of the
+// vocabulary fills one of them.
+constexpr int kGatherThreads = 256;
+constexpr int kGatherRows = 2;  // of a request, at a time
+constexpr int kGatherBlocks = 2048;
+template <int DT>
+__global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArgs a) {
+  using E = Elem<DT>;
+  using Bits = typename E::Bits;
+  __shared__ uint32_t gathered;
+  const int share = (int)blockIdx.x, request = (int)blockIdx.y, t = (int)threadIdx.x;
+  const Needed needed = a.needed[request];
+  if (!(needed.slots[0] | needed.slots[1])) return;
+  const Place place = place_of(a, request);
+  const uint32_t room = share_room(a);
+  each_needed(needed, (int)blockIdx.z, kGatherRows, [&](int slot) {
+    const int row = request * a.slots + slot;
+    const RowCut window = a.cuts[row];
+    const Bits *const base = (const Bits *)row_of<DT>(a, place, kWhole, slot).base;
+    uint64_t *const list = a.bins + (int64_t)row * a.parts * kBins + (int64_t)share * room;
+    __syncthreads();
+    if (t == 0) gathered = 0;
+    __syncthreads();
+    constexpr int kAhead = 4, kLoad = kGatherThreads * E::kVec;
+    const int loads = (a.vocab + kLoad - 1) / kLoad;
+#pragma unroll 1
+    for (int first = share; first < loads; first += kAhead * a.shares) {
+      u32x4 raw[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = (first + u * a.shares) * kLoad + t * E::kVec;
+        raw[u] = at < a.vocab ? load_values<DT, false>(base, at, a.vocab) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int at = (first + u * a.shares) * kLoad + t * E::kVec;
+        float v[E::kVec];
+        E::widen16(raw[u], v);
+        uint32_t own = 0;
+        bool in[E::kVec];
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) {
+          in[j] = at + j < a.vocab && v[j] >= window.least && v[j] < window.most && v[j] > -INFINITY;
+          own += in[j] ? 1u : 0u;
+        }
+        if (own == 0) continue;
+        uint32_t to = atomicAdd(&gathered, own);
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) {
+          if (in[j] && to < room) list[to] = composite(key_of(v[j]), (uint32_t)(at + j));
+          to += in[j] ? 1u : 0u;
+        }
+      }
+    }
+    __syncthreads();
+    if (t == 0) a.gathered[(int64_t)row * kSharesMax + share] = gathered;
+  });
+}
+
+// The exact cuts of a request's rows that need it, by as many workgroups as there are rows, up to kGatherRows; the last of
+// them decides.
+template <int DT>
+__global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArgs a) {
+  using E = Elem<DT>;
+  __shared__ SettleScratch s;
+  const int request = (int)blockIdx.x, t = (int)threadIdx.x;
+  const Needed needed = a.needed[request];
+  const int workgroups = min((int)(__popcll(needed.slots[0]) + __popcll(needed.slots[1])), kGatherRows);
+  if ((int)blockIdx.y >= workgroups) return;
+  const Setting set = setting_of(a, request);
+  const Place place = place_of(a, request);
+  each_needed(needed, (int)blockIdx.y, kGatherRows, [&](int slot) {
+    const int row = request * a.slots + slot;
+    RowDist d = a.dists[row];
+    const RowCut window = a.cuts[row];
+    const SlotRow source = row_of<DT>(a, place, set.kind, slot);
+    Candidates<DT> left(source.base, a.vocab, window, s);
+    if (a.bins) left.take(a.bins + (int64_t)row * a.parts * kBins, a.gathered + (int64_t)row * kSharesMax, a.shares, share_room(a));
+    if (!left.resident) left.fill();
+    settle_row<DT>(a, set, window, left, d, s);
+    if (t == 0) {
+      if (source.drafted >= 0) {
+        const int token = a.drafts[source.drafted];
+        const float x = token >= 0 && token < a.vocab ? E::widen(((const typename E::Bits *)source.base)[token]) : -INFINITY;
+        d.drafted = share_of(d, set, token, a.vocab, x);
+      }
+      a.dists[row] = d;
+    }
+  });
+  if (workgroups > 1) {
+    if (t == 0) s.last = __hip_atomic_fetch_add(&a.needed[request].settled, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)workgroups - 1;
+    __syncthreads();
+    if (!s.last) return;
+  }
+  __syncthreads();
+  for (int slot = t; slot < a.slots; slot += kSettleThreads) s.dists[slot] = a.dists[request * a.slots + slot];
+  __syncthreads();
+  const Verdict verdict = verdict_of(a, request, set, place, s.dists, s.shared);
+  if (t == 0) a.decisions[request] = decision_of(a, request, set, place, s.dists, verdict);
+}
+
 // What a thread's elements of a segment weigh in a request's draw: `rest` of them is drawn from, or `all` where nothing rests.
 template <int DT>
 struct RestOf {
@@ -1058,19 +1329,20 @@ struct RestOf {
   }
   __device__ __forceinline__ RestOf(const VerifyArgs &a, const Decision &d, int first) {
     const int vocab = a.vocab;
-    float x[E::kVec], y[E::kVec];
     const bool both = d.draw == kFromRest;
     const u32x4 none = {0, 0, 0, 0};
     const u32x4 p = first < vocab ? load_values<DT, false>((const Bits *)a.logits + d.target, first, vocab) : none;
     const u32x4 q = both && first < vocab ? load_values<DT, false>((const Bits *)a.draft_logits + d.draft, first, vocab) : none;
+    float x[E::kVec], y[E::kVec];
     E::widen16(p, x);
     E::widen16(q, y);
 #pragma unroll
     for (int j = 0; j < E::kVec; ++j) {
-      const bool in = first + j < vocab;
-      all[j] = in ? share(d.threshold, d.max, d.inverse, d.of_target, x[j], first + j) : 0.0;
-      rest[j] = both ? fmax(all[j] - (in ? share(d.draft_threshold, d.draft_max, d.inverse, d.of_draft, y[j], first + j) : 0.0), 0.0)
-                     : first + j == d.token ? 0.0 : all[j];
+      const int e = first + j;
+      const bool in = e < vocab;
+      all[j] = in ? share(d.threshold, d.max, d.inverse, d.of_target, x[j], e) : 0.0;
+      rest[j] = e == d.token ? 0.0 : all[j];
+      if (both) rest[j] = fmax(all[j] - (in ? share(d.draft_threshold, d.draft_max, d.inverse, d.of_draft, y[j], e) : 0.0), 0.0);
     }
   }
 };
@@ -1190,10 +1462,13 @@ int verify_parts(int64_t rows, int vocab) {
   return (int)std::max<int64_t>(parts, 1);
 }
 
+// Lists (parts of rows) that there may be: rows that are cut make at most kBlocksAimed of them.
+int64_t lists_max(int64_t rows) { return std::max<int64_t>(rows, kBlocksAimed); }
+
 int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // The workspace's arrays: where each begins, and the end.
-struct Space { int64_t sums, entries, dists, bins, pools, decisions, segments, end; };
+struct Space { int64_t sums, entries, dists, bins, groups, pools, decisions, cuts, needed, gathered, segments, end; };
 constexpr int64_t kBinnedMax = 4096;  // lists (parts of rows) that have bins, 16 KB each
 Space space_of(int64_t requests, int64_t slots, int64_t lists, int64_t segments) {
   Space s;
@@ -1201,9 +1476,13 @@ Space space_of(int64_t requests, int64_t slots, int64_t lists, int64_t segments)
   s.entries = s.sums + aligned(lists * (int64_t)sizeof(PartSum));
   s.dists = s.entries + aligned(lists * kPoolMax * 8);
   s.bins = s.dists + aligned(requests * slots * (int64_t)sizeof(RowDist));
-  s.pools = s.bins + std::min(lists, kBinnedMax) * kBins * 8;
+  s.groups = s.bins + std::min(lists, kBinnedMax) * kBins * 8;
+  s.pools = s.groups + std::min(lists, kBinnedMax) * kGroups * (int64_t)sizeof(double2);
   s.decisions = s.pools + aligned(requests * slots * kPoolMax * 8);
-  s.segments = s.decisions + aligned(requests * (int64_t)sizeof(Decision));
+  s.cuts = s.decisions + aligned(requests * (int64_t)sizeof(Decision));
+  s.needed = s.cuts + aligned(requests * slots * (int64_t)sizeof(RowCut));
+  s.gathered = s.needed + aligned(requests * (int64_t)sizeof(Needed));
+  s.segments = s.gathered + aligned(requests * slots * kSharesMax * 4);
   s.end = s.segments + aligned(requests * segments * (int64_t)sizeof(double2));
   return s;
 }
@@ -1216,14 +1495,21 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
   else if (blocks <= 256u && a.part_len > 8 * kChunk) hipLaunchKernelGGL((verify_rows_kernel<DT, 16>), dim3(blocks), dim3(1024), 0, s, a);
   else hipLaunchKernelGGL((verify_rows_kernel<DT, 8>), dim3(blocks), dim3(512), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
-  if (a.whole) {
-    hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3(rows), dim3(kSettleThreads), 0, s, a);
+  auto decide = [&](auto full) {
+    constexpr bool kFull = decltype(full)::value;
+    if (a.slots <= 4) hipLaunchKernelGGL((verify_decide_kernel<DT, 4, kFull>), dim3((unsigned)a.requests), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((verify_decide_kernel<DT, 16, kFull>), dim3((unsigned)a.requests), dim3(1024), 0, s, a);
+    return hipGetLastError();
+  };
+  if (a.whole) TABBY_HIP_CHECK(decide(std::true_type{}));
+  else TABBY_HIP_CHECK(decide(std::false_type{}));
+  if (!a.whole) return TABBY_OK;
+  if (a.bins) {
+    hipLaunchKernelGGL(verify_gather_kernel<DT>, dim3((unsigned)a.shares, (unsigned)a.requests, kGatherRows), dim3(kGatherThreads), 0, s, a);
     TABBY_HIP_CHECK(hipGetLastError());
   }
-  if (a.slots <= 4) hipLaunchKernelGGL((verify_decide_kernel<DT, 4>), dim3((unsigned)a.requests), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((verify_decide_kernel<DT, 16>), dim3((unsigned)a.requests), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3((unsigned)a.requests, kGatherRows), dim3(kSettleThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
-  if (!a.whole) return TABBY_OK;
   hipLaunchKernelGGL(verify_weigh_kernel<DT>, dim3((unsigned)a.segments, (unsigned)a.requests), dim3(RestOf<DT>::kThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL(verify_pick_kernel<DT>, dim3((unsigned)a.requests), dim3(RestOf<DT>::kThreads), 0, s, a);
@@ -1240,9 +1526,9 @@ extern "C" int tabby_draft_workspace(int32_t requests, int32_t drafts_max, int32
   if (!bytes) return record_failure(TABBY_EINVAL, "null pointer");
   const int rc = check_verify_shape(requests, drafts_max, vocab);
   if (rc) return rc;
-  // For these sizes and every smaller one: rows that are cut make at most kBlocksAimed parts.
-  const int64_t slots = 2 * drafts_max + 1, lists = std::max<int64_t>(requests * slots, kBlocksAimed);
-  *bytes = space_of(requests, slots, lists, ((int64_t)vocab + kSegment - 1) / kSegment).end;
+  // For these sizes and every smaller one.
+  const int64_t slots = 2 * drafts_max + 1;
+  *bytes = space_of(requests, slots, lists_max(requests * slots), ((int64_t)vocab + kSegment - 1) / kSegment).end;
   return TABBY_OK;
 }
 
@@ -1279,18 +1565,21 @@ extern "C" int tabby_draft_verify_device(const void *logits_dev, int32_t dtype, 
   const int slots = drafts_max + 1 + (draft_logits_dev ? drafts_max : 0);
   const int parts = verify_parts(rows + (draft_logits_dev ? total : 0), vocab);
   // Slots that no row fills take parts as well, which the workspace has to hold.
-  const int fit = (int)std::max<int64_t>(1, std::min<int64_t>(parts, std::max<int64_t>((int64_t)requests * (2 * drafts_max + 1), kBlocksAimed) / ((int64_t)requests * slots)));
+  const int fit = (int)std::max<int64_t>(1, std::min<int64_t>(parts, lists_max((int64_t)requests * slots) / ((int64_t)requests * slots)));
   const int part_len = (int)((((int64_t)vocab + fit - 1) / fit + 31) / 32 * 32);
   const int used = (int)(((int64_t)vocab + part_len - 1) / part_len);
   const int segments = (vocab + kSegment - 1) / kSegment;
   const int64_t lists = (int64_t)requests * slots * used;
+  // As many workgroups as the chip holds at once, with some loads each.
+  const int shares = std::max(std::min({kGatherBlocks / requests, vocab / 4096, kSharesMax}), 1);
   const Space space = space_of(requests, slots, lists, segments);
   char *w = (char *)workspace_dev;
   VerifyArgs a{logits_dev, draft_logits_dev, row_stride, draft_row_stride, drafts_dev, uniforms_dev, offsets_dev, params_dev,
                rows, requests, drafts_max, vocab, slots, (flags & TABBY_FLAG_FULL_VOCAB) != 0, used, part_len, segments,
                tokens_dev, accepted_dev, status_dev, (PartSum *)(w + space.sums), (uint64_t *)(w + space.entries),
                (RowDist *)(w + space.dists), lists <= kBinnedMax ? (uint64_t *)(w + space.bins) : nullptr,
-               (uint64_t *)(w + space.pools), (Decision *)(w + space.decisions), (double2 *)(w + space.segments)};
+               (uint64_t *)(w + space.pools), (Decision *)(w + space.decisions), (double2 *)(w + space.segments),
+               (RowCut *)(w + space.cuts), (Needed *)(w + space.needed), (double2 *)(w + space.groups), (uint32_t *)(w + space.gathered), shares};
   // What is written lies apart from what is read.
   const RowSpan outputs[] = {row_span(tokens_dev, 1, (int64_t)requests * (drafts_max + 1), 0, 4), row_span(accepted_dev, 1, requests, 0, 4),
                              row_span(status_dev, 1, status_dev ? requests : 0, 0, 4), row_span(workspace_dev, 1, need, 0, 1)};
