@@ -1454,7 +1454,7 @@ int check_verify_shape(int32_t requests, int32_t drafts_max, int32_t vocab) {
   return TABBY_OK;
 }
 
-constexpr int kPartMin = 8192;  // a chunk to each of eight waves
+constexpr int kPartMin = 16384;  // half as much makes twice the lists to bring together: one request of four tokens, 24.7 us against 23.2
 
 // Rows are cut into parts, a workgroup each, until there are some to a compute unit.
 int verify_parts(int64_t rows, int vocab) {
