@@ -348,8 +348,8 @@ TABBY_API int tabby_fp8_pack_device(const void *row_codes_dev, const float *bloc
  * both sides are FP8: out_dev [rows, n] of `out_dtype` (rows out_stride elements apart) =
  * x [rows, k] (block_rows 1) times the transpose of w [n, k] (block_rows 128), plus bias_dev [n] (f32, may be
  * NULL). Products of codes are exact, their sums and the scales' application f32, rounded once to
- * out_dtype. For an f16 or bf16 result of many rows (more than 64, and of 128 tiles of 128 x 128 or more) the matrix
- * instruction adds eight products at a time, each to 2^-13 of the largest of them or better.
+ * out_dtype. For an f16 or bf16 result of more than 64 rows the matrix instruction adds eight products
+ * at a time, each to 2^-13 of the largest of them or better.
  * Asynchronous on `stream`; no scratch.
  */
 TABBY_API int tabby_fp8_matmul_device(const void *x_codes_dev, const void *x_scales_dev, int32_t rows,

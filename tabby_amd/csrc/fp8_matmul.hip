@@ -11,7 +11,7 @@
 // Or one 16 x 16 x 128 instruction on the codes themselves, at twice the rate, which adds eight products at a time and
 // keeps of each what lies above 2^-14 or so of the group's largest (measured: 1.5e-5 of the result's norm for normal
 // values, 5e-5 for codes drawn alike). The first is taken where the result is f32, and wherever memory and not the
-// matrix cores are the bound; the second where many rows go to f16 or bf16, whose own rounding, 1.4e-4 and
+// matrix cores are the bound; the second where more than 64 rows go to f16 or bf16, whose own rounding, 1.4e-4 and
 // 1.1e-3 of the norm, is far larger.
 
 #include <hip/hip_runtime.h>
@@ -67,6 +67,10 @@ struct CodeOperand {
     for (int i = 0; i < 8; ++i) codes[i] = (int)t.half[i / 4][i % 4];
   }
 };
+
+// What many rows are multiplied as.
+template <int DT>
+using MostOperand = typename std::conditional<DT == TABBY_F32, HalfOperand, CodeOperand>::type;
 
 // The 16 x 16 product of one tile of each side.
 __device__ __forceinline__ f32x4 tile_product(const HalfOperand &w, const HalfOperand &x) {
@@ -127,7 +131,7 @@ __device__ __forceinline__ void bring_scales(const uint8_t *from, uint8_t *to) {
 template <int DT, int PM, int PN, int WM, int WN, int KG>
 __global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, int tiles_w, int tiles_x) {
   using S = TileShape<PM, PN, WM, WN, KG>;
-  using Operand = typename std::conditional<DT == TABBY_F32, HalfOperand, CodeOperand>::type;
+  using Operand = MostOperand<DT>;
   __shared__ __align__(1024) uint8_t all_lds[S::kLds];
   const int lane = (int)threadIdx.x & 63;
   const int all_waves = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -254,9 +258,10 @@ __host__ __device__ constexpr int sums_bytes(int waves, int tiles) { return wave
 constexpr int kStepBytes = kF8TileBytes + 64;  // codes and scales of 16 rows, 128 columns
 
 // The tiles of X as they are held.
-template <int NT>
+template <int NT, typename OP = HalfOperand>
 struct HeldTiles {
   using Args = Fp8Matrix;
+  using Operand = OP;
   static constexpr int kTiles = NT;
   static constexpr bool kFills = false;
   static constexpr int kAhead = NT == 1 ? 2 : 1;
@@ -281,9 +286,9 @@ struct HeldTiles {
       r.scale[u] = scales[(int64_t)k * kF8PanelRows + u * kF8TileRows];
     }
   }
-  __device__ __forceinline__ HalfOperand tile(const Raw &r, int, int u, float &scale) const {
+  __device__ __forceinline__ Operand tile(const Raw &r, int, int u, float &scale) const {
     scale = r.scale[u];
-    return HalfOperand(r.x[u]);
+    return Operand(r.x[u]);
   }
 };
 
@@ -301,6 +306,7 @@ template <int XDT>
 struct FloatTiles {
   using E = Elem<XDT>;
   using Args = FloatRows;
+  using Operand = HalfOperand;
   static constexpr int kTiles = 1;
   static constexpr bool kFills = true;
   static constexpr int kAhead = 2;
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
   f32x4 acc[4][NT] = {};
   auto multiply = [&](int at, Step &s, auto more) {
     constexpr bool kMore = decltype(more)::value != 0;
-    HalfOperand x[NT];
+    typename Rows::Operand x[NT];
     float both[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -382,7 +388,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
     if constexpr (kMore) s.scale = block_scale_at(ws, at + kAhead);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const HalfOperand w(s.w[t]);
+      const typename Rows::Operand w(s.w[t]);
       if constexpr (kMore) bring(at + kAhead, s, t);
 #pragma unroll
       for (int u = 0; u < NT; ++u) add_scaled(acc[t][u], tile_product(w, x[u]), both[u]);
@@ -452,8 +458,8 @@ constexpr int64_t kTilesMax = 1 << 22;  // of a launch: 2^32 threads are too man
 int64_t small_tiles(int n, int rows) { return f8_parts(n, 128) * f8_parts(rows, 128); }
 
 // Whether W is streamed into registers: up to 64 rows, which one wave takes, and where tiles of 128 x 128 would leave half
-// of the units idle (300 rows, W of 4,864 x 4,096: 25 us, in tiles 26 us to bf16 and 41 us to f32; 512 rows: 36 us, in
-// tiles 27 us to bf16).
+// of the units idle (300 rows, W of 4,864 x 4,096: to bf16 21 us, in tiles 26; to f32 25 us, in tiles 41. 512 rows: to bf16 36 us,
+// in tiles 27).
 bool few_rows(int n, int rows) { return rows <= kF8PanelRows || small_tiles(n, rows) < kCus / 2; }
 
 template <int DT, int PM, int PN, int WM, int WN, int KG>
@@ -502,7 +508,8 @@ int launch_product(const Fp8Product &p, hipStream_t s) {
     case 1: return launch_few<DT, HeldTiles<1>>(p, p.x, s);
     case 2: return launch_few<DT, HeldTiles<2>>(p, p.x, s);
     case 3: return launch_few<DT, HeldTiles<3>>(p, p.x, s);
-    default: return launch_few<DT, HeldTiles<4>>(p, p.x, s);
+    case 4: return launch_few<DT, HeldTiles<4>>(p, p.x, s);
+    default: return launch_few<DT, HeldTiles<4, MostOperand<DT>>>(p, p.x, s);
   }
 }
 

@@ -125,8 +125,8 @@ def matmul(x, w: Fp8Matrix, bias=None, dtype=None, out=None, stream=None):
     """x W^T (+ bias), [rows, w.rows] of ``dtype`` (float32 by default): ``w`` has square blocks, ``x``
     is an ``Fp8Matrix`` with blocks of one row or a float tensor ([rows, k] or [k]), which is quantised
     in the call and may share memory with ``out``. Products of codes are exact, their sums float32,
-    rounded once to ``dtype``; for a float16 or bfloat16 result of many rows (more than 64, and of 128
-    tiles of 128 x 128 or more) eight products at a time are added to 2^-13 of the largest of them."""
+    rounded once to ``dtype``; for a float16 or bfloat16 result of more than 64 rows eight
+    products at a time are added to 2^-13 of the largest of them."""
     device = w.data.device
     if w.block_rows != BLOCK:
         raise ValueError(f"the weights must have blocks of {BLOCK} rows, got {w.block_rows}")

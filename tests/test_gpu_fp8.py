@@ -177,8 +177,8 @@ def _weights(n, k, seed, powers=False):
 
 
 def _in_tiles(rows, n, out):
-    """Whether the product adds codes eight at a time: many rows, f16 or bf16."""
-    return out != "f32" and rows > 64 and -(-n // 128) * -(-rows // 128) >= 128
+    """Whether the product adds codes eight at a time: more than 64 rows, f16 or bf16."""
+    return out != "f32" and rows > 64
 
 
 def _bound(x, w, y, k, out, bias=None):
