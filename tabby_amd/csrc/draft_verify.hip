@@ -265,6 +265,11 @@ __device__ __forceinline__ float reference_of(const void *base, int vocab) {
   return top > -INFINITY && top < INFINITY ? top : 0.0f;
 }
 
+// A workgroup to a part of a row, 16 chunks of it on their way at once in eight waves. 16 x 9 rows of 128,000 f32 that are
+// cut: 25 us, three parts to a row; of a workgroup's time 6.5 us do not depend on its length (the request's settings, the
+// reference, the bins cleared and written), so that more parts take longer (eight: 37). 576 rows of 151,936 f32: 77 us, 4.6
+// TB/s, of which the last 64 rows take the end for themselves; more copies of the bins against lanes that meet in
+// one: slower, by their clearing.
 template <int DT, int NW>
 __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
   using Reader = PartReader<DT, false>;
@@ -819,7 +824,9 @@ __device__ __forceinline__ Needed needed_of(const VerifyArgs &a, const Place &pl
 }
 
 // A workgroup of NW waves to a request: a wave to a row gives its distribution and the probability of its drafted token;
-// then the first refusal; then, for pools, the draw.
+// then the first refusal; then, for pools, the draw. A chain of latencies: of 12.5 us for nine rows of ten lists of 40 each,
+// the lists' entries take 3, their bound 2, compaction and ranks 2, the wait for the other rows 3, the draw 2. Rows that are
+// cut take their bounds here (16 requests of nine rows: 12 us), which spares the settling of seven rows in nine.
 template <int DT, int NW, bool FULL>
 __global__ __launch_bounds__(NW * 64) void verify_decide_kernel(VerifyArgs a) {
   using E = Elem<DT>;
@@ -1216,7 +1223,8 @@ __device__ __forceinline__ void each_needed(const Needed &needed, int first, int
 __device__ __forceinline__ uint32_t share_room(const VerifyArgs &a) { return (uint32_t)(a.parts * kBins / a.shares); }
 
 // A row's entries in its window, to the row's lists, a workgroup to a share: loads far apart, so that no order of the
-// vocabulary fills one of them.
+// vocabulary fills one of them. (One workgroup to a row passes over it at 25 GB/s: 20 us for 128,000 f32; 32 take 7. The last
+// of them going on to settle the row instead of a launch of its own: 41 us against 20, for the order it asks of memory.)
 constexpr int kGatherThreads = 256;
 constexpr int kGatherRows = 2;  // of a request, at a time
 constexpr int kGatherBlocks = 2048;
@@ -1275,7 +1283,8 @@ __global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArg
 }
 
 // The exact cuts of a request's rows that need it, by as many workgroups as there are rows, up to kGatherRows; the last of
-// them decides.
+// them decides. 13 us for top_p alone (about 300 entries in the window: a round among cells, then ranks), 24 where top_k 1,000
+// comes first.
 template <int DT>
 __global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArgs a) {
   using E = Elem<DT>;
