@@ -1,5 +1,5 @@
-"""FP8 (e4m3) in blocks of 128 from its definition, in numpy's 64 bits: the checker of the tabby_fp8_*
-operators."""
+"""FP8 (e4m3) in blocks of 128 from its definition, in numpy's 64 bits: what the tabby_fp8_* operators are tested
+against."""
 import numpy as np
 
 BLOCK = 128
