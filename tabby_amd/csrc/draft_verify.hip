@@ -1268,8 +1268,11 @@ __global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArg
           in[j] = at + j < a.vocab && v[j] >= window.least && v[j] < window.most && v[j] > -INFINITY;
           own += in[j] ? 1u : 0u;
         }
-        if (own == 0) continue;
-        uint32_t to = atomicAdd(&gathered, own);
+        if (!__ballot(own != 0)) continue;
+        const uint32_t upto = wave_inclusive_scan_u32(own);
+        uint32_t to = 0;
+        if (wave_lane() == 63) to = atomicAdd(&gathered, upto);
+        to = (uint32_t)__builtin_amdgcn_readlane((int)to, 63) + upto - own;
 #pragma unroll
         for (int j = 0; j < E::kVec; ++j) {
           if (in[j] && to < room) list[to] = composite(key_of(v[j]), (uint32_t)(at + j));
@@ -1386,8 +1389,9 @@ __global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_weigh_kernel(Veri
 template <int DT>
 __global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_pick_kernel(VerifyArgs a) {
   constexpr int kThreads = RestOf<DT>::kThreads, kWavesN = kThreads / 64;
-  __shared__ double wave_space[kWavesN], before_;
-  __shared__ int segment_, last_, token_, last_token_;
+  __shared__ double wave_space[kWavesN], befores[kWavesN];
+  __shared__ int places[kWavesN], tokens[kWavesN];
+  __shared__ bool reaches[kWavesN];
   const int request = (int)blockIdx.x, t = (int)threadIdx.x;
   const Decision d = a.decisions[request];
   if (d.draw == kDone) return;
@@ -1398,12 +1402,6 @@ __global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_pick_kernel(Verif
   for (int i = begin; i < end; ++i) {
     own += sums[i].x;
     own_all += sums[i].y;
-  }
-  if (t == 0) {
-    segment_ = a.segments;
-    last_ = -1;
-    token_ = a.vocab;
-    last_token_ = -1;
   }
   double before = block_prefix<kWavesN>(own, wave_space, total) - own;
   const bool plain = !(total > 0.0);  // nothing left: P is Q, but for roundings
@@ -1425,18 +1423,41 @@ __global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_pick_kernel(Verif
     }
     at += v;
   }
-  if (found < a.segments) atomicMin(&segment_, found);
-  if (last >= 0) atomicMax(&last_, last);
+  // Of a wave: its first lane that has one, or its last with a weight. Then of the waves. (Atomics on one word go lane by
+  // lane: 2 us here and 4 below.)
+  auto settle_on = [&](bool reach, bool some) {
+    const uint64_t reached = __ballot(reach), weighted = __ballot(some);
+    return reached ? (int)__builtin_ctzll(reached) : weighted ? 63 - (int)__builtin_clzll(weighted) : -1;
+  };
+  auto first_wave = [&]() {
+    int wave = -1;
+    bool sure = false;
+#pragma unroll
+    for (int w = 0; w < kWavesN; ++w) {
+      if (!sure && places[w] >= 0) {
+        wave = w;
+        sure = reaches[w];
+      }
+    }
+    return wave;
+  };
+  const int wave = t >> 6, lane = t & 63;
+  const bool reach = found < a.segments;
+  const int owner = settle_on(reach, last >= 0);
+  if (lane == max(owner, 0)) {
+    places[wave] = owner < 0 ? -1 : reach ? found : last;
+    befores[wave] = reach ? found_before : last_before;
+    reaches[wave] = reach;
+  }
   __syncthreads();
-  const bool reached = segment_ < a.segments;
-  const int chosen = reached ? segment_ : max(last_, 0);
-  if ((reached ? found : last) == chosen) before_ = reached ? found_before : last_before;
+  const int of = first_wave(), chosen = of < 0 ? 0 : places[of];
+  const double chosen_before = of < 0 ? 0.0 : befores[of];
   const int first = chosen * kSegment + t * RestOf<DT>::E::kVec;
   const RestOf<DT> weights(a, d, first);
   double sum = 0.0, all;
 #pragma unroll
   for (int j = 0; j < RestOf<DT>::E::kVec; ++j) sum += plain ? weights.all[j] : weights.rest[j];
-  double run = block_prefix<kWavesN>(sum, wave_space, all) - sum + before_;
+  double run = block_prefix<kWavesN>(sum, wave_space, all) - sum + chosen_before;
   int token = a.vocab, some = -1;
 #pragma unroll
   for (int j = 0; j < RestOf<DT>::E::kVec; ++j) {
@@ -1447,10 +1468,18 @@ __global__ __launch_bounds__(RestOf<DT>::kThreads) void verify_pick_kernel(Verif
       if (token == a.vocab && run > goal) token = first + j;
     }
   }
-  if (token < a.vocab) atomicMin(&token_, token);
-  if (some >= 0) atomicMax(&last_token_, some);
+  const bool in = token < a.vocab;
+  const int holder = settle_on(in, some >= 0);
+  if (lane == max(holder, 0)) {
+    places[wave] = holder;
+    reaches[wave] = in;
+    tokens[wave] = in ? token : some;
+  }
   __syncthreads();
-  if (t == 0) a.tokens[d.out] = token_ < a.vocab ? token_ : max(last_token_, 0);
+  if (t == 0) {
+    const int w = first_wave();
+    a.tokens[d.out] = w < 0 ? 0 : tokens[w];
+  }
 }
 
 int check_verify_shape(int32_t requests, int32_t drafts_max, int32_t vocab) {
