@@ -1228,6 +1228,7 @@ __device__ __forceinline__ uint32_t share_room(const VerifyArgs &a) { return (ui
 constexpr int kGatherThreads = 256;
 constexpr int kGatherRows = 2;  // of a request, at a time
 constexpr int kGatherBlocks = 2048;
+constexpr int kSettleRows = 4;
 template <int DT>
 __global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArgs a) {
   using E = Elem<DT>;
@@ -1235,8 +1236,8 @@ __global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArg
   __shared__ uint32_t gathered;
   const int share = (int)blockIdx.x, request = (int)blockIdx.y, t = (int)threadIdx.x;
   const Needed needed = a.needed[request];
+  const Place place = place_of(a, request);  // (on its way beside the line above)
   if (!(needed.slots[0] | needed.slots[1])) return;
-  const Place place = place_of(a, request);
   const uint32_t room = share_room(a);
   each_needed(needed, (int)blockIdx.z, kGatherRows, [&](int slot) {
     const int row = request * a.slots + slot;
@@ -1285,7 +1286,7 @@ __global__ __launch_bounds__(kGatherThreads) void verify_gather_kernel(VerifyArg
   });
 }
 
-// The exact cuts of a request's rows that need it, by as many workgroups as there are rows, up to kGatherRows; the last of
+// The exact cuts of a request's rows that need it, by as many workgroups as there are rows, up to kSettleRows; the last of
 // them decides. 13 us for top_p alone (about 300 entries in the window: a round among cells, then ranks), 24 where top_k 1,000
 // comes first.
 template <int DT>
@@ -1294,11 +1295,11 @@ __global__ __launch_bounds__(kSettleThreads) void verify_settle_kernel(VerifyArg
   __shared__ SettleScratch s;
   const int request = (int)blockIdx.x, t = (int)threadIdx.x;
   const Needed needed = a.needed[request];
-  const int workgroups = min((int)(__popcll(needed.slots[0]) + __popcll(needed.slots[1])), kGatherRows);
-  if ((int)blockIdx.y >= workgroups) return;
   const Setting set = setting_of(a, request);
-  const Place place = place_of(a, request);
-  each_needed(needed, (int)blockIdx.y, kGatherRows, [&](int slot) {
+  const Place place = place_of(a, request);  // (three loads on their way together)
+  const int workgroups = min((int)(__popcll(needed.slots[0]) + __popcll(needed.slots[1])), kSettleRows);
+  if ((int)blockIdx.y >= workgroups) return;
+  each_needed(needed, (int)blockIdx.y, kSettleRows, [&](int slot) {
     const int row = request * a.slots + slot;
     RowDist d = a.dists[row];
     const RowCut window = a.cuts[row];
@@ -1546,7 +1547,7 @@ int launch_verify(const VerifyArgs &a, hipStream_t s) {
     hipLaunchKernelGGL(verify_gather_kernel<DT>, dim3((unsigned)a.shares, (unsigned)a.requests, kGatherRows), dim3(kGatherThreads), 0, s, a);
     TABBY_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3((unsigned)a.requests, kGatherRows), dim3(kSettleThreads), 0, s, a);
+  hipLaunchKernelGGL(verify_settle_kernel<DT>, dim3((unsigned)a.requests, kSettleRows), dim3(kSettleThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
   hipLaunchKernelGGL(verify_weigh_kernel<DT>, dim3((unsigned)a.segments, (unsigned)a.requests), dim3(RestOf<DT>::kThreads), 0, s, a);
   TABBY_HIP_CHECK(hipGetLastError());
