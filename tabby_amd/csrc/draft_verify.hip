@@ -20,7 +20,7 @@
 //           comparisons need no more
 //   gather  (whole vocabularies that are cut) workgroups to a request: of the rows for which that is not enough, and of those
 //           that the last token is drawn from, the entries among which the cut lies
-//   settle  a workgroup to a request: the exact cuts of these rows, then the decision
+//   settle  workgroups to a request: the exact cuts of these rows, then, by the last of them, the decision
 //   weigh   (whole vocabularies) a workgroup to a segment of a deciding row: the sum of what is drawn from
 //   pick    (whole vocabularies) a workgroup to a request: the draw, among segments, then within one
 // Sums are in 64 bits, and exponentials within 5.5e-11: which token comes out hangs on comparisons of sums.
@@ -543,7 +543,7 @@ struct BinSums {
   int parts;
   bool counts;           // numbers and masses, else masses
   double count = 0.0, mass = 0.0, count_before, mass_before;  // the lane's, and what lies above
-  double all_count, all_mass;
+  double all_mass;
 
   __device__ __forceinline__ BinSums(const VerifyArgs &a, int row, bool counts_)
       : bins(a.bins + (int64_t)row * a.parts * kBins), parts(a.parts), counts(counts_) {
@@ -561,7 +561,6 @@ struct BinSums {
     }
     count_before = wave_prefix(count);
     mass_before = wave_prefix(mass);
-    all_count = __shfl(count_before, 63);
     all_mass = __shfl(mass_before, 63);
     count_before -= count;
     mass_before -= mass;

@@ -37,7 +37,6 @@ struct BlockWalk {
 template <int DT, int BR, bool WHOLE>
 __global__ __launch_bounds__(BR == 1 ? 256 : 512) void fp8_quantize_kernel(const typename Elem<DT>::Bits *x, int rows, int cols,
                                                                            int64_t stride, uint8_t *codes, float *scales) {
-  using E = Elem<DT>;
   using Walk = BlockWalk<DT, BR>;
   __shared__ __align__(16) uint8_t held[Walk::kPanels * kF8PanelBytes];
   __shared__ float row_scales[kF8PanelRows];
