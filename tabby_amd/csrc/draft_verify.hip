@@ -674,8 +674,9 @@ __device__ __forceinline__ RowDist pool_row(const VerifyArgs &a, int row, const 
     for (int u = 0; u < 8; ++u) {
       const int i = first + u * 64 + lane, p = (int)(((float)i + 0.5f) * per), turned = i - p * set.k + 5 * p;
       const int at = turned - (int)(((float)turned + 0.5f) * per) * set.k;
-      const bool here = i < slots && at < __shfl(own.count, p & 63);
-      e[u] = here ? entries[p * kPoolMax + at] : 0;
+      // By all lanes: what a lane that is switched off holds is not read.
+      const int listed = __shfl(own.count, p & 63);
+      e[u] = i < slots && at < listed ? entries[p * kPoolMax + at] : 0;
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {

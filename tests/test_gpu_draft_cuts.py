@@ -1,0 +1,74 @@
+"""The verification's cuts where they are easily wrong: pools brought together from every number of lists, the largest
+vocabulary, equal entries under a mask, tails of entries far lighter than the largest, and rows that cannot be used."""
+import numpy as np
+import pytest
+
+import draft_oracle as D
+import test_gpu_draft as V
+from tabby_amd import sampler as S
+
+pytestmark = pytest.mark.gpu
+
+INF = float("inf")
+NAN = float("nan")
+LAST = np.nextafter(1.0, 0.0)  # the largest uniform
+
+
+def _pools_agree(x, y, tokens, uniforms, lasts, settings, ctx):
+    """Requests of as many drafted tokens each, top_k up to 128: x [requests, n + 1, vocab] and y [requests, n, vocab] of f32
+    values. The oracle has only what lies among some row's first 128 entries, which keeps the vocabulary's order."""
+    torch = V._torch()
+    requests, n, vocab = y.shape
+    print(f"pools {ctx}: {requests} requests of {n} x {vocab}", flush=True)
+    v = V._draft().DraftVerify(vocab_max=vocab, requests_max=requests, drafts_max=n)
+    status = torch.full((requests,), -5, dtype=torch.int32, device="cuda")
+    got = v(x.view(-1, vocab), torch.from_numpy(tokens.reshape(-1).astype(np.int32)).cuda(), V._params(settings, lasts),
+            torch.from_numpy(uniforms.reshape(-1)).cuda(), draft_logits=y.view(-1, vocab), status=status)
+    assert status.tolist() == [0] * requests
+    out, accepted = got.tokens.tolist(), got.accepted.tolist()
+    # Of equal entries the lower index comes first: a stable sort.
+    first = [torch.sort(t, dim=-1, descending=True, stable=True).indices[..., :128].cpu().numpy() for t in (x, y)]
+    for r in range(requests):
+        ids = np.unique(np.concatenate([f[r].ravel() for f in first] + [tokens[r]]))
+        at = torch.from_numpy(ids).cuda()
+        want, taken = D.decide(x[r][:, at].double().cpu().numpy(), np.searchsorted(ids, tokens[r]), uniforms[r], lasts[r], settings[r],
+                               y[r][:, at].double().cpu().numpy())
+        want = [int(ids[i]) for i in want]
+        assert accepted[r] == taken and out[r] == want + [-1] * (n + 1 - len(want)), (ctx, r, settings[r], out[r], want)
+
+
+def _rows_with_a_tail(shape, vocab, seed):
+    """Rows whose largest entries lie among the last twentieth of the vocabulary, in part, and anywhere."""
+    torch = V._torch()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(*shape, vocab, device="cuda", generator=g)
+    last = vocab // 20
+    x[..., -last:] += 6.0 * (torch.rand(*shape, last, device="cuda", generator=g) < 100.0 / last)
+    return x + 5.0 * (torch.rand(*shape, vocab, device="cuda", generator=g) < 100.0 / vocab)
+
+
+@pytest.mark.parametrize("vocab", [32768, 49152, 65536, 100352, 114688, 131072, 151936, 201088, 256000])
+def test_pools_of_every_size_over_every_number_of_lists(vocab):
+    # A row is cut into a list for each 16,384 entries, with so few rows: two to sixteen, brought together 64 entries at a
+    # time, whatever the pool's size leaves of the last 64. The entries that matter lie in the last list.
+    rng = np.random.default_rng(vocab)
+    lists = -(-vocab // 16384)
+    each = 512 // (3 * lists)  # requests of three rows, before rows are cut into fewer
+    for first in range(1, 129, each):
+        ks = list(range(first, min(first + each, 129)))
+        x = _rows_with_a_tail((len(ks), 2), vocab, vocab + first)
+        y = x[:, :1] + 0.3 * _rows_with_a_tail((len(ks), 1), vocab, vocab + first + 1)
+        tokens = y.argmax(2).cpu().numpy()
+        settings = [(1.0, k, 1.0 if k % 3 else 0.9) for k in ks]
+        _pools_agree(x, y, tokens, rng.random((len(ks), 1)), rng.random(len(ks)), settings, f"top_k {ks[0]} to {ks[-1]}")
+
+
+@pytest.mark.parametrize("top_k", [20, 50])
+@pytest.mark.parametrize("requests,vocab", [(1, 151936), (6, 151936), (8, 151936), (1, 200064)])
+def test_usual_pools_over_usual_vocabularies(requests, vocab, top_k):
+    rng = np.random.default_rng(top_k)
+    for seed in range(6):
+        x = _rows_with_a_tail((requests, 5), vocab, seed)
+        y = x[:, :4] + 0.2 * _rows_with_a_tail((requests, 4), vocab, seed + 100)
+        tokens = y.argmax(2).cpu().numpy()
+        _pools_agree(x, y, tokens, rng.random((requests, 4)), rng.random(requests), [(0.8, top_k, 0.95)] * requests, f"seed {seed}")
