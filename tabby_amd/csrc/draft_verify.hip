@@ -194,9 +194,11 @@ __device__ __forceinline__ SlotRow row_of(const VerifyArgs &a, const Place &p, K
 // sum in units of 2^(n/16) 2^-14: whole numbers, so that no order matters. The reference is the largest of 256 loads spread
 // over the row, which all of its parts find alike.
 constexpr int kPerOctave = 16, kBinsBelow = 96 * kPerOctave, kBinsAbove = kBins - kBinsBelow;
-constexpr int kMassBits = 38, kSmallBits = 14, kCountShift = 40;
-static_assert((int64_t)kVerifyVocabMax << (kMassBits + 1) <= INT64_MAX && (int64_t)kVerifyVocabMax << (kSmallBits + 1) < (1ll << kCountShift),
-              "all of a row in one bin");
+constexpr int kMassBits = 38, kSmallBits = 14, kCountShift = 39;
+// All of a row in one bin: its number, and masses of at most 2^(1/32) < 33/32.
+static_assert((uint64_t)kVerifyVocabMax <= UINT64_MAX / ((33ull << kMassBits) / 32 + 1) && (uint64_t)kVerifyVocabMax <= UINT64_MAX >> kCountShift &&
+                  (uint64_t)kVerifyVocabMax <= ((1ull << kCountShift) - 1) / ((33ull << kSmallBits) / 32 + 1),
+              "a bin's word holds them");
 
 constexpr int kGroups = 64, kGroupBins = kBins / kGroups;  // the highest bins' group first
 

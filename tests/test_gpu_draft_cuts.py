@@ -72,3 +72,30 @@ def test_usual_pools_over_usual_vocabularies(requests, vocab, top_k):
         y = x[:, :4] + 0.2 * _rows_with_a_tail((requests, 4), vocab, seed + 100)
         tokens = y.argmax(2).cpu().numpy()
         _pools_agree(x, y, tokens, rng.random((requests, 4)), rng.random(requests), [(0.8, top_k, 0.95)] * requests, f"seed {seed}")
+
+
+def _plain(x, settings, lasts):
+    """The tokens drawn from rows without drafted ones."""
+    torch = V._torch()
+    none = torch.zeros(0, device="cuda")
+    v = V._draft().DraftVerify(vocab_max=x.shape[1], requests_max=x.shape[0], drafts_max=0)
+    status = torch.full((x.shape[0],), -5, dtype=torch.int32, device="cuda")
+    got = v(x, none.int(), V._params(settings, lasts), none.double(), status=status, flags=S.TABBY_FLAG_FULL_VOCAB)
+    assert status.tolist() == [0] * x.shape[0]
+    return got.tokens[:, 0].tolist()
+
+
+def test_a_number_of_entries_that_is_the_largest_vocabulary():
+    # 2^24 equal entries: all of them in one bin.
+    torch = V._torch()
+    vocab = 2 ** 24
+    settings = [(1.0, 200, 1.0), (0.5, 1000, 0.5), (1.0, 2 ** 24 - 1, 1.0), (2.0, 0, 0.25), (1e30, 4096, 1.0)]
+    left = [200, 500, 2 ** 24 - 1, 2 ** 22, 4096]
+    x = torch.full((1, vocab), 1.5, dtype=torch.bfloat16, device="cuda")
+    for setting, n in zip(settings, left):
+        print(f"largest vocabulary {setting}", flush=True)
+        assert _plain(x, [setting], [0.0]) == [0]
+        assert _plain(x, [setting], [LAST]) == [n - 1]
+    # The same among several lists with some entries that are left out.
+    x[:, ::2] = -INF
+    assert _plain(x, [(1.0, 300, 1.0)], [LAST]) == [599]
