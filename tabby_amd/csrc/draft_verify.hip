@@ -360,7 +360,8 @@ __global__ __launch_bounds__(NW * 64) void verify_rows_kernel(VerifyArgs a) {
         bad |= !(top < INFINITY);
         far |= bins.height(top) > (double)(kBinsAbove - 1);
         largest = fmaxf(largest, top);
-        if (__ballot(far) != 0) continue;
+        // What is no number, or far, has no bin; nor has what lies beside a NaN, which hides it in `top`.
+        if (__ballot(bad || far) != 0) continue;
         // Entries below the bins are no number of theirs, and far less than a sum tells: they count as the lowest bin's.
         if (masses) {
 #pragma unroll

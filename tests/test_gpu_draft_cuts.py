@@ -99,3 +99,22 @@ def test_a_number_of_entries_that_is_the_largest_vocabulary():
     # The same among several lists with some entries that are left out.
     x[:, ::2] = -INF
     assert _plain(x, [(1.0, 300, 1.0)], [LAST]) == [599]
+
+
+@pytest.mark.parametrize("dtype", V.TYPES)
+@pytest.mark.parametrize("setting", [(1.0, 0, 0.9), (0.8, 600, 0.95), (0.5, 2000, 1.0)])
+def test_entries_that_no_bin_holds_beside_a_nan(setting, dtype):
+    # A row's largest entries lie far above its reference and share 16 elements with a NaN: the row is refused, and no other.
+    torch = V._torch()
+    rng = np.random.default_rng(4)
+    vocab, requests = 8192, 8
+    x = V._logits(rng, 2 * requests, vocab)
+    at = 64 * rng.integers(0, vocab // 64, requests) + 33
+    far = 6e4 if dtype == "f16" else 1e30
+    for r in range(0, requests, 2):
+        for i, v in enumerate((40.0, 60.0, 75.0, far)):
+            x[2 * r, (at[r] + 64 * i) % vocab] = NAN
+            x[2 * r, (at[r] + 64 * i + 1) % vocab] = v
+    tokens = np.where(np.isnan(x[::2]), -INF, x[::2]).argmax(1)
+    target = torch.from_numpy(x).to(V._dtype(dtype)).cuda()
+    V._check(target, tokens, rng.random(requests), rng.random(requests), [setting], [1] * requests, uniform_rows=True, bad_ok=True)
