@@ -343,14 +343,15 @@ TABBY_API int tabby_fp8_dequantize_device(const void *codes_dev, const void *sca
  */
 TABBY_API int tabby_fp8_pack_device(const void *row_codes_dev, const float *block_scales_dev, int32_t rows, int32_t cols,
                                     void *codes_dev, void *scales_dev, void *stream);
+#define TABBY_FP8_FAST_SUMS 0x100
 /*
  * The product that stands in encodeQuantMatmul's place (src/engine/forward.ts:732-770) where
  * both sides are FP8: out_dev [rows, n] of `out_dtype` (rows out_stride elements apart) =
  * x [rows, k] (block_rows 1) times the transpose of w [n, k] (block_rows 128), plus bias_dev [n] (f32, may be
  * NULL). Products of codes are exact, their sums and the scales' application f32, rounded once to
- * out_dtype. For an f16 or bf16 result of more than 64 rows the matrix instruction adds eight products
- * at a time, each to 2^-13 of the largest of them or better.
- * Asynchronous on `stream`; no scratch.
+ * out_dtype. TABBY_FP8_FAST_SUMS, added to an out_dtype of TABBY_F16 or TABBY_BF16, lets more than 64 rows go through the
+ * matrix cores as codes, at twice the rate: eight products at a time are added, each to 2^-13 of the
+ * largest of them or better. Asynchronous on `stream`; no scratch.
  */
 TABBY_API int tabby_fp8_matmul_device(const void *x_codes_dev, const void *x_scales_dev, int32_t rows,
                                       const void *w_codes_dev, const void *w_scales_dev, const float *bias_dev,

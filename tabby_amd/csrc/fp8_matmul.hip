@@ -9,10 +9,10 @@
 // Two ways to the inner sum. Codes converted to f16, where all of them are exact, and four 16 x 16 x 32 f16
 // instructions: their products are exact and their sums f32's (measured: within 2^-22 of the sum of the magnitudes).
 // Or one 16 x 16 x 128 instruction on the codes themselves, at twice the rate, which adds eight products at a time and
-// keeps of each what lies above 2^-14 or so of the group's largest (measured: 1.5e-5 of the result's norm for normal
-// values, 5e-5 for codes drawn alike). The first is taken where the result is f32, and wherever memory and not the
-// matrix cores are the bound; the second where more than 64 rows go to f16 or bf16, whose own rounding, 1.4e-4 and
-// 1.1e-3 of the norm, is far larger.
+// keeps of each what lies above 2^-13 of the group's largest, or better (measured: 1.5e-5 of the result's norm for normal
+// values, 5e-5 for codes drawn alike; where large products cancel it is what is left). The first is taken unless the caller
+// asks for the second (TABBY_FP8_FAST_SUMS), which more than 64 rows to f16 or bf16 then take: fewer are bound by
+// memory, and f32 would show the difference.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -67,10 +67,6 @@ struct CodeOperand {
     for (int i = 0; i < 8; ++i) codes[i] = (int)t.half[i / 4][i % 4];
   }
 };
-
-// What many rows are multiplied as.
-template <int DT>
-using MostOperand = typename std::conditional<DT == TABBY_F32, HalfOperand, CodeOperand>::type;
 
 // The 16 x 16 product of one tile of each side.
 __device__ __forceinline__ f32x4 tile_product(const HalfOperand &w, const HalfOperand &x) {
@@ -130,10 +126,9 @@ __device__ __forceinline__ void bring_scales(const uint8_t *from, uint8_t *to) {
   __builtin_amdgcn_global_load_lds((GlobalVoid *)from, (LdsVoid *)to, 4, 0, 0);
 }
 
-template <int DT, int PM, int PN, int WM, int WN, int KG>
+template <int DT, typename Operand, int PM, int PN, int WM, int WN, int KG>
 __global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product p, int tiles_w, int tiles_x) {
   using S = TileShape<PM, PN, WM, WN, KG>;
-  using Operand = MostOperand<DT>;
   __shared__ __align__(1024) uint8_t all_lds[S::kLds];
   const int lane = (int)threadIdx.x & 63;
   const int all_waves = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -260,7 +255,7 @@ __host__ __device__ constexpr int sums_bytes(int waves, int tiles) { return wave
 constexpr int kStepBytes = kF8TileBytes + 64;  // codes and scales of 16 rows, 128 columns
 
 // The tiles of X as they are held.
-template <int NT, typename OP = HalfOperand>
+template <int NT, typename OP>
 struct HeldTiles {
   using Args = Fp8Matrix;
   using Operand = OP;
@@ -453,6 +448,13 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
     store_panel<DT>(p.y, (tile + u) * kF8TileRows + (lane & 15), panel * kF8PanelRows, acc[0][u], acc[1][u], acc[2][u], acc[3][u]);
 }
 
+// What the caller asks for: the result's type, and whether its sums may be the codes' own.
+struct OutType {
+  int32_t dtype;
+  bool fast;
+  explicit OutType(int32_t asked) : dtype(asked & ~TABBY_FP8_FAST_SUMS), fast((asked & TABBY_FP8_FAST_SUMS) != 0) {}
+};
+
 constexpr int kCus = 256;               // an MI355X's compute units
 constexpr int64_t kTilesMax = 1 << 22;  // of a launch: 2^32 threads are too many
 
@@ -464,11 +466,11 @@ int64_t small_tiles(int n, int rows) { return f8_parts(n, 128) * f8_parts(rows, 
 // in tiles 27).
 bool few_rows(int n, int rows) { return rows <= kF8PanelRows || small_tiles(n, rows) < kCus / 2; }
 
-template <int DT, int PM, int PN, int WM, int WN, int KG>
+template <int DT, typename Operand, int PM, int PN, int WM, int WN, int KG>
 int launch_tiles(const Fp8Product &p, hipStream_t s) {
   const int64_t tiles_w = f8_parts(p.w.rows, kF8PanelRows * PM * WM), tiles_x = f8_parts(p.x.rows, kF8PanelRows * PN * WN);
   if (tiles_w * tiles_x > kTilesMax) return record_failure(TABBY_EINVAL, "the product is too large for one launch");
-  hipLaunchKernelGGL((fp8_tile_kernel<DT, PM, PN, WM, WN, KG>), dim3((unsigned)(tiles_w * tiles_x)), dim3(KG * WM * WN * 64), 0, s, p,
+  hipLaunchKernelGGL((fp8_tile_kernel<DT, Operand, PM, PN, WM, WN, KG>), dim3((unsigned)(tiles_w * tiles_x)), dim3(KG * WM * WN * 64), 0, s, p,
                      (int)tiles_w, (int)tiles_x);
   TABBY_HIP_CHECK(hipGetLastError());
   return TABBY_OK;
@@ -495,31 +497,31 @@ int launch_few(const Fp8Product &p, const typename Rows::Args &xs, hipStream_t s
   return TABBY_OK;
 }
 
-// X as it is held.
-template <int DT>
+// X as it is held; `Most` is what more than 64 rows are multiplied as.
+template <int DT, typename Most>
 int launch_product(const Fp8Product &p, hipStream_t s) {
   if (!few_rows(p.w.rows, p.x.rows)) {
     // (As f16, X's tiles take twice the registers: the large ones do not fit.)
-    if constexpr (DT != TABBY_F32) {
-      if (large_tiles(p.w.rows, p.x.rows)) return launch_tiles<DT, 2, 1, 2, 4, 1>(p, s);
+    if constexpr (std::is_same<Most, CodeOperand>::value) {
+      if (large_tiles(p.w.rows, p.x.rows)) return launch_tiles<DT, Most, 2, 1, 2, 4, 1>(p, s);
     }
     // (512 rows, W of 4,864 x 4,096: 27 us with two groups of waves, 31 us with one.)
-    return small_tiles(p.w.rows, p.x.rows) <= kCus ? launch_tiles<DT, 1, 1, 2, 2, 2>(p, s) : launch_tiles<DT, 1, 1, 2, 2, 1>(p, s);
+    return small_tiles(p.w.rows, p.x.rows) <= kCus ? launch_tiles<DT, Most, 1, 1, 2, 2, 2>(p, s) : launch_tiles<DT, Most, 1, 1, 2, 2, 1>(p, s);
   }
   switch (f8_parts(p.x.rows, kF8TileRows)) {
-    case 1: return launch_few<DT, HeldTiles<1>>(p, p.x, s);
-    case 2: return launch_few<DT, HeldTiles<2>>(p, p.x, s);
-    case 3: return launch_few<DT, HeldTiles<3>>(p, p.x, s);
-    case 4: return launch_few<DT, HeldTiles<4>>(p, p.x, s);
-    default: return launch_few<DT, HeldTiles<4, MostOperand<DT>>>(p, p.x, s);
+    case 1: return launch_few<DT, HeldTiles<1, HalfOperand>>(p, p.x, s);
+    case 2: return launch_few<DT, HeldTiles<2, HalfOperand>>(p, p.x, s);
+    case 3: return launch_few<DT, HeldTiles<3, HalfOperand>>(p, p.x, s);
+    case 4: return launch_few<DT, HeldTiles<4, HalfOperand>>(p, p.x, s);
+    default: return launch_few<DT, HeldTiles<4, Most>>(p, p.x, s);
   }
 }
 
-int product(const Fp8Product &p, int32_t out_dtype, hipStream_t s) {
-  switch (out_dtype) {
-    case TABBY_F32: return launch_product<TABBY_F32>(p, s);
-    case TABBY_F16: return launch_product<TABBY_F16>(p, s);
-    default: return launch_product<TABBY_BF16>(p, s);
+int product(const Fp8Product &p, const OutType &out, hipStream_t s) {
+  switch (out.dtype) {
+    case TABBY_F32: return launch_product<TABBY_F32, HalfOperand>(p, s);
+    case TABBY_F16: return out.fast ? launch_product<TABBY_F16, CodeOperand>(p, s) : launch_product<TABBY_F16, HalfOperand>(p, s);
+    default: return out.fast ? launch_product<TABBY_BF16, CodeOperand>(p, s) : launch_product<TABBY_BF16, HalfOperand>(p, s);
   }
 }
 
@@ -552,6 +554,12 @@ int check_apart(const RowSpan &rows, const Fp8Product &p) {
   return TABBY_OK;
 }
 
+int check_result(const void *out_dev, const OutType &out, int32_t rows, int32_t n, int64_t stride) {
+  const int rc = check_output(out_dev, out.dtype, rows, n, stride);
+  if (!rc && out.fast && out.dtype == TABBY_F32) return record_failure(TABBY_EINVAL, "TABBY_FP8_FAST_SUMS is for f16 and bf16 results");
+  return rc;
+}
+
 int check_bias(const float *bias) {
   if ((uintptr_t)bias % 4 != 0) return record_failure(TABBY_EINVAL, "bias must be aligned to its elements");
   return TABBY_OK;
@@ -570,17 +578,18 @@ extern "C" int tabby_fp8_matmul_device(const void *x_codes_dev, const void *x_sc
   if (!rc) rc = check_fp8_operand(w_codes_dev, w_scales_dev);
   if (!rc) rc = check_fp8_shape(rows, k, 1);
   if (!rc) rc = check_fp8_shape(n, k, kF8Block);
-  if (!rc) rc = check_output(out_dev, out_dtype, rows, n, out_stride);
+  const OutType type(out_dtype);
+  if (!rc) rc = check_result(out_dev, type, rows, n, out_stride);
   if (!rc) rc = check_bias(bias_dev);
   if (rc) return rc;
   const Fp8Product p{{(const uint8_t *)w_codes_dev, (const float *)w_scales_dev, n, k},
                      {(const uint8_t *)x_codes_dev, (const float *)x_scales_dev, rows, k},
                      {rows, n, bias_dev, out_dev, out_stride}};
-  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
+  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(type.dtype));
   rc = check_apart(out, p);
   if (!rc) rc = check_fp8_apart(out, x_codes_dev, x_scales_dev, rows, k, 1);
   if (rc) return rc;
-  return product(p, out_dtype, (hipStream_t)stream);
+  return product(p, type, (hipStream_t)stream);
 }
 
 extern "C" int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64_t x_stride, int32_t rows,
@@ -591,7 +600,8 @@ extern "C" int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64
   int rc = check_fp8_operand(w_codes_dev, w_scales_dev);
   if (!rc) rc = check_fp8_shape(rows, k, 1);
   if (!rc) rc = check_fp8_shape(n, k, kF8Block);
-  if (!rc) rc = check_output(out_dev, out_dtype, rows, n, out_stride);
+  const OutType type(out_dtype);
+  if (!rc) rc = check_result(out_dev, type, rows, n, out_stride);
   if (!rc) rc = check_bias(bias_dev);
   if (rc) return rc;
   if (!known_dtype(x_dtype)) return record_failure(TABBY_EINVAL, "dtype must be TABBY_F32, TABBY_F16 or TABBY_BF16");
@@ -607,7 +617,7 @@ extern "C" int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64
   const Fp8Product p{{(const uint8_t *)w_codes_dev, (const float *)w_scales_dev, n, k},
                      {codes, scales, rows, k}, {rows, n, bias_dev, out_dev, out_stride}};
   const RowSpan x = row_span(x_dev, rows, k, x_stride, dtype_size(x_dtype));
-  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(out_dtype));
+  const RowSpan out = row_span(out_dev, rows, n, out_stride, dtype_size(type.dtype));
   rc = check_apart(out, p);
   if (!rc) rc = check_apart(row_span(workspace_dev, 1, need, 0, 1), p);
   if (rc) return rc;
@@ -617,8 +627,8 @@ extern "C" int tabby_fp8_linear_device(const void *x_dev, int32_t x_dtype, int64
   // all of x; in the product's own launch some workgroups would read what others have written.
   const bool apart = !rows_meet({out_dev, 1, out.bytes(), 0}, x_dev, x.bytes());
   if (apart && fills(rows, p.w.col_panels()))
-    return linear(p, FloatRows{x_dev, x_stride, rows, k}, x_dtype, out_dtype, (hipStream_t)stream);
+    return linear(p, FloatRows{x_dev, x_stride, rows, k}, x_dtype, type.dtype, (hipStream_t)stream);
   rc = fp8_quantize(x_dev, x_dtype, rows, k, x_stride, 1, codes, scales, (hipStream_t)stream);
   if (rc) return rc;
-  return product(p, out_dtype, (hipStream_t)stream);
+  return product(p, type, (hipStream_t)stream);
 }

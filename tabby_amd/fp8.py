@@ -19,6 +19,7 @@ import torch
 from .mx4 import INT32_MAX, _result_code, call_on, dtype_code, on_device, rows_of
 from .sampler import _check, load_library
 
+FAST_SUMS = 0x100  # TABBY_FP8_FAST_SUMS
 BLOCK = 128  # columns to a scale, and rows of a weight's block
 PANEL_ROWS, PANEL_COLS = 64, 128  # a panel's codes take 8,192 bytes, the scales of its rows 256
 
@@ -121,12 +122,13 @@ class Fp8Matrix:
         return out
 
 
-def matmul(x, w: Fp8Matrix, bias=None, dtype=None, out=None, stream=None):
+def matmul(x, w: Fp8Matrix, bias=None, dtype=None, out=None, stream=None, fast_sums: bool = False):
     """x W^T (+ bias), [rows, w.rows] of ``dtype`` (float32 by default): ``w`` has square blocks, ``x``
     is an ``Fp8Matrix`` with blocks of one row or a float tensor ([rows, k] or [k]), which is quantised
     in the call and may share memory with ``out``. Products of codes are exact, their sums float32,
-    rounded once to ``dtype``; for a float16 or bfloat16 result of more than 64 rows eight
-    products at a time are added to 2^-13 of the largest of them."""
+    rounded once to ``dtype``. ``fast_sums``, for float16 and bfloat16, lets more than 64 rows go through the
+    matrix cores as codes, at twice the rate: eight products at a time are added to 2^-13 of the largest of
+    them."""
     device = w.data.device
     if w.block_rows != BLOCK:
         raise ValueError(f"the weights must have blocks of {BLOCK} rows, got {w.block_rows}")
@@ -155,6 +157,8 @@ def matmul(x, w: Fp8Matrix, bias=None, dtype=None, out=None, stream=None):
     else:
         code = _result_code(out, dtype, rows, n, device)
         out = rows_of(out, "out")
+    if fast_sums:
+        code |= FAST_SUMS
     lib = load_library()
     w_at = w.data.data_ptr()
     ctx, handle = call_on(device, stream)
@@ -184,6 +188,7 @@ class LmHeadFp8:
         self.weight, self.bias = weight, bias
         self.vocab, self.hidden = weight.rows, weight.cols
 
-    def logits(self, hidden_states, dtype=None, out=None, stream=None):
-        """Logits [rows, vocab] (float32 by default) of hidden states [rows, hidden] or [hidden]."""
-        return matmul(hidden_states, self.weight, self.bias, dtype=dtype, out=out, stream=stream)
+    def logits(self, hidden_states, dtype=None, out=None, stream=None, fast_sums: bool = False):
+        """Logits [rows, vocab] (float32 by default) of hidden states [rows, hidden] or [hidden]; ``fast_sums`` as
+        in ``matmul``."""
+        return matmul(hidden_states, self.weight, self.bias, dtype=dtype, out=out, stream=stream, fast_sums=fast_sums)

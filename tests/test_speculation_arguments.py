@@ -146,3 +146,15 @@ def test_verification_arguments(lib):
     _refused(lib, call(tokens=7 * step), "overlap")
     _refused(lib, call(status=9 * step + 64), "overlap")
     _refused(lib, call(offsets=6 * step), "overlap")
+
+
+def test_fast_sums_arguments(lib):
+    m, f = lib.tabby_fp8_matmul_device, lib.tabby_fp8_linear_device
+    fast = 0x100
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, E, fast | S.TABBY_F32, 64, None), "f16 and bf16 results")
+    _refused(lib, f(A, 0, 128, 1, C, D, None, 64, 128, E, fast | S.TABBY_F32, 64, B, 8192 + 256, None), "f16 and bf16 results")
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, E, fast | 3, 64, None), "dtype")
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, E, -1, 64, None), "dtype")
+    _refused(lib, m(A, B, 1, C, D, None, 64, 128, E + 1, fast | S.TABBY_BF16, 64, None), "elements")
+    _refused(lib, m(A, B, 2, C, D, None, 64, 128, E, fast | S.TABBY_F16, 63, None), "out_stride")
+    _refused(lib, f(A, fast, 128, 1, C, D, None, 64, 128, E, 1, 64, B, 8192 + 256, None), "dtype")
