@@ -79,6 +79,11 @@ struct RowCut {
   float least, most;   // the window: logits at or above `least` and below `most`
 };
 
+// What top_p of a row's total may be short of, relative to it, where that total comes from the row's bins or its parts' sums: up to
+// three exponentials, 5.5e-11 each, on top of the one in the entries' own masses. Without it the last of the entries that make up
+// the share exactly (nine of ten equal ones, for 0.9) would not do.
+constexpr double kTotalOff = 2.5e-10;
+
 enum Draw : int32_t { kDone = 0, kFromTarget, kFromRest, kWithoutToken };
 
 // What a request's last token is drawn from, where that is not a pool.
@@ -614,7 +619,7 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
     const double all = sums.all_mass;
     // The cut lies in the bins from `low` to `high`; `last` is the one of the k-th entry. (One loop: the code of one search.)
     BinSums::Found low{0, 0.0, 0.0}, high = low, last = low;
-    double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - 1e-12);
+    double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - kTotalOff);
 #pragma unroll 1
     for (int search = 0; search < (by_count && by_mass ? 3 : 1); ++search) {
       const BinSums::Found found = sums.find(goal, by_count && search == 0);
@@ -1113,9 +1118,10 @@ __device__ __forceinline__ void settle_row(const VerifyArgs &a, const Setting &s
   const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
   double total = window.total;  // of what top_p is a share of, in units; 0: not known
   uint64_t goal = 0, entry = 0, left_mass = 0;  // the last entry that is left; of what is left
-  // The smallest whole number of units that is top_p of the total, within the rounding of sums and masses (so that
-  // 900 of 1,000 equal entries are 0.9 of them); at least one.
-  auto aim = [&]() { goal = (uint64_t)fmax(ceil(set.top_p * total * (1.0 - 1e-12 - 1.0 / unit)), 1.0); };
+  // The smallest whole number of units that is top_p of the total, within what that may be off by, or the rounding of the
+  // masses where it is their own sum (so that 900 of 1,000 equal entries are 0.9 of them); at least one.
+  const double off = window.total > 0.0 && !by_count ? kTotalOff : 1e-12;
+  auto aim = [&]() { goal = (uint64_t)fmax(ceil(set.top_p * total * (1.0 - off - 1.0 / unit)), 1.0); };
 #pragma unroll 1
   for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {
     const bool masses = stage == 1;

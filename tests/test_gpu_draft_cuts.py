@@ -118,3 +118,19 @@ def test_entries_that_no_bin_holds_beside_a_nan(setting, dtype):
     tokens = np.where(np.isnan(x[::2]), -INF, x[::2]).argmax(1)
     target = torch.from_numpy(x).to(V._dtype(dtype)).cuda()
     V._check(target, tokens, rng.random(requests), rng.random(requests), [setting], [1] * requests, uniform_rows=True, bad_ok=True)
+
+
+@pytest.mark.parametrize("count,top_p", [(10, 0.9), (10, 0.5), (1000, 0.9), (64, 0.25), (96, 0.75), (500, 0.2)])
+@pytest.mark.parametrize("floor", [-INF, -80.0])
+def test_equal_entries_under_a_mask(count, top_p, floor):
+    # The tokens that a mask leaves are equally likely, at any logit, and lie where the row is not sampled for its
+    # reference: top_p of `count` of them are a whole number.
+    torch = V._torch()
+    vocab, rows = 8192, 64
+    left = int((np.cumsum(np.ones(count)) < top_p * count).sum()) + 1
+    ids = 32 * np.arange(256)[:, None] + np.array([4, 9, 15, 21, 30])
+    ids = np.sort(np.random.default_rng(count).permutation(ids.ravel())[:count])
+    x = np.full((rows, vocab), floor)
+    x[:, ids] = np.linspace(0.03, 9.0, rows)[:, None]
+    got = _plain(torch.from_numpy(x).float().cuda(), [(0.7, 0, top_p)], [LAST] * rows)
+    assert got == [int(ids[left - 1])] * rows
