@@ -683,7 +683,7 @@ __device__ __forceinline__ RowDist pool_row(const VerifyArgs &a, int row, const 
       const int i = first + u * 64 + lane, p = (int)(((float)i + 0.5f) * per), turned = i - p * set.k + 5 * p;
       const int at = turned - (int)(((float)turned + 0.5f) * per) * set.k;
       // By all lanes: what a lane that is switched off holds is not read.
-      const int listed = __shfl(own.count, p & 63);
+      const int listed = __builtin_amdgcn_ds_bpermute((p & 63) << 2, own.count);
       e[u] = i < slots && at < listed ? entries[p * kPoolMax + at] : 0;
     }
 #pragma unroll
