@@ -23,7 +23,9 @@
 //   settle  workgroups to a request: the exact cuts of these rows, then, by the last of them, the decision
 //   weigh   (whole vocabularies) a workgroup to a segment of a deciding row: the sum of what is drawn from
 //   pick    (whole vocabularies) a workgroup to a request: the draw, among segments, then within one
-// Sums are in 64 bits, and exponentials within 5.5e-11: which token comes out hangs on comparisons of sums.
+// Sums are in 64 bits, and exponentials within 5.5e-11: which token comes out hangs on comparisons of sums. Of whole
+// vocabularies that are cut, running sums are compared with top_p of the total to within 2.5e-10 of it and 2^-52 of the
+// largest weight to an entry (3.4e-11 at 151,936 entries, 3.7e-9 at 2^24); pools to the last bits.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -75,8 +77,9 @@ struct RowDist {
 
 // Where the cut of a whole vocabulary's distribution lies, as its row's bins tell.
 struct RowCut {
-  double from, total;  // the mass above the window; what top_p is a share of, or 0: not known
+  double from, total;  // the mass above the window; what top_p is a share of, or 0: not known. Both in units of 2^-shift.
   float least, most;   // the window: logits at or above `least` and below `most`
+  int32_t shift;       // of the masses of its entries; 0: not known, and the window is all of the row
 };
 
 // What top_p of a row's total may be short of, relative to it, where that total comes from the row's bins or its parts' sums: up to
@@ -520,8 +523,10 @@ __device__ __forceinline__ T block_prefix(T v, T *scratch, T &total) {
   return before + v;
 }
 
-// Masses of a row's entries are whole multiples of 2^-shift: their sums are exact and do not depend on an order.
-__device__ __forceinline__ int mass_shift(int vocab) { return min(62 - (32 - __clz(vocab)), 51); }
+// Masses of a row's entries are whole multiples of 2^-shift: their sums are exact and do not depend on an order. As many bits as
+// the sum of all of them, `total` times the largest at most, leaves of 61, and 51 at most, which the rounding below has
+// room for: together they are off by 2^-52 of the largest to an entry, 2^-62 of the total where that is large.
+__device__ __forceinline__ int mass_shift(double total) { return min(60 - ilogb(total), 51); }
 __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, double unit) {
   // At most 2^51: added to 2^52 it is rounded to a whole number, in the low bits.
   const double whole = __builtin_fma(exp_or_none(((double)x - (double)max) * inverse), unit, 0x1p52);
@@ -603,9 +608,9 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
                                               double &most_share) {
   RowDist dist = whole_row(a, row, set);
   const float m = dist.max;
-  const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
   const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
-  window = {0.0, dist.total * unit, -INFINITY, INFINITY};
+  int shift = dist.total > 0.0 ? mass_shift(dist.total) : 0;  // (with room for what the total is off by)
+  window = {0.0, __builtin_ldexp(dist.total, shift), -INFINITY, INFINITY, shift};
   least_share = 0.0;
   most_share = INFINITY;
   if (dist.bad) return dist;
@@ -617,6 +622,8 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
     // What the sums may be off by: masses beside numbers are held in few bits.
     const double off = by_count ? 1e-4 : 1e-9, less = 1.0 - off, more = 1.0 + off;
     const double all = sums.all_mass;
+    shift = mass_shift(all * scale * more);
+    window.shift = shift;
     // The cut lies in the bins from `low` to `high`; `last` is the one of the k-th entry. (One loop: the code of one search.)
     BinSums::Found low{0, 0.0, 0.0}, high = low, last = low;
     double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - kTotalOff);
@@ -632,7 +639,7 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
     if (by_count) window.least = bin_begin(bins, last.bin);
     if (low.bin > 0) {  // (the lowest bin holds what lies below it as well)
       const float least = bin_begin(bins, low.bin);
-      if (!by_count) window = {high.above * scale * unit, all * scale * unit, least, bin_begin(bins, high.bin + 1)};
+      if (!by_count) window = {__builtin_ldexp(high.above * scale, shift), __builtin_ldexp(all * scale, shift), least, bin_begin(bins, high.bin + 1), shift};
       const double total_least = fmax(high.above, goal) * scale * less, total_most = (low.above + low.mass) * scale * more;
       dist.total = 0.5 * (total_least + total_most);
       dist.threshold = (uint64_t)key_of(least) << 32;
@@ -646,7 +653,7 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
       }
       return dist;
     }
-    window = {0.0, 0.0, -INFINITY, INFINITY};
+    window = {0.0, 0.0, -INFINITY, INFINITY, shift};
   } else if (!by_count && window.total > 0.0) {
     // Entries below (1 - top_p) total / vocab hold less than 1 - top_p together. (A margin for roundings.)
     const double low = (1.0 - set.top_p) * dist.total / (double)a.vocab * (1.0 - 1e-6);
@@ -1114,7 +1121,16 @@ template <int DT>
 __device__ __forceinline__ void settle_row(const VerifyArgs &a, const Setting &set, const RowCut &window, const Candidates<DT> &left, RowDist &dist, SettleScratch &s) {
   const int t = (int)threadIdx.x;
   const float m = dist.max;
-  const double unit = __builtin_ldexp(1.0, mass_shift(a.vocab));
+  int shift = window.shift;
+  if (shift == 0) {
+    // Their sum first, in the masses that as many entries alike would leave.
+    const double coarse = __builtin_ldexp(1.0, mass_shift((double)a.vocab));
+    uint64_t sum = 0, all;
+    left.each([&](float x, uint64_t) { sum += mass_of(x, m, set.inverse, coarse); });
+    block_prefix<kSettleWaves>(sum, s.wave64, all);
+    shift = mass_shift(((double)all + (double)a.vocab) / coarse);
+  }
+  const double unit = __builtin_ldexp(1.0, shift);
   const bool by_count = set.k < a.vocab, by_mass = set.top_p < 1.0;
   double total = window.total;  // of what top_p is a share of, in units; 0: not known
   uint64_t goal = 0, entry = 0, left_mass = 0;  // the last entry that is left; of what is left

@@ -134,3 +134,25 @@ def test_equal_entries_under_a_mask(count, top_p, floor):
     x[:, ids] = np.linspace(0.03, 9.0, rows)[:, None]
     got = _plain(torch.from_numpy(x).float().cuda(), [(0.7, 0, top_p)], [LAST] * rows)
     assert got == [int(ids[left - 1])] * rows
+
+
+@pytest.mark.parametrize("vocab,tail,top_p,dtype", [(151936, -31.5, 1 - 1e-9, "f32"),
+                                                    (2 ** 24, -27.0, 1 - 1e-5, "bf16"), (2 ** 24, -31.0, 1 - 2e-7, "bf16")])
+@pytest.mark.parametrize("top_k", [0, -1])
+@pytest.mark.parametrize("sampled", [True, False])
+def test_a_wide_tail_far_below_the_largest(vocab, tail, top_p, dtype, sampled, top_k):
+    # One entry, and all others alike and so light that only their number makes them matter: the cut lies among them where
+    # the running sum says, to what the sums may be off by: 2^-52 of the largest to an entry, 2.5e-10 of the total where
+    # it comes from the row's bins, and twice an exponential's 5.5e-11.
+    torch = V._torch()
+    peak = 0 if sampled else vocab // 3 // 4096 * 4096 + 1111  # the row's reference, or far above it
+    x = torch.full((1, vocab), tail, dtype=V._dtype(dtype), device="cuda")
+    x[0, peak] = 0.0
+    weight = float(np.exp(x[0, 5].double().item()))
+    k = vocab + top_k if top_k else 0
+    entries = (k or vocab) - 1
+    want = (top_p * (1 + entries * weight) - 1) / weight  # of the tail's entries; the index of the last, but for the peak's place
+    off = (2.5e-10 + 1.2e-10 + vocab * 2.0 ** -52) / weight + 2
+    assert 0.05 * vocab < off + want < 0.95 * vocab and off < 0.4 * vocab
+    got = _plain(x, [(1.0, k, top_p)], [LAST])[0]
+    assert abs(got - want) <= off, (got, want, off)
