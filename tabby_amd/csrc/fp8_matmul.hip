@@ -85,6 +85,30 @@ __device__ __forceinline__ void add_scaled(f32x4 &acc, f32x4 t, float s) {
   for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(t[i], s, acc[i]);
 }
 
+// Both scales' product is formed first, in f32: t, 0 or from 2^-18 to 2^25, is then one multiplication and addition away from
+// the sum. That product may be no ordinary number (blocks whose scales lie near f32's ends), although s_x s_w t is one: a wave that has met
+// such a block goes over its part again, in 64 bits, which hold s_x s_w exactly.
+struct ScaleRange {
+  float least = 1.0f, most = 1.0f;  // of the products' magnitudes; NaN is as good as any
+  template <int N>
+  __device__ __forceinline__ void see(const float (&s)[N], float sw) {
+    float low = __builtin_fabsf(s[0]), high = low;
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      low = __builtin_fminf(low, __builtin_fabsf(s[i]));
+      high = __builtin_fmaxf(high, __builtin_fabsf(s[i]));
+    }
+    least = __builtin_fminf(least, __builtin_fmaxf(low, sw == 0.0f ? 1.0f : 0.0f));  // (a weights' block that is empty; X's are not)
+    most = __builtin_fmaxf(most, high);
+  }
+  __device__ __forceinline__ bool odd() const { return __ballot(least < 0x1p-100f || most > 0x1p100f) != 0; }
+};
+__device__ __forceinline__ void add_scaled_wide(f32x4 &acc, f32x4 t, float sx, float sw) {
+  const double s = (double)sx * (double)sw;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = (float)__builtin_fma((double)t[i], s, (double)acc[i]);
+}
+
 // A square block's scale, the same for the whole wave: by the scalar unit, whose loads no wait for the vector ones holds up.
 __device__ __forceinline__ float block_scale_at(const float *scales, int64_t at) {
   typedef const __attribute__((address_space(4))) float Constant;
@@ -177,6 +201,7 @@ __global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product
   bring(lds[0]);
   int now = 0;
   float sw = block_scale_at(w_scales, at);
+  ScaleRange range;
   for (int first = 0; first < kp; first += KG) {
     const bool works = first + group < kp;  // the last group may have a panel less
     wait_and_meet<0>();
@@ -213,7 +238,24 @@ __global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product
     }
 #pragma unroll
     for (int c = 0; c < kX; ++c) add_scaled(acc[kW - 1][c], t[(kW - 1) & 1][c], s[c]);
+    range.see(s, sw);
     sw = sw_next;
+  }
+  if (range.odd()) {
+#pragma unroll
+    for (int i = 0; i < kW * kX; ++i) {
+      const int r = i / kX, c = i % kX;
+      const int64_t w_panel = panel_at(wm * PM + r / 4), x_panel = panel_at(WM * PM + wn * PN + c / 4);
+      const uint8_t *w_from_memory = p.w.codes + w_panel * kF8PanelBytes + r % 4 * kF8TileBytes + lane * 16;
+      const uint8_t *x_from_memory = p.x.codes + x_panel * kF8PanelBytes + c % 4 * kF8TileBytes + lane * 16;
+      const float *sx = p.x.scales + x_panel * kF8PanelRows + c % 4 * kF8TileRows + (lane & 15);
+      f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 1
+      for (int64_t k = group; k < kp; k += KG)
+        add_scaled_wide(sum, tile_product(Operand(read_tile(w_from_memory + k * kF8PanelBytes)), Operand(read_tile(x_from_memory + k * kF8PanelBytes))),
+                        sx[k * kF8PanelRows], block_scale_at(w_scales, k));
+      acc[r][c] = sum;
+    }
   }
   wait_and_meet<0>();
   if constexpr (KG > 1) {
@@ -313,7 +355,8 @@ struct FloatTiles {
   static_assert(kLds >= sums_bytes(kFewWaves, 1), "the slices' sums find room");
   struct Raw {};
   const uint8_t *codes;
-  __device__ __forceinline__ FloatTiles(const FloatRows &, const uint8_t *lds, int, int lane) : codes(lds + lane * 16) {}
+  bool held;  // the lane's row is one of x
+  __device__ __forceinline__ FloatTiles(const FloatRows &a, const uint8_t *lds, int, int lane) : codes(lds + lane * 16), held((lane & 15) < a.rows) {}
   static __device__ __forceinline__ void fill(const FloatRows &a, uint8_t *lds, int kp) {
     const int row_lanes = kp * kBlockLanes, all = a.rows * row_lanes;
     const float per_row = 1.0f / (float)row_lanes;  // all <= 2^10: (i + 1/2) / row_lanes has bits to spare
@@ -342,6 +385,7 @@ struct FloatTiles {
   __device__ __forceinline__ HalfOperand tile(const Raw &, int k, int, float &scale) const {
     const uint8_t *at = codes + k * kStepBytes;
     scale = *reinterpret_cast<const float *>(at - (int)(threadIdx.x & 63) * 16 + kF8TileBytes + (threadIdx.x & 15) * 4);
+    if (!held) scale = 1.0f;  // (nothing has been written there)
     return HalfOperand(read_tile(at));
   }
 };
@@ -372,6 +416,8 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
   auto bring = [&](int at, Step &s, int t) { s.w[t] = read_tile(wc + (int64_t)at * kF8PanelBytes + t * kF8TileBytes); };
   typename Rows::Raw raw;
   f32x4 acc[4][NT] = {};
+  const int begin = k;
+  ScaleRange range;
   auto multiply = [&](int at, Step &s, auto more) {
     constexpr bool kMore = decltype(more)::value != 0;
     typename Rows::Operand x[NT];
@@ -381,6 +427,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
       x[u] = rows.tile(raw, at, u, both[u]);
       both[u] *= s.scale;
     }
+    range.see(both, s.scale);
     rows.load(min(at + 1, end - 1), raw);
     if constexpr (kMore) s.scale = block_scale_at(ws, at + kAhead);
 #pragma unroll
@@ -422,6 +469,25 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void fp8_few_kernel(Fp8Product p
     } else {
       if (k < end) multiply(k, steps[0], kWithout);
       if (k + 1 < end) multiply(k + 1, steps[1], kWithout);
+    }
+  }
+  if (range.odd()) {
+#pragma unroll
+    for (int i = 0; i < 4 * NT; ++i) acc[i / NT][i % NT] = f32x4{0, 0, 0, 0};
+#pragma unroll 1
+    for (k = begin; k < end; ++k) {
+      rows.load(k, raw);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        float sx;
+        const typename Rows::Operand x = rows.tile(raw, k, u, sx);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const typename Rows::Operand w(read_tile(wc + (int64_t)k * kF8PanelBytes + t * kF8TileBytes));
+          add_scaled_wide(acc[t][u], tile_product(w, x), sx, block_scale_at(ws, k));
+          __builtin_amdgcn_sched_barrier(0);  // one at a time, in few registers
+        }
+      }
     }
   }
   // The slices in halves: the upper half's sums go through LDS to the lower half's waves.

@@ -117,3 +117,51 @@ def test_fast_sums_where_they_make_no_difference_and_where_they_are_refused():
         P._fp8().matmul(x, w, fast_sums=True)
     with pytest.raises(S.SamplingError, match="f16 and bf16 results"):
         P._fp8().matmul(P._fp8().Fp8Matrix.quantize(x), w, out=torch.empty(64, 700, device="cuda"), fast_sums=True)
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", SIZES)
+def test_scales_whose_product_is_no_f32(rows, n, out):
+    # Both sides' scales lie within f32, their product above its largest value or below its smallest one, the result within
+    # it: a block whose codes' sum is zero or small enough; or all of it among the smallest, with ordinary blocks beside.
+    torch = P._torch()
+    k = 640
+    rng = np.random.default_rng(rows + n)
+    x = np.zeros((rows, k))
+    w = np.zeros((n, k))
+    # Block 0: 2^110 times 2^25 and nothing that meets; block 1: the smallest codes, 2^-18 of 2^(110 + 20).
+    x[:, 0], w[:, 1] = 448.0 * 2.0 ** 110, 448.0
+    x[:, 128], x[:, 129], w[:, 129] = 448.0 * 2.0 ** 110, 2.0 ** -9 * 2.0 ** 110, 2.0 ** -9
+    # Block 2: 2^-126 times 2^-20 or so of 3 x 448^2; block 3 as ordinary as can be; block 4 ordinary but for one row.
+    x[:, 256:259], w[:, 256:259] = 448.0 * 2.0 ** -126, 448.0
+    x[:, 384:400], w[:, 384:400] = rng.integers(-16, 17, (rows, 16)), rng.integers(-16, 17, (n, 16))
+    x[:, 512:520], w[:, 512:520] = rng.integers(-16, 17, (rows, 8)), rng.integers(-16, 17, (n, 8))
+    x[rows // 2, 512:520] *= 2.0 ** -100
+    blocks = -(-n // 128)
+    scales = np.ones((blocks, 5))
+    scales[:, 0], scales[:, 1], scales[:, 2] = 2.0 ** 25, 2.0 ** 20, 1.37 * 2.0 ** -20
+    scales[:, 3], scales[:, 4] = 0.9 * 2.0 ** -10, 0.7 * 2.0 ** -14
+
+    def check(xs, ws, ss):
+        m = _held(ws, ss)
+        xv = F.rounded(xs.astype(np.float32))
+        wv = ws * ss.astype(np.float32).astype(np.float64).repeat(128, 0)[:n].repeat(128, 1)[:, :k]
+        want = xv @ wv.T
+        # To f32's sums, and among the smallest values half a step to each block and one to the result.
+        limit = P._bound(xv, wv, want, k, "f32") + 6 * 2.0 ** -150
+        if out == "bf16":
+            limit = limit + 2.0 ** -8 * (np.abs(want) + limit) + 2.0 ** -134
+        got = P._fp8().matmul(torch.from_numpy(xs).float().cuda(), m, dtype=P._dtype(out)).double().cpu().numpy()
+        assert np.isfinite(want).all() and (np.abs(got - want) <= limit).all(), np.argwhere(~(np.abs(got - want) <= limit))[:4]
+
+    print(f"far scales {rows} x {n} to {out}", flush=True)
+    check(x, w, scales)
+    low, few = x.copy(), w.copy()
+    low[:, :256] = 0.0
+    low[:, 384:] = 0.0
+    check(low, few, scales)  # only what lies among the smallest
+    some = x.copy()
+    some[: rows // 2, :384] = 0.0
+    check(some, w, scales)   # rows of ordinary scales beside others
+    scales[:, :3] = 0.0
+    check(x, w, scales)      # weights' blocks that are empty
