@@ -114,7 +114,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       // only; ref + 600 would be 1,024 above a ref of 2^33.)
       const float m = wave_max(top);
       if (m < INFINITY) {
-        sum *= exp_or_none((double)ref - (double)m);
+        sum *= exp_or_none<false>((double)ref - (double)m);
         ref = m;
       }
     }
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
       const double at = (double)ref;
       double part_sum[2] = {0.0, 0.0};
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) part_sum[i & 1] += exp_or_none((double)x[i] - at);
+      for (int i = 0; i < kLane; ++i) part_sum[i & 1] += exp_or_none<false>((double)x[i] - at);
       sum += part_sum[0] + part_sum[1];
     }
   };
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {
   if (wave == 0) {
     const float m = wave_max(lane < NW ? wave_max_[lane] : -INFINITY);
     double term = lane < NW ? wave_sum_[lane] : 0.0;
-    if (term > 0.0) term *= exp_or_none((double)wave_ref[lane] - (double)m);
+    if (term > 0.0) term *= exp_or_none<false>((double)wave_ref[lane] - (double)m);
     term = wave_sum(term);
     if (t == 0) a.sums[blockIdx.x] = RowSum{term, m, (int)need, 0, 0};
   }
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(NW * 64) void beam_merge_kernel(BeamArgs a, int wid
 #pragma unroll
   for (int stride = 1; stride < kPartsMax; stride *= 2)
     if (stride < width) m = fmaxf(m, xor_lane_by(m, stride));
-  double sum = rs.count > 0 ? rs.sum * exp_or_none((double)rs.max - (double)m) : 0.0;
+  double sum = rs.count > 0 ? rs.sum * exp_or_none<false>((double)rs.max - (double)m) : 0.0;
 #pragma unroll
   for (int stride = 1; stride < kPartsMax; stride *= 2)
     if (stride < width) sum += xor_lane_by(sum, stride);

@@ -232,10 +232,10 @@ struct RowBins {
   static __device__ __forceinline__ uint64_t mass(double f) {
     constexpr double kUnit = 274877906944.0;
     static_assert(kUnit == (double)(1ll << kMassBits), "the unit");
-    double p = fma_const(f, 1.4676387238435006e-07 * kUnit, 1.3551205154935067e-05 * kUnit);
-    p = fma_const(p, f, 0.0009383847926296646 * kUnit);
-    p = fma_const(p, f, 0.043321698760160544 * kUnit);
-    return (uint64_t)__double_as_longlong(fma_const(p, f, kUnit + 0x1p52)) & ((1ull << 52) - 1);
+    double p = fma_const<true>(f, 1.4676387238435006e-07 * kUnit, 1.3551205154935067e-05 * kUnit);
+    p = fma_const<true>(p, f, 0.0009383847926296646 * kUnit);
+    p = fma_const<true>(p, f, 0.043321698760160544 * kUnit);
+    return (uint64_t)__double_as_longlong(fma_const<true>(p, f, kUnit + 0x1p52)) & ((1ull << 52) - 1);
   }
   // What a bin holds: its number, if it has one, and its mass, relative to the reference's.
   static __device__ __forceinline__ double2 worth(uint64_t v, int bin, bool counts) {

@@ -20,38 +20,45 @@ constexpr int kListMax = 4096;                // entries above the bound that LD
 
 typedef uint32_t uint32x2 __attribute__((ext_vector_type(2)));
 
-// a b + c, c a constant: written out, because the compiler copies c to registers first to add to it there.
+// a b + c, c a constant. HELD: written out, so that c stays in scalar registers, where the compiler copies it to vector ones first to
+// add to it there: for kernels that have none to spare (the verification's decision spills 13 without it). The beam selection has, and
+// takes 67 us with the copies and 70 without (64 groups of eight beams over 151,936 f32).
+template <bool HELD>
 __device__ __forceinline__ double fma_const(double a, double b, double c) {
+  if constexpr (!HELD) return __builtin_fma(a, b, c);
   double r;
   asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
   return r;
 }
 
 // 2^f in 64 bits for f in [-1/2, 1/2]: the polynomial of degree 7 through it at the Chebyshev nodes, within 5.5e-11 of it.
+template <bool HELD = true>
 __device__ __forceinline__ double exp2_64(double f) {
-  double p = fma_const(f, 1.530370102315244e-05, 0.0001546972921563772);
-  p = fma_const(p, f, 0.0013333478472326247);
-  p = fma_const(p, f, 0.009618025613309008);
-  p = fma_const(p, f, 0.055504109063275894);
-  p = fma_const(p, f, 0.24022651213498245);
-  p = fma_const(p, f, 0.6931471805568318);
-  return fma_const(p, f, 0.9999999999595618);
+  double p = fma_const<HELD>(f, 1.530370102315244e-05, 0.0001546972921563772);
+  p = fma_const<HELD>(p, f, 0.0013333478472326247);
+  p = fma_const<HELD>(p, f, 0.009618025613309008);
+  p = fma_const<HELD>(p, f, 0.055504109063275894);
+  p = fma_const<HELD>(p, f, 0.24022651213498245);
+  p = fma_const<HELD>(p, f, 0.6931471805568318);
+  return fma_const<HELD>(p, f, 0.9999999999595618);
 }
 
 // exp(d) in 64 bits for d in [-690, 690]: t = d log2(e) is split into the nearest whole number, found by adding
 // and taking away 1.5 * 2^52, whose low word then holds it, and the rest f in [-1/2, 1/2]. A sum of such terms
 // decides the order of two beams' continuations only where their scores are that close.
+template <bool HELD = true>
 __device__ __forceinline__ double exp_64(double d) {
   constexpr double kLog2e = 1.4426950408889634;
   const double magic = 6755399441055744.0;
   const double shifted = __builtin_fma(d, kLog2e, magic);
-  uint32x2 bits = __builtin_bit_cast(uint32x2, exp2_64(__builtin_fma(d, kLog2e, -(shifted - magic))));
+  uint32x2 bits = __builtin_bit_cast(uint32x2, exp2_64<HELD>(__builtin_fma(d, kLog2e, -(shifted - magic))));
   bits.y += __builtin_bit_cast(uint32x2, shifted).x << 20;
   return __builtin_bit_cast(double, bits);
 }
 // The same for any d <= 690, -inf too: below -690 nothing is left that a sum of at least 1 would hold. Above 690 the
 // exponent's field runs over, and the result, NaN included, has nothing to do with exp.
-__device__ __forceinline__ double exp_or_none(double d) { return exp_64(fmax(d, -690.0)); }
+template <bool HELD = true>
+__device__ __forceinline__ double exp_or_none(double d) { return exp_64<HELD>(fmax(d, -690.0)); }
 
 // The larger of two, NaN if either is: a chunk's maximum shows that it holds a NaN.
 __device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
