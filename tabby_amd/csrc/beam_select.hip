@@ -69,7 +69,7 @@ __device__ __forceinline__ bool beam_reads(const BeamArgs &a, int row) {
 // One workgroup of NW waves to a part of a row, every element read once. Many rows are bound by the issue of
 // the 64-bit terms (16 operations an element) and by HBM, which one wave does not overlap: it asks for its next
 // chunk before it looks at this one, but waits for it at the loop's end, and the unit's other waves cover that.
-// 512 rows of 151,936 f32 in 65 us, 4.8 TB/s; the whole call 66, from f16 63, from bf16 59. Few rows are bound by
+// 512 rows of 151,936 f32 in 65 us, 4.8 TB/s; the whole call 67, from f16 63, from bf16 59. Few rows are bound by
 // latency: the load, the bound, the list, the ranks (four rows in 19 parts each: 7.7 us).
 template <int DT, bool MASK, int NW>
 __global__ __launch_bounds__(NW * 64) void beam_row_kernel(BeamArgs a) {

@@ -123,10 +123,12 @@ struct Fp8Product {
 // A workgroup of WM x WN waves has a tile of WM PM x WN PN panels of Y (64 x 64), PM x PN to a wave, and takes a
 // panel of k (128) at a time. The panels of a stage lie in LDS as they do in memory, W's before X's, then X's scales,
 // brought there without passing through registers, a stage ahead. A wave holds the tiles of X and goes through those
-// of W; a tile's results are added while the next one's products run. 4,096 rows, W of 16,384 x 4,096 to bf16: 237 us, 2.3
-// PFLOP/s; the chip's power bounds it (orders of a step that take 674,000, 600,000 and 544,000 cycles, 262,000 of them the matrix
-// cores', take the same time, at 2.2 to 1.87 GHz; without the scaled additions 13 % less), so the order is the simplest. Where there are few tiles, KG groups of such waves
-// take every KG-th panel of k, each with stages of its own, and add up through LDS.
+// of W; a tile's results are added while the next one's products run. 4,096 rows, W of 16,384 x 4,096 to bf16: 460 us, 1.2
+// PFLOP/s, of which the f16 instructions' rate allows some 450 (the library's bf16 product runs at 1.23); to f32 499. As codes, in
+// tiles of 256 x 256: 252 us, 2.2 PFLOP/s, and the chip's power bounds it (orders of a step that take 674,000, 600,000 and 544,000 cycles,
+// 262,000 of them the matrix cores', take the same time, at 2.2 to 1.87 GHz; without the scaled additions 13 % less), so the
+// order is the simplest. Where there are few tiles, KG groups of such waves take every KG-th panel of k, each with stages of
+// its own, and add up through LDS.
 template <int PM, int PN, int WM, int WN, int KG>
 struct TileShape {
   static constexpr int kWaves = WM * WN;
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(KG *WM *WN * 64, 2) void fp8_tile_kernel(Fp8Product
 // NT tiles of 16 rows; where there are few panels, `slices` waves of the workgroup take a part of k each and add up
 // through LDS. The registers of a tile of W take the next panel's as soon as the tile is read, so a panel is on its way
 // all the time (two for one tile of rows, which leaves the registers). Workgroups of four waves where the slices allow:
-// one token, W of 151,936 x 896: 27 us, of which the weights' 136 MB need 21 to 26; workgroups of eight took 30 us.
+// one token, W of 151,936 x 896: 22 us, 6.2 TB/s, and 27 us a call; with workgroups of eight the call took 30 us.
 struct FewShape {
   int waves, slices;  // of a workgroup; powers of two
 };
@@ -528,8 +530,8 @@ constexpr int64_t kTilesMax = 1 << 22;  // of a launch: 2^32 threads are too man
 int64_t small_tiles(int n, int rows) { return f8_parts(n, 128) * f8_parts(rows, 128); }
 
 // Whether W is streamed into registers: up to 64 rows, which one wave takes, and where tiles of 128 x 128 would leave half
-// of the units idle (300 rows, W of 4,864 x 4,096: to bf16 21 us, in tiles 26; to f32 25 us, in tiles 41. 512 rows: to bf16 36 us,
-// in tiles 27).
+// of the units idle (W of 4,864 x 4,096 to bf16, the product alone. 300 rows: 19 us, in tiles 33; as codes 15, in tiles 20. 512 rows: 30 us, in
+// tiles 33; as codes 26, in tiles 21).
 bool few_rows(int n, int rows) { return rows <= kF8PanelRows || small_tiles(n, rows) < kCus / 2; }
 
 template <int DT, typename Operand, int PM, int PN, int WM, int WN, int KG>
@@ -571,7 +573,7 @@ int launch_product(const Fp8Product &p, hipStream_t s) {
     if constexpr (std::is_same<Most, CodeOperand>::value) {
       if (large_tiles(p.w.rows, p.x.rows)) return launch_tiles<DT, Most, 2, 1, 2, 4, 1>(p, s);
     }
-    // (512 rows, W of 4,864 x 4,096: 27 us with two groups of waves, 31 us with one.)
+    // (512 rows, W of 4,864 x 4,096 to bf16: 33 us with two groups of waves, 41 us with one; as codes 21 and 25.)
     return small_tiles(p.w.rows, p.x.rows) <= kCus ? launch_tiles<DT, Most, 1, 1, 2, 2, 2>(p, s) : launch_tiles<DT, Most, 1, 1, 2, 2, 1>(p, s);
   }
   switch (f8_parts(p.x.rows, kF8TileRows)) {
