@@ -525,7 +525,7 @@ __device__ __forceinline__ T block_prefix(T v, T *scratch, T &total) {
 
 // Masses of a row's entries are whole multiples of 2^-shift: their sums are exact and do not depend on an order. As many bits as
 // the sum of all of them, `total` times the largest at most, leaves of 61, and 51 at most, which the rounding below has
-// room for: together they are off by 2^-52 of the largest to an entry, 2^-62 of the total where that is large.
+// room for: together they are off by 2^-52 of the largest to an entry, or by 2^-61 of the total where that is large.
 __device__ __forceinline__ int mass_shift(double total) { return min(60 - ilogb(total), 51); }
 __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, double unit) {
   // At most 2^51: added to 2^52 it is rounded to a whole number, in the low bits.

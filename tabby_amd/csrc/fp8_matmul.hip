@@ -98,7 +98,7 @@ struct ScaleRange {
       low = __builtin_fminf(low, __builtin_fabsf(s[i]));
       high = __builtin_fmaxf(high, __builtin_fabsf(s[i]));
     }
-    least = __builtin_fminf(least, __builtin_fmaxf(low, sw == 0.0f ? 1.0f : 0.0f));  // (a weights' block that is empty; X's are not)
+    least = __builtin_fminf(least, sw == 0.0f ? 1.0f : low);  // (a weights' block that is empty; X's are not)
     most = __builtin_fmaxf(most, high);
   }
   __device__ __forceinline__ bool odd() const { return __ballot(least < 0x1p-100f || most > 0x1p100f) != 0; }
