@@ -1365,7 +1365,9 @@ struct RestOf {
   double rest[E::kVec], all[E::kVec];
   static __device__ __forceinline__ double share(uint64_t threshold, float max, double inverse, double scale, float x, int e) {
     if (!(x > -INFINITY) || composite(key_of(x), (uint32_t)e) < threshold) return 0.0;
-    return exp_or_none(((double)x - (double)max) * inverse) * scale;
+    // Below e^-690 there is nothing: what is left of a P that is Q, or comes first at a uniform of zero, must not be that.
+    const double d = ((double)x - (double)max) * inverse;
+    return d >= -690.0 ? exp_64(d) * scale : 0.0;
   }
   __device__ __forceinline__ RestOf(const VerifyArgs &a, const Decision &d, int first) {
     const int vocab = a.vocab;

@@ -156,3 +156,26 @@ def test_a_wide_tail_far_below_the_largest(vocab, tail, top_p, dtype, sampled, t
     assert 0.05 * vocab < off + want < 0.95 * vocab and off < 0.4 * vocab
     got = _plain(x, [(1.0, k, top_p)], [LAST])[0]
     assert abs(got - want) <= off, (got, want, off)
+
+
+@pytest.mark.parametrize("with_draft", [True, False])
+@pytest.mark.parametrize("dtype", V.TYPES)
+def test_rows_of_one_possible_token(dtype, with_draft):
+    # All but one entry lie so far below it that they have no probability in 64 bits: a drafted token among them is refused, and
+    # the one comes out, for uniforms of zero too, whichever of the others top_k left beside it.
+    torch = V._torch()
+    rng = np.random.default_rng(12)
+    settings = [(0.05, 0, 1.0), (0.05, 0, 0.9), (0.05, 1102, 1.0), (0.05, 400, 0.99), (0.05, 40, 1.0), (0.05, 3000, 1.0)]
+    vocab, requests = 3875, 12
+    x = rng.normal(size=(2 * requests, vocab)) * 3
+    y = x[::2] + rng.normal(size=(requests, vocab))
+    for r in range(requests):
+        peak = int(rng.integers(0, vocab))
+        x[2 * r, peak] = y[r, peak] = 200.0
+        x[2 * r + 1, rng.integers(0, vocab)] = 200.0
+    target, draft = (torch.from_numpy(v).to(V._dtype(dtype)).cuda() for v in (x, y))
+    for seed in range(4):
+        rng = np.random.default_rng(seed)
+        tokens = rng.integers(0, vocab, requests) if seed % 2 else x[::2].argmax(1)
+        lasts = rng.random(requests) if seed < 2 else np.zeros(requests)
+        V._check(target, tokens, rng.random(requests), lasts, settings, [1] * requests, draft if with_draft else None, uniform_rows=True)
