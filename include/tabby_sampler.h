@@ -385,8 +385,8 @@ TABBY_API int tabby_draft_workspace(int32_t requests, int32_t drafts_max, int32_
  * settings, those of the target and of the draft, and the uniform of its last draw.
  * P and Q are what sampleFromTopK draws from for a row of the target and of the draft: the first top_k
  * entries by (logit, lower index), weights exp((x - max) / temperature), those up to and with the first at
- * which their running sum reaches top_p of the total (of more than 128 entries: to within 2.5e-10 of it and 2^-52 of the
- * largest weight to an entry), divided by their sum; temperature <= 0: the first
+ * which their running sum reaches top_p of the total (of more than 128 entries: to within 1e-11 of it, 2.5e-10
+ * where the call has more than 4,096 rows, and 2^-52 of the largest weight to an entry), divided by their sum; temperature <= 0: the first
  * entry. A drafted token d is accepted while uniform * Q(d) < P(d), Q(d) being 1 where the tokens were certain and where
  * temperature <= 0. The next token is drawn from max(P - Q, 0) at the first refusal (from P without d where d was
  * certain), from the last row's P if there is none: the first token in the vocabulary's order at which the

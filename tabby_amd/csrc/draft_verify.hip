@@ -24,8 +24,9 @@
 //   weigh   (whole vocabularies) a workgroup to a segment of a deciding row: the sum of what is drawn from
 //   pick    (whole vocabularies) a workgroup to a request: the draw, among segments, then within one
 // Sums are in 64 bits, and exponentials within 5.5e-11: which token comes out hangs on comparisons of sums. Of whole
-// vocabularies that are cut, running sums are compared with top_p of the total to within 2.5e-10 of it and 2^-52 of the
-// largest weight to an entry (3.4e-11 at 151,936 entries, 3.7e-9 at 2^24); pools to the last bits.
+// vocabularies that are cut, running sums are compared with top_p of the total to within 1e-11 of it (2.5e-10 where there are more
+// lists than have bins) and 2^-52 of the largest weight to an entry (3.4e-11 at 151,936 entries, 3.7e-9 at 2^24, at most); pools to the
+// last bits.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -82,10 +83,11 @@ struct RowCut {
   int32_t shift;       // of the masses of its entries; 0: not known, and the window is all of the row
 };
 
-// What top_p of a row's total may be short of, relative to it, where that total comes from the row's bins or its parts' sums: up to
-// three exponentials, 5.5e-11 each, on top of the one in the entries' own masses. Without it the last of the entries that make up
-// the share exactly (nine of ten equal ones, for 0.9) would not do.
-constexpr double kTotalOff = 2.5e-10;
+// What top_p of a row's total may be short of, relative to it, where that total is not the sum of the entries' own masses: from the
+// bins, their polynomial's 2.5e-12 and its rounding's 1.9e-12, and as much for what lies above the window; from the parts' sums,
+// up to three exponentials of 5.5e-11 each. Without it the last of the entries that make up the share exactly (nine of ten equal ones, for
+// 0.9) would not do.
+constexpr double kBinsOff = 1e-11, kSumsOff = 2.5e-10;
 
 enum Draw : int32_t { kDone = 0, kFromTarget, kFromRest, kWithoutToken };
 
@@ -241,8 +243,12 @@ struct RowBins {
   static __device__ __forceinline__ double2 worth(uint64_t v, int bin, bool counts) {
     const double number = counts ? (double)(uint32_t)(v >> kCountShift) : 0.0;
     if (counts) v &= (1ull << kCountShift) - 1;
-    const double power = (double)(bin - kBinsBelow) * (1.0 / kPerOctave), whole = rint(power);
-    return {number, __builtin_ldexp((double)v * exp2_64(power - whole), (int)whole - (counts ? kSmallBits : kMassBits))};
+    static_assert(kPerOctave == 16 && kBinsBelow % kPerOctave == 0, "four bits of a bin are its sixteenths");
+    double sixteenths = (bin & 8) != 0 ? 1.4142135623730951 : 1.0;
+    sixteenths *= (bin & 4) != 0 ? 1.189207115002721 : 1.0;
+    sixteenths *= (bin & 2) != 0 ? 1.0905077326652577 : 1.0;
+    sixteenths *= (bin & 1) != 0 ? 1.0442737824274138 : 1.0;
+    return {number, __builtin_ldexp((double)v * sixteenths, bin / kPerOctave - kBinsBelow / kPerOctave - (counts ? kSmallBits : kMassBits))};
   }
   // One entry and its mass, within 2^-14 of it.
   static __device__ __forceinline__ uint64_t one_and_mass(double f) {
@@ -529,7 +535,7 @@ __device__ __forceinline__ T block_prefix(T v, T *scratch, T &total) {
 __device__ __forceinline__ int mass_shift(double total) { return min(60 - ilogb(total), 51); }
 __device__ __forceinline__ uint64_t mass_of(float x, float max, double inverse, double unit) {
   // At most 2^51: added to 2^52 it is rounded to a whole number, in the low bits.
-  const double whole = __builtin_fma(exp_or_none(((double)x - (double)max) * inverse), unit, 0x1p52);
+  const double whole = __builtin_fma(exp_nonpos(((double)x - (double)max) * inverse), unit, 0x1p52);
   return (uint64_t)__double_as_longlong(whole) & ((1ull << 52) - 1);
 }
 
@@ -626,7 +632,7 @@ __device__ __forceinline__ RowDist screen_row(const VerifyArgs &a, int row, cons
     window.shift = shift;
     // The cut lies in the bins from `low` to `high`; `last` is the one of the k-th entry. (One loop: the code of one search.)
     BinSums::Found low{0, 0.0, 0.0}, high = low, last = low;
-    double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - kTotalOff);
+    double goal = by_count ? (double)set.k : set.top_p * all * (1.0 - kBinsOff);
 #pragma unroll 1
     for (int search = 0; search < (by_count && by_mass ? 3 : 1); ++search) {
       const BinSums::Found found = sums.find(goal, by_count && search == 0);
@@ -1138,7 +1144,7 @@ __device__ __forceinline__ void settle_row(const VerifyArgs &a, const Setting &s
   uint64_t goal = 0, entry = 0, left_mass = 0;  // the last entry that is left; of what is left
   // The smallest whole number of units that is top_p of the total, within what that may be off by, or the rounding of the
   // masses where it is their own sum (so that 900 of 1,000 equal entries are 0.9 of them); at least one.
-  const double off = window.total > 0.0 && !by_count ? kTotalOff : 1e-12;
+  const double off = by_count || !(window.total > 0.0) ? 1e-12 : a.bins ? kBinsOff : kSumsOff;
   auto aim = [&]() { goal = (uint64_t)fmax(ceil(set.top_p * total * (1.0 - off - 1.0 / unit)), 1.0); };
 #pragma unroll 1
   for (int stage = by_count ? 0 : 1; stage < (by_mass ? 2 : 1); ++stage) {

@@ -179,3 +179,22 @@ def test_rows_of_one_possible_token(dtype, with_draft):
         tokens = rng.integers(0, vocab, requests) if seed % 2 else x[::2].argmax(1)
         lasts = rng.random(requests) if seed < 2 else np.zeros(requests)
         V._check(target, tokens, rng.random(requests), lasts, settings, [1] * requests, draft if with_draft else None, uniform_rows=True)
+
+
+@pytest.mark.parametrize("gap", [21.8, 22.0, 23.0])
+def test_a_share_that_all_but_equals_top_p(gap):
+    # Two equal entries, half of the total each but for a third one, the row's reference, of 1.7e-10 to 5e-11 of it: top_p 0.5
+    # takes both.
+    torch = V._torch()
+    vocab, rows = 60000, 32
+    x = np.full((rows, vocab), -300.0)
+    rng = np.random.default_rng(3)
+    want = []
+    for r in range(rows):
+        pair = 64 * np.sort(rng.permutation(vocab // 64 - 1)[:2]) + 37
+        x[r, pair], x[r, 0] = 2.0 + r, 2.0 + r - gap
+        share = np.nonzero(D.shares(x[r].astype(np.float32), 1.0, 0, 0.5))[0]
+        assert share.tolist() == pair.tolist()
+        want.append(int(pair[1]))
+    got = _plain(torch.from_numpy(x).float().cuda(), [(1.0, 0, 0.5)], [LAST] * rows)
+    assert got == want
