@@ -123,9 +123,9 @@ struct Fp8Product {
 // A workgroup of WM x WN waves has a tile of WM PM x WN PN panels of Y (64 x 64), PM x PN to a wave, and takes a
 // panel of k (128) at a time. The panels of a stage lie in LDS as they do in memory, W's before X's, then X's scales,
 // brought there without passing through registers, a stage ahead. A wave holds the tiles of X and goes through those
-// of W; a tile's results are added while the next one's products run. 4,096 rows, W of 16,384 x 4,096 to bf16: 460 us, 1.2
-// PFLOP/s, of which the f16 instructions' rate allows some 450 (the library's bf16 product runs at 1.23); to f32 499. As codes, in
-// tiles of 256 x 256: 252 us, 2.2 PFLOP/s, and the chip's power bounds it (orders of a step that take 674,000, 600,000 and 544,000 cycles,
+// of W; a tile's results are added while the next one's products run. 4,096 rows, W of 16,384 x 4,096 to bf16: 460 to 473 us, one card or
+// another, 1.2 PFLOP/s, of which the f16 instructions' rate allows some 450 (the library's bf16 product runs at 1.23); to f32 499 to
+// 511. As codes, in tiles of 256 x 256: 252 us, 2.2 PFLOP/s, and the chip's power bounds it (orders of a step that take 674,000, 600,000 and 544,000 cycles,
 // 262,000 of them the matrix cores', take the same time, at 2.2 to 1.87 GHz; without the scaled additions 13 % less), so the
 // order is the simplest. Where there are few tiles, KG groups of such waves take every KG-th panel of k, each with stages of
 // its own, and add up through LDS.
